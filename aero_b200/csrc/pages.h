@@ -1,0 +1,86 @@
+// The paged key/value cache (include/aero_cuda_pages.h): what its translation
+// units share. pages.cu owns the handle and the books, pages_decode.cu the
+// attention.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/aero_cuda_pages.h"
+
+namespace aero {
+
+// The cache as kernels see it.
+struct PageView {
+    int32_t* table;   // (n_seq, max_pages)
+    int32_t* length;  // (n_seq)
+    int32_t* refs;    // (n_page)
+    int32_t* status;  // first code recorded, 0: none
+    int32_t n_page, page_shift, HK, D, n_seq, max_pages, n_layer;
+};
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ void pages_flag(const PageView& c, int code) { atomicCAS(c.status, 0, code); }
+// Length of sequence s as kernels may use it: 0 for a number outside the table,
+// never past what its row of the table can hold.
+__device__ __forceinline__ int pages_length(const PageView& c, int s) {
+    if (s < 0 || s >= c.n_seq) return 0;
+    const int64_t cap = (int64_t)c.max_pages << c.page_shift;
+    const int n = c.length[s];
+    return n < 0 ? 0 : (int64_t)n > cap ? (int)cap : n;
+}
+#endif
+
+// One attention call. Strides are in elements; vec: q and out rows may be read and
+// written 16 bytes at a time.
+struct AttendArgs {
+    PageView c;
+    const void* q;
+    int64_t q_token, q_head;
+    void* out;
+    int64_t o_token, o_head;
+    const int32_t* seqs;
+    const int32_t* q_start;  // null: one token per sequence
+    int layer, T, n, H, window, sinks;
+    float scale_log2;  // scale * log2(e): scores are in powers of two
+    int vec;
+    float* part;        // partial results of units that several CTAs share
+    uint32_t* counters; // arrivals per shared unit; zero between launches
+};
+
+#if defined(__CUDACC__)
+// Which sequence token t is of, and how many of its positions the token sees at most
+// (its own position + 1). q_start is searched within its n + 1 entries whatever they hold.
+__device__ __forceinline__ void token_rows(const AttendArgs& a, int t, int& seq, int& n) {
+    if (!a.q_start) {
+        seq = a.seqs[t];
+        n = pages_length(a.c, seq);
+        return;
+    }
+    int lo = 0, hi = a.n;  // the last i < n with q_start[i] <= t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.q_start[mid] <= t)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    seq = a.seqs[lo];
+    const int q0 = a.q_start[lo], q1 = a.q_start[lo + 1], len = pages_length(a.c, seq);
+    n = len - (q1 - q0) + (t - q0) + 1;
+    if (t < q0 || t >= q1 || q1 - q0 > len) {
+        pages_flag(a.c, AERO_CUDA_PAGES_BAD_ROWS);
+        n = 0;
+    }
+}
+#endif
+
+// Workspace the kernel needs for a cache of this shape.
+size_t pages_decode_part_floats(int D, int n_sm);
+int pages_decode_max_grid(int n_sm);
+// kmap / vmap: (n_layer * n_page * HK * page rows, D) with boxes of min(page, 64)
+// rows by 64 columns, 128-byte swizzle.
+cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                                int n_sm, cudaStream_t s);
+
+}  // namespace aero

@@ -1,0 +1,505 @@
+// Attention of one new token per sequence over the paged cache
+// (include/aero_cuda_pages.h): o = sum_j softmax_j(scale q . k_j) v_j over the visible
+// positions, one pass over K and V with a running maximum m and sum l:
+//   m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),
+//   o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j     (s in powers of two),
+// and two partial results join by the same rule.
+//
+// Bound by HBM: every visible K and V row is read once (up to 16 query heads share it,
+// at most 16 operations a byte).
+//
+// Split: the work of the call is one line of units, unit = 64 positions of one
+// (sequence, kv head); each CTA takes an equal piece of the line, wherever it begins, so
+// sequences of any lengths load the GPU evenly and one long sequence is split over all of
+// it. A (sequence, head) whose units lie in one CTA is finished there; the others leave
+// partial results (o, m, l), and the CTA that arrives last joins them in the line's
+// order, so the sums do not depend on timing.
+//
+// A CTA: one producer warp brings units into a ring of stages by TMA (a page is a run of
+// rows per head; a box of min(page, 64) rows by 64 columns, swizzled), four consumer warps
+// take 16 positions of each unit: S = Q K^T and O += P V as m16n8k16 products, the kv
+// head's query heads as the 16 rows, each warp with its own m, l, o until the segment's
+// end. The consumers never wait for one another within a segment. The matrix pipes are
+// mostly idle: at 16 rows the tile's bytes, not its products, set the time.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "pages.h"
+#include "pages_mma.cuh"
+#include "tc_common.cuh"
+
+namespace aero {
+namespace {
+
+constexpr int kUnit = 64;          // positions per unit
+constexpr int kConsumers = 4;      // warps; each takes 16 positions of a unit
+constexpr int kThreads = 32 * (kConsumers + 1);
+constexpr int kMinUnits = 2;       // a CTA takes at least this many, so that few partials are joined
+constexpr int kHalf = kUnit * 128; // bytes of a unit's 64-column half
+
+template <int D>
+struct Cfg {
+    // two CTAs of an SM hide one another's segment ends; wide heads fill it alone
+    static constexpr int ctas = D <= 128 ? 2 : 1;
+    static constexpr int stages = D == 64 ? 6 : D == 128 ? 3 : D == 192 ? 4 : 3;
+    static constexpr int stage_bytes = 2 * (D / 64) * kHalf;
+    static constexpr int red_bytes = 2 * 16 * D * 4;
+    static constexpr int smem = stages * stage_bytes + red_bytes + 1024;
+};
+
+// The units of one token's kv head: tiles of 64 positions that hold a visible one,
+// first those of the first tokens (sinks), then the window's.
+struct Span {
+    int seq;
+    int n;      // positions that the token may see: its own and those before it
+    int lo;     // first position of the window
+    int sinks;  // positions visible before it
+    int first;  // tiles of the sinks in front of the window's
+    int tile0;  // the window's first tile
+    int tiles;  // at least 1: an empty sequence has a unit that writes zeros
+};
+
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int e) {
+    Span p;
+    token_rows(a, e, p.seq, p.n);
+    if (p.seq < 0 || p.seq >= a.c.n_seq) pages_flag(a.c, AERO_CUDA_PAGES_BAD_SEQ);
+    p.lo = a.window && p.n > a.window ? p.n - a.window : 0;
+    p.sinks = min(a.sinks, p.lo);
+    p.tile0 = p.lo / kUnit;
+    p.first = min((p.sinks + kUnit - 1) / kUnit, p.tile0);
+    p.tiles = p.n > 0 ? p.first + (p.n - 1) / kUnit + 1 - p.tile0 : 1;
+    return p;
+}
+__device__ __forceinline__ int tile_at(const Span& p, int t) { return t < p.first ? t : p.tile0 + t - p.first; }
+__device__ __forceinline__ bool visible(const Span& p, int j) { return j < p.n && (j >= p.lo || j < p.sinks); }
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
+    decode_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
+                         const __grid_constant__ CUtensorMap vmap) {
+    constexpr int ST = Cfg<D>::stages;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    float* red = reinterpret_cast<float*>(sm + ST * Cfg<D>::stage_bytes);        // [2][16][D], columns swizzled by row
+    float2* ml = reinterpret_cast<float2*>(sm + ST * Cfg<D>::stage_bytes + Cfg<D>::red_bytes);  // [4][16] (m, l)
+    float2* joint = ml + 64;                                                     // [16]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(joint + 16);                    // full[ST], empty[ST]
+    int64_t* begin_s = reinterpret_cast<int64_t*>(bars + 2 * ST);                // entry base, total
+    int* misc = reinterpret_cast<int*>(begin_s + 2);                             // entry, abort, last, warp sums
+    volatile int* abort_flag = misc + 1;
+    const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int HK = a.c.HK, G = a.H / HK;
+    const uint32_t ring = smem_u32(sm);
+
+    // ---- this CTA's piece of the line of units
+    {
+        int64_t* sums = reinterpret_cast<int64_t*>(red);  // [kThreads / 32]
+        const int per = (a.T + kThreads - 1) / kThreads;
+        const int e0 = min(a.T, tid * per), e1 = min(a.T, e0 + per);
+        int64_t mine = 0;
+        for (int e = e0; e < e1; ++e) mine += span_of(a, e).tiles;
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) sums[warp] = incl;
+        if (tid == 0) {
+            for (int i = 0; i < ST; ++i) {
+                mbar_init(smem_u32(bars + i), 1);
+                mbar_init(smem_u32(bars + ST + i), kConsumers);
+            }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            *abort_flag = 0;
+        }
+        __syncthreads();
+        int64_t before = incl - mine, total = 0;
+        for (int i = 0; i < kThreads / 32; ++i) {
+            if (i < warp) before += sums[i];
+            total += sums[i];
+        }
+        total *= HK;
+        const int64_t w = max((int64_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
+        const int64_t u0 = w * blockIdx.x;
+        if (u0 >= before * HK && u0 < (before + mine) * HK) {
+            int64_t base = before * HK;
+            int e = e0;
+            for (;; ++e) {
+                const int64_t next = base + (int64_t)span_of(a, e).tiles * HK;
+                if (u0 < next) break;
+                base = next;
+            }
+            begin_s[0] = base;
+            misc[0] = e;
+        }
+        if (tid == 0) begin_s[1] = total;
+        __syncthreads();
+    }
+    const int64_t total = begin_s[1];
+    const int64_t w = max((int64_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
+    const int64_t u0 = w * blockIdx.x, u1 = min(total, u0 + w);
+    if (u0 >= u1) return;
+
+    int e = misc[0];
+    int64_t base = begin_s[0];
+    Span sp = span_of(a, e);
+    int stage = 0;
+    uint32_t phase = 0;
+
+    if (warp == kConsumers) {
+        // ---------------------------------------------------------- producer
+        const int P = 1 << a.c.page_shift, rows = min(P, kUnit), boxes = kUnit / rows;
+        int64_t loaded = 0;
+        bool good = true;
+        for (int64_t u = u0; u < u1 && good;) {
+            const int64_t in = u - base;
+            const int h = (int)(in / sp.tiles), t0 = (int)(in % sp.tiles);
+            const int cnt = (int)min((int64_t)(sp.tiles - t0), u1 - u);
+            const int s = sp.seq;
+            for (int t = t0; t < t0 + cnt; ++t) {
+                // lane i brings box i, if a position in it is visible
+                const int j0 = tile_at(sp, t) * kUnit + lane * rows;
+                bool want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
+                int page = 0;
+                if (want) {
+                    page = a.c.table[(int64_t)s * a.c.max_pages + (j0 >> a.c.page_shift)];
+                    if ((uint32_t)page >= (uint32_t)a.c.n_page) {
+                        pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
+                        want = false;
+                    }
+                }
+                if (!mbar_wait(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
+                    good = false;
+                    break;
+                }
+                const uint32_t full = smem_u32(bars + stage);
+                const int n_box = __popc(__ballot_sync(0xffffffffu, want));
+                if (lane == 0) {
+                    if (n_box)
+                        mbar_expect_tx(full, (uint32_t)(n_box * rows * D * 2 * 2));
+                    else
+                        mbar_arrive(full);
+                }
+                __syncwarp();
+                if (want) {
+                    const int64_t row0 = (((int64_t)a.layer * a.c.n_page + page) * HK + h) << a.c.page_shift;
+                    const int row = (int)row0 + (j0 & (P - 1));  // < 2^31: checked when the cache was opened
+                    const uint32_t dst = ring + (uint32_t)stage * Cfg<D>::stage_bytes + (uint32_t)(lane * rows * 128);
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) tma_load_2d(dst + c * kHalf, &kmap, c * 64, row, full);
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) tma_load_2d(dst + (D / 64 + c) * kHalf, &vmap, c * 64, row, full);
+                }
+                __syncwarp();
+                ++loaded;
+                if (++stage == ST) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            }
+            u += cnt;
+            if (u == base + (int64_t)sp.tiles * HK && u < u1) {
+                base = u;
+                sp = span_of(a, ++e);
+            }
+        }
+        if (!good) {
+            *abort_flag = 1;
+            if (lane == 0) pages_flag(a.c, AERO_CUDA_PAGES_WAIT);
+            // copies in flight land before the CTA's memory is given up
+            for (int i = 0; i < ST && i < loaded; ++i) {
+                const int64_t k = loaded - 1 - i;
+                mbar_wait_timed(smem_u32(bars + (int)(k % ST)), (uint32_t)((k / ST) & 1));
+            }
+        }
+        return;
+    }
+
+    // -------------------------------------------------------------- consumers
+    const int g = lane >> 2, tq = lane & 3;
+    bool dead = false;
+    // this lane's rows of the K fragments (keys (lane / 16) * 8 + lane % 8, 8 columns by bit 3)
+    // and of the V fragments (keys (bit 3) * 8 + lane % 8, 8 columns by lane / 16)
+    const int krow = warp * 16 + (lane >> 4) * 8 + (lane & 7), kcol = (lane >> 3) & 1;
+    const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), vcol = lane >> 4;
+    for (int64_t u = u0; u < u1;) {
+        const int64_t in = u - base;
+        const int h = (int)(in / sp.tiles), t0 = (int)(in % sp.tiles);
+        const int cnt = (int)min((int64_t)(sp.tiles - t0), u1 - u);
+        // the query heads as the products' rows g and g + 8; rows past G are zero
+        uint32_t qf[D / 16][4];
+        {
+            const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)e * a.q_token + (int64_t)(h * G) * a.q_head;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = g + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + 2 * tq;
+                    const uint16_t* x = q + (int64_t)r * a.q_head + col;
+                    qf[ks][i] = r >= G ? 0u
+                                : a.vec ? *reinterpret_cast<const uint32_t*>(x)
+                                        : (uint32_t)x[0] | ((uint32_t)x[1] << 16);
+                }
+        }
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        for (int t = t0; t < t0 + cnt; ++t) {
+            // a warp whose wait gave up goes on without waiting (its results are void, the status
+            // says so): the other warps still meet it at the barriers below
+            if (!dead && !mbar_wait(smem_u32(bars + stage), phase, abort_flag)) {
+                dead = true;
+                *abort_flag = 1;
+                if (lane == 0) pages_flag(a.c, AERO_CUDA_PAGES_WAIT);
+            }
+            const uint32_t kb = ring + (uint32_t)stage * Cfg<D>::stage_bytes, vb = kb + (D / 64) * kHalf;
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                uint32_t b[4];
+                const int c16 = (ks & 3) * 2 + kcol;
+                ldsm4<false>(b, kb + (ks >> 2) * kHalf + krow * 128 + ((c16 ^ (krow & 7)) << 4));
+                mma16<BF16>(s[0], qf[ks], b[0], b[1]);
+                mma16<BF16>(s[1], qf[ks], b[2], b[3]);
+            }
+            // positions that the token does not see: their scores are -inf and their V rows
+            // are taken as zero, whatever their memory holds
+            const int j = tile_at(sp, t) * kUnit + warp * 16 + 2 * tq;
+            const bool s00 = visible(sp, j), s01 = visible(sp, j + 1), s10 = visible(sp, j + 8), s11 = visible(sp, j + 9);
+            const uint32_t keep0 = (s00 ? 0x0000FFFFu : 0u) | (s01 ? 0xFFFF0000u : 0u);
+            const uint32_t keep1 = (s10 ? 0x0000FFFFu : 0u) | (s11 ? 0xFFFF0000u : 0u);
+            const float sc = a.scale_log2;
+            s[0][0] = s00 ? s[0][0] * sc : -INFINITY;
+            s[0][1] = s01 ? s[0][1] * sc : -INFINITY;
+            s[0][2] = s00 ? s[0][2] * sc : -INFINITY;
+            s[0][3] = s01 ? s[0][3] * sc : -INFINITY;
+            s[1][0] = s10 ? s[1][0] * sc : -INFINITY;
+            s[1][1] = s11 ? s[1][1] * sc : -INFINITY;
+            s[1][2] = s10 ? s[1][2] * sc : -INFINITY;
+            s[1][3] = s11 ? s[1][3] * sc : -INFINITY;
+            float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+            float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+                // (a row without a visible position stays at -inf; its sums are zero)
+                const float f0 = n0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 0.f : ex2(m1 - n1);
+                m0 = n0;
+                m1 = n1;
+                l0 *= f0;
+                l1 *= f1;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    o[i][0] *= f0;
+                    o[i][1] *= f0;
+                    o[i][2] *= f1;
+                    o[i][3] *= f1;
+                }
+            }
+            const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+            float p[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                p[i][0] = ex2(s[i][0] - z0);
+                p[i][1] = ex2(s[i][1] - z0);
+                p[i][2] = ex2(s[i][2] - z1);
+                p[i][3] = ex2(s[i][3] - z1);
+                l0 += p[i][0] + p[i][1];
+                l1 += p[i][2] + p[i][3];
+            }
+            // P in the cache's type: a relative rounding of 2^-11 (f16) or 2^-8 (bf16) / 2 per
+            // weight, below the output's own; the sums l stay f32
+            const uint32_t pa[4] = {pack16<BF16>(p[0][0], p[0][1]), pack16<BF16>(p[0][2], p[0][3]),
+                                    pack16<BF16>(p[1][0], p[1][1]), pack16<BF16>(p[1][2], p[1][3])};
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                uint32_t b[4];
+                const int c16 = (i & 3) * 2 + vcol;
+                ldsm4<true>(b, vb + (i >> 2) * kHalf + vrow * 128 + ((c16 ^ (vrow & 7)) << 4));
+                mma16<BF16>(o[2 * i], pa, b[0] & keep0, b[1] & keep1);
+                mma16<BF16>(o[2 * i + 1], pa, b[2] & keep0, b[3] & keep1);
+            }
+            __syncwarp();
+            if (lane == 0 && !dead) mbar_arrive(smem_u32(bars + ST + stage));
+            if (++stage == ST) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        // ---- the four warps' results into one: o[row][d] = red[0] + red[1], (m, l) in joint
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        if (tq == 0) {
+            ml[warp * 16 + g] = make_float2(m0, l0);
+            ml[warp * 16 + g + 8] = make_float2(m1, l1);
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        {
+            float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < kConsumers; ++i) {
+                M0 = fmaxf(M0, ml[i * 16 + g].x);
+                M1 = fmaxf(M1, ml[i * 16 + g + 8].x);
+            }
+#pragma unroll
+            for (int i = 0; i < kConsumers; ++i) {
+                const float2 v0 = ml[i * 16 + g], v1 = ml[i * 16 + g + 8];
+                L0 += v0.x == -INFINITY ? 0.f : v0.y * ex2(v0.x - M0);
+                L1 += v1.x == -INFINITY ? 0.f : v1.y * ex2(v1.x - M1);
+            }
+            const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M1);
+            if (warp == 0 && tq == 0) {
+                joint[g] = make_float2(M0, L0);
+                joint[g + 8] = make_float2(M1, L1);
+            }
+            float* r = red + (warp & 1) * 16 * D;
+            const int sw = (g & 3) * 8;  // columns of row g and g + 8 exchanged in blocks of 8: no bank twice
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                o[i][0] *= f0;
+                o[i][1] *= f0;
+                o[i][2] *= f1;
+                o[i][3] *= f1;
+                if (warp >= 2) {
+                    const int col = (8 * i + 2 * tq) ^ sw;
+                    *reinterpret_cast<float2*>(r + g * D + col) = make_float2(o[i][0], o[i][1]);
+                    *reinterpret_cast<float2*>(r + (g + 8) * D + col) = make_float2(o[i][2], o[i][3]);
+                }
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (warp < 2) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const int col = (8 * i + 2 * tq) ^ sw;
+                    float2* a0 = reinterpret_cast<float2*>(r + g * D + col);
+                    float2* a1 = reinterpret_cast<float2*>(r + (g + 8) * D + col);
+                    const float2 v0 = *a0, v1 = *a1;
+                    *a0 = make_float2(o[i][0] + v0.x, o[i][1] + v0.y);
+                    *a1 = make_float2(o[i][2] + v1.x, o[i][3] + v1.y);
+                }
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+        const int64_t seg0 = base + (int64_t)h * sp.tiles;  // the (sequence, head)'s units: [seg0, seg0 + tiles)
+        uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)e * a.o_token + (int64_t)(h * G) * a.o_head;
+        const auto put = [&](int row, int d, float4 v) {
+            uint16_t* y = out + (int64_t)row * a.o_head + d;
+            const uint32_t w0 = pack16<BF16>(v.x, v.y), w1 = pack16<BF16>(v.z, v.w);
+            if (a.vec) {
+                *reinterpret_cast<uint2*>(y) = make_uint2(w0, w1);
+            } else {
+                y[0] = (uint16_t)w0;
+                y[1] = (uint16_t)(w0 >> 16);
+                y[2] = (uint16_t)w1;
+                y[3] = (uint16_t)(w1 >> 16);
+            }
+        };
+        const auto summed = [&](int row, int d) {
+            const int col = d ^ ((row & 3) * 8);
+            const float4 x = *reinterpret_cast<const float4*>(red + row * D + col),
+                         y = *reinterpret_cast<const float4*>(red + (16 + row) * D + col);
+            return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        };
+        if (cnt == sp.tiles) {
+            for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
+                const int row = i / (D / 4), d = i % (D / 4) * 4;
+                const float inv = joint[row].y > 0.f ? 1.f / joint[row].y : 0.f;
+                const float4 v = summed(row, d);
+                // a sum that is not a number stays one
+                const float k = joint[row].y == joint[row].y ? inv : joint[row].y;
+                put(row, d, make_float4(v.x * k, v.y * k, v.z * k, v.w * k));
+            }
+        } else {
+            // partial results: slot 1 of the CTA where the (sequence, head) begins, slot 0 of the others
+            constexpr int64_t slot = 16 * (D + 2);
+            float* mine = a.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * slot;
+            for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
+                const int row = i / (D / 4), d = i % (D / 4) * 4;
+                *reinterpret_cast<float4*>(mine + row * D + d) = summed(row, d);
+            }
+            if (tid < G) *reinterpret_cast<float2*>(mine + 16 * D + 2 * tid) = joint[tid];
+            __threadfence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const int64_t c0 = seg0 / w, c1 = (seg0 + sp.tiles - 1) / w;
+            if (tid == 0) {
+                const uint32_t was = atomicAdd(a.counters + c0, 1u);
+                misc[2] = was == (uint32_t)(c1 - c0);
+                if (misc[2]) a.counters[c0] = 0;  // for the next launch
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (misc[2]) {
+                __threadfence();
+                for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
+                    const int row = i / (D / 4), d = i % (D / 4) * 4;
+                    float M = -INFINITY, L = 0.f;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int64_t c = c0; c <= c1; ++c) {
+                        const float* p = a.part + (c * 2 + (c == c0)) * slot;
+                        const float2 x = __ldcg(reinterpret_cast<const float2*>(p + 16 * D + 2 * row));
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
+                        const float N = fmaxf(M, x.x);
+                        const float f = N == -INFINITY ? 0.f : ex2(M - N), k = N == -INFINITY ? 0.f : ex2(x.x - N);
+                        M = N;
+                        L = L * f + x.y * k;
+                        acc.x = acc.x * f + v.x * k;
+                        acc.y = acc.y * f + v.y * k;
+                        acc.z = acc.z * f + v.z * k;
+                        acc.w = acc.w * f + v.w * k;
+                    }
+                    const float k = L > 0.f ? 1.f / L : L == L ? 0.f : L;
+                    put(row, d, make_float4(acc.x * k, acc.y * k, acc.z * k, acc.w * k));
+                }
+            }
+        }
+        u += cnt;
+        if (u == base + (int64_t)sp.tiles * HK && u < u1) {
+            base = u;
+            sp = span_of(a, ++e);
+        }
+    }
+}
+
+template <int D, bool BF16>
+cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int n_sm, cudaStream_t s) {
+    static thread_local int prepared = -1;  // the device whose attribute this thread has set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (prepared != dev) {
+        e = cudaFuncSetAttribute(decode_attend_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem);
+        if (e != cudaSuccess) return e;
+        prepared = dev;
+    }
+    // no more CTAs than units the tables can hold
+    const int64_t cap = ((int64_t)a.c.max_pages << a.c.page_shift) / kUnit + 2;
+    const int64_t units = (int64_t)a.T * a.c.HK * cap;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((int64_t)n_sm * Cfg<D>::ctas, (units + kMinUnits - 1) / kMinUnits));
+    decode_attend_kernel<D, BF16><<<grid, kThreads, Cfg<D>::smem, s>>>(a, kmap, vmap);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+int pages_decode_max_grid(int n_sm) { return 2 * n_sm; }
+size_t pages_decode_part_floats(int D, int n_sm) { return (size_t)pages_decode_max_grid(n_sm) * 2 * 16 * (size_t)(D + 2); }
+
+cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                                int n_sm, cudaStream_t s) {
+    switch (a.c.D) {
+        case 64: return bf16 ? launch<64, true>(a, kmap, vmap, n_sm, s) : launch<64, false>(a, kmap, vmap, n_sm, s);
+        case 128: return bf16 ? launch<128, true>(a, kmap, vmap, n_sm, s) : launch<128, false>(a, kmap, vmap, n_sm, s);
+        case 192: return bf16 ? launch<192, true>(a, kmap, vmap, n_sm, s) : launch<192, false>(a, kmap, vmap, n_sm, s);
+        case 256: return bf16 ? launch<256, true>(a, kmap, vmap, n_sm, s) : launch<256, false>(a, kmap, vmap, n_sm, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace aero

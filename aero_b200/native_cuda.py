@@ -26,6 +26,11 @@ DTYPE_F16 = 1
 DTYPE_Q8_0 = 8
 DTYPE_Q4_K = 12
 
+# element types of the paged cache and of logits (include/aero_cuda_pages.h)
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 30
+
 # memory classes (src/memory_guard.cpp MemClass order)
 MEM_WEIGHTS_RESIDENT, MEM_WEIGHTS_CACHE, MEM_KV_CACHE, MEM_SCRATCH, MEM_RUNTIME = range(5)
 
@@ -70,6 +75,13 @@ class DecoderDesc(Structure):
                 ("token_embd", Tensor), ("output", Tensor), ("output_norm", c_void_p), ("layers", POINTER(DecoderLayer))]
 
 
+class PagesDesc(Structure):
+    """aero_cuda_pages_desc (include/aero_cuda_pages.h)."""
+    _fields_ = [("n_layer", c_int32), ("n_page", c_int32), ("page_size", c_int32), ("n_head_kv", c_int32),
+                ("head_dim", c_int32), ("n_seq", c_int32), ("max_pages", c_int32), ("dtype", c_int32),
+                ("device", c_int32), ("reserved", c_int32)]
+
+
 EVICT_FN = CFUNCTYPE(c_size_t, c_void_p, c_size_t)
 BREACH_FN = CFUNCTYPE(None, c_void_p, c_size_t, c_size_t)
 
@@ -101,6 +113,24 @@ SYMBOLS = [
     ("aero_cuda_decoder_info", c_int, [_P, _P]),
     ("aero_cuda_decoder_last_error", c_char_p, [_P]),
     ("aero_cuda_decoder_close", None, [_P]),
+    ("aero_cuda_pages_open", c_void_p, [POINTER(PagesDesc), c_char_p, c_int]),
+    ("aero_cuda_pages_plan_bytes", c_int64, [POINTER(PagesDesc), _P]),
+    ("aero_cuda_pages_close", None, [_P]),
+    ("aero_cuda_pages_set_stream", c_int, [_P, _P]),
+    ("aero_cuda_pages_buffers", c_int, [_P, _P, _P, _P, _P, _P]),
+    ("aero_cuda_pages_status", c_int, [_P]),
+    ("aero_cuda_pages_last_error", c_char_p, [_P]),
+    ("aero_cuda_pages_set_tables", c_int, [_P, _P, _P, _P]),
+    ("aero_cuda_pages_extend", c_int, [_P, _P, _P, c_int]),
+    ("aero_cuda_pages_append", c_int, [_P, c_int, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, _P, c_int]),
+    ("aero_cuda_pages_fork", c_int, [_P, _P, _P, c_int]),
+    ("aero_cuda_pages_free", c_int, [_P, _P, c_int]),
+    ("aero_cuda_pages_copy", c_int, [_P, _P, _P, c_int]),
+    ("aero_cuda_pages_compact", c_int, [_P]),
+    ("aero_cuda_pages_attend", c_int, [_P, c_int, _P, c_int64, c_int64, c_int, c_int, _P, _P, c_int, c_float, c_int,
+                                       c_int, _P, c_int64, c_int64]),
+    ("aero_cuda_logits_adjust", c_int, [_P, c_int64, c_int, c_int, c_int, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P,
+                                        _P, c_int64, _P, c_int64, _P]),
     ("aero_cuda_moe_forward", c_int, [_P, c_int, _P, c_int, c_int, _P]),
     ("aero_cuda_moe_submit", c_int, [_P, c_int, _P, c_int, _P]),
     ("aero_cuda_moe_wait", c_int, [_P, c_int]),
