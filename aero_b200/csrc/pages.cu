@@ -432,8 +432,8 @@ struct Pages {
     BooksWork work{};
     void *k = nullptr, *v = nullptr, *books = nullptr;
     size_t pool_bytes = 0, books_bytes = 0;  // pool_bytes: K or V alone
-    float* decode_part = nullptr;
-    uint32_t* decode_count = nullptr;
+    float *decode_part = nullptr, *prompt_part = nullptr;
+    uint32_t *decode_count = nullptr, *prompt_count = nullptr;
     CUtensorMap kmap{}, vmap{};
     std::string err;
 
@@ -503,7 +503,7 @@ const char* bad_desc(const aero_cuda_pages_desc& d) {
 struct Layout {
     size_t pool, books;                                                        // bytes of K (or V); of the books block
     size_t table, length, refs, status, list, to, mark, first, len, jobs, counts;  // offsets in the books block
-    size_t dpart, dcount;
+    size_t dpart, dcount, ppart, pcount;
 };
 
 Layout layout(const aero_cuda_pages_desc& d, int n_sm) {
@@ -528,6 +528,8 @@ Layout layout(const aero_cuda_pages_desc& d, int n_sm) {
     l.counts = take(8);
     l.dpart = take(pages_decode_part_floats(d.head_dim, n_sm) * 4);
     l.dcount = take((size_t)pages_decode_max_grid(n_sm) * 4);
+    l.ppart = take(pages_prompt_part_floats(d.head_dim, n_sm) * 4);
+    l.pcount = take((size_t)pages_prompt_max_grid(n_sm) * 4);
     l.books = at;
     return l;
 }
@@ -587,6 +589,8 @@ Pages* open_pages(const aero_cuda_pages_desc* desc, std::string* why) {
     w.n_live = w.n_jobs + 1;
     g->decode_part = reinterpret_cast<float*>(b + l.dpart);
     g->decode_count = reinterpret_cast<uint32_t*>(b + l.dcount);
+    g->prompt_part = reinterpret_cast<float*>(b + l.ppart);
+    g->prompt_count = reinterpret_cast<uint32_t*>(b + l.pcount);
     if (cudaMemsetAsync(g->k, 0, l.pool, g->stream) != cudaSuccess ||
         cudaMemsetAsync(g->v, 0, l.pool, g->stream) != cudaSuccess ||
         cudaMemsetAsync(g->books, 0, l.books, g->stream) != cudaSuccess ||
@@ -848,6 +852,11 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
         a.scale_log2 = scale * 1.4426950408889634f;
         a.vec = aero::vec16(q, q_token, q_head) && aero::vec16(out, o_token, o_head);
         const bool bf16 = g.d.dtype == AERO_CUDA_TYPE_BF16;
+        if (q_start) {
+            a.part = g.prompt_part;
+            a.counters = g.prompt_count;
+            return g.ok(aero::launch_pages_prompt(a, bf16, g.kmap, g.vmap, g.k, g.v, g.n_sm, g.stream), "attend");
+        }
         a.part = g.decode_part;
         a.counters = g.decode_count;
         return g.ok(aero::launch_pages_decode(a, bf16, g.kmap, g.vmap, g.n_sm, g.stream), "attend");

@@ -1,6 +1,6 @@
 // The paged key/value cache (include/aero_cuda_pages.h): what its translation
 // units share. pages.cu owns the handle and the books, pages_decode.cu the
-// attention.
+// attention of single tokens, pages_prompt.cu that of several tokens a sequence.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -75,12 +75,17 @@ __device__ __forceinline__ void token_rows(const AttendArgs& a, int t, int& seq,
 }
 #endif
 
-// Workspace the kernel needs for a cache of this shape.
+// Workspace the two kernels need for a cache of this shape.
 size_t pages_decode_part_floats(int D, int n_sm);
+size_t pages_prompt_part_floats(int D, int n_sm);
 int pages_decode_max_grid(int n_sm);
+int pages_prompt_max_grid(int n_sm);
 // kmap / vmap: (n_layer * n_page * HK * page rows, D) with boxes of min(page, 64)
 // rows by 64 columns, 128-byte swizzle.
 cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                 int n_sm, cudaStream_t s);
+// k, v: the pool itself.
+cudaError_t launch_pages_prompt(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                                const void* k, const void* v, int n_sm, cudaStream_t s);
 
 }  // namespace aero
