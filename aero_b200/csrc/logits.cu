@@ -18,6 +18,7 @@
 
 #include "../../include/aero_cuda_pages.h"
 #include "internal.h"
+#include "pages.h"
 
 namespace aero {
 namespace {
@@ -168,7 +169,12 @@ extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype
         if (rows == 0) return 0;
         if (ld < vocab || ld_out < vocab) return refuse("ld and ld_out must be at least vocab"), -1;
         const uintptr_t size = dtype == AERO_CUDA_TYPE_F32 ? 4 : 2;
-        if (!is_device_ptr(logits) || !is_device_ptr(out)) return refuse("logits and out must be device memory"), -1;
+        cudaPointerAttributes where{};
+        if (cudaPointerGetAttributes(&where, logits) != cudaSuccess) {
+            cudaGetLastError();
+            where.type = cudaMemoryTypeUnregistered;
+        }
+        if ((where.type != cudaMemoryTypeDevice && where.type != cudaMemoryTypeManaged) || !is_device_ptr(out)) return refuse("logits and out must be device memory"), -1;
         if (((uintptr_t)logits | (uintptr_t)out) % size) return refuse("logits and out must be aligned to their type"), -1;
         if (history && !n_history) return refuse("a history needs n_history"), -1;
         if (bias_start && (!bias_token || !bias_value)) return refuse("bias_start needs bias_token and bias_value"), -1;
@@ -176,6 +182,8 @@ extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype
         const void* arrays[] = {history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask};
         for (const void* p : arrays)
             if (!device_or_null(p)) return refuse("histories, penalties, biases and masks must be device memory, aligned to 4 bytes"), -1;
+        OnDevice on(where.device);
+        if (!on.good) return refuse("cudaSetDevice failed"), -1;
         LogitArgs a{logits, out, ld, ld_out, vocab, 0, history, ld_history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask};
         a.slice = 8192;
         const size_t smem = (size_t)a.slice * (bias_start ? 8 : 4);

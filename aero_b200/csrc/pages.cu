@@ -461,21 +461,6 @@ struct Pages {
     }
 };
 
-// The caller's current device, put back on the way out.
-struct OnDevice {
-    int was = -1;
-    bool good;
-    explicit OnDevice(int device) {
-        if (cudaGetDevice(&was) != cudaSuccess) was = -1;
-        good = was == device || cudaSetDevice(device) == cudaSuccess;
-        if (!good) cudaGetLastError();
-        if (was == device) was = -1;
-    }
-    ~OnDevice() {
-        if (was >= 0) cudaSetDevice(was);
-    }
-};
-
 int log2_exact(int v) {
     int s = 0;
     while ((1 << s) < v) ++s;

@@ -10,6 +10,21 @@
 
 namespace aero {
 
+// The caller's current device, put back on the way out.
+struct OnDevice {
+    int was = -1;
+    bool good;
+    explicit OnDevice(int device) {
+        if (cudaGetDevice(&was) != cudaSuccess) was = -1;
+        good = was == device || cudaSetDevice(device) == cudaSuccess;
+        if (!good) cudaGetLastError();
+        if (was == device) was = -1;
+    }
+    ~OnDevice() {
+        if (was >= 0) cudaSetDevice(was);
+    }
+};
+
 // The cache as kernels see it.
 struct PageView {
     int32_t* table;   // (n_seq, max_pages)

@@ -35,7 +35,7 @@ namespace {
 constexpr int kUnit = 64;          // positions per unit
 constexpr int kConsumers = 4;      // warps; each takes 16 positions of a unit
 constexpr int kThreads = 32 * (kConsumers + 1);
-constexpr int kMinUnits = 2;       // a CTA takes at least this many, so that few partials are joined
+constexpr int kMinUnits = 4;       // a CTA takes at least this many, so that few partials are joined
 constexpr int kHalf = kUnit * 128; // bytes of a unit's 64-column half
 
 template <int D>
@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     float2* joint = ml + 64;                                                     // [16]
     uint64_t* bars = reinterpret_cast<uint64_t*>(joint + 16);                    // full[ST], empty[ST]
     int64_t* begin_s = reinterpret_cast<int64_t*>(bars + 2 * ST);                // entry base, total
-    int* misc = reinterpret_cast<int*>(begin_s + 2);                             // entry, abort, last, warp sums
+    int* misc = reinterpret_cast<int*>(begin_s + 2);                             // entry, abort, last
+    Span* span_s = reinterpret_cast<Span*>(misc + 4);                            // the first entry's
     volatile int* abort_flag = misc + 1;
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int HK = a.c.HK, G = a.H / HK;
@@ -125,13 +126,16 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         if (u0 >= before * HK && u0 < (before + mine) * HK) {
             int64_t base = before * HK;
             int e = e0;
+            Span at;
             for (;; ++e) {
-                const int64_t next = base + (int64_t)span_of(a, e).tiles * HK;
+                at = span_of(a, e);
+                const int64_t next = base + (int64_t)at.tiles * HK;
                 if (u0 < next) break;
                 base = next;
             }
             begin_s[0] = base;
             misc[0] = e;
+            *span_s = at;
         }
         if (tid == 0) begin_s[1] = total;
         __syncthreads();
@@ -143,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
 
     int e = misc[0];
     int64_t base = begin_s[0];
-    Span sp = span_of(a, e);
+    Span sp = *span_s;
     int stage = 0;
     uint32_t phase = 0;
 
@@ -255,15 +259,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 if (lane == 0) pages_flag(a.c, AERO_CUDA_PAGES_WAIT);
             }
             const uint32_t kb = ring + (uint32_t)stage * Cfg<D>::stage_bytes, vb = kb + (D / 64) * kHalf;
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            // (two sums each, of the even and the odd steps: a shorter chain of products)
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, so[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
                 uint32_t b[4];
                 const int c16 = (ks & 3) * 2 + kcol;
                 ldsm4<false>(b, kb + (ks >> 2) * kHalf + krow * 128 + ((c16 ^ (krow & 7)) << 4));
-                mma16<BF16>(s[0], qf[ks], b[0], b[1]);
-                mma16<BF16>(s[1], qf[ks], b[2], b[3]);
+                mma16<BF16>(ks & 1 ? so[0] : s[0], qf[ks], b[0], b[1]);
+                mma16<BF16>(ks & 1 ? so[1] : s[1], qf[ks], b[2], b[3]);
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] += so[i >> 2][i & 3];
             // positions that the token does not see: their scores are -inf and their V rows
             // are taken as zero, whatever their memory holds
             const int j = tile_at(sp, t) * kUnit + warp * 16 + 2 * tq;
@@ -425,34 +432,57 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 *reinterpret_cast<float4*>(mine + row * D + d) = summed(row, d);
             }
             if (tid < G) *reinterpret_cast<float2*>(mine + 16 * D + 2 * tid) = joint[tid];
-            __threadfence();
             asm volatile("bar.sync 1, 128;" ::: "memory");
-            const int64_t c0 = seg0 / w, c1 = (seg0 + sp.tiles - 1) / w;
+            const int64_t c0 = seg0 / w;
+            const int parts = (int)((seg0 + sp.tiles - 1) / w - c0) + 1;
             if (tid == 0) {
+                __threadfence();  // the CTA's stores, ordered before by the barrier
                 const uint32_t was = atomicAdd(a.counters + c0, 1u);
-                misc[2] = was == (uint32_t)(c1 - c0);
+                misc[2] = was == (uint32_t)(parts - 1);
                 if (misc[2]) a.counters[c0] = 0;  // for the next launch
+                __threadfence();
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
             if (misc[2]) {
-                __threadfence();
+                // part c of the line: the first one's slot is 1, the others' 0
+                const float* first = a.part + (c0 * 2 + 1) * slot;
+                const float* rest = a.part + (c0 * 2) * slot;
+                const auto part_at = [&](int c) { return c == 0 ? first : rest + (int64_t)c * 2 * slot; };
+                // four columns of a row a thread; the loads of kBatch parts are in flight at once
+                // (an L2 round trip each batch is what this costs)
+                constexpr int kBatch = 16;
                 for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
                     const int row = i / (D / 4), d = i % (D / 4) * 4;
                     float M = -INFINITY, L = 0.f;
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int64_t c = c0; c <= c1; ++c) {
-                        const float* p = a.part + (c * 2 + (c == c0)) * slot;
-                        const float2 x = __ldcg(reinterpret_cast<const float2*>(p + 16 * D + 2 * row));
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
-                        const float N = fmaxf(M, x.x);
-                        const float f = N == -INFINITY ? 0.f : ex2(M - N), k = N == -INFINITY ? 0.f : ex2(x.x - N);
+                    for (int b0 = 0; b0 < parts; b0 += kBatch) {
+                        float2 x[kBatch];
+                        float4 v[kBatch];
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) {
+                            const float* p = part_at(min(b0 + k, parts - 1));
+                            x[k] = __ldcg(reinterpret_cast<const float2*>(p + 16 * D + 2 * row));
+                            v[k] = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
+                        }
+                        float N = M;
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) {
+                            if (b0 + k >= parts) x[k] = make_float2(-INFINITY, 0.f);
+                            N = fmaxf(N, x[k].x);
+                        }
+                        const float z = N == -INFINITY ? 0.f : N, f = ex2(M - z);
                         M = N;
-                        L = L * f + x.y * k;
-                        acc.x = acc.x * f + v.x * k;
-                        acc.y = acc.y * f + v.y * k;
-                        acc.z = acc.z * f + v.z * k;
-                        acc.w = acc.w * f + v.w * k;
+                        L *= f;
+                        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+                        for (int k = 0; k < kBatch; ++k) {  // (past the last part: its values again, weight 0)
+                            const float y = ex2(x[k].x - z);
+                            L = fmaf(x[k].y, y, L);
+                            acc.x = fmaf(v[k].x, y, acc.x);
+                            acc.y = fmaf(v[k].y, y, acc.y);
+                            acc.z = fmaf(v[k].z, y, acc.z);
+                            acc.w = fmaf(v[k].w, y, acc.w);
+                        }
                     }
                     const float k = L > 0.f ? 1.f / L : L == L ? 0.f : L;
                     put(row, d, make_float4(acc.x * k, acc.y * k, acc.z * k, acc.w * k));

@@ -83,7 +83,10 @@ class PagedCache:
         self.n_head_kv, self.head_dim, self.n_seq, self.max_pages = int(n_head_kv), int(head_dim), int(n_seq), int(max_pages)
         self.dtype, self.device = dtype, torch.device("cuda", int(device))
         self._torch = torch
+        self._index = int(device)
         self._follow, self._stream = True, None
+        self._current_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream builds an object each call
+        self._i32_type, self._scale = torch.int32, 1.0 / math.sqrt(self.head_dim)
         p = [ctypes.c_void_p() for _ in range(5)]
         self._lib.aero_cuda_pages_buffers(h, *(ctypes.byref(x) for x in p))
         self._ptr = [x.value for x in p]
@@ -128,7 +131,9 @@ class PagedCache:
         if self.handle is None:
             raise RuntimeError("the cache is closed")
         if self._follow:
-            self._use(self._torch.cuda.current_stream(self.device).cuda_stream)
+            raw = self._current_stream(self._index)
+            if raw != self._stream:
+                self._use(raw)
 
     def _refused(self, what: str):
         raise ValueError(f"{what} refused: {self.last_error()}")
@@ -148,21 +153,24 @@ class PagedCache:
             raise RuntimeError(f"paged cache: {STATUS.get(code, f'status {code}')}")
 
     # ---- arguments
-    def _i32(self, t, name: str, n: Optional[int] = None):
-        if t.dtype != self._torch.int32 or t.device != self.device or not t.is_contiguous():
+    def _i32(self, t, name: str, n: Optional[int] = None) -> int:
+        if t.dtype is not self._i32_type or t.get_device() != self._index or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor on {self.device}")
         if n is not None and t.numel() != n:
             raise ValueError(f"{name} has {t.numel()} entries, expected {n}")
         return t.data_ptr()
 
     def _rows(self, t, name: str, heads: Optional[int]):
-        if t.dtype != self.dtype or t.device != self.device:
+        """(address, token stride, head stride) of rows (tokens, heads, head_dim)."""
+        if t.dtype is not self.dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must be {self.dtype} on {self.device}, got {t.dtype} on {t.device}")
-        if t.dim() != 3 or t.shape[2] != self.head_dim or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{name} must be (tokens, {heads or 'heads'}, {self.head_dim}), got {tuple(t.shape)}")
-        if t.stride(2) != 1:
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != self.head_dim or (heads is not None and shape[1] != heads):
+            raise ValueError(f"{name} must be (tokens, {heads or 'heads'}, {self.head_dim}), got {tuple(shape)}")
+        token, head, one = t.stride()
+        if one != 1:
             raise ValueError(f"{name} must be contiguous along head_dim")
-        return t.data_ptr(), t.stride(0), t.stride(1)
+        return t.data_ptr(), token, head
 
     # ---- books
     def set_tables(self, table, length, refs) -> None:
@@ -228,17 +236,23 @@ class PagedCache:
         [q_start[i], q_start[i + 1]) are the last positions of seqs[i]. scale: 1 /
         sqrt(head_dim) by default. Returns out (T, n_head, head_dim)."""
         self._on()
-        T, H = q.shape[0], q.shape[1]
+        qp, q_token, q_head = self._rows(q, "q", None)
+        T, H, _ = q.shape
         if out is None:
-            out = self._torch.empty((T, H, self.head_dim), dtype=self.dtype, device=self.device)
-        elif out.shape != q.shape:
-            raise ValueError(f"out has shape {tuple(out.shape)}, expected {tuple(q.shape)}")
+            if q.is_contiguous():
+                out, o_token, o_head = self._torch.empty_like(q), q_token, q_head
+            else:
+                out, o_token, o_head = q.new_empty(q.shape), H * self.head_dim, self.head_dim
+            op = out.data_ptr()
+        else:
+            if out.shape != q.shape:
+                raise ValueError(f"out has shape {tuple(out.shape)}, expected {tuple(q.shape)}")
+            op, o_token, o_head = self._rows(out, "out", H)
         n = seqs.numel()
-        rc = self._lib.aero_cuda_pages_attend(
-            self.handle, layer, *self._rows(q, "q", None), T, H, self._i32(seqs, "seqs"),
-            None if q_start is None else self._i32(q_start, "q_start", n + 1), n,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, window, sinks, *self._rows(out, "out", H))
-        if rc != 0:
+        if self._lib.aero_cuda_pages_attend(
+                self.handle, layer, qp, q_token, q_head, T, H, self._i32(seqs, "seqs"),
+                None if q_start is None else self._i32(q_start, "q_start", n + 1), n,
+                self._scale if scale is None else scale, window, sinks, op, o_token, o_head) != 0:
             self._refused("attend")
         return out
 
