@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                         want = false;
                     }
                 }
-                if (!mbar_wait(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
+                if (!wait_phase(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
                     good = false;
                     break;
                 }
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         for (int t = t0; t < t0 + cnt; ++t) {
             // a warp whose wait gave up goes on without waiting (its results are void, the status
             // says so): the other warps still meet it at the barriers below
-            if (!dead && !mbar_wait(smem_u32(bars + stage), phase, abort_flag)) {
+            if (!dead && !wait_phase(smem_u32(bars + stage), phase, abort_flag)) {
                 dead = true;
                 *abort_flag = 1;
                 if (lane == 0) pages_flag(a.c, AERO_CUDA_PAGES_WAIT);

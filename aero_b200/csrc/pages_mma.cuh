@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "tc_common.cuh"
+
 namespace aero {
 namespace {
 
@@ -45,6 +47,19 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Bounded wait for a phase of an mbarrier without reading a timer between its tries (one read
+// of the global timer costs more than most of these waits last). A try may suspend the
+// thread for a time that the hardware sets; after kWaitTries of them, each some 20 cycles at
+// least (half a second or more), or when another warp has given up, it returns false.
+constexpr int kWaitTries = 1 << 26;
+__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    for (int i = 0; i < kWaitTries; ++i) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 63) == 63 && *abort_flag) return false;
+    }
+    return false;
 }
 
 // 2^x, the hardware's approximation (relative error about 2^-22; 2^-inf = 0).

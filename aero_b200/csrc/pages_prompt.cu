@@ -40,22 +40,32 @@ namespace aero {
 namespace {
 
 constexpr int kTileRows = 128;
+// Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly): the
+// special-function pipe, at 16 a cycle and SM, is what the softmax waits for otherwise.
+#ifndef POLY
+#define POLY 4
+#endif
+constexpr int kPolyEvery = POLY;
 
 template <int D>
 struct PCfg {
     static constexpr int NQ = D <= 128 ? 2 : 1;        // row tiles of a CTA
-    static constexpr int BN = D <= 128 ? 128 : 64;     // positions per tile
     static constexpr int rows = NQ * kTileRows;
+    static constexpr int BN = D <= 128 ? 128 : 64;     // positions per tile
+    // TMEM columns. Two row tiles share one S buffer and have a P each; one row tile has two S
+    // buffers and writes P over S. O last.
+    static constexpr bool shared_s = NQ == 2;
+    static constexpr int SA = shared_s ? 1 : 2;        // tiles that S runs ahead of P V
+    static constexpr int p_col0 = shared_s ? BN : 0;
+    static constexpr int o_col0 = 2 * BN;
+    static constexpr int tmem = 512;
+    static constexpr int PH = D <= 128 ? 2 : 1;        // parts in which a tile's P is handed over
     static constexpr int stages = D == 64 ? 4 : 2;     // of K and of V
     static constexpr int half = BN * 128;              // bytes of a tile's 64-column part
     static constexpr int kv_bytes = (D / 64) * half;
     static constexpr int q_bytes = (D / 64) * kTileRows * 128;  // of one row tile
-    static constexpr int smem = NQ * q_bytes + 2 * stages * kv_bytes + 256;
-    static constexpr int threads = 32 * (4 * NQ + 2);
-    // TMEM columns: two S buffers (of the two row tiles, or of one), then O
-    static constexpr int s_col = BN;
-    static constexpr int o_col0 = 2 * BN;
-    static constexpr int tmem = 512;
+    static constexpr int smem = NQ * q_bytes + 2 * stages * kv_bytes + 512;
+    static constexpr int threads = 32 * (5 * NQ + 2);
 };
 
 // What a CTA works on.
@@ -115,24 +125,33 @@ __device__ __forceinline__ bool find_work(const AttendArgs& a, int slot, Work& w
     return true;
 }
 
-// Row-major K x N operand with N (the head's columns) contiguous, 128-byte swizzle: 8-row
-// groups 1024 bytes apart, 64-column parts `part` bytes apart.
-__device__ __forceinline__ uint64_t sw128_mn_desc(uint32_t saddr, uint32_t part) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(part >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// D (TMEM) += A B, both from shared memory, 16-bit types.
-__device__ __forceinline__ void umma16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// Shared-memory operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart: the low
+// word holds the address (in 16 bytes) and, for an operand whose N (the head's columns) is
+// contiguous, the distance of its 64-column parts; the high word is the same for all.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t part) { return (saddr >> 4) | ((part >> 4) << 16); }
+__device__ __forceinline__ uint64_t desc(uint32_t low) { return (uint64_t)kDescHigh << 32 | low; }
+// D (TMEM) (+)= A B, 16-bit types, A from shared memory or from TMEM.
+template <bool ADD>
+__device__ __forceinline__ void umma16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
             d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc));
+        "l"(adesc), "l"(bdesc), "r"(idesc), "n"(ADD ? 1 : 0));
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+    return one != 0;
 }
 // Instruction descriptor: f32 sums, both operands f16 or both bf16; B with N contiguous if bn.
 template <bool BF16>
 __device__ __forceinline__ uint32_t idesc16(int N, bool bn) {
     return idesc_f16(kTileRows, N) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (bn ? 1u << 16 : 0u);
 }
+
+// The lowest n bits set (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
 // Any of the 8 16-bit values infinite or not a number?
 template <bool BF16>
@@ -148,6 +167,56 @@ __device__ __forceinline__ float to_f32(uint16_t v) {
         return __uint_as_float((uint32_t)v << 16);
     else
         return __half2float(__ushort_as_half(v));
+}
+
+// Pairs of f32 in a 64-bit register, and their packed arithmetic.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// Largest of three; not a number if one is none.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float v;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+    return v;
+}
+
+// 2^x of a pair on the multiply-add pipe: x = n + f with n the nearest integer and |f| <= 1/2,
+// 2^f by a polynomial of degree 4 (least largest relative error with a constant term of 1,
+// fitted over [-1/2, 1/2]: 3e-6), n added to the exponent. Below -127, -inf among them,
+// exactly 0; x at most 127 and no NaN.
+__device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
+    float a, b;
+    unpair(x, a, b);
+    x = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
+    const uint64_t r = add2(x, pair(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's last bits are n
+    const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
+    uint64_t t = fma2(f, pair(0.009585382416844368f, 0.009585382416844368f), pair(0.05590662732720375f, 0.05590662732720375f));
+    t = fma2(t, f, pair(0.24024038016796112f, 0.24024038016796112f));
+    t = fma2(t, f, pair(0.6931241750717163f, 0.6931241750717163f));
+    t = fma2(t, f, pair(1.f, 1.f));
+    float t0, t1, r0, r1;
+    unpair(t, t0, t1);
+    unpair(r, r0, r1);
+    p0 = __uint_as_float(__float_as_uint(t0) + (__float_as_uint(r0) << 23));
+    p1 = __uint_as_float(__float_as_uint(t1) + (__float_as_uint(r1) << 23));
 }
 
 // One row over the tiles [ta, tb), position by position in f32: 32 columns of o at a time to
@@ -192,20 +261,23 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                          const __grid_constant__ CUtensorMap vmap, const uint16_t* __restrict__ kp,
                          const uint16_t* __restrict__ vp, int n_slot, int splits) {
     using C = PCfg<D>;
-    constexpr int NQ = C::NQ, BN = C::BN, ST = C::stages, SW = 4 * NQ;  // SW: softmax warps
+    constexpr int NQ = C::NQ, BN = C::BN, SA = C::SA, PH = C::PH, ST = C::stages, SW = 4 * NQ;  // SW: softmax warps
     extern __shared__ __align__(1024) uint8_t sm[];
     const uint32_t q_s = smem_u32(sm), k_s = q_s + NQ * C::q_bytes, v_s = k_s + ST * C::kv_bytes;
     uint8_t* v_gen = sm + NQ * C::q_bytes + ST * C::kv_bytes;
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + NQ * C::q_bytes + 2 * ST * C::kv_bytes);
     const auto bar = [&](int i) { return smem_u32(bars + i); };
-    // barriers: K full / empty, V full / empty by stage; S full, P full by S buffer; O done, Q full by row
-    // tile; AB: the products of a CTA that gives up
-    enum { KF = 0, KE = KF + ST, VF = KE + ST, VE = VF + ST, SF = VE + ST, PF = SF + 2, OD = PF + 2, QF = OD + 2, AB = QF + 2, NB = AB + 1 };
+    // S runs SA tiles ahead of P V. A stage holds V of tile i and K of tile i + SA, which one
+    // step of the products uses; K of the first SA tiles comes first, to where K of tiles ST and
+    // on will be. Barriers: full, looked through and empty by stage; K of the first tiles there, and used; S there,
+    // S read and P there (by part), by row tile or by S buffer; O added to, and Q there, by row
+    // tile; the products of a row tile that is given up.
+    enum { F = 0, V = F + ST, E = V + ST, KF = E + ST, KU = KF + 2, SF = KU + 2, SR = SF + 2, PF = SR + 2, OD = PF + 4, QF = OD + 2, AB = QF + 2, NB = AB + 2 };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NB);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // [NQ]
     int* last = poison + 2;
-    static_assert(NB * 8 + 24 <= 256, "barrier area");
+    static_assert(NB * 8 + 24 <= 512, "barrier area");
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int HK = a.c.HK, G = a.H / HK;
     const int h = (int)blockIdx.x % HK;
@@ -227,7 +299,10 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     const int ta = part * per, tb = min(w.tiles, ta + per), nt = tb - ta;
 
     if (tid == 0) {
-        for (int i = 0; i < NB; ++i) mbar_init(bar(i), (i >= PF && i < OD) || (i >= QF && i < AB) ? 128u : 1u);
+        for (int i = 0; i < NB; ++i) {
+            const bool frees = (i >= E && i < KF) || (i >= KU && i < SF), rows = (i >= SR && i < OD) || (i >= QF && i < AB);
+            mbar_init(bar(i), frees ? (uint32_t)NQ : rows ? 4u : 1u);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *abort_flag = 0;
         poison[0] = poison[1] = 0;
@@ -241,124 +316,199 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // the S buffer (and its barriers) of row tile q and tile i, and how often it was used before
+    const auto buffer = [](int q, int i) { return C::shared_s ? q : i % C::SA; };
+    const auto uses = [](int i) { return C::shared_s ? i : i / C::SA; };
+    const auto s_col = [](int i) { return C::shared_s ? 0 : i % C::SA * C::BN; };
+    const auto p_col = [](int q, int i) { return C::shared_s ? C::p_col0 + q * (C::BN / 2) : i % C::SA * C::BN; };
+    // every position of the tile at j0 is seen by rows at positions first .. last
+    const auto all_see = [&](int j0, int first, int last_pos) {
+        return j0 + C::BN - 1 <= first && (!a.window || j0 > last_pos - a.window || j0 + C::BN <= a.sinks);
+    };
     const auto give_up = [&]() {
         *abort_flag = 1;
         pages_flag(a.c, AERO_CUDA_PAGES_WAIT);
     };
 
-    if (warp == SW + 1) {
+    if (warp == SW + NQ) {
         // ------------------------------------------------------------ K and V tiles by TMA
         const int P = 1 << a.c.page_shift, box = min(P, 64), boxes = BN / box;
         bool good = true;
-        int done = 0;  // tiles whose copies were issued
-        for (int i = 0; i < nt && good; ++i) {
+        // this lane's box of tile i: the pool's row, or -1
+        const auto find = [&](int i) {
             const int j0 = tile_pos<BN>(w, ta + i) + lane * box;
-            bool want = lane < boxes && j0 <= w.p1;
-            int row = 0;
-            if (want) {
-                const int page = a.c.table[(int64_t)w.seq * a.c.max_pages + (j0 >> a.c.page_shift)];
-                if ((uint32_t)page >= (uint32_t)a.c.n_page) {
-                    pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
-                    want = false;
-                }
-                // < 2^31: checked when the cache was opened
-                row = want ? (int)((((int64_t)a.layer * a.c.n_page + page) * HK + h) << a.c.page_shift) + (j0 & (P - 1)) : 0;
+            if (i >= nt || lane >= boxes || j0 > w.p1) return -1;
+            const int page = a.c.table[(int64_t)w.seq * a.c.max_pages + (j0 >> a.c.page_shift)];
+            if ((uint32_t)page >= (uint32_t)a.c.n_page) {
+                pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
+                return -1;
             }
-            const int n_box = __popc(__ballot_sync(0xffffffffu, want));
+            // < 2^31: checked when the cache was opened
+            return (int)(((((int64_t)a.layer * a.c.n_page + page) * HK + h) << a.c.page_shift) + (j0 & (P - 1)));
+        };
+        const auto load = [&](const CUtensorMap& map, uint32_t tile, int row, int full) {
+            if (row < 0) return;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) tma_load_2d(tile + lane * box * 128 + c * C::half, &map, c * 64, row, bar(full));
+        };
+        const auto expect = [&](int n_box, int full) {
+            if (lane == 0) {
+                if (n_box)
+                    mbar_expect_tx(bar(full), (uint32_t)(n_box * box * D * 2));
+                else
+                    mbar_arrive(bar(full));
+            }
+            __syncwarp();
+        };
+        const auto count = [&](int row) { return __popc(__ballot_sync(0xffffffffu, row >= 0)); };
+        // rows of the tiles i .. i + SA - 1, whose K is on its way
+        int row[SA + 1];
+#pragma unroll
+        for (int i = 0; i < SA; ++i) {
+            row[i] = find(i);
+            expect(count(row[i]), KF + i);
+            load(kmap, k_s + ((i + ST - SA) % ST) * C::kv_bytes, row[i], KF + i);
+        }
+        int done = 0;  // stages whose copies were issued
+        for (int i = 0; i < nt; ++i) {
+            row[SA] = find(i + SA);
             const int st = i % ST;
-            const uint32_t ph = (uint32_t)(i / ST) & 1u;
+            // the stage's last use; of the places of the first tiles' K, that use
+            if (i >= ST) good = good && wait_phase(bar(E + st), (uint32_t)(i / ST - 1) & 1u, abort_flag);
+            if (i + SA < nt && i < ST && i >= ST - SA) good = good && wait_phase(bar(KU + i - (ST - SA)), 0, abort_flag);
+            if (!good) break;
+            expect(count(row[0]) + count(row[SA]), F + st);
+            load(vmap, v_s + st * C::kv_bytes, row[0], F + st);
+            load(kmap, k_s + st * C::kv_bytes, row[SA], F + st);
 #pragma unroll
-            for (int kv = 0; kv < 2; ++kv) {
-                const uint32_t full = bar((kv ? VF : KF) + st);
-                if (!mbar_wait(bar((kv ? VE : KE) + st), ph ^ 1u, abort_flag)) {
-                    good = false;
-                    break;
-                }
-                if (lane == 0) {
-                    if (n_box)
-                        mbar_expect_tx(full, (uint32_t)(n_box * box * D * 2));
-                    else
-                        mbar_arrive(full);
-                }
-                __syncwarp();
-                if (want) {
-                    const uint32_t dst = (kv ? v_s : k_s) + (uint32_t)(st * C::kv_bytes + lane * box * 128);
-#pragma unroll
-                    for (int c = 0; c < D / 64; ++c) tma_load_2d(dst + c * C::half, kv ? &vmap : &kmap, c * 64, row, full);
-                }
-                __syncwarp();
-            }
-            done += good;
+            for (int k = 0; k < SA; ++k) row[k] = row[k + 1];
+            ++done;
         }
         if (!good) {
             if (lane == 0) give_up();
-            for (int i = std::max(0, done - ST); i < done; ++i) {  // copies in flight land before the memory is given up
-                mbar_wait_timed(bar(KF + i % ST), (uint32_t)(i / ST) & 1u);
-                mbar_wait_timed(bar(VF + i % ST), (uint32_t)(i / ST) & 1u);
-            }
+            // copies in flight land before the memory is given up
+            for (int i = 0; i < SA; ++i) mbar_wait_timed(bar(KF + i), 0);
+            for (int i = std::max(0, done - ST); i < done; ++i) mbar_wait_timed(bar(F + i % ST), (uint32_t)(i / ST) & 1u);
         }
-    } else if (warp == SW) {
-        // ------------------------------------------------------------ the products
-        if (lane == 0 && nt > 0) {
-            const uint32_t iqk = idesc16<BF16>(BN, false), ipv = idesc16<BF16>(D, true);
-            bool good = true;
-            const auto wait = [&](int b, int n) {  // the n-th completion (from 0) of barrier b
-                if (good && !mbar_wait(bar(b), (uint32_t)n & 1u, abort_flag)) {
-                    good = false;
-                    give_up();
-                }
-                tc_fence_after();
-            };
-            const auto qk = [&](int q, int buf, int i) {
-                const uint32_t qa = q_s + q * C::q_bytes, kb = k_s + (i % ST) * C::kv_bytes;
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    umma16_ss(tmem + buf * C::s_col, sw128_desc(qa + (ks >> 2) * (kTileRows * 128) + (ks & 3) * 32),
-                              sw128_desc(kb + (ks >> 2) * C::half + (ks & 3) * 32), iqk, ks > 0);
-                umma_commit(bar(SF + buf));
-            };
-            const auto pv = [&](int q, int buf, int i) {
-                const uint32_t vb = v_s + (i % ST) * C::kv_bytes;
-#pragma unroll
-                for (int ks = 0; ks < BN / 16; ++ks)
-                    umma_ts(tmem + C::o_col0 + q * D, tmem + buf * C::s_col + ks * 8,
-                            sw128_mn_desc(vb + ks * 2048, C::half), ipv, i > 0 || ks > 0);
-            };
-            for (int q = 0; q < NQ; ++q) wait(QF + q, 0);
-            wait(KF, 0);
-            if (good) {
-                for (int q = 0; q < NQ; ++q) qk(q, q, 0);
-                umma_commit(bar(KE));
-            }
-            for (int i = 0; i < nt && good; ++i) {
-                const bool next = i + 1 < nt;
-                if (next) wait(KF + (i + 1) % ST, (i + 1) / ST);
-                if constexpr (NQ == 2) {
-                    for (int q = 0; q < 2 && good; ++q) {
-                        wait(PF + q, i);
-                        if (q == 0) wait(VF + i % ST, i / ST);
-                        if (!good) break;
-                        pv(q, q, i);
-                        if (next)
-                            qk(q, q, i + 1);
+    } else if (warp == SW + NQ + 1) {
+        // ------------------------------------------------------------ V tiles that not every row sees
+        bool good = true;
+        for (int i = 0; i < nt && good; ++i) {
+            const int j0 = tile_pos<BN>(w, ta + i);
+            good = wait_phase(bar(F + i % ST), (uint32_t)(i / ST) & 1u, abort_flag);
+            if (good && !all_see(j0, w.p0, w.p1)) {
+                uint8_t* vt = v_gen + (i % ST) * C::kv_bytes;
+                bool odd = false;
+                for (int r = lane; r < BN; r += 32) {
+                    const int j = j0 + r;
+                    const bool dead = j > w.p1 || (a.window && j < w.lo && j >= a.sinks);
+                    // (the swizzle only orders the 16-byte pieces of a row)
+#pragma unroll 8
+                    for (int c = 0; c < D / 8; ++c) {
+                        uint4* at = reinterpret_cast<uint4*>(vt + (c >> 3) * C::half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                        if (dead)
+                            *at = make_uint4(0u, 0u, 0u, 0u);
                         else
-                            umma_commit(bar(OD + q));
+                            odd |= not_finite<BF16>(*at);
                     }
-                } else {
-                    if (next && good) qk(0, (i + 1) & 1, i + 1);
-                    wait(PF + (i & 1), i >> 1);
-                    wait(VF + i % ST, i / ST);
+                }
+                if (odd)
+                    for (int q = 0; q < NQ; ++q) {
+                        const int r0 = w.row0 + q * kTileRows, r1 = min(w.rows, r0 + kTileRows) - 1;
+                        if (r0 <= r1 && !all_see(j0, w.len - w.n_new + r0 / G, w.len - w.n_new + r1 / G)) poison[q] = 1;
+                    }
+                fence_proxy_async();
+            }
+            __syncwarp();
+            if (good && lane == 0) mbar_arrive(bar(V + i % ST));
+        }
+        if (!good && lane == 0) give_up();
+        __syncwarp();
+        asm volatile("bar.arrive 1, %0;" ::"n"(128 * NQ + 32) : "memory");
+    } else if (warp >= SW) {
+        // ------------------------------------------------------------ the products of row tile q
+        // (a warp each: while one waits for its softmax, the other's products run)
+        const int q = warp - SW;
+        // The whole warp walks the loop, with values that are visibly the same in every lane, so
+        // descriptors are made by the uniform pipe; one lane issues. (With one lane walking it, the
+        // arithmetic and its moves took longer than the products.)
+        const int n = __shfl_sync(0xffffffffu, nt, 0);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const bool leads = elect_one();
+        const uint32_t iqk = idesc16<BF16>(BN, false), ipv = idesc16<BF16>(D, true);
+        bool good = true;
+        const auto wait = [&](int b, int nth) {  // the nth completion (from 0) of barrier b
+            if (good && !wait_phase(bar(b), (uint32_t)nth & 1u, abort_flag)) {
+                good = false;
+                if (leads) give_up();
+            }
+        };
+        const auto qk = [&](int i) {
+            const uint32_t qa = desc_low(q_s + q * C::q_bytes, 16), kb = desc_low(k_s + ((i + ST - SA) % ST) * C::kv_bytes, 16);
+            const uint32_t d = tm + s_col(i);
+            if (leads) {
+                umma16_ss<false>(d, desc(qa), desc(kb), iqk);
+#pragma unroll
+                for (int ks = 1; ks < D / 16; ++ks)
+                    umma16_ss<true>(d, desc(qa + (((ks >> 2) * (kTileRows * 128) + (ks & 3) * 32) >> 4)),
+                                    desc(kb + (((ks >> 2) * C::half + (ks & 3) * 32) >> 4)), iqk);
+                umma_commit(bar(SF + buffer(q, i)));
+            }
+            __syncwarp();
+        };
+        const auto pv = [&](int i, int part) {
+            const int k0 = part * (BN / 16 / PH);
+            const uint32_t vb = desc_low(v_s + (i % ST) * C::kv_bytes + k0 * 2048, C::half);
+            const uint32_t d = tm + C::o_col0 + q * D, p = tm + p_col(q, i) + k0 * 8;
+            if (leads) {
+#pragma unroll
+                for (int k = 0; k < BN / 16 / PH; ++k)
+                    umma_ts(d, p + k * 8, desc(vb + (k * 2048 >> 4)), ipv, i > 0 || part > 0 || k > 0);
+            }
+            __syncwarp();
+        };
+        const auto commit = [&](int b) {
+            if (leads) umma_commit(bar(b));
+            __syncwarp();
+        };
+        if (n > 0) {
+            wait(QF + q, 0);
+            // S of tile i may be written when the buffer's last S has been read: the other row
+            // tile's of this tile or the one before, or (P over S) when P V of tile i - 2, in front
+            // of it, has read P
+            const auto s_free = [&](int i) {
+                if (C::shared_s && (q == 1 || i > 0)) wait(SR + (q ^ 1), q == 1 ? i : i - 1);
+            };
+            for (int i = 0; i < SA && i < n && good; ++i) {
+                wait(KF + i, 0);
+                s_free(i);
+                if (!good) break;
+                tc_fence_after();
+                qk(i);
+                commit(KU + i);
+            }
+            for (int i = 0; i < n && good; ++i) {
+                wait(V + i % ST, i / ST);
+                if (C::shared_s && i + SA < n) {
+                    s_free(i + SA);
                     if (!good) break;
-                    pv(0, i & 1, i);
-                    umma_commit(bar(OD));
+                    tc_fence_after();
+                    qk(i + SA);
+                }
+                for (int part = 0; part < PH && good; ++part) {
+                    wait(PF + buffer(q, i) * PH + part, uses(i));
+                    if (!good) break;
+                    tc_fence_after();
+                    pv(i, part);
                 }
                 if (!good) break;
-                umma_commit(bar(VE + i % ST));
-                if (next) umma_commit(bar(KE + (i + 1) % ST));
+                if (!C::shared_s && i + SA < n) qk(i + SA);
+                if (C::shared_s || i + SA >= n) commit(OD + q);
+                commit(E + i % ST);
             }
             if (!good) {  // products in flight end before TMEM is given up
-                umma_commit(bar(AB));
-                mbar_wait_timed(bar(AB), 0);
+                commit(AB + q);
+                mbar_wait_timed(bar(AB + q), 0);
             }
         }
         __syncwarp();
@@ -393,61 +543,71 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             }
         }
         fence_proxy_async();
-        mbar_arrive(bar(QF + q));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(QF + q));
 
-        // positions of this warp's rows (ascending with the row) and of this row tile's
+        // positions of this warp's rows (ascending with the row)
         const int pw0 = __shfl_sync(0xffffffffu, pos, 0);
         const int pw1 = __reduce_max_sync(0xffffffffu, pos);
         const bool full_warp = __all_sync(0xffffffffu, real);
-        const int tile_row0 = w.row0 + q * kTileRows;
-        const int pt0 = w.len - w.n_new + min(tile_row0, w.rows - 1) / G;
-        const int pt1 = w.len - w.n_new + (min(w.rows, tile_row0 + kTileRows) - 1) / G;
-        const auto all_see = [&](int j0, int first, int lastp) {  // every position of the tile, for rows at first .. lastp
-            return j0 + BN - 1 <= first && (!a.window || j0 > lastp - a.window || j0 + BN <= a.sinks);
-        };
         const float sc = a.scale_log2;
         float m = -INFINITY, l = 0.f;
         bool good = true;
         for (int i = 0; i < nt && good; ++i) {
-            const int buf = NQ == 2 ? q : i & 1, use = NQ == 2 ? i : i >> 1;
+            const int buf = buffer(q, i);
             const int j0 = tile_pos<BN>(w, ta + i);
-            if (!mbar_wait(bar(SF + buf), (uint32_t)use & 1u, abort_flag)) {
+            if (!wait_phase(bar(SF + buf), (uint32_t)uses(i) & 1u, abort_flag)) {
                 good = false;
                 break;
             }
             tc_fence_after();
-            const uint32_t st = tmem + lanes + buf * C::s_col;
+            const uint32_t st = tmem + lanes + s_col(i), pt = tmem + lanes + p_col(q, i);
             uint32_t s[BN / 32][32];
 #pragma unroll
             for (int c = 0; c < BN / 32; ++c) tmem_ld32(st + c * 32, s[c]);
             tmem_wait_ld();
+            if constexpr (C::shared_s) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(SR + q));
+            }
             if (!(full_warp && all_see(j0, pw0, pw1))) {
+                // bit k of a word: does the row see position k of its 32?
                 const int hi = pos - j0, lo = a.window ? pos - a.window - j0 : -1, sk = a.window ? a.sinks - j0 : 0;
 #pragma unroll
-                for (int c = 0; c < BN / 32; ++c)
+                for (int c = 0; c < BN / 32; ++c) {
+                    const uint32_t see = low_bits(hi + 1 - 32 * c) & (~low_bits(lo + 1 - 32 * c) | low_bits(sk - 32 * c));
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int k = c * 32 + e;
-                        if (!(k <= hi && (k > lo || k < sk))) s[c][e] = 0xFF800000u;  // -inf
-                    }
+                    for (int e = 0; e < 32; ++e)
+                        if (!(see >> e & 1u)) s[c][e] = 0xFF800000u;  // -inf
+                }
             }
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < BN / 32; ++c)
 #pragma unroll
-                for (int e = 0; e < 32; ++e) x[e & 3] = fmaxf(x[e & 3], __uint_as_float(s[c][e]));
-            const float mt = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * sc;
+                for (int e = 0; e < 32; e += 2)
+                    x[(e >> 1) & 3] = max3(x[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+            const float mt = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])) * sc;
+            // P V of the tile before has ended: O may be rescaled and P written
+            if (C::shared_s && i > 0) {
+                if (!wait_phase(bar(OD + q), (uint32_t)(i - 1) & 1u, abort_flag)) {
+                    good = false;
+                    break;
+                }
+                tc_fence_after();
+            }
             if (i == 0) {
                 m = mt;
-            } else if (__any_sync(0xffffffffu, mt > m + 8.f)) {
-                const float mn = fmaxf(m, mt);
+            } else if (__any_sync(0xffffffffu, !(mt <= m + 8.f) && mt != -INFINITY)) {
+                const float mn = max_nan(m, mt);
                 const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
                 l *= f;
-                // O += P V of the tile before has ended: with two row tiles it was issued before
-                // this tile's S; with one it has a barrier of its own
-                if constexpr (NQ == 1) {
-                    if (!mbar_wait(bar(OD), (uint32_t)(i - 1) & 1u, abort_flag)) {
+                if constexpr (!C::shared_s) {
+                    // P V of the tile before has ended when S of the next tile, issued after it, is there
+                    if (!(i + 1 < nt ? wait_phase(bar(SF + (buf ^ 1)), (uint32_t)uses(i + 1) & 1u, abort_flag)
+                                     : wait_phase(bar(OD + q), 0, abort_flag))) {
                         good = false;
                         break;
                     }
@@ -464,55 +624,48 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                     tmem_st16(ot + c * 16, o);
                 }
             }
-            const float z = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            // (m + (m - m) is m, or no number where m is infinite or none: then the whole row is
+            // none, as its formula says, and ex2_poly's result does not matter)
+            const float z = m == -INFINITY ? 0.f : m + (m - m);
+            const uint64_t sc2 = pair(sc, sc), nz2 = pair(-z, -z);
+            uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
             for (int c = 0; c < BN / 32; ++c) {
                 uint32_t p[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float p0 = ex2(fmaf(__uint_as_float(s[c][e]), sc, -z));
-                    const float p1 = ex2(fmaf(__uint_as_float(s[c][e + 1]), sc, -z));
-                    sum[e & 2] += p0;
-                    sum[(e & 2) + 1] += p1;
+                for (int e = 0; e < 16; ++e) {
+                    const uint64_t y = fma2(pair(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc2, nz2);
+                    float p0, p1;
+                    if (e % kPolyEvery == kPolyEvery - 1) {
+                        ex2_poly(y, p0, p1);
+                    } else {
+                        unpair(y, p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                    }
+                    sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
                     // the weights meet V in its type: a relative rounding of 2^-11 (f16) or 2^-8
                     // (bf16) each, below the output's own; their sum l stays f32
-                    p[e / 2] = pack16<BF16>(p0, p1);
+                    p[e] = pack16<BF16>(p0, p1);
                 }
-                tmem_st16(st + c * 16, p);
+                tmem_st16(pt + c * 16, p);
+                if ((c + 1) % (BN / 32 / PH) == 0) {  // a part of P is there
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(PF + buf * PH + c / (BN / 32 / PH)));
+                }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            const bool some = !all_see(j0, pt0, pt1);  // a position of the tile that some row does not see
-            if (some) {
-                if (!mbar_wait(bar(VF + i % ST), (uint32_t)(i / ST) & 1u, abort_flag)) {
-                    good = false;
-                    break;
-                }
-                uint8_t* vt = v_gen + (i % ST) * C::kv_bytes;
-                bool odd = false;
-                const int r = ((warp & 3) * 32 + lane) % BN;  // the row of V this thread looks after
-                const int j = j0 + r;
-                const bool dead = j > w.p1 || (a.window && j < w.lo && j >= a.sinks);
-                // (the swizzle only orders the 16-byte pieces of a row)
-                for (int c = (warp & 3) * 32 + lane >= BN ? D / 16 : 0; c < (BN == 64 && (warp & 3) < 2 ? D / 16 : D / 8); ++c) {
-                    uint4* at = reinterpret_cast<uint4*>(vt + (c >> 3) * C::half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                    if (dead)
-                        *at = make_uint4(0u, 0u, 0u, 0u);
-                    else
-                        odd |= not_finite<BF16>(*at);
-                }
-                if (odd) poison[q] = 1;
-                fence_proxy_async();
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(bar(PF + buf));
+            float l0, l1;
+            unpair(add2(sum[0], sum[1]), l0, l1);
+            l += l0 + l1;
         }
-        if (good && nt > 0 && !mbar_wait(bar(OD + q), NQ == 2 ? 0u : (uint32_t)(nt - 1) & 1u, abort_flag)) good = false;
+        for (int i = max(nt - SA, 0); i < nt; ++i)  // one by one: a wait tells neighbouring phases apart only
+            if (good && !wait_phase(bar(OD + q), (uint32_t)(C::shared_s ? i : i - max(nt - SA, 0)) & 1u, abort_flag)) good = false;
         tc_fence_after();
         if (!good) give_up();
-        // every thread of the row tile has said what it met
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + q) : "memory");
+        // the V tiles have been looked through
+        asm volatile("bar.sync 1, %0;" ::"n"(128 * NQ + 32) : "memory");
         const bool slow = poison[q] != 0;
         uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head;
         const bool stores = row < w.rows;

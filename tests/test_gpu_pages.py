@@ -247,6 +247,32 @@ def test_prompt_masked_places_hold_anything():
     assert not torch.isfinite(got[~clean]).any()
 
 
+@pytest.mark.parametrize("dtype,bad", [(F16, math.nan), (BF16, math.nan), (F16, math.inf), (BF16, -math.inf)])
+def test_keys_that_are_no_numbers(dtype, bad):
+    """One key at a time not finite, V finite: a token that sees it has no result (infinite
+    scores of both signs, or none), the others theirs."""
+    c, K, V = open_cache([300], 16, 1, 64, dtype)
+    q = (torch.rand((40, 2, 64), device="cuda") + 0.5).to(dtype)  # scores of an infinite key: infinite
+    for j in (270, 279, 285, 291):
+        row = c.k(0)[int(c.tables()[0][0, j // 16]), :, j % 16]
+        keep = row.clone()
+        row.fill_(bad)
+        many = c.attend(0, q, i32([0]), i32([0, 40]))
+        one = c.attend(0, q[39:], i32([0]))
+        k = K[0].clone()
+        row.copy_(keep)
+        want = reference(q[:j - 260], k, V[0], list(range(260, j)), 0, 0, 0.125)
+        close(many[:j - 260], want, dtype)
+        if bad == -math.inf:  # scores of -inf: a weight of 0
+            k = torch.cat([k[:j], k[j + 1:]])
+            v = torch.cat([V[0][:j], V[0][j + 1:]])
+            close(many[j - 260:], reference(q[j - 260:], k, v, list(range(j - 1, 299)), 0, 0, 0.125), dtype)
+            close(one, reference(q[39:], k, v, [298], 0, 0, 0.125), dtype)
+        else:
+            assert not torch.isfinite(many[j - 260:]).any() and not torch.isfinite(one).any()
+    c.check()
+
+
 def test_prompt_strides_and_bad_rows():
     c, K, V = open_cache([150, 60], 16, 2, 64, BF16)
     wide = torch.randn((101, 9, 67), device="cuda").to(BF16)
