@@ -24,10 +24,10 @@
 // CTAs that leave (o, m, l); the last to arrive joins them in order.
 //
 // Positions that no token of the CTA sees are zeroed in the V tile (their memory may
-// hold anything, and 0 x NaN is NaN). Where only some rows see a position (diagonal, ends of
-// the window), V tiles are searched for values that are not finite; if there are any, the
-// row tile is computed again in f32 by row_slow, position by position: rows that do not see
-// them come out as without them.
+// hold anything, and 0 x NaN is NaN). A position that only some rows see (diagonal, ends of the
+// window) may hold values that are not finite; then the rows that do not see it come out not
+// finite too. So a row whose result is not finite is computed again in f32 by row_slow,
+// position by position over what it sees: one that sees such a value keeps its result.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -42,10 +42,7 @@ namespace {
 constexpr int kTileRows = 128;
 // Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly): the
 // special-function pipe, at 16 a cycle and SM, is what the softmax waits for otherwise.
-#ifndef POLY
-#define POLY 4
-#endif
-constexpr int kPolyEvery = POLY;
+constexpr int kPolyEvery = 8;
 
 template <int D>
 struct PCfg {
@@ -152,14 +149,6 @@ __device__ __forceinline__ uint32_t idesc16(int N, bool bn) {
 
 // The lowest n bits set (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
-
-// Any of the 8 16-bit values infinite or not a number?
-template <bool BF16>
-__device__ __forceinline__ bool not_finite(uint4 v) {
-    // the exponent bits alone; adding one step of them to all-ones carries into the sign bit
-    constexpr uint32_t ex = BF16 ? 0x7F807F80u : 0x7C007C00u, one = BF16 ? 0x00800080u : 0x04000400u;
-    return (((v.x & ex) + one) | ((v.y & ex) + one) | ((v.z & ex) + one) | ((v.w & ex) + one)) & 0x80008000u;
-}
 
 template <bool BF16>
 __device__ __forceinline__ float to_f32(uint16_t v) {
@@ -269,14 +258,13 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     const auto bar = [&](int i) { return smem_u32(bars + i); };
     // S runs SA tiles ahead of P V. A stage holds V of tile i and K of tile i + SA, which one
     // step of the products uses; K of the first SA tiles comes first, to where K of tiles ST and
-    // on will be. Barriers: full, looked through and empty by stage; K of the first tiles there, and used; S there,
+    // on will be. Barriers: full, V's unseen rows zero, and empty by stage; K of the first tiles there, and used; S there,
     // S read and P there (by part), by row tile or by S buffer; O added to, and Q there, by row
     // tile; the products of a row tile that is given up.
     enum { F = 0, V = F + ST, E = V + ST, KF = E + ST, KU = KF + 2, SF = KU + 2, SR = SF + 2, PF = SR + 2, OD = PF + 4, QF = OD + 2, AB = QF + 2, NB = AB + 2 };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NB);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* poison = reinterpret_cast<int*>(tmem_slot + 2);  // [NQ]
-    int* last = poison + 2;
+    int* last = reinterpret_cast<int*>(tmem_slot + 2);
     static_assert(NB * 8 + 24 <= 512, "barrier area");
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int HK = a.c.HK, G = a.H / HK;
@@ -305,7 +293,6 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *abort_flag = 0;
-        poison[0] = poison[1] = 0;
     }
     if (warp == SW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -391,40 +378,26 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             for (int i = std::max(0, done - ST); i < done; ++i) mbar_wait_timed(bar(F + i % ST), (uint32_t)(i / ST) & 1u);
         }
     } else if (warp == SW + NQ + 1) {
-        // ------------------------------------------------------------ V tiles that not every row sees
+        // ------------------------------------------------------------ V rows that no row sees, to zero
         bool good = true;
         for (int i = 0; i < nt && good; ++i) {
             const int j0 = tile_pos<BN>(w, ta + i);
             good = wait_phase(bar(F + i % ST), (uint32_t)(i / ST) & 1u, abort_flag);
             if (good && !all_see(j0, w.p0, w.p1)) {
                 uint8_t* vt = v_gen + (i % ST) * C::kv_bytes;
-                bool odd = false;
                 for (int r = lane; r < BN; r += 32) {
                     const int j = j0 + r;
-                    const bool dead = j > w.p1 || (a.window && j < w.lo && j >= a.sinks);
-                    // (the swizzle only orders the 16-byte pieces of a row)
-#pragma unroll 8
-                    for (int c = 0; c < D / 8; ++c) {
-                        uint4* at = reinterpret_cast<uint4*>(vt + (c >> 3) * C::half + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-                        if (dead)
-                            *at = make_uint4(0u, 0u, 0u, 0u);
-                        else
-                            odd |= not_finite<BF16>(*at);
-                    }
+                    if (j <= w.p1 && (!a.window || j >= w.lo || j < a.sinks)) continue;
+                    for (int c = 0; c < D / 8; ++c)  // (the swizzle only orders a row's pieces)
+                        *reinterpret_cast<uint4*>(vt + (c >> 3) * C::half + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                            make_uint4(0u, 0u, 0u, 0u);
                 }
-                if (odd)
-                    for (int q = 0; q < NQ; ++q) {
-                        const int r0 = w.row0 + q * kTileRows, r1 = min(w.rows, r0 + kTileRows) - 1;
-                        if (r0 <= r1 && !all_see(j0, w.len - w.n_new + r0 / G, w.len - w.n_new + r1 / G)) poison[q] = 1;
-                    }
                 fence_proxy_async();
             }
             __syncwarp();
             if (good && lane == 0) mbar_arrive(bar(V + i % ST));
         }
         if (!good && lane == 0) give_up();
-        __syncwarp();
-        asm volatile("bar.arrive 1, %0;" ::"n"(128 * NQ + 32) : "memory");
     } else if (warp >= SW) {
         // ------------------------------------------------------------ the products of row tile q
         // (a warp each: while one waits for its softmax, the other's products run)
@@ -521,25 +494,40 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         const int pos = real ? w.len - w.n_new + tok : -1;
         const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(w.q0 + tok) * a.q_token + (int64_t)head * a.q_head;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        // The warp's 32 rows, 16 bytes a lane, neighbouring lanes neighbouring pieces: piece x of the
+        // x-th of 32 * D / 8, where it lies in shared memory (as the products read it), and the
+        // offset of its row, which the row's own lane knows.
+        constexpr int kPieces = D / 8;
+        const auto at = [&](int x) {
+            const int r = x / kPieces, c = x % kPieces;
+            return (uint32_t)(q * C::q_bytes + (c >> 3) * (kTileRows * 128) + ((warp & 3) * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4));
+        };
+        const auto of_row = [&](int64_t mine, int r) {
+            const uint32_t low = __shfl_sync(0xffffffffu, (uint32_t)mine, r), high = __shfl_sync(0xffffffffu, (uint32_t)(mine >> 32), r);
+            return (int64_t)((uint64_t)high << 32 | low);
+        };
         {
-            const uint32_t dst = q_s + q * C::q_bytes + ((warp & 3) * 32 + lane) * 128;
-            const int sw = lane & 7;
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (real) {
-                    if (a.vec) {
-                        v = *reinterpret_cast<const uint4*>(qp + 8 * c);
-                    } else {
-                        const uint16_t* x = qp + 8 * c;
-                        v = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16,
-                                       x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
+            const int64_t mine = real ? (int64_t)(w.q0 + tok) * a.q_token + (int64_t)head * a.q_head : -1;
+            const uint16_t* all = static_cast<const uint16_t*>(a.q);
+#pragma unroll 1
+            for (int x0 = 0; x0 < kPieces; x0 += 8) {
+                uint4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int x = (x0 + k) * 32 + lane;
+                    const int64_t row_at = of_row(mine, x / kPieces);
+                    v[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row_at >= 0) {
+                        const uint16_t* y = all + row_at + x % kPieces * 8;
+                        if (a.vec)
+                            v[k] = *reinterpret_cast<const uint4*>(y);
+                        else
+                            v[k] = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16,
+                                              y[4] | (uint32_t)y[5] << 16, y[6] | (uint32_t)y[7] << 16);
                     }
                 }
-                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
-                                 dst + (uint32_t)((c >> 3) * (kTileRows * 128) + (((c & 7) ^ sw) << 4))),
-                             "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                             : "memory");
+#pragma unroll
+                for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(sm + at((x0 + k) * 32 + lane)) = v[k];
             }
         }
         fence_proxy_async();
@@ -577,6 +565,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
 #pragma unroll
                 for (int c = 0; c < BN / 32; ++c) {
                     const uint32_t see = low_bits(hi + 1 - 32 * c) & (~low_bits(lo + 1 - 32 * c) | low_bits(sk - 32 * c));
+                    if (__all_sync(0xffffffffu, see == 0xFFFFFFFFu)) continue;
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         if (!(see >> e & 1u)) s[c][e] = 0xFF800000u;  // -inf
@@ -664,9 +653,6 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             if (good && !wait_phase(bar(OD + q), (uint32_t)(C::shared_s ? i : i - max(nt - SA, 0)) & 1u, abort_flag)) good = false;
         tc_fence_after();
         if (!good) give_up();
-        // the V tiles have been looked through
-        asm volatile("bar.sync 1, %0;" ::"n"(128 * NQ + 32) : "memory");
-        const bool slow = poison[q] != 0;
         uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head;
         const bool stores = row < w.rows;
         const auto put_out = [&](int d0, const float* o, float k, int n) {
@@ -682,6 +668,12 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                 }
             }
         };
+        const auto put_row = [&](int d0, const float* o, float k) {  // 32 columns of the row, to Q's place
+            for (int e = 0; e < 32; e += 8)
+                *reinterpret_cast<uint4*>(sm + at(lane * kPieces + (d0 + e) / 8)) =
+                    make_uint4(pack16<BF16>(o[e] * k, o[e + 1] * k), pack16<BF16>(o[e + 2] * k, o[e + 3] * k),
+                               pack16<BF16>(o[e + 4] * k, o[e + 5] * k), pack16<BF16>(o[e + 6] * k, o[e + 7] * k));
+        };
         const auto inverse = [](float sum) { return sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum; };
         // partial results: columns in front of rows, so a warp's stores are contiguous
         constexpr int64_t slot_f = (int64_t)C::rows * (D + 2);
@@ -690,35 +682,65 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         const auto put_part = [&](int d0, const float* o, int n) {
             for (int e = 0; e < n; ++e) mine[(int64_t)(d0 + e) * C::rows + lrow] = o[e];
         };
-        if (slow && real) {
+        const float k = inverse(l);
+        const uint32_t ot = tmem + lanes + C::o_col0 + q * D;
+        bool odd = false;  // a value of the row that is not finite
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            if (nt > 0) {
+                tmem_ld32(ot + c * 32, o);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) odd |= (o[e] & 0x7F800000u) == 0x7F800000u;
+            if (parts > 1) {
+                float f[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]);
+                put_part(c * 32, f, 32);
+            } else {
+                // into Q's place, which no product reads any more
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint4 v;
+                    v.x = pack16<BF16>(__uint_as_float(o[e]) * k, __uint_as_float(o[e + 1]) * k);
+                    v.y = pack16<BF16>(__uint_as_float(o[e + 2]) * k, __uint_as_float(o[e + 3]) * k);
+                    v.z = pack16<BF16>(__uint_as_float(o[e + 4]) * k, __uint_as_float(o[e + 5]) * k);
+                    v.w = pack16<BF16>(__uint_as_float(o[e + 6]) * k, __uint_as_float(o[e + 7]) * k);
+                    *reinterpret_cast<uint4*>(sm + at(lane * kPieces + c * 4 + e / 8)) = v;
+                }
+            }
+        }
+        if (odd && real && l == l)  // (a score that is no number leaves none in the whole row)
             row_slow<D, BF16>(
                 a, w, h, qp, pos, ta, tb, kp, vp,
                 [&](int d0, const float* o, float sum) {
-                    if (parts == 1)
-                        put_out(d0, o, inverse(sum), 32);
-                    else
+                    if (parts > 1)
                         put_part(d0, o, 32);
+                    else
+                        put_row(d0, o, inverse(sum));
                 },
-                [&](float sm_, float sl) { m = sm_, l = sl; });
-        } else {
-            const float k = inverse(l);
-            const uint32_t ot = tmem + lanes + C::o_col0 + q * D;
-            if (!slow) {
-#pragma unroll 1
-                for (int c = 0; c < D / 16; ++c) {
-                    uint32_t o[16];
-                    if (nt > 0) {
-                        tmem_ld16(ot + c * 16, o);
-                        tmem_wait_ld();
-                    } else {
+                [&](float slow_m, float slow_l) { m = slow_m, l = slow_l; });
+        if (parts == 1) {
+            __syncwarp();
+            const int64_t to = stores ? (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head : -1;
+#pragma unroll 2
+            for (int x0 = 0; x0 < kPieces; ++x0) {
+                const int x = x0 * 32 + lane;
+                const int64_t row_at = of_row(to, x / kPieces);
+                if (row_at < 0) continue;
+                const uint4 v = *reinterpret_cast<const uint4*>(sm + at(x));
+                uint16_t* y = static_cast<uint16_t*>(a.out) + row_at + x % kPieces * 8;
+                if (a.vec) {
+                    *reinterpret_cast<uint4*>(y) = v;
+                } else {
+                    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = 0u;
-                    }
-                    float f[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]);
-                    if (stores && parts == 1) put_out(c * 16, f, k, 16);
-                    if (parts > 1) put_part(c * 16, f, 16);
+                    for (int b = 0; b < 8; ++b) y[b] = (uint16_t)(u[b >> 1] >> (16 * (b & 1)));
                 }
             }
         }
