@@ -837,7 +837,13 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
         a.scale_log2 = scale * 1.4426950408889634f;
         a.vec = aero::vec16(q, q_token, q_head) && aero::vec16(out, o_token, o_head);
         const bool bf16 = g.d.dtype == AERO_CUDA_TYPE_BF16;
-        if (q_start) {
+        // Few tokens, or hardly more than one a sequence, go token by token: a tile of 128 rows
+        // would be mostly empty, and its CTA costs some 15 us before it is done (B200, 4 x 8 heads of
+        // 128, tokens against tiles: 16 tokens over 4096 positions 27 / 34 us, 32 of 16 sequences
+        // over 2000 28 / 33, 64 of 64 over 2000 57 / 82; but 64 of one over 4096 61 / 47, 128 of 64
+        // over 2000 95 / 84).
+        const bool by_token = !q_start || T <= 32 || T < 2 * (int64_t)n;
+        if (!by_token) {
             a.part = g.prompt_part;
             a.counters = g.prompt_count;
             return g.ok(aero::launch_pages_prompt(a, bf16, g.kmap, g.vmap, g.k, g.v, g.n_sm, g.stream), "attend");

@@ -64,6 +64,13 @@ struct AttendArgs {
 };
 
 #if defined(__CUDACC__)
+// By one CTA of a launch: q_start ascends from 0 to T.
+__device__ __forceinline__ void check_q_start(const AttendArgs& a) {
+    bool bad = false;
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x) bad |= a.q_start[i] > a.q_start[i + 1];
+    if (threadIdx.x == 0) bad |= a.q_start[0] != 0 || a.q_start[a.n] != a.T;
+    if (bad) pages_flag(a.c, AERO_CUDA_PAGES_BAD_ROWS);
+}
 // Which sequence token t is of, and how many of its positions the token sees at most
 // (its own position + 1). q_start is searched within its n + 1 entries whatever they hold.
 __device__ __forceinline__ void token_rows(const AttendArgs& a, int t, int& seq, int& n) {

@@ -1,5 +1,5 @@
-// Attention of one new token per sequence over the paged cache
-// (include/aero_cuda_pages.h): o = sum_j softmax_j(scale q . k_j) v_j over the visible
+// Attention over the paged cache (include/aero_cuda_pages.h), token by token: one new
+// token per sequence, or few of several. o = sum_j softmax_j(scale q . k_j) v_j over the visible
 // positions, one pass over K and V with a running maximum m and sum l:
 //   m' = max(m, max_j s_j),  l' = l 2^(m - m') + sum_j 2^(s_j - m'),
 //   o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j     (s in powers of two),
@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     const int HK = a.c.HK, G = a.H / HK;
     const uint32_t ring = smem_u32(sm);
 
+    if (blockIdx.x == 0 && a.q_start) check_q_start(a);
     // ---- this CTA's piece of the line of units
     {
         int64_t* sums = reinterpret_cast<int64_t*>(red);  // [kThreads / 32]

@@ -40,6 +40,10 @@ namespace aero {
 namespace {
 
 constexpr int kTileRows = 128;
+// How far a row tile is split: a part more saves the others its tiles and costs the CTA that
+// joins the reading of rows * D sums. A tile takes about as long as the sums of kJoinRows
+// rows, so nt / parts + parts * rows / kJoinRows is least at sqrt(nt * kJoinRows / rows) parts.
+constexpr float kJoinRows = 220.f;
 // Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly): the
 // special-function pipe, at 16 a cycle and SM, is what the softmax waits for otherwise.
 constexpr int kPolyEvery = 8;
@@ -271,16 +275,12 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     const int h = (int)blockIdx.x % HK;
     const int slot = n_slot - 1 - (int)blockIdx.x / HK;  // the longest rows first
 
-    if (blockIdx.x == 0 && blockIdx.y == 0) {  // the whole of q_start
-        bool bad = false;
-        for (int i = tid; i < a.n; i += C::threads) bad |= a.q_start[i] > a.q_start[i + 1];
-        if (tid == 0) bad |= a.q_start[0] != 0 || a.q_start[a.n] != a.T;
-        if (bad) pages_flag(a.c, AERO_CUDA_PAGES_BAD_ROWS);
-    }
+    if (blockIdx.x == 0 && blockIdx.y == 0) check_q_start(a);
     Work w;
     if (!find_work<D>(a, slot, w)) return;
-    // this CTA's share of the tiles; a share holds at least 4 of them
-    const int per = splits > 1 ? max(4, (w.tiles + splits - 1) / splits) : max(w.tiles, 1);
+    // this CTA's share of the tiles
+    const int most = min(splits, (int)sqrtf((float)w.tiles * kJoinRows / (float)min(C::rows, w.rows - w.row0)) + 1);
+    const int per = max(1, (w.tiles + most - 1) / most);
     const int parts = max(1, (w.tiles + per - 1) / per);
     const int part = (int)blockIdx.y;
     if (part >= parts) return;
@@ -653,21 +653,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             if (good && !wait_phase(bar(OD + q), (uint32_t)(C::shared_s ? i : i - max(nt - SA, 0)) & 1u, abort_flag)) good = false;
         tc_fence_after();
         if (!good) give_up();
-        uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head;
         const bool stores = row < w.rows;
-        const auto put_out = [&](int d0, const float* o, float k, int n) {
-            for (int e = 0; e < n; e += 8) {
-                const uint4 v = make_uint4(pack16<BF16>(o[e] * k, o[e + 1] * k), pack16<BF16>(o[e + 2] * k, o[e + 3] * k),
-                                           pack16<BF16>(o[e + 4] * k, o[e + 5] * k), pack16<BF16>(o[e + 6] * k, o[e + 7] * k));
-                uint16_t* y = out + d0 + e;
-                if (a.vec) {
-                    *reinterpret_cast<uint4*>(y) = v;
-                } else {
-                    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-                    for (int b = 0; b < 8; ++b) y[b] = (uint16_t)(x[b >> 1] >> (16 * (b & 1)));
-                }
-            }
-        };
         const auto put_row = [&](int d0, const float* o, float k) {  // 32 columns of the row, to Q's place
             for (int e = 0; e < 32; e += 8)
                 *reinterpret_cast<uint4*>(sm + at(lane * kPieces + (d0 + e) / 8)) =
@@ -680,7 +666,8 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         const int64_t unit = (int64_t)(blockIdx.x) * splits;
         float* mine = a.part + (unit + part) * slot_f;
         const auto put_part = [&](int d0, const float* o, int n) {
-            for (int e = 0; e < n; ++e) mine[(int64_t)(d0 + e) * C::rows + lrow] = o[e];
+            if (stores)
+                for (int e = 0; e < n; ++e) mine[(int64_t)(d0 + e) * C::rows + lrow] = o[e];
         };
         const float k = inverse(l);
         const uint32_t ot = tmem + lanes + C::o_col0 + q * D;
@@ -745,35 +732,73 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             }
         }
         if (parts > 1) {
-            mine[(int64_t)D * C::rows + lrow] = m;
-            mine[(int64_t)(D + 1) * C::rows + lrow] = l;
-            __threadfence();
+            if (stores) {
+                mine[(int64_t)D * C::rows + lrow] = m;
+                mine[(int64_t)(D + 1) * C::rows + lrow] = l;
+            }
             asm volatile("bar.sync 4, %0;" ::"n"(128 * NQ) : "memory");
             if (tid == 0) {
+                __threadfence();  // the CTA's stores, ordered before by the barrier
                 *last = atomicAdd(a.counters + blockIdx.x, 1u) == (uint32_t)(parts - 1);
                 if (*last) a.counters[blockIdx.x] = 0;  // for the next launch
+                __threadfence();
             }
             asm volatile("bar.sync 4, %0;" ::"n"(128 * NQ) : "memory");
             if (*last) {
-                __threadfence();
-                const float* p0 = a.part + unit * slot_f + lrow;
-                float M = -INFINITY, L = 0.f;
-                for (int c = 0; c < parts; ++c) M = fmaxf(M, __ldcg(p0 + c * slot_f + (int64_t)D * C::rows));
-                const float z = M == -INFINITY ? 0.f : M;
-                for (int c = 0; c < parts; ++c)
-                    L += __ldcg(p0 + c * slot_f + (int64_t)(D + 1) * C::rows) *
-                         ex2(__ldcg(p0 + c * slot_f + (int64_t)D * C::rows) - z);
-                const float k = inverse(L);
-                for (int d0 = 0; d0 < D; d0 += 16) {
-                    float o[16];
+                // 16 columns of a row a thread, however few rows there are; the loads of kBatch parts are in
+                // flight at once (an L2 round trip each batch is what this costs)
+                constexpr int kBatch = 4, kCols = 16;
+                const int nrows = min(C::rows, w.rows - w.row0);
+                for (int x = tid; x < nrows * (D / kCols); x += 128 * NQ) {
+                    const int r = x % nrows, d0 = x / nrows * kCols;
+                    const float* p0 = a.part + unit * slot_f + r;
+                    float M = -INFINITY, L = 0.f, o[kCols];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = 0.f;
-                    for (int c = 0; c < parts; ++c) {
-                        const float f = ex2(__ldcg(p0 + c * slot_f + (int64_t)D * C::rows) - z);
+                    for (int e = 0; e < kCols; ++e) o[e] = 0.f;
+                    for (int c0 = 0; c0 < parts; c0 += kBatch) {
+                        float pm[kBatch], pl[kBatch], v[kBatch][kCols];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = fmaf(f, __ldcg(p0 + c * slot_f + (int64_t)(d0 + e) * C::rows), o[e]);
+                        for (int b = 0; b < kBatch; ++b) {
+                            const float* p = p0 + min(c0 + b, parts - 1) * slot_f;
+                            pm[b] = __ldcg(p + (int64_t)D * C::rows);
+                            pl[b] = __ldcg(p + (int64_t)(D + 1) * C::rows);
+#pragma unroll
+                            for (int e = 0; e < kCols; ++e) v[b][e] = __ldcg(p + (int64_t)(d0 + e) * C::rows);
+                        }
+                        float N = M;
+#pragma unroll
+                        for (int b = 0; b < kBatch; ++b) {
+                            if (c0 + b >= parts) pm[b] = -INFINITY, pl[b] = 0.f;  // (the last part again, weight 0)
+                            N = max_nan(N, pm[b]);
+                        }
+                        const float z = N == -INFINITY ? 0.f : N, f = ex2(M - z);
+                        M = N;
+                        L *= f;
+#pragma unroll
+                        for (int e = 0; e < kCols; ++e) o[e] *= f;
+#pragma unroll
+                        for (int b = 0; b < kBatch; ++b) {
+                            const float y = ex2(pm[b] - z);
+                            L = fmaf(pl[b], y, L);
+#pragma unroll
+                            for (int e = 0; e < kCols; ++e) o[e] = fmaf(v[b][e], y, o[e]);
+                        }
                     }
-                    if (stores) put_out(d0, o, k, 16);
+                    const float inv = inverse(L);
+                    const int t = (w.row0 + r) / G, hd = h * G + (w.row0 + r) % G;
+                    uint16_t* y = static_cast<uint16_t*>(a.out) + (int64_t)(w.q0 + t) * a.o_token + (int64_t)hd * a.o_head + d0;
+#pragma unroll
+                    for (int e = 0; e < kCols; e += 8) {
+                        const uint4 u = make_uint4(pack16<BF16>(o[e] * inv, o[e + 1] * inv), pack16<BF16>(o[e + 2] * inv, o[e + 3] * inv),
+                                                   pack16<BF16>(o[e + 4] * inv, o[e + 5] * inv), pack16<BF16>(o[e + 6] * inv, o[e + 7] * inv));
+                        if (a.vec) {
+                            *reinterpret_cast<uint4*>(y + e) = u;
+                        } else {
+                            const uint32_t half[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int b = 0; b < 8; ++b) y[e + b] = (uint16_t)(half[b >> 1] >> (16 * (b & 1)));
+                        }
+                    }
                 }
             }
         }
@@ -802,8 +827,10 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorM
     const int G = a.H / a.c.HK;
     const int n_slot = (int)((int64_t)a.T * G / C::rows) + a.n;  // see find_work
     const int64_t ctas = (int64_t)n_slot * a.c.HK;
-    // fewer CTAs than SMs: split the positions (the kernel splits no further than they reach)
-    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(n_sm / ctas, 64));
+    // fewer CTAs with work than SMs: split the positions (the kernel splits no further than pays);
+    // slots without rows end at once, so they are not counted, up to the workspace's size
+    const int64_t busy = std::max<int64_t>(a.n, ((int64_t)a.T * G + C::rows - 1) / C::rows) * a.c.HK;
+    const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(n_sm / busy, pages_prompt_max_grid(n_sm) / ctas), 64));
     prompt_attend_kernel<D, BF16><<<dim3((unsigned)ctas, (unsigned)splits), C::threads, C::smem, s>>>(
         a, kmap, vmap, static_cast<const uint16_t*>(kp), static_cast<const uint16_t*>(vp), n_slot, splits);
     return cudaGetLastError();
@@ -811,9 +838,9 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorM
 
 }  // namespace
 
-int pages_prompt_max_grid(int n_sm) { return n_sm; }
+int pages_prompt_max_grid(int n_sm) { return 2 * n_sm; }
 size_t pages_prompt_part_floats(int D, int n_sm) {
-    return (size_t)n_sm * (size_t)((D <= 128 ? 2 : 1) * kTileRows) * (size_t)(D + 2);
+    return (size_t)pages_prompt_max_grid(n_sm) * (size_t)((D <= 128 ? 2 : 1) * kTileRows) * (size_t)(D + 2);
 }
 
 cudaError_t launch_pages_prompt(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,

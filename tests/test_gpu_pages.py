@@ -198,6 +198,14 @@ PROMPT = [
     ([900, 150], [500, 150], 64, 1, 8, 64, F16, 200, 1),
     ([900, 150], [300, 150], 8, 2, 2, 128, F16, 130, 300),
     ([700, 33], [140, 33], 32, 1, 6, 256, BF16, 100, 129),
+    # few rows over long caches: split over CTAs and joined, one with a part that sees nothing
+    ([4000], [33], 64, 1, 8, 128, F16, 0, 0),
+    ([3000, 200], [40, 5], 16, 2, 3, 64, BF16, 0, 0),
+    ([2500, 50], [30, 4], 32, 1, 4, 256, F16, 0, 0),
+    ([3000], [260], 16, 1, 1, 192, BF16, 700, 40),
+    # few tokens: one by one
+    ([700, 90, 64], [9, 20, 1], 8, 2, 8, 128, F16, 0, 0),
+    ([700, 90, 64, 5], [2, 1, 1, 0], 16, 1, 4, 192, BF16, 100, 4),
 ]
 
 
@@ -283,6 +291,10 @@ def test_prompt_strides_and_bad_rows():
     close(out[[0, 30, 31, 100]], join([reference(q[[0, 30]], K[1], V[1], [29, 59], 0, 0, 0.125),
                                        reference(q[[31, 100]], K[0], V[0], [80, 149], 0, 0, 0.125)]), BF16)
     assert c.status() == 0
+    few, table = q[:31].contiguous(), i32([1, 0])
+    for start in ([0, 31, 32], [1, 20, 31], [0, 25, 20]):
+        c.attend(0, few, table, i32(start))
+        assert c.status() == 6, start
     for start in ([0, 90, 101], [0, 40, 30], [5, 31, 101], [0, 31, 100]):  # more tokens than positions; not ascending; ends
         c.attend(0, q, i32([1, 0]), i32(start))
         assert c.status() == 6, start
