@@ -3,11 +3,13 @@
 // mask.
 //
 // Bound by HBM: the logits are read and written once, in one launch. A CTA owns a slice
-// of one row's vocabulary: it notes in shared memory what the row's history and biases
-// say about the slice's tokens (counts are integer sums, so their order does not
-// matter; biases of one token are added by one lane in the list's order), then streams
-// the slice. Every CTA of a row reads the whole history (from L2 but for the first): a
-// wider slice reads it fewer times, a narrower one fills the GPU at few rows.
+// of one row's vocabulary. It notes in shared memory what the row's history and biases say
+// about the slice's tokens, while the slice's first logits are on their way, then streams the
+// slice. Slices are as wide as shared memory allows and the number of rows asks for, so that all
+// CTAs run at once and a history is read few times: with slices of 8192 tokens every CTA of the
+// 19 of a row read it, and three waves of CTAs each waited for it (64 rows of 151936 with 8192
+// tokens of history: 31 us). Counts are integer sums, so their order does not matter; the
+// biases of one token are added by its own thread in the list's order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -15,6 +17,7 @@
 #include <algorithm>
 #include <cstdio>
 #include <string>
+#include <type_traits>
 
 #include "../../include/aero_cuda_pages.h"
 #include "internal.h"
@@ -24,7 +27,10 @@ namespace aero {
 namespace {
 
 constexpr int kLogitThreads = 512;
-constexpr uint32_t kInPrompt = 0x80000000u;  // note of a token that the history holds, beside its count after the prompt
+constexpr int kLogitCtas = 2;     // of an SM
+constexpr int kLogitBatch = 4;    // 16-byte pieces of the slice in flight a thread
+constexpr int kBiasList = 512;    // biases of a slice kept in shared memory; with more, the row's list is read
+constexpr int kNotesBytes = 81920;
 
 struct LogitArgs {
     const void* in;
@@ -60,88 +66,170 @@ __device__ __forceinline__ E from_f(float v) {
         return __float2bfloat16_rn(v);
 }
 
-template <typename E>
-__global__ void __launch_bounds__(kLogitThreads) adjust_kernel(const LogitArgs a) {
-    extern __shared__ __align__(16) uint32_t notes[];                 // [slice], then [slice] biases
-    float* bias = reinterpret_cast<float*>(notes + a.slice);
-    const int r = (int)blockIdx.y, v0 = (int)blockIdx.x * a.slice, nv = min(a.slice, a.vocab - v0);
+// NB: bits of a token's note, its count after the prompt below a bit that says the prompt holds
+// it: 16 for histories of at most 32767 tokens, else 32.
+template <typename E, int NB>
+__global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const LogitArgs a) {
+    constexpr int V = 16 / (int)sizeof(E), U = kLogitBatch;
+    constexpr uint32_t kInPrompt = 1u << (NB - 1);
+    extern __shared__ __align__(16) uint32_t notes[];                    // slice * NB / 32
+    const int S = a.slice;
+    uint32_t* biased = notes + S / 32 * NB;                              // slice / 32: a bit for a token with biases
+    int* listed = reinterpret_cast<int*>(biased + S / 32);               // number of the slice's biases, padded
+    int* list_token = listed + 4;                                        // [kBiasList]
+    float* list_value = reinterpret_cast<float*>(list_token + kBiasList);
+    const int r = (int)blockIdx.y, v0 = (int)blockIdx.x * S, nv = min(S, a.vocab - v0);
     const int tid = (int)threadIdx.x;
-    const int nh = a.history ? max(0, a.n_history[r]) : 0;
-    const int np = nh && a.n_prompt ? a.n_prompt[r] : 0;
-    const int b0 = a.bias_start ? a.bias_start[r] : 0, b1 = a.bias_start ? a.bias_start[r + 1] : 0;
-    if (nh > 0) {
-        for (int i = tid; i < nv; i += kLogitThreads) notes[i] = 0;
-        __syncthreads();
-        const int32_t* h = a.history + (int64_t)r * a.ld_history;
-        for (int i = tid; i < nh; i += kLogitThreads) {
-            const uint32_t t = (uint32_t)(h[i] - v0);
-            if (h[i] >= 0 && t < (uint32_t)nv) {
-                if (i < np)
-                    atomicOr(notes + t, kInPrompt);
-                else
-                    atomicAdd(notes + t, 1u);
-            }
-        }
-    }
-    if (b1 > b0) {
-        for (int i = tid; i < nv; i += kLogitThreads) bias[i] = 0.f;
-        __syncthreads();
-        if (tid < 32) {
-            for (int i = b0 + tid; i - tid < b1; i += 32) {
-                const int t = i < b1 ? a.bias_token[i] : -1;
-                const float x = i < b1 ? a.bias_value[i] : 0.f;
-                const bool in = t >= v0 && t < v0 + nv;
-                const uint32_t same = __match_any_sync(0xffffffffu, in ? t - v0 : -1);
-                const bool leads = in && (same & ((1u << tid) - 1u)) == 0;
-                float sum = leads ? bias[t - v0] : 0.f;
-                // entries of one token, in the list's order
-                uint32_t todo = same;
-                while (__any_sync(0xffffffffu, leads && todo)) {
-                    const int from = leads && todo ? __ffs((int)todo) - 1 : tid;
-                    const float y = __shfl_sync(0xffffffffu, x, from);
-                    if (leads && todo) {
-                        sum += y;
-                        todo &= todo - 1;
-                    }
-                }
-                if (leads) bias[t - v0] = sum;
-                __syncwarp();
-            }
-        }
-    }
-    __syncthreads();
-    const float rep = a.repetition ? a.repetition[r] : 1.f;
-    const float fr = a.frequency ? a.frequency[r] : 0.f, pr = a.presence ? a.presence[r] : 0.f;
-    const uint32_t* bits = a.mask ? reinterpret_cast<const uint32_t*>(a.mask) + (int64_t)r * a.ld_mask : nullptr;
-    const auto one = [&](float x, int i) {
-        if (nh > 0) {
-            const uint32_t note = notes[i];
-            if (note) {
-                x = x > 0.f ? x / rep : x * rep;
-                const uint32_t c = note & ~kInPrompt;
-                if (c) x = x - fr * (float)c - pr;
-            }
-        }
-        if (b1 > b0) x += bias[i];
-        return x;
-    };
     const E* in = static_cast<const E*>(a.in) + (int64_t)r * a.ld + v0;
     E* out = static_cast<E*>(a.out) + (int64_t)r * a.ld_out + v0;
-    constexpr int V = 16 / (int)sizeof(E);
     const bool vec = (((uintptr_t)in | (uintptr_t)out) & 15) == 0;
-    const int whole = vec ? nv / V * V : 0;
-    for (int i = tid * V; i < whole; i += kLogitThreads * V) {
-        uint4 raw = __ldcs(reinterpret_cast<const uint4*>(in + i));
-        // the bits of tokens v0 + i .. + V: one word, V divides 32 and the slice is a multiple of 32
-        const uint32_t allow = bits ? bits[(v0 + i) >> 5] >> ((v0 + i) & 31) : 0xFFFFFFFFu;
-        E* x = reinterpret_cast<E*>(&raw);
+    const uint32_t* bits = a.mask ? reinterpret_cast<const uint32_t*>(a.mask) + (int64_t)r * a.ld_mask : nullptr;
+    const int nh = a.history ? (int)min((int64_t)max(0, a.n_history[r]), a.ld_history) : 0;
+    const int np = nh && a.n_prompt ? a.n_prompt[r] : 0;
+    const int b0 = a.bias_start ? a.bias_start[r] : 0, b1 = a.bias_start ? a.bias_start[r + 1] : 0;
+    const float rep = a.repetition ? a.repetition[r] : 1.f;
+    const float per = 1.f / rep;  // x * (1 / rep) for x / rep: one f32 rounding more
+    const float fr = a.frequency ? a.frequency[r] : 0.f, pr = a.presence ? a.presence[r] : 0.f;
+    uint4 raw[U];
+    uint32_t allow[U];
+    const auto load = [&](int base) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = from_f<E>((allow >> j) & 1u ? one(to_f(x[j]), i + j) : -INFINITY);
-        __stcs(reinterpret_cast<uint4*>(out + i), raw);
+        for (int k = 0; k < U; ++k) {
+            const int i = base + (k * kLogitThreads + tid) * V;
+            // the bits of tokens v0 + i .. + V: of one word, since V divides 32 and S is a multiple of 32
+            allow[k] = bits && i < nv ? __ldg(bits + ((v0 + i) >> 5)) >> ((v0 + i) & 31) : 0xFFFFFFFFu;
+            E* x = reinterpret_cast<E*>(raw + k);
+            if (vec && i + V <= nv) {
+                raw[k] = __ldcs(reinterpret_cast<const uint4*>(in + i));
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (i + j < nv) x[j] = in[i + j];
+            }
+        }
+    };
+    load(0);
+    if (nh > 0 || b1 > b0) {
+        const int clear = S / 32 * (NB + 1);  // (slices are multiples of 128)
+        for (int i = tid; i < clear / 4; i += kLogitThreads) reinterpret_cast<uint4*>(notes)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+        // warp 0: the slice's biases, in the list's order
+        if (b1 > b0 && tid < 32) {
+            int n = 0;
+            for (int i = b0 + tid; i - tid < b1; i += 32) {
+                const int t = i < b1 ? a.bias_token[i] - v0 : -1;
+                const bool mine = t >= 0 && t < nv;
+                const uint32_t who = __ballot_sync(0xffffffffu, mine);
+                const int at = n + __popc(who & ((1u << tid) - 1u));
+                if (mine) {
+                    atomicOr(biased + (t >> 5), 1u << (t & 31));
+                    if (at < kBiasList) {
+                        list_token[at] = t;
+                        list_value[at] = a.bias_value[i];
+                    }
+                }
+                n += __popc(who);
+            }
+            if (tid == 0) *listed = n;
+        }
+        if (nh > 0) {
+            const int32_t* h = a.history + (int64_t)r * a.ld_history;
+            const auto note = [&](int token, int i) {
+                const uint32_t t = (uint32_t)token - (uint32_t)v0;  // (past every slice for a negative token)
+                if (t < (uint32_t)nv) {
+                    const int shift = NB == 16 ? 16 * (int)(t & 1) : 0;
+                    uint32_t* at = notes + (NB == 16 ? t >> 1 : t);
+                    if (i < np)
+                        atomicOr(at, kInPrompt << shift);
+                    else
+                        atomicAdd(at, 1u << shift);
+                }
+            };
+            const int whole = ((uintptr_t)h & 15) == 0 ? nh & ~3 : 0;
+            constexpr int kBatch = 4;  // 16-byte loads in flight a thread
+            for (int i0 = 4 * tid; i0 < whole; i0 += 4 * kLogitThreads * kBatch) {
+                int4 t[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int i = i0 + 4 * kLogitThreads * k;
+                    t[k] = i < whole ? __ldg(reinterpret_cast<const int4*>(h + i)) : make_int4(-1, -1, -1, -1);
+                }
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const int i = i0 + 4 * kLogitThreads * k;
+                    note(t[k].x, i);
+                    note(t[k].y, i + 1);
+                    note(t[k].z, i + 2);
+                    note(t[k].w, i + 3);
+                }
+            }
+            for (int i = whole + tid; i < nh; i += kLogitThreads) note(h[i], i);
+        }
+        __syncthreads();
     }
-    for (int i = whole + tid; i < nv; i += kLogitThreads) {
-        const bool allow = !bits || (bits[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1u;
-        out[i] = from_f<E>(allow ? one(to_f(in[i]), i) : -INFINITY);
+    // the sum of token v0 + t's biases, in the list's order
+    const auto add_biases = [&](float y, int t) {
+        const int n = *listed;
+        if (n <= kBiasList) {
+            float sum = 0.f;
+            for (int i = 0; i < n; ++i)
+                if (list_token[i] == t) sum += list_value[i];
+            return y + sum;
+        }
+        float sum = 0.f;
+        for (int i = b0; i < b1; ++i)
+            if (a.bias_token[i] - v0 == t) sum += a.bias_value[i];
+        return y + sum;
+    };
+    for (int base = 0; base < nv; base += kLogitThreads * V * U) {
+        if (base) load(base);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = base + (k * kLogitThreads + tid) * V;
+            if (i >= nv) break;
+            E* x = reinterpret_cast<E*>(raw + k);
+            const uint32_t bb = b1 > b0 ? biased[i >> 5] >> (i & 31) : 0u;
+#pragma unroll
+            for (int j0 = 0; j0 < V; j0 += 4) {
+                float y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = to_f(x[j0 + j]);
+                uint32_t n[4] = {0u, 0u, 0u, 0u};
+                if (nh > 0) {
+                    if constexpr (NB == 16) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(notes + (i + j0) / 2);
+                        n[0] = w.x & 0xFFFFu, n[1] = w.x >> 16, n[2] = w.y & 0xFFFFu, n[3] = w.y >> 16;
+                    } else {
+                        const uint4 w = *reinterpret_cast<const uint4*>(notes + i + j0);
+                        n[0] = w.x, n[1] = w.y, n[2] = w.z, n[3] = w.w;
+                    }
+                }
+                if (n[0] | n[1] | n[2] | n[3] | (bb >> j0 & 15u)) {
+                    // (without branches: one token in twenty has a note, so nearly every warp comes here)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t c = n[j] & (kInPrompt - 1u);
+                        // c as f32: below 2^23 in the last bits of 2^23
+                        const float cf = NB == 16 ? __uint_as_float(0x4B000000u | c) - 8388608.f : (float)c;
+                        const float f = n[j] ? y[j] > 0.f ? per : rep : 1.f;
+                        y[j] = y[j] * f - (c ? fmaf(fr, cf, pr) : 0.f);
+                    }
+                    if (bb >> j0 & 15u)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (bb >> (j0 + j) & 1u) y[j] = add_biases(y[j], i + j0 + j);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j0 + j] = from_f<E>(allow[k] >> (j0 + j) & 1u ? y[j] : -INFINITY);
+            }
+            if (vec && i + V <= nv) {
+                __stcs(reinterpret_cast<uint4*>(out + i), raw[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (i + j < nv) out[i + j] = x[j];
+            }
+        }
     }
 }
 
@@ -176,6 +264,7 @@ extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype
         }
         if ((where.type != cudaMemoryTypeDevice && where.type != cudaMemoryTypeManaged) || !is_device_ptr(out)) return refuse("logits and out must be device memory"), -1;
         if (((uintptr_t)logits | (uintptr_t)out) % size) return refuse("logits and out must be aligned to their type"), -1;
+        if (history && ld_history < 1) return refuse("ld_history must be positive"), -1;
         if (history && !n_history) return refuse("a history needs n_history"), -1;
         if (bias_start && (!bias_token || !bias_value)) return refuse("bias_start needs bias_token and bias_value"), -1;
         if (mask && ld_mask < (vocab + 31) / 32) return refuse("ld_mask must be at least (vocab + 31) / 32"), -1;
@@ -185,19 +274,31 @@ extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype
         OnDevice on(where.device);
         if (!on.good) return refuse("cudaSetDevice failed"), -1;
         LogitArgs a{logits, out, ld, ld_out, vocab, 0, history, ld_history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask};
-        a.slice = 8192;
-        const size_t smem = (size_t)a.slice * (bias_start ? 8 : 4);
-        const dim3 grid((unsigned)((vocab + a.slice - 1) / a.slice), (unsigned)rows);
         const cudaStream_t s = static_cast<cudaStream_t>(stream);
+        int n_sm = 148;
+        cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, where.device);
+        // As many slices as leave two CTAs for each SM in one wave, none narrower than a CTA's first
+        // batch of loads (f32; 16-bit logits: half of it), none wider than the notes' place.
+        const int nb = ld_history <= 32767 ? 16 : 32, widest = kNotesBytes / 4 * 32 / nb;
+        const int64_t fill = std::max(1, kLogitCtas * n_sm / rows), least = ((int64_t)vocab + widest - 1) / widest;
+        const int64_t most = std::max<int64_t>(least, vocab / (kLogitThreads * 4 * kLogitBatch) + 1);
+        const int64_t slices = std::min(std::max(fill, least), most);
+        a.slice = (int)std::min<int64_t>((((int64_t)vocab + slices - 1) / slices + 127) / 128 * 128, widest);
         const auto launch = [&](auto kernel) {
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 65536);
+            const size_t smem = (size_t)a.slice / 8 * (size_t)(nb + 1) + 16 + kBiasList * 8;
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 98304);
             if (e != cudaSuccess) return e;
-            kernel<<<grid, kLogitThreads, smem, s>>>(a);
+            const unsigned ctas = (unsigned)(((int64_t)vocab + a.slice - 1) / a.slice);
+            kernel<<<dim3(ctas, (unsigned)rows), kLogitThreads, smem, s>>>(a);
             return cudaGetLastError();
         };
-        const cudaError_t e = dtype == AERO_CUDA_TYPE_F32   ? launch(adjust_kernel<float>)
-                              : dtype == AERO_CUDA_TYPE_F16 ? launch(adjust_kernel<__half>)
-                                                            : launch(adjust_kernel<__nv_bfloat16>);
+        const auto typed = [&](auto zero) {
+            using E = decltype(zero);
+            return nb == 16 ? launch(adjust_kernel<E, 16>) : launch(adjust_kernel<E, 32>);
+        };
+        const cudaError_t e = dtype == AERO_CUDA_TYPE_F32   ? typed(float{})
+                              : dtype == AERO_CUDA_TYPE_F16 ? typed(__half{})
+                                                            : typed(__nv_bfloat16{});
         if (e != cudaSuccess) {
             cudaGetLastError();
             set_free_error(std::string("logits_adjust: ") + cudaGetErrorString(e));

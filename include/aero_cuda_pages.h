@@ -114,7 +114,7 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
 
 /* Adjusts `rows` rows of `vocab` logits (type dtype, row stride ld elements) into out
  * (same type, row stride ld_out; may be logits itself), on `stream`. Per row r, with
- * its history's first n_history[r] token ids (row stride ld_history) of which the
+ * its history's first n_history[r] token ids (row stride ld_history; at most ld_history count) of which the
  * first n_prompt[r] are the prompt:
  *   x = a token of the history? (x > 0 ? x / repetition[r] : x * repetition[r]) : x
  *   x -= frequency[r] * c + presence[r], c > 0 times in the history after the prompt
