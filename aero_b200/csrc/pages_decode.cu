@@ -85,8 +85,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     float2* joint = ml + 64;                                                     // [16]
     uint64_t* bars = reinterpret_cast<uint64_t*>(joint + 16);                    // full[ST], empty[ST]
     int64_t* begin_s = reinterpret_cast<int64_t*>(bars + 2 * ST);                // entry base, total
-    int* misc = reinterpret_cast<int*>(begin_s + 2);                             // entry, abort, last
-    Span* span_s = reinterpret_cast<Span*>(misc + 4);                            // the first entry's
+    int4* joins = reinterpret_cast<int4*>(begin_s + 2);                          // [2]: parts to join (or 0), first CTA, token, head
+    int* misc = reinterpret_cast<int*>(joins + 2);                               // entry, abort
+    Span* span_s = reinterpret_cast<Span*>(misc + 2);                            // the first entry's
     volatile int* abort_flag = misc + 1;
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int HK = a.c.HK, G = a.H / HK;
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                         want = false;
                     }
                 }
-                if (!wait_phase(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
+                if (!warp_wait(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
                     good = false;
                     break;
                 }
@@ -228,6 +229,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     // and of the V fragments (keys (bit 3) * 8 + lane % 8, 8 columns by lane / 16)
     const int krow = warp * 16 + (lane >> 4) * 8 + (lane & 7), kcol = (lane >> 3) & 1;
     const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), vcol = lane >> 4;
+    constexpr int64_t slot = 16 * (D + 2);  // floats of a partial result
+    if (tid < 2) joins[tid] = make_int4(0, 0, 0, 0);  // (read after later barriers)
+    const auto out_of = [&](int tok, int h) {
+        return static_cast<uint16_t*>(a.out) + (int64_t)tok * a.o_token + (int64_t)(h * G) * a.o_head;
+    };
+    const auto put = [&](uint16_t* to, int row, int d, float4 v) {
+        uint16_t* y = to + (int64_t)row * a.o_head + d;
+        const uint32_t w0 = pack16<BF16>(v.x, v.y), w1 = pack16<BF16>(v.z, v.w);
+        if (a.vec) {
+            *reinterpret_cast<uint2*>(y) = make_uint2(w0, w1);
+        } else {
+            y[0] = (uint16_t)w0;
+            y[1] = (uint16_t)(w0 >> 16);
+            y[2] = (uint16_t)w1;
+            y[3] = (uint16_t)(w1 >> 16);
+        }
+    };
+    const auto summed = [&](int row, int d) {
+        const int col = d ^ ((row & 3) * 8);
+        const float4 x = *reinterpret_cast<const float4*>(red + row * D + col),
+                     y = *reinterpret_cast<const float4*>(red + (16 + row) * D + col);
+        return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+    };
     for (int64_t u = u0; u < u1;) {
         const int64_t in = u - base;
         const int h = (int)(in / sp.tiles), t0 = (int)(in % sp.tiles);
@@ -254,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         for (int t = t0; t < t0 + cnt; ++t) {
             // a warp whose wait gave up goes on without waiting (its results are void, the status
             // says so): the other warps still meet it at the barriers below
-            if (!dead && !wait_phase(smem_u32(bars + stage), phase, abort_flag)) {
+            if (!dead && !warp_wait(smem_u32(bars + stage), phase, abort_flag)) {
                 dead = true;
                 *abort_flag = 1;
                 if (lane == 0) pages_flag(a.c, AERO_CUDA_PAGES_WAIT);
@@ -274,26 +298,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] += so[i >> 2][i & 3];
             // positions that the token does not see: their scores are -inf and their V rows
             // are taken as zero, whatever their memory holds
-            const int j = tile_at(sp, t) * kUnit + warp * 16 + 2 * tq;
-            const bool s00 = visible(sp, j), s01 = visible(sp, j + 1), s10 = visible(sp, j + 8), s11 = visible(sp, j + 9);
-            const uint32_t keep0 = (s00 ? 0x0000FFFFu : 0u) | (s01 ? 0xFFFF0000u : 0u);
-            const uint32_t keep1 = (s10 ? 0x0000FFFFu : 0u) | (s11 ? 0xFFFF0000u : 0u);
+            const int j0 = tile_at(sp, t) * kUnit;
+            uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
             const float sc = a.scale_log2;
-            s[0][0] = s00 ? s[0][0] * sc : -INFINITY;
-            s[0][1] = s01 ? s[0][1] * sc : -INFINITY;
-            s[0][2] = s00 ? s[0][2] * sc : -INFINITY;
-            s[0][3] = s01 ? s[0][3] * sc : -INFINITY;
-            s[1][0] = s10 ? s[1][0] * sc : -INFINITY;
-            s[1][1] = s11 ? s[1][1] * sc : -INFINITY;
-            s[1][2] = s10 ? s[1][2] * sc : -INFINITY;
-            s[1][3] = s11 ? s[1][3] * sc : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] *= sc;
+            if (j0 + kUnit > sp.n || (j0 < sp.lo && j0 + kUnit > sp.sinks)) {
+                const int j = j0 + warp * 16 + 2 * tq;
+                const bool s00 = visible(sp, j), s01 = visible(sp, j + 1), s10 = visible(sp, j + 8), s11 = visible(sp, j + 9);
+                keep0 = (s00 ? 0x0000FFFFu : 0u) | (s01 ? 0xFFFF0000u : 0u);
+                keep1 = (s10 ? 0x0000FFFFu : 0u) | (s11 ? 0xFFFF0000u : 0u);
+                if (!s00) s[0][0] = s[0][2] = -INFINITY;
+                if (!s01) s[0][1] = s[0][3] = -INFINITY;
+                if (!s10) s[1][0] = s[1][2] = -INFINITY;
+                if (!s11) s[1][1] = s[1][3] = -INFINITY;
+            }
             float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
             float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+            // o and l are rescaled only when a maximum has grown by more than 2^8 since they were last:
+            // weights of up to 2^8 are as exact as any in f16, bf16 and the f32 sums
+            if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f)) {
                 const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
                 // (a row without a visible position stays at -inf; its sums are zero)
                 const float f0 = n0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 0.f : ex2(m1 - n1);
@@ -395,105 +423,90 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        const int64_t seg0 = base + (int64_t)h * sp.tiles;  // the (sequence, head)'s units: [seg0, seg0 + tiles)
-        uint16_t* out = static_cast<uint16_t*>(a.out) + (int64_t)e * a.o_token + (int64_t)(h * G) * a.o_head;
-        const auto put = [&](int row, int d, float4 v) {
-            uint16_t* y = out + (int64_t)row * a.o_head + d;
-            const uint32_t w0 = pack16<BF16>(v.x, v.y), w1 = pack16<BF16>(v.z, v.w);
-            if (a.vec) {
-                *reinterpret_cast<uint2*>(y) = make_uint2(w0, w1);
-            } else {
-                y[0] = (uint16_t)w0;
-                y[1] = (uint16_t)(w0 >> 16);
-                y[2] = (uint16_t)w1;
-                y[3] = (uint16_t)(w1 >> 16);
-            }
-        };
-        const auto summed = [&](int row, int d) {
-            const int col = d ^ ((row & 3) * 8);
-            const float4 x = *reinterpret_cast<const float4*>(red + row * D + col),
-                         y = *reinterpret_cast<const float4*>(red + (16 + row) * D + col);
-            return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-        };
         if (cnt == sp.tiles) {
             for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4;
-                const float inv = joint[row].y > 0.f ? 1.f / joint[row].y : 0.f;
+                const float L = joint[row].y, k = L > 0.f ? 1.f / L : L == L ? 0.f : L;  // a sum that is no number stays none
                 const float4 v = summed(row, d);
-                // a sum that is not a number stays one
-                const float k = joint[row].y == joint[row].y ? inv : joint[row].y;
-                put(row, d, make_float4(v.x * k, v.y * k, v.z * k, v.w * k));
+                put(out_of(e, h), row, d, make_float4(v.x * k, v.y * k, v.z * k, v.w * k));
             }
         } else {
             // partial results: slot 1 of the CTA where the (sequence, head) begins, slot 0 of the others
-            constexpr int64_t slot = 16 * (D + 2);
-            float* mine = a.part + ((int64_t)blockIdx.x * 2 + (t0 == 0)) * slot;
+            const int which = t0 == 0;
+            float* mine = a.part + ((int64_t)blockIdx.x * 2 + which) * slot;
             for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
                 const int row = i / (D / 4), d = i % (D / 4) * 4;
                 *reinterpret_cast<float4*>(mine + row * D + d) = summed(row, d);
             }
             if (tid < G) *reinterpret_cast<float2*>(mine + 16 * D + 2 * tid) = joint[tid];
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            const int64_t seg0 = base + (int64_t)h * sp.tiles;  // its units: [seg0, seg0 + tiles)
             const int64_t c0 = seg0 / w;
             const int parts = (int)((seg0 + sp.tiles - 1) / w - c0) + 1;
+            asm volatile("bar.sync 1, 128;" ::: "memory");
             if (tid == 0) {
                 __threadfence();  // the CTA's stores, ordered before by the barrier
-                const uint32_t was = atomicAdd(a.counters + c0, 1u);
-                misc[2] = was == (uint32_t)(parts - 1);
-                if (misc[2]) a.counters[c0] = 0;  // for the next launch
-                __threadfence();
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (misc[2]) {
-                // part c of the line: the first one's slot is 1, the others' 0
-                const float* first = a.part + (c0 * 2 + 1) * slot;
-                const float* rest = a.part + (c0 * 2) * slot;
-                const auto part_at = [&](int c) { return c == 0 ? first : rest + (int64_t)c * 2 * slot; };
-                // four columns of a row a thread; the loads of kBatch parts are in flight at once
-                // (an L2 round trip each batch is what this costs)
-                constexpr int kBatch = 16;
-                for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
-                    const int row = i / (D / 4), d = i % (D / 4) * 4;
-                    float M = -INFINITY, L = 0.f;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int b0 = 0; b0 < parts; b0 += kBatch) {
-                        float2 x[kBatch];
-                        float4 v[kBatch];
-#pragma unroll
-                        for (int k = 0; k < kBatch; ++k) {
-                            const float* p = part_at(min(b0 + k, parts - 1));
-                            x[k] = __ldcg(reinterpret_cast<const float2*>(p + 16 * D + 2 * row));
-                            v[k] = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
-                        }
-                        float N = M;
-#pragma unroll
-                        for (int k = 0; k < kBatch; ++k) {
-                            if (b0 + k >= parts) x[k] = make_float2(-INFINITY, 0.f);
-                            N = fmaxf(N, x[k].x);
-                        }
-                        const float z = N == -INFINITY ? 0.f : N, f = ex2(M - z);
-                        M = N;
-                        L *= f;
-                        acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-#pragma unroll
-                        for (int k = 0; k < kBatch; ++k) {  // (past the last part: its values again, weight 0)
-                            const float y = ex2(x[k].x - z);
-                            L = fmaf(x[k].y, y, L);
-                            acc.x = fmaf(v[k].x, y, acc.x);
-                            acc.y = fmaf(v[k].y, y, acc.y);
-                            acc.z = fmaf(v[k].z, y, acc.z);
-                            acc.w = fmaf(v[k].w, y, acc.w);
-                        }
-                    }
-                    const float k = L > 0.f ? 1.f / L : L == L ? 0.f : L;
-                    put(row, d, make_float4(acc.x * k, acc.y * k, acc.z * k, acc.w * k));
-                }
+                const bool last = atomicAdd(a.counters + c0, 1u) == (uint32_t)(parts - 1);
+                if (last) a.counters[c0] = 0;  // for the next launch
+                joins[which] = make_int4(last ? parts : 0, (int)c0, e, h);
             }
         }
         u += cnt;
         if (u == base + (int64_t)sp.tiles * HK && u < u1) {
             base = u;
             sp = span_of(a, ++e);
+        }
+    }
+    // ---- joins of the (at most two) shared (sequence, head)s whose last part this CTA wrote; here,
+    // so that neither the arrivals nor the joins hold up the units
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    __threadfence();
+    for (int which = 0; which < 2; ++which) {
+        const int parts = joins[which].x;
+        if (!parts) continue;
+        const int64_t c0 = joins[which].y;
+        uint16_t* to = out_of(joins[which].z, joins[which].w);
+        // part c of the line: the first one's slot is 1, the others' 0
+        const float* first = a.part + (c0 * 2 + 1) * slot;
+        const float* rest = a.part + (c0 * 2) * slot;
+        const auto part_at = [&](int c) { return c == 0 ? first : rest + (int64_t)c * 2 * slot; };
+        // four columns of a row a thread; the loads of kBatch parts are in flight at once
+        // (an L2 round trip each batch is what this costs)
+        constexpr int kBatch = 16;
+        for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
+            const int row = i / (D / 4), d = i % (D / 4) * 4;
+            float M = -INFINITY, L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int b0 = 0; b0 < parts; b0 += kBatch) {
+                float2 x[kBatch];
+                float4 v[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    const float* p = part_at(min(b0 + k, parts - 1));
+                    x[k] = __ldcg(reinterpret_cast<const float2*>(p + 16 * D + 2 * row));
+                    v[k] = __ldcg(reinterpret_cast<const float4*>(p + row * D + d));
+                }
+                float N = M;
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {
+                    if (b0 + k >= parts) x[k] = make_float2(-INFINITY, 0.f);
+                    N = fmaxf(N, x[k].x);
+                }
+                const float z = N == -INFINITY ? 0.f : N, f = ex2(M - z);
+                M = N;
+                L *= f;
+                acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) {  // (past the last part: its values again, weight 0)
+                    const float y = ex2(x[k].x - z);
+                    L = fmaf(x[k].y, y, L);
+                    acc.x = fmaf(v[k].x, y, acc.x);
+                    acc.y = fmaf(v[k].y, y, acc.y);
+                    acc.z = fmaf(v[k].z, y, acc.z);
+                    acc.w = fmaf(v[k].w, y, acc.w);
+                }
+            }
+            const float k = L > 0.f ? 1.f / L : L == L ? 0.f : L;
+            put(to, row, d, make_float4(acc.x * k, acc.y * k, acc.z * k, acc.w * k));
         }
     }
 }

@@ -49,17 +49,26 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Bounded wait for a phase of an mbarrier without reading a timer between its tries (one read
-// of the global timer costs more than most of these waits last). A try may suspend the
-// thread for a time that the hardware sets; after kWaitTries of them, each some 20 cycles at
-// least (half a second or more), or when another warp has given up, it returns false.
-constexpr int kWaitTries = 1 << 26;
-__device__ __forceinline__ bool wait_phase(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-    for (int i = 0; i < kWaitTries; ++i) {
-        if (mbar_try(bar, parity)) return true;
-        if ((i & 63) == 63 && *abort_flag) return false;
+// Bounded wait of a whole warp for a phase of an mbarrier: true in every lane, or false in every
+// lane after kWaitNs or when another warp has given up. Lanes may leave the polling at different
+// tries; the vote brings them together again, as the .aligned instructions that follow need.
+// The global timer is read now and then only (a read costs more than most of these waits last).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    bool ok = mbar_try(bar, parity);
+    if (!ok) {
+        uint64_t t0 = 0;
+        for (int i = 1;; ++i) {
+            ok = mbar_try(bar, parity);
+            if (ok) break;
+            if ((i & 63) == 0) {
+                if (*abort_flag) break;
+                const uint64_t now = gtimer();
+                if (t0 == 0) t0 = now;
+                if (now - t0 > kWaitNs) break;
+            }
+        }
     }
-    return false;
+    return __all_sync(0xffffffffu, ok);
 }
 
 // 2^x, the hardware's approximation (relative error about 2^-22; 2^-inf = 0).

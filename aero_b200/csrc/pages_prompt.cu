@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             row[SA] = find(i + SA);
             const int st = i % ST;
             // the stage's last use; of the places of the first tiles' K, that use
-            if (i >= ST) good = good && wait_phase(bar(E + st), (uint32_t)(i / ST - 1) & 1u, abort_flag);
-            if (i + SA < nt && i < ST && i >= ST - SA) good = good && wait_phase(bar(KU + i - (ST - SA)), 0, abort_flag);
+            if (i >= ST) good = good && warp_wait(bar(E + st), (uint32_t)(i / ST - 1) & 1u, abort_flag);
+            if (i + SA < nt && i < ST && i >= ST - SA) good = good && warp_wait(bar(KU + i - (ST - SA)), 0, abort_flag);
             if (!good) break;
             expect(count(row[0]) + count(row[SA]), F + st);
             load(vmap, v_s + st * C::kv_bytes, row[0], F + st);
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         bool good = true;
         for (int i = 0; i < nt && good; ++i) {
             const int j0 = tile_pos<BN>(w, ta + i);
-            good = wait_phase(bar(F + i % ST), (uint32_t)(i / ST) & 1u, abort_flag);
+            good = warp_wait(bar(F + i % ST), (uint32_t)(i / ST) & 1u, abort_flag);
             if (good && !all_see(j0, w.p0, w.p1)) {
                 uint8_t* vt = v_gen + (i % ST) * C::kv_bytes;
                 for (int r = lane; r < BN; r += 32) {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         const uint32_t iqk = idesc16<BF16>(BN, false), ipv = idesc16<BF16>(D, true);
         bool good = true;
         const auto wait = [&](int b, int nth) {  // the nth completion (from 0) of barrier b
-            if (good && !wait_phase(bar(b), (uint32_t)nth & 1u, abort_flag)) {
+            if (good && !warp_wait(bar(b), (uint32_t)nth & 1u, abort_flag)) {
                 good = false;
                 if (leads) give_up();
             }
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         for (int i = 0; i < nt && good; ++i) {
             const int buf = buffer(q, i);
             const int j0 = tile_pos<BN>(w, ta + i);
-            if (!wait_phase(bar(SF + buf), (uint32_t)uses(i) & 1u, abort_flag)) {
+            if (!warp_wait(bar(SF + buf), (uint32_t)uses(i) & 1u, abort_flag)) {
                 good = false;
                 break;
             }
@@ -578,9 +578,12 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                 for (int e = 0; e < 32; e += 2)
                     x[(e >> 1) & 3] = max3(x[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
             const float mt = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3])) * sc;
-            // P V of the tile before has ended: O may be rescaled and P written
-            if (C::shared_s && i > 0) {
-                if (!wait_phase(bar(OD + q), (uint32_t)(i - 1) & 1u, abort_flag)) {
+            // P V of the tile before has ended: O may be rescaled and, where P has a place of its own,
+            // P written. With two S buffers O's barrier counts the last two tiles alone, and the
+            // first of them is waited for here, before this tile's P lets the second complete: a
+            // wait that came after both would take its phase for one still to come.
+            if (C::shared_s ? i > 0 : i > 0 && i == nt - 1) {
+                if (!warp_wait(bar(OD + q), C::shared_s ? (uint32_t)(i - 1) & 1u : 0u, abort_flag)) {
                     good = false;
                     break;
                 }
@@ -593,10 +596,9 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                 const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
                 l *= f;
-                if constexpr (!C::shared_s) {
+                if (!C::shared_s && i + 1 < nt) {
                     // P V of the tile before has ended when S of the next tile, issued after it, is there
-                    if (!(i + 1 < nt ? wait_phase(bar(SF + (buf ^ 1)), (uint32_t)uses(i + 1) & 1u, abort_flag)
-                                     : wait_phase(bar(OD + q), 0, abort_flag))) {
+                    if (!warp_wait(bar(SF + (buf ^ 1)), (uint32_t)uses(i + 1) & 1u, abort_flag)) {
                         good = false;
                         break;
                     }
@@ -649,8 +651,8 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             unpair(add2(sum[0], sum[1]), l0, l1);
             l += l0 + l1;
         }
-        for (int i = max(nt - SA, 0); i < nt; ++i)  // one by one: a wait tells neighbouring phases apart only
-            if (good && !wait_phase(bar(OD + q), (uint32_t)(C::shared_s ? i : i - max(nt - SA, 0)) & 1u, abort_flag)) good = false;
+        if (good && nt > 0)  // the last addition to O
+            good = warp_wait(bar(OD + q), C::shared_s ? (uint32_t)(nt - 1) & 1u : (uint32_t)(nt > 1), abort_flag);
         tc_fence_after();
         if (!good) give_up();
         const bool stores = row < w.rows;
@@ -712,8 +714,8 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                         put_row(d0, o, inverse(sum));
                 },
                 [&](float slow_m, float slow_l) { m = slow_m, l = slow_l; });
+        __syncwarp();
         if (parts == 1) {
-            __syncwarp();
             const int64_t to = stores ? (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head : -1;
 #pragma unroll 2
             for (int x0 = 0; x0 < kPieces; ++x0) {

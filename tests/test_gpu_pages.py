@@ -281,6 +281,21 @@ def test_keys_that_are_no_numbers(dtype, bad):
     c.check()
 
 
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+def test_prompt_repeats_with_growing_maxima(D):
+    """Rows whose maxima grow from tile to tile (O rescaled often), again and again: the same
+    result, and no device wait that gives up."""
+    for T, n in ((303, 303), (40, 900), (64, 100), (130, 129 + 130)):
+        c, K, V = open_cache([n], 64, 1, D, F16)
+        c.k().mul_(torch.linspace(0.1, 6, c.n_page * 64, device="cuda").reshape(1, -1, 1, 64, 1).half())
+        q = (3 * torch.randn((T, 4, D), device="cuda")).half()
+        first = c.attend(0, q, i32([0]), i32([0, T]))
+        for _ in range(40):
+            again = c.attend(0, q, i32([0]), i32([0, T]))
+        c.check()
+        assert torch.equal(again, first) and torch.isfinite(first).all()
+
+
 def test_prompt_strides_and_bad_rows():
     c, K, V = open_cache([150, 60], 16, 2, 64, BF16)
     wide = torch.randn((101, 9, 67), device="cuda").to(BF16)
