@@ -84,6 +84,7 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
     E* out = static_cast<E*>(a.out) + (int64_t)r * a.ld_out + v0;
     const bool vec = (((uintptr_t)in | (uintptr_t)out) & 15) == 0;
     const uint32_t* bits = a.mask ? reinterpret_cast<const uint32_t*>(a.mask) + (int64_t)r * a.ld_mask : nullptr;
+    stream_turn();
     const int nh = a.history ? (int)min((int64_t)max(0, a.n_history[r]), a.ld_history) : 0;
     const int np = nh && a.n_prompt ? a.n_prompt[r] : 0;
     const int b0 = a.bias_start ? a.bias_start[r] : 0, b1 = a.bias_start ? a.bias_start[r + 1] : 0;
@@ -289,8 +290,7 @@ extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype
             cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 98304);
             if (e != cudaSuccess) return e;
             const unsigned ctas = (unsigned)(((int64_t)vocab + a.slice - 1) / a.slice);
-            kernel<<<dim3(ctas, (unsigned)rows), kLogitThreads, smem, s>>>(a);
-            return cudaGetLastError();
+            return launch_in_turn(kernel, dim3(ctas, (unsigned)rows), kLogitThreads, smem, s, a);
         };
         const auto typed = [&](auto zero) {
             using E = decltype(zero);

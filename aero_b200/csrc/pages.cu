@@ -108,6 +108,7 @@ __device__ bool lowest_free(const PageView& c, int want, int32_t* list) {
 
 __global__ void set_tables_kernel(PageView c, const int32_t* __restrict__ table, const int32_t* __restrict__ length,
                                   const int32_t* __restrict__ refs) {
+    stream_turn();
     const int64_t nt = (int64_t)c.n_seq * c.max_pages, all = nt + c.n_seq + c.n_page;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
         if (i < nt)
@@ -157,6 +158,7 @@ __device__ int place_needs(int n, int n_page, int32_t* first, F need) {
 
 __global__ void __launch_bounds__(kBooksThreads) extend_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs,
                                                                const int32_t* __restrict__ counts, int n) {
+    stream_turn();
     const int P = 1 << c.page_shift;
     if (!distinct_seqs(c, seqs, n, w.mark)) {
         if (threadIdx.x == 0) pages_flag(c, AERO_CUDA_PAGES_BAD_SEQ);
@@ -193,6 +195,7 @@ __global__ void __launch_bounds__(kBooksThreads) extend_kernel(PageView c, Books
 __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWork w,
                                                              const int32_t* __restrict__ parents,
                                                              const int32_t* __restrict__ children, int n) {
+    stream_turn();
     const int P = 1 << c.page_shift;
     if (threadIdx.x == 0) *w.n_jobs = 0;
     bool bad = false;
@@ -252,6 +255,7 @@ __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWo
 // A CTA per listed sequence. The exchange of the length hands the sequence's pages to
 // one CTA even when the list names it twice.
 __global__ void __launch_bounds__(256) free_kernel(PageView c, const int32_t* __restrict__ seqs, int n) {
+    stream_turn();
     __shared__ int held;
     const int P = 1 << c.page_shift;
     const int s = seqs[blockIdx.x];
@@ -281,6 +285,7 @@ __global__ void __launch_bounds__(256) free_kernel(PageView c, const int32_t* __
 // below L takes the i-th live page at or above L (there are equally many). Sources lie
 // at or above L and targets below, so the moves do not touch one another.
 __global__ void __launch_bounds__(kBooksThreads) compact_kernel(PageView c, BooksWork w) {
+    stream_turn();
     int live = 0;
     for (int base = 0; base < c.n_page; base += 4 * (int)blockDim.x) {
         const int p0 = base + 4 * (int)threadIdx.x;
@@ -334,6 +339,7 @@ __global__ void __launch_bounds__(kBooksThreads) compact_kernel(PageView c, Book
 
 __global__ void copy_jobs_kernel(PageView c, BooksWork w, const int32_t* __restrict__ src,
                                  const int32_t* __restrict__ dst, int n) {
+    stream_turn();
     const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
     if (i == 0) *w.n_jobs = n;
     if (i >= n) return;
@@ -353,6 +359,7 @@ constexpr int kMoveUnit = 256 * kMoveVec;
 // from n_live on follow their pages.
 __global__ void __launch_bounds__(256) move_kernel(PageView c, BooksWork w, uint4* __restrict__ k, uint4* __restrict__ v,
                                                    int retable) {
+    stream_turn();
     const int P = 1 << c.page_shift, row_vec = c.D / 8;
     const int page_vec = c.HK * P * row_vec;
     const int pieces = (page_vec + kMoveUnit - 1) / kMoveUnit;
@@ -396,6 +403,7 @@ __global__ void __launch_bounds__(256) append_kernel(PageView c, int layer, cons
                                                      int64_t v_head, const int32_t* __restrict__ seqs,
                                                      const int32_t* __restrict__ positions, int T, E* __restrict__ kp,
                                                      E* __restrict__ vp) {
+    stream_turn();
     // E counts in pieces of the row: strides and D come in those
     constexpr int PER = sizeof(E) / 2;
     const int rowp = c.D / PER;
@@ -625,8 +633,8 @@ cudaError_t launch_move(Pages& g, int64_t max_jobs, int retable) {
     const int64_t units = max_jobs * c.n_layer * 2 * ((page_vec + kMoveUnit - 1) / kMoveUnit);
     const int64_t books = retable ? ((int64_t)c.n_seq * c.max_pages + 255) / 256 : 0;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::max(units, books), (int64_t)g.n_sm * 8));
-    move_kernel<<<grid, 256, 0, g.stream>>>(c, g.work, static_cast<uint4*>(g.k), static_cast<uint4*>(g.v), retable);
-    return cudaGetLastError();
+    return launch_in_turn(move_kernel, grid, 256, 0, g.stream, c, g.work, static_cast<uint4*>(g.k), static_cast<uint4*>(g.v),
+                          retable);
 }
 
 bool layer_ok(Pages& g, int layer) {
@@ -725,8 +733,7 @@ int aero_cuda_pages_set_tables(void* cache, const int32_t* table, const int32_t*
             return false;
         const int64_t all = (int64_t)g.d.n_seq * g.d.max_pages + g.d.n_seq + g.d.n_page;
         const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, (int64_t)g.n_sm * 8);
-        aero::set_tables_kernel<<<grid, 256, 0, g.stream>>>(g.view, table, length, refs);
-        return g.ok(cudaGetLastError(), "set_tables");
+        return g.ok(aero::launch_in_turn(aero::set_tables_kernel, grid, 256, 0, g.stream, g.view, table, length, refs), "set_tables");
     });
 }
 
@@ -735,8 +742,8 @@ int aero_cuda_pages_extend(void* cache, const int32_t* seqs, const int32_t* coun
         if (!aero::listed(g, seqs, "seqs", counts, "counts", n)) return false;
         if (n > 0 && !counts) return g.fail("counts is required");
         if (n == 0) return true;
-        aero::extend_kernel<<<1, aero::kBooksThreads, 0, g.stream>>>(g.view, g.work, seqs, counts, n);
-        return g.ok(cudaGetLastError(), "extend");
+        return g.ok(aero::launch_in_turn(aero::extend_kernel, 1, aero::kBooksThreads, 0, g.stream, g.view, g.work, seqs, counts, n),
+                    "extend");
     });
 }
 
@@ -753,15 +760,13 @@ int aero_cuda_pages_append(void* cache, int layer, const void* k, int64_t k_toke
         const int per = vec ? 8 : 1;
         const int64_t all = (int64_t)T * g.d.n_head_kv * (g.d.head_dim / per);
         const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, (int64_t)g.n_sm * 16);
-        if (vec)
-            aero::append_kernel<uint4><<<grid, 256, 0, g.stream>>>(
-                g.view, layer, static_cast<const uint4*>(k), k_token / 8, k_head / 8, static_cast<const uint4*>(v),
-                v_token / 8, v_head / 8, seqs, positions, T, static_cast<uint4*>(g.k), static_cast<uint4*>(g.v));
-        else
-            aero::append_kernel<uint16_t><<<grid, 256, 0, g.stream>>>(
-                g.view, layer, static_cast<const uint16_t*>(k), k_token, k_head, static_cast<const uint16_t*>(v),
-                v_token, v_head, seqs, positions, T, static_cast<uint16_t*>(g.k), static_cast<uint16_t*>(g.v));
-        return g.ok(cudaGetLastError(), "append");
+        const auto launch = [&](auto piece) {
+            using E = decltype(piece);
+            return aero::launch_in_turn(aero::append_kernel<E>, grid, 256, 0, g.stream, g.view, layer, static_cast<const E*>(k),
+                                        k_token / per, k_head / per, static_cast<const E*>(v), v_token / per, v_head / per,
+                                        seqs, positions, T, static_cast<E*>(g.k), static_cast<E*>(g.v));
+        };
+        return g.ok(vec ? launch(uint4{}) : launch(uint16_t{}), "append");
     });
 }
 
@@ -770,8 +775,9 @@ int aero_cuda_pages_fork(void* cache, const int32_t* parents, const int32_t* chi
         if (!aero::listed(g, parents, "parents", children, "children", n)) return false;
         if (n > 0 && !children) return g.fail("children is required");
         if (n == 0) return true;
-        aero::fork_kernel<<<1, aero::kBooksThreads, 0, g.stream>>>(g.view, g.work, parents, children, n);
-        return g.ok(cudaGetLastError(), "fork") && g.ok(aero::launch_move(g, n, 0), "fork");
+        return g.ok(aero::launch_in_turn(aero::fork_kernel, 1, aero::kBooksThreads, 0, g.stream, g.view, g.work, parents, children, n),
+                    "fork") &&
+               g.ok(aero::launch_move(g, n, 0), "fork");
     });
 }
 
@@ -779,8 +785,7 @@ int aero_cuda_pages_free(void* cache, const int32_t* seqs, int n) {
     return aero::entry(cache, [&](Pages& g) {
         if (!aero::listed(g, seqs, "seqs", nullptr, "", n)) return false;
         if (n == 0) return true;
-        aero::free_kernel<<<(unsigned)n, 256, 0, g.stream>>>(g.view, seqs, n);
-        return g.ok(cudaGetLastError(), "free");
+        return g.ok(aero::launch_in_turn(aero::free_kernel, (unsigned)n, 256, 0, g.stream, g.view, seqs, n), "free");
     });
 }
 
@@ -789,15 +794,16 @@ int aero_cuda_pages_copy(void* cache, const int32_t* src, const int32_t* dst, in
         if (n < 0 || n > g.d.n_page) return g.fail("n must be from 0 to n_page = %d, got %d", g.d.n_page, n);
         if (n == 0) return true;
         if (!aero::device_i32(g, src, "src") || !aero::device_i32(g, dst, "dst")) return false;
-        aero::copy_jobs_kernel<<<(unsigned)(n + 255) / 256, 256, 0, g.stream>>>(g.view, g.work, src, dst, n);
-        return g.ok(cudaGetLastError(), "copy") && g.ok(aero::launch_move(g, n, 0), "copy");
+        return g.ok(aero::launch_in_turn(aero::copy_jobs_kernel, (unsigned)(n + 255) / 256, 256, 0, g.stream, g.view, g.work, src, dst, n),
+                    "copy") &&
+               g.ok(aero::launch_move(g, n, 0), "copy");
     });
 }
 
 int aero_cuda_pages_compact(void* cache) {
     return aero::entry(cache, [&](Pages& g) {
-        aero::compact_kernel<<<1, aero::kBooksThreads, 0, g.stream>>>(g.view, g.work);
-        return g.ok(cudaGetLastError(), "compact") && g.ok(aero::launch_move(g, (g.d.n_page + 1) / 2, 1), "compact");
+        return g.ok(aero::launch_in_turn(aero::compact_kernel, 1, aero::kBooksThreads, 0, g.stream, g.view, g.work), "compact") &&
+               g.ok(aero::launch_move(g, (g.d.n_page + 1) / 2, 1), "compact");
     });
 }
 

@@ -25,6 +25,23 @@ struct OnDevice {
     }
 };
 
+// Launches a kernel that begins while the one before it in the stream ends: such a kernel calls
+// stream_turn() before it touches any memory that another kernel may have written or reads.
+template <typename... P, typename... A>
+cudaError_t launch_in_turn(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A&&... args) {
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = grid;
+    c.blockDim = block;
+    c.dynamicSmemBytes = smem;
+    c.stream = s;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);
+}
+
 // The cache as kernels see it.
 struct PageView {
     int32_t* table;   // (n_seq, max_pages)
@@ -35,6 +52,12 @@ struct PageView {
 };
 
 #if defined(__CUDACC__)
+// The next kernel of the stream may be brought up from here on; this one's turn comes when all
+// before it have ended and what they wrote is visible.
+__device__ __forceinline__ void stream_turn() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 __device__ __forceinline__ void pages_flag(const PageView& c, int code) { atomicCAS(c.status, 0, code); }
 // Length of sequence s as kernels may use it: 0 for a number outside the table,
 // never past what its row of the table can hold.

@@ -93,6 +93,15 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     const int HK = a.c.HK, G = a.H / HK;
     const uint32_t ring = smem_u32(sm);
 
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(smem_u32(bars + i), 1);
+            mbar_init(smem_u32(bars + ST + i), kConsumers);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *abort_flag = 0;
+    }
+    stream_turn();
     if (blockIdx.x == 0 && a.q_start) check_q_start(a);
     // ---- this CTA's piece of the line of units
     {
@@ -108,14 +117,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             if (lane >= o) incl += y;
         }
         if (lane == 31) sums[warp] = incl;
-        if (tid == 0) {
-            for (int i = 0; i < ST; ++i) {
-                mbar_init(smem_u32(bars + i), 1);
-                mbar_init(smem_u32(bars + ST + i), kConsumers);
-            }
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            *abort_flag = 0;
-        }
         __syncthreads();
         int64_t before = incl - mine, total = 0;
         for (int i = 0; i < kThreads / 32; ++i) {
@@ -526,8 +527,7 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorM
     const int64_t cap = ((int64_t)a.c.max_pages << a.c.page_shift) / kUnit + 2;
     const int64_t units = (int64_t)a.T * a.c.HK * cap;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((int64_t)n_sm * Cfg<D>::ctas, (units + kMinUnits - 1) / kMinUnits));
-    decode_attend_kernel<D, BF16><<<grid, kThreads, Cfg<D>::smem, s>>>(a, kmap, vmap);
-    return cudaGetLastError();
+    return launch_in_turn(decode_attend_kernel<D, BF16>, grid, kThreads, Cfg<D>::smem, s, a, kmap, vmap);
 }
 
 }  // namespace

@@ -275,6 +275,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     const int h = (int)blockIdx.x % HK;
     const int slot = n_slot - 1 - (int)blockIdx.x / HK;  // the longest rows first
 
+    stream_turn();
     if (blockIdx.x == 0 && blockIdx.y == 0) check_q_start(a);
     Work w;
     if (!find_work<D>(a, slot, w)) return;
@@ -833,9 +834,8 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorM
     // slots without rows end at once, so they are not counted, up to the workspace's size
     const int64_t busy = std::max<int64_t>(a.n, ((int64_t)a.T * G + C::rows - 1) / C::rows) * a.c.HK;
     const int splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(n_sm / busy, pages_prompt_max_grid(n_sm) / ctas), 64));
-    prompt_attend_kernel<D, BF16><<<dim3((unsigned)ctas, (unsigned)splits), C::threads, C::smem, s>>>(
-        a, kmap, vmap, static_cast<const uint16_t*>(kp), static_cast<const uint16_t*>(vp), n_slot, splits);
-    return cudaGetLastError();
+    return launch_in_turn(prompt_attend_kernel<D, BF16>, dim3((unsigned)ctas, (unsigned)splits), C::threads, C::smem, s, a, kmap,
+                          vmap, static_cast<const uint16_t*>(kp), static_cast<const uint16_t*>(vp), n_slot, splits);
 }
 
 }  // namespace
