@@ -82,6 +82,7 @@ struct AttendArgs {
     int layer, T, n, H, window, sinks;
     float scale_log2;  // scale * log2(e): scores are in powers of two
     int vec;
+    int over;           // places of pages_decode.cu's line that stand for a beginning and an end
     float* part;        // partial results of units that several CTAs share
     uint32_t* counters; // arrivals per shared unit; zero between launches
 };

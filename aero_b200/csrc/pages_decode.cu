@@ -36,6 +36,7 @@ constexpr int kUnit = 64;          // positions per unit
 constexpr int kConsumers = 4;      // warps; each takes 16 positions of a unit
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kMinUnits = 4;       // a CTA takes at least this many, so that few partials are joined
+constexpr int kWhole = 8;
 constexpr int kHalf = kUnit * 128; // bytes of a unit's 64-column half
 
 template <int D>
@@ -74,6 +75,30 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int e) {
 __device__ __forceinline__ int tile_at(const Span& p, int t) { return t < p.first ? t : p.tile0 + t - p.first; }
 __device__ __forceinline__ bool visible(const Span& p, int j) { return j < p.n && (j >= p.lo || j < p.sinks); }
 
+// Places of the line that a CTA takes: an equal share, but at least kMinUnits, or a whole (sequence,
+// head) where those have up to kWhole: joining parts costs more than those few units one after another.
+__device__ __forceinline__ int64_t piece_length(int64_t total, int64_t segments) {
+    const int64_t each = (total + segments - 1) / segments;
+    return max(each <= kWhole ? each : (int64_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
+}
+
+// What [u, u1) of the line holds of the (sequence, head) at u: on the line each begins with a.over
+// places for the cost of having it at all, so that CTAs with more beginnings get fewer units.
+struct Piece {
+    int h, t0, cnt, line;  // kv head, units [t0, t0 + cnt), places on the line
+};
+__device__ __forceinline__ Piece piece_at(const AttendArgs& a, const Span& p, int64_t u, int64_t u1, int64_t base) {
+    const int line = p.tiles + a.over;
+    const int64_t in = u - base;
+    Piece c;
+    c.h = (int)(in / line);
+    const int at = (int)(in % line);
+    c.line = (int)min((int64_t)(line - at), u1 - u);
+    c.t0 = max(at - a.over, 0);
+    c.cnt = max(at + c.line - a.over, 0) - c.t0;
+    return c;
+}
+
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     decode_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
@@ -109,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         const int per = (a.T + kThreads - 1) / kThreads;
         const int e0 = min(a.T, tid * per), e1 = min(a.T, e0 + per);
         int64_t mine = 0;
-        for (int e = e0; e < e1; ++e) mine += span_of(a, e).tiles;
+        for (int e = e0; e < e1; ++e) mine += span_of(a, e).tiles + a.over;
         int64_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -124,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             total += sums[i];
         }
         total *= HK;
-        const int64_t w = max((int64_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
+        const int64_t w = piece_length(total, (int64_t)a.T * HK);
         const int64_t u0 = w * blockIdx.x;
         if (u0 >= before * HK && u0 < (before + mine) * HK) {
             int64_t base = before * HK;
@@ -132,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             Span at;
             for (;; ++e) {
                 at = span_of(a, e);
-                const int64_t next = base + (int64_t)at.tiles * HK;
+                const int64_t next = base + (int64_t)(at.tiles + a.over) * HK;
                 if (u0 < next) break;
                 base = next;
             }
@@ -144,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         __syncthreads();
     }
     const int64_t total = begin_s[1];
-    const int64_t w = max((int64_t)kMinUnits, (total + gridDim.x - 1) / gridDim.x);
+    const int64_t w = piece_length(total, (int64_t)a.T * HK);
     const int64_t u0 = w * blockIdx.x, u1 = min(total, u0 + w);
     if (u0 >= u1) return;
 
@@ -160,9 +185,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         int64_t loaded = 0;
         bool good = true;
         for (int64_t u = u0; u < u1 && good;) {
-            const int64_t in = u - base;
-            const int h = (int)(in / sp.tiles), t0 = (int)(in % sp.tiles);
-            const int cnt = (int)min((int64_t)(sp.tiles - t0), u1 - u);
+            const Piece pc = piece_at(a, sp, u, u1, base);
+            const int h = pc.h, t0 = pc.t0, cnt = pc.cnt;
             const int s = sp.seq;
             for (int t = t0; t < t0 + cnt; ++t) {
                 // lane i brings box i, if a position in it is visible
@@ -205,8 +229,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                     phase ^= 1u;
                 }
             }
-            u += cnt;
-            if (u == base + (int64_t)sp.tiles * HK && u < u1) {
+            u += pc.line;
+            if (u == base + (int64_t)(sp.tiles + a.over) * HK && u < u1) {
                 base = u;
                 sp = span_of(a, ++e);
             }
@@ -254,9 +278,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
     };
     for (int64_t u = u0; u < u1;) {
-        const int64_t in = u - base;
-        const int h = (int)(in / sp.tiles), t0 = (int)(in % sp.tiles);
-        const int cnt = (int)min((int64_t)(sp.tiles - t0), u1 - u);
+        const Piece pc = piece_at(a, sp, u, u1, base);
+        const int h = pc.h, t0 = pc.t0, cnt = pc.cnt;
+        if (cnt > 0) {
         // the query heads as the products' rows g and g + 8; rows past G are zero
         uint32_t qf[D / 16][4];
         {
@@ -440,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 *reinterpret_cast<float4*>(mine + row * D + d) = summed(row, d);
             }
             if (tid < G) *reinterpret_cast<float2*>(mine + 16 * D + 2 * tid) = joint[tid];
-            const int64_t seg0 = base + (int64_t)h * sp.tiles;  // its units: [seg0, seg0 + tiles)
+            const int64_t seg0 = base + (int64_t)h * (sp.tiles + a.over) + a.over;  // its units: [seg0, seg0 + tiles)
             const int64_t c0 = seg0 / w;
             const int parts = (int)((seg0 + sp.tiles - 1) / w - c0) + 1;
             asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -451,8 +475,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 joins[which] = make_int4(last ? parts : 0, (int)c0, e, h);
             }
         }
-        u += cnt;
-        if (u == base + (int64_t)sp.tiles * HK && u < u1) {
+        }
+        u += pc.line;
+        if (u == base + (int64_t)(sp.tiles + a.over) * HK && u < u1) {
             base = u;
             sp = span_of(a, ++e);
         }
@@ -513,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
 }
 
 template <int D, bool BF16>
-cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, int n_sm, cudaStream_t s) {
+cudaError_t launch(AttendArgs a, const CUtensorMap& kmap, const CUtensorMap& vmap, int n_sm, cudaStream_t s) {
     static thread_local int prepared = -1;  // the device whose attribute this thread has set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -523,10 +548,14 @@ cudaError_t launch(const AttendArgs& a, const CUtensorMap& kmap, const CUtensorM
         if (e != cudaSuccess) return e;
         prepared = dev;
     }
+    // Beginnings and ends of (sequence, head)s cost about three units each, and are counted where they
+    // are many (16 sequences of up to 4096 positions, 4 kv heads: 24.3 -> 22.7 us); where a few long ones
+    // are split over all CTAs that would only shift the cuts (one sequence of 4096: 12.9 -> 14.5 us).
+    a.over = (int64_t)a.T * a.c.HK >= 32 ? 3 : 0;
     // no more CTAs than units the tables can hold
-    const int64_t cap = ((int64_t)a.c.max_pages << a.c.page_shift) / kUnit + 2;
+    const int64_t cap = ((int64_t)a.c.max_pages << a.c.page_shift) / kUnit + 2 + a.over;
     const int64_t units = (int64_t)a.T * a.c.HK * cap;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((int64_t)n_sm * Cfg<D>::ctas, (units + kMinUnits - 1) / kMinUnits));
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((int64_t)n_sm * Cfg<D>::ctas, units));
     return launch_in_turn(decode_attend_kernel<D, BF16>, grid, kThreads, Cfg<D>::smem, s, a, kmap, vmap);
 }
 
