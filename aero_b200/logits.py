@@ -31,6 +31,7 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
     word token // 32 set where the token is allowed. Runs on torch's current stream."""
     import torch
     L, kinds = nc.lib(), _kinds()
+    f32, i32 = torch.float32, torch.int32
     index = logits.get_device()
     if logits.dim() != 2 or logits.dtype not in kinds or index < 0 or logits.stride(1) != 1:
         raise ValueError("logits must be a (rows, vocab) CUDA tensor of float32, float16 or bfloat16, contiguous along vocab")
@@ -40,21 +41,24 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != index or out.stride(1) != 1:
         raise ValueError("out must have the logits' shape, type and device")
 
-    def vec(t, name, dtype, n):
+    def vec(t, name, dtype, shape):
         if t is None:
             return None
-        if t.dtype is not dtype or t.get_device() != index or t.dim() != 1 or (n >= 0 and t.numel() != n) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} vector" + (f" of {n} entries" if n >= 0 else "") +
+        if t.dtype is not dtype or t.get_device() != index or (t.shape != shape if shape else t.dim() != 1) or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} vector" + (f" of {shape[0]} entries" if shape else "") +
                              f" on {logits.device}")
         return t.data_ptr()
 
     def mat(t, name, width):
         if t is None:
             return None, 0
-        if t.dtype is not torch.int32 or t.get_device() != index or t.dim() != 2 or t.shape[0] != rows or \
-                t.shape[1] < width or (t.shape[1] > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name} must be int32 ({rows}, at least {width}) on {logits.device}, contiguous along its rows")
-        return t.data_ptr(), t.stride(0) if rows > 1 else max(t.shape[1], 1)
+        shape = t.shape
+        if t.dtype is not i32 or t.get_device() != index or len(shape) != 2 or shape[0] != rows or shape[1] < width:
+            raise ValueError(f"{name} must be int32 ({rows}, at least {width}) on {logits.device}")
+        stride, one = t.stride()
+        if one != 1 and shape[1] > 1:
+            raise ValueError(f"{name} must be contiguous along its rows")
+        return t.data_ptr(), stride if rows > 1 else max(shape[1], 1)
 
     if (history is None) != (n_history is None):
         raise ValueError("history and n_history come together")
@@ -69,13 +73,13 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
         history = n_history = None
     hp, hl = mat(history, "history", 0)
     mp, mlw = mat(mask, "mask", (vocab + 31) // 32)
-    f32, i32 = torch.float32, torch.int32
+    row = (rows,)
     if L.aero_cuda_logits_adjust(
             logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kinds[logits.dtype], rows, vocab, hp, hl,
-            vec(n_history, "n_history", i32, rows), vec(n_prompt, "n_prompt", i32, rows),
-            vec(repetition, "repetition", f32, rows), vec(frequency, "frequency", f32, rows),
-            vec(presence, "presence", f32, rows), vec(bias_start, "bias_start", i32, rows + 1),
-            vec(bias_token, "bias_token", i32, -1), vec(bias_value, "bias_value", f32, -1), mp, mlw, out.data_ptr(),
+            vec(n_history, "n_history", i32, row), vec(n_prompt, "n_prompt", i32, row),
+            vec(repetition, "repetition", f32, row), vec(frequency, "frequency", f32, row),
+            vec(presence, "presence", f32, row), vec(bias_start, "bias_start", i32, (rows + 1,)),
+            vec(bias_token, "bias_token", i32, None), vec(bias_value, "bias_value", f32, None), mp, mlw, out.data_ptr(),
             out.stride(0) if rows > 1 else vocab, torch._C._cuda_getCurrentRawStream(index) or None) != 0:
         raise ValueError(f"logits_adjust refused: {nc.last_error()}")
     return out
