@@ -692,6 +692,15 @@ int aero_cuda_pages_set_stream(void* cache, void* stream) {
     return aero::entry(cache, [&](Pages& g) {
         const cudaStream_t to = stream ? static_cast<cudaStream_t>(stream) : g.own_stream;
         if (to == g.stream) return true;
+        // a captured stream cannot wait for work outside its graph, nor other work for it: who
+        // captures has waited for what went before
+        cudaStreamCaptureStatus was = cudaStreamCaptureStatusNone, is = cudaStreamCaptureStatusNone;
+        if (!g.ok(cudaStreamIsCapturing(g.stream, &was), "set_stream") || !g.ok(cudaStreamIsCapturing(to, &is), "set_stream"))
+            return false;
+        if (was != cudaStreamCaptureStatusNone || is != cudaStreamCaptureStatusNone) {
+            g.stream = to;
+            return true;
+        }
         if (!g.ok(cudaEventRecord(g.moved, g.stream), "set_stream") ||
             !g.ok(cudaStreamWaitEvent(to, g.moved, 0), "set_stream"))
             return false;

@@ -718,19 +718,27 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         __syncwarp();
         if (parts == 1) {
             const int64_t to = stores ? (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head : -1;
-#pragma unroll 2
-            for (int x0 = 0; x0 < kPieces; ++x0) {
-                const int x = x0 * 32 + lane;
-                const int64_t row_at = of_row(to, x / kPieces);
-                if (row_at < 0) continue;
-                const uint4 v = *reinterpret_cast<const uint4*>(sm + at(x));
-                uint16_t* y = static_cast<uint16_t*>(a.out) + row_at + x % kPieces * 8;
-                if (a.vec) {
-                    *reinterpret_cast<uint4*>(y) = v;
-                } else {
-                    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll 1
+            for (int x0 = 0; x0 < kPieces; x0 += 8) {
+                uint4 v[8];
+                int64_t row_at[8];
 #pragma unroll
-                    for (int b = 0; b < 8; ++b) y[b] = (uint16_t)(u[b >> 1] >> (16 * (b & 1)));
+                for (int k = 0; k < 8; ++k) {
+                    const int x = (x0 + k) * 32 + lane;
+                    row_at[k] = of_row(to, x / kPieces);
+                    v[k] = *reinterpret_cast<const uint4*>(sm + at(x));
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    if (row_at[k] < 0) continue;
+                    uint16_t* y = static_cast<uint16_t*>(a.out) + row_at[k] + ((x0 + k) * 32 + lane) % kPieces * 8;
+                    if (a.vec) {
+                        *reinterpret_cast<uint4*>(y) = v[k];
+                    } else {
+                        const uint32_t u[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) y[b] = (uint16_t)(u[b >> 1] >> (16 * (b & 1)));
+                    }
                 }
             }
         }

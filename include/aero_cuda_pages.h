@@ -66,7 +66,9 @@ int64_t aero_cuda_pages_plan_bytes(const aero_cuda_pages_desc* desc, int64_t* by
 void aero_cuda_pages_close(void* cache);
 
 /* Run on a cudaStream_t (NULL: the handle's own); work enqueued from now on waits
- * for what the handle has enqueued before. 0 / -1. */
+ * for what the handle has enqueued before, unless one of the two streams is being
+ * captured (synchronise before the capture). A stream given here must exist until
+ * another one is set or the cache is closed. 0 / -1. */
 int aero_cuda_pages_set_stream(void* cache, void* stream);
 /* Device addresses of the pool and the books; any of them may be NULL. 0 / -1. */
 int aero_cuda_pages_buffers(void* cache, void** k, void** v, int32_t** table, int32_t** length, int32_t** refs);
@@ -105,7 +107,7 @@ int aero_cuda_pages_compact(void* cache);
  * q_start[i + 1]) are the last positions of sequence seqs[i]. A sequence may be
  * listed more than once. A token at position p sees position j when j <= p and
  * (window == 0 or j > p - window or j < sinks); where none is visible (an empty
- * sequence) its output is 0. scores = scale * q . k; softmax statistics and sums
+ * sequence) its output is 0. scores = scale * q . k with a positive, finite scale; softmax statistics and sums
  * are f32, the probabilities meet V in the cache's type. Values of positions past a
  * sequence's length are never used. */
 int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
@@ -118,8 +120,8 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
  * first n_prompt[r] are the prompt:
  *   x = a token of the history? (x > 0 ? x / repetition[r] : x * repetition[r]) : x
  *   x -= frequency[r] * c + presence[r], c > 0 times in the history after the prompt
- *   x += bias_value[i] for the entries i in [bias_start[r], bias_start[r + 1]) that
- *        name the token (bias_token[i]), in the list's order
+ *   x += the sum, in the list's order, of bias_value[i] for the entries i in
+ *        [bias_start[r], bias_start[r + 1]) that name the token (bias_token[i])
  *   x = -infinity where bit (token % 32) of mask[r * ld_mask + token / 32] is 0
  * computed in f32. history, n_prompt (none), repetition (1), frequency (0), presence
  * (0), bias_start and mask may be NULL. Token ids outside [0, vocab) are passed over.

@@ -544,6 +544,23 @@ def test_streams_and_graph():
     c.check()
 
 
+def test_capture_on_a_stream_of_its_own():
+    """A capture whose stream the cache has not run on before, then calls on the old stream again."""
+    c, K, V = open_cache([100, 40], 16, 2, 64, F16)
+    q, seqs = torch.randn((2, 4, 64), device="cuda").to(F16), i32([0, 1])
+    want = c.attend(0, q, seqs)
+    out = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.attend(0, q, seqs, out=out)
+    g.replay()
+    assert torch.equal(out, want) and torch.equal(c.attend(0, q, seqs), want)
+    q.mul_(0.5)
+    g.replay()
+    assert torch.equal(out, c.attend(0, q, seqs))
+    c.check()
+
+
 def test_refusals():
     from aero_b200.pages import PagedCache, plan_bytes
     for bad in (dict(page_size=12), dict(page_size=4), dict(page_size=512), dict(head_dim=96), dict(n_page=0),
