@@ -344,9 +344,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
             x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
             x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-            // o and l are rescaled only when a maximum has grown by more than 2^8 since they were last:
-            // weights of up to 2^8 are as exact as any in f16, bf16 and the f32 sums
-            if (__any_sync(0xffffffffu, x0 > m0 + 8.f || x1 > m1 + 8.f)) {
+            // (with the exact maximum the largest weight is 1, which the cache's type holds exactly)
+            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
                 const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
                 // (a row without a visible position stays at -inf; its sums are zero)
                 const float f0 = n0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 0.f : ex2(m1 - n1);

@@ -510,11 +510,12 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         {
             const int64_t mine = real ? (int64_t)(w.q0 + tok) * a.q_token + (int64_t)head * a.q_head : -1;
             const uint16_t* all = static_cast<const uint16_t*>(a.q);
+            constexpr int kLoads = kPieces % 16 == 0 ? 16 : 8;  // in flight a lane
 #pragma unroll 1
-            for (int x0 = 0; x0 < kPieces; x0 += 8) {
-                uint4 v[8];
+            for (int x0 = 0; x0 < kPieces; x0 += kLoads) {
+                uint4 v[kLoads];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < kLoads; ++k) {
                     const int x = (x0 + k) * 32 + lane;
                     const int64_t row_at = of_row(mine, x / kPieces);
                     v[k] = make_uint4(0u, 0u, 0u, 0u);
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(sm + at((x0 + k) * 32 + lane)) = v[k];
+                for (int k = 0; k < kLoads; ++k) *reinterpret_cast<uint4*>(sm + at((x0 + k) * 32 + lane)) = v[k];
             }
         }
         fence_proxy_async();
@@ -674,7 +675,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         };
         const float k = inverse(l);
         const uint32_t ot = tmem + lanes + C::o_col0 + q * D;
-        bool odd = false;  // a value of the row that is not finite
+        uint64_t zero = pair(0.f, 0.f);
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -686,7 +687,8 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                 for (int e = 0; e < 32; ++e) o[e] = 0u;
             }
 #pragma unroll
-            for (int e = 0; e < 32; ++e) odd |= (o[e] & 0x7F800000u) == 0x7F800000u;
+            for (int e = 0; e < 32; e += 2)  // 0 x o is no number where o is infinite or none
+                zero = fma2(pair(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), pair(0.f, 0.f), zero);
             if (parts > 1) {
                 float f[32];
 #pragma unroll
@@ -705,7 +707,9 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                 }
             }
         }
-        if (odd && real && l == l)  // (a score that is no number leaves none in the whole row)
+        float z0, z1;
+        unpair(zero, z0, z1);
+        if (!(z0 + z1 == 0.f) && real && l == l)  // (a score that is no number leaves none in the whole row)
             row_slow<D, BF16>(
                 a, w, h, qp, pos, ta, tb, kp, vp,
                 [&](int d0, const float* o, float sum) {
