@@ -472,6 +472,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 const bool last = atomicAdd(a.counters + c0, 1u) == (uint32_t)(parts - 1);
                 if (last) a.counters[c0] = 0;  // for the next launch
                 joins[which] = make_int4(last ? parts : 0, (int)c0, e, h);
+                __threadfence();  // what the others stored, ordered by the barrier below for the whole CTA
             }
         }
         }
@@ -484,7 +485,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     // ---- joins of the (at most two) shared (sequence, head)s whose last part this CTA wrote; here,
     // so that neither the arrivals nor the joins hold up the units
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    __threadfence();
     for (int which = 0; which < 2; ++which) {
         const int parts = joins[which].x;
         if (!parts) continue;
