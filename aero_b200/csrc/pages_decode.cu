@@ -6,7 +6,9 @@
 // and two partial results join by the same rule.
 //
 // Bound by HBM: every visible K and V row is read once (up to 16 query heads share it,
-// at most 16 operations a byte).
+// at most 16 operations a byte). Measured: 48 sequences of 8192 to 32768 positions, 32 query
+// heads on 4 kv heads of 128, 288 us (1.85 GB: 6.4 TB/s); one sequence of 4096 13 us, of 20 6.5 us,
+// where a launch, the chain from lengths to pages to rows, and the join set the time.
 //
 // Split: the work of the call is one line of units, unit = 64 positions of one
 // (sequence, kv head); each CTA takes an equal piece of the line, wherever it begins, so
@@ -19,8 +21,9 @@
 // rows per head; a box of min(page, 64) rows by 64 columns, swizzled), four consumer warps
 // take 16 positions of each unit: S = Q K^T and O += P V as m16n8k16 products, the kv
 // head's query heads as the 16 rows, each warp with its own m, l, o until the segment's
-// end. The consumers never wait for one another within a segment. The matrix pipes are
-// mostly idle: at 16 rows the tile's bytes, not its products, set the time.
+// end. The consumers never wait for one another within a segment. A unit takes a warp some
+// 1000 cycles, an SM's share of HBM 1400 for its 32 KB (head size 128): the tile's bytes, not its
+// products, set the time, so tcgen05's 128 rows would not help.
 #include <cuda_runtime.h>
 
 #include <algorithm>

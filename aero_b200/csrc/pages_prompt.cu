@@ -3,22 +3,30 @@
 // visible, one pass over K and V with a running maximum and sum (pages_decode.cu has
 // the formulas).
 //
-// Bound by the tensor cores and, as much, by the exponentials: a tile of 128 rows by 128
-// positions at head size 128 is 2 x 2.1 M multiply-adds (about 1000 cycles of an SM's
-// tcgen05 pipe) and 16384 exponentials (1024 cycles at 16 a cycle).
+// Bound by the tensor cores and, as much, by the exponentials: a step of two row tiles of 128
+// rows by 128 positions at head size 128 is 4 x 2.1 M multiply-adds (2048 cycles of an SM's
+// tcgen05 pipe) and 2 x 16384 exponentials (2048 cycles at 16 a cycle). Measured: 2600 cycles a
+// step; a prompt of 4096 tokens of 32 query heads on 4 kv heads 134 us (1020 TFLOP/s of the causal
+// half), of 16384 tokens 1.75 ms cold (1257), 1.9 ms in a row under the power cap.
 //
 // Layout: a row is one (token, query head); the rows of a sequence's kv head, its group of
 // query heads innermost, are cut into tiles of 128, so a K/V tile in shared memory serves
 // every query head of the group and a short prompt still fills rows. A CTA takes two row
 // tiles (one at head sizes 192 and 256, where two do not fit TMEM) over the tiles of
-// positions that any of its tokens sees. Warps: four per row tile (a thread a row) for
-// the softmax, one that issues the products, one that brings K and V by TMA (a box per
-// page and 64 columns). S = Q K^T goes to TMEM, its thread takes the row's 128 scores,
-// writes P over them in the cache's type, and O += P V reads P from TMEM and V from shared
-// memory. The two row tiles alternate, so one's products run under the other's softmax;
-// with one row tile S has two buffers instead. O stays in TMEM and is rescaled only
-// when a row's maximum has grown by more than 2^8 since it was last: until then the
-// weights are at most 2^8, which f16, bf16 and the f32 sums hold as exactly as any.
+// positions that any of its tokens sees. Warps: four per row tile (a thread a row) for the
+// softmax, one per row tile that issues its products, one that brings K and V by TMA (a box per
+// page and 64 columns), one that zeroes V rows no token sees. S = Q K^T goes to TMEM, its
+// thread takes the row's scores and writes P to TMEM in the cache's type, O += P V reads P
+// there and V from shared memory.
+//
+// TMEM holds O and P of both row tiles and one S for both: a row tile's S is written when the
+// other's has been read, so the two are always half a step apart and one's products run under the
+// other's softmax. (With an S of its own for each, which P then overwrites, the two fall into
+// step and wait together: 881 against 1100 TFLOP/s at 16384 tokens; with two S of 64 positions
+// each, Q is read twice as often from shared memory, whose 128 bytes a cycle then bind: 1000.) One
+// row tile has two S buffers instead and writes P over S. O is rescaled only when a row's
+// maximum has grown by more than 2^8 since it was last: until then the weights are at most
+// 2^8, which f16, bf16 and the f32 sums hold as exactly as any.
 //
 // Few row tiles over a long cache: the positions of a row tile are split over several
 // CTAs that leave (o, m, l); the last to arrive joins them in order.
@@ -44,8 +52,9 @@ constexpr int kTileRows = 128;
 // joins the reading of rows * D sums. A tile takes about as long as the sums of kJoinRows
 // rows, so nt / parts + parts * rows / kJoinRows is least at sqrt(nt * kJoinRows / rows) parts.
 constexpr float kJoinRows = 220.f;
-// Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly): the
-// special-function pipe, at 16 a cycle and SM, is what the softmax waits for otherwise.
+// Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly), to
+// relieve the special-function pipe. Head size 64, 8192 tokens: none 393 us, every 8th pair 374,
+// every 4th 371; head size 128: alike within 1 %, more of them cost power.
 constexpr int kPolyEvery = 8;
 
 template <int D>
@@ -262,10 +271,14 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     const auto bar = [&](int i) { return smem_u32(bars + i); };
     // S runs SA tiles ahead of P V. A stage holds V of tile i and K of tile i + SA, which one
     // step of the products uses; K of the first SA tiles comes first, to where K of tiles ST and
-    // on will be. Barriers: full, V's unseen rows zero, and empty by stage; K of the first tiles there, and used; S there,
-    // S read and P there (by part), by row tile or by S buffer; O added to, and Q there, by row
-    // tile; the products of a row tile that is given up.
-    enum { F = 0, V = F + ST, E = V + ST, KF = E + ST, KU = KF + 2, SF = KU + 2, SR = SF + 2, PF = SR + 2, OD = PF + 4, QF = OD + 2, AB = QF + 2, NB = AB + 2 };
+    // on will be. Barriers: full (F), V's unseen rows zero (V) and empty (E) by stage; K of the first
+    // tiles there (KF) and used (KU); S there (SF), S read (SR) and P there by part (PF), by row
+    // tile or by S buffer; O added to (OD) and Q there (QF) by row tile; AB: the products of a row
+    // tile that is given up.
+    enum {
+        F = 0, V = F + ST, E = V + ST, KF = E + ST, KU = KF + 2, SF = KU + 2, SR = SF + 2, PF = SR + 2, OD = PF + 4,
+        QF = OD + 2, AB = QF + 2, NB = AB + 2
+    };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NB);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* last = reinterpret_cast<int*>(tmem_slot + 2);
