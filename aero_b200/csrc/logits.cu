@@ -234,6 +234,19 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
     }
 }
 
+template <typename E, int NB>
+cudaError_t launch_adjust(const LogitArgs& a, int rows, int device, cudaStream_t s) {
+    static thread_local int prepared = -1;  // the device whose attribute this thread has set
+    if (prepared != device) {
+        const cudaError_t e = cudaFuncSetAttribute(adjust_kernel<E, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, 98304);
+        if (e != cudaSuccess) return e;
+        prepared = device;
+    }
+    const size_t smem = (size_t)a.slice / 8 * (size_t)(NB + 1) + 16 + kBiasList * 8;
+    const unsigned slices = (unsigned)(((int64_t)a.vocab + a.slice - 1) / a.slice);
+    return launch_in_turn(adjust_kernel<E, NB>, dim3(slices, (unsigned)rows), kLogitThreads, smem, s, a);
+}
+
 bool refuse(const char* what) {
     set_free_error(what);
     return false;
@@ -285,16 +298,9 @@ extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype
         const int64_t most = std::max<int64_t>(least, vocab / (kLogitThreads * 4 * kLogitBatch) + 1);
         const int64_t slices = std::min(std::max(fill, least), most);
         a.slice = (int)std::min<int64_t>((((int64_t)vocab + slices - 1) / slices + 127) / 128 * 128, widest);
-        const auto launch = [&](auto kernel) {
-            const size_t smem = (size_t)a.slice / 8 * (size_t)(nb + 1) + 16 + kBiasList * 8;
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 98304);
-            if (e != cudaSuccess) return e;
-            const unsigned ctas = (unsigned)(((int64_t)vocab + a.slice - 1) / a.slice);
-            return launch_in_turn(kernel, dim3(ctas, (unsigned)rows), kLogitThreads, smem, s, a);
-        };
         const auto typed = [&](auto zero) {
             using E = decltype(zero);
-            return nb == 16 ? launch(adjust_kernel<E, 16>) : launch(adjust_kernel<E, 32>);
+            return nb == 16 ? launch_adjust<E, 16>(a, rows, where.device, s) : launch_adjust<E, 32>(a, rows, where.device, s);
         };
         const cudaError_t e = dtype == AERO_CUDA_TYPE_F32   ? typed(float{})
                               : dtype == AERO_CUDA_TYPE_F16 ? typed(__half{})

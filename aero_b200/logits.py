@@ -41,12 +41,11 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
     elif out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != index or out.stride(1) != 1:
         raise ValueError("out must have the logits' shape, type and device")
 
-    def vec(t, name, dtype, shape):
+    def vec(t, name, dtype, n):
         if t is None:
             return None
-        if t.dtype is not dtype or t.get_device() != index or (t.shape != shape if shape else t.dim() != 1) or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} vector" + (f" of {shape[0]} entries" if shape else "") +
-                             f" on {logits.device}")
+        if t.dtype is not dtype or t.get_device() != index or (n >= 0 and t.numel() != n) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dtype}" + (f", {n} entries," if n >= 0 else "") + f" on {logits.device}")
         return t.data_ptr()
 
     def mat(t, name, width):
@@ -73,13 +72,12 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
         history = n_history = None
     hp, hl = mat(history, "history", 0)
     mp, mlw = mat(mask, "mask", (vocab + 31) // 32)
-    row = (rows,)
     if L.aero_cuda_logits_adjust(
             logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kinds[logits.dtype], rows, vocab, hp, hl,
-            vec(n_history, "n_history", i32, row), vec(n_prompt, "n_prompt", i32, row),
-            vec(repetition, "repetition", f32, row), vec(frequency, "frequency", f32, row),
-            vec(presence, "presence", f32, row), vec(bias_start, "bias_start", i32, (rows + 1,)),
-            vec(bias_token, "bias_token", i32, None), vec(bias_value, "bias_value", f32, None), mp, mlw, out.data_ptr(),
+            vec(n_history, "n_history", i32, rows), vec(n_prompt, "n_prompt", i32, rows),
+            vec(repetition, "repetition", f32, rows), vec(frequency, "frequency", f32, rows),
+            vec(presence, "presence", f32, rows), vec(bias_start, "bias_start", i32, rows + 1),
+            vec(bias_token, "bias_token", i32, -1), vec(bias_value, "bias_value", f32, -1), mp, mlw, out.data_ptr(),
             out.stride(0) if rows > 1 else vocab, torch._C._cuda_getCurrentRawStream(index) or None) != 0:
         raise ValueError(f"logits_adjust refused: {nc.last_error()}")
     return out
