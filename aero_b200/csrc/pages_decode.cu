@@ -7,7 +7,7 @@
 //
 // Bound by HBM: every visible K and V row is read once (up to 16 query heads share it,
 // at most 16 operations a byte). Measured: 48 sequences of 8192 to 32768 positions, 32 query
-// heads on 4 kv heads of 128, 288 us (1.85 GB: 6.4 TB/s); one sequence of 4096 13 us, of 20 6.5 us,
+// heads on 4 kv heads of 128, 279 us (1.85 GB: 6.6 TB/s); one sequence of 4096 12.6 us, of 20 5.4 us,
 // where a launch, the chain from lengths to pages to rows, and the join set the time.
 //
 // Split: the work of the call is one line of units, unit = 64 positions of one
@@ -19,14 +19,17 @@
 //
 // A CTA: one producer warp brings units into a ring of stages by TMA (a page is a run of
 // rows per head; a box of min(page, 64) rows by 64 columns, swizzled), four consumer warps
-// take 16 positions of each unit: S = Q K^T and O += P V as m16n8k16 products, the kv
-// head's query heads as the 16 rows, each warp with its own m, l, o until the segment's
-// end. The consumers never wait for one another within a segment. A unit takes a warp some
-// 1000 cycles, an SM's share of HBM 1400 for its 32 KB (head size 128): the tile's bytes, not its
-// products, set the time, so tcgen05's 128 rows would not help.
+// take 16 positions of each unit as S^T = K Q^T and O^T += V^T P^T in m16n8k16 products, the kv
+// head's query heads as the 8 or 16 columns (as rows they would be padded to 16, with twice the
+// products and sums: 13.6 against 12.6 us for one sequence of 4096, 288 against 279 us for the long
+// ones), each warp with its own m, l, o until the segment's end. The consumers never wait for one
+// another within a segment. An SM's share of HBM takes 1400 cycles for a unit's 32 KB (head size
+// 128), a warp's part of it some 800: the unit's bytes, not its products, set the time, so
+// tcgen05's 128 rows would not help.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pages.h"
 #include "pages_mma.cuh"
@@ -102,13 +105,14 @@ __device__ __forceinline__ Piece piece_at(const AttendArgs& a, const Span& p, in
     return c;
 }
 
-template <int D, bool BF16>
+// NT: tiles of 8 query heads (a kv head's group is up to 8 or up to 16 of them).
+template <int D, bool BF16, int NT>
 __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     decode_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap) {
     constexpr int ST = Cfg<D>::stages;
     extern __shared__ __align__(1024) uint8_t sm[];
-    float* red = reinterpret_cast<float*>(sm + ST * Cfg<D>::stage_bytes);        // [2][16][D], columns swizzled by row
+    float* red = reinterpret_cast<float*>(sm + ST * Cfg<D>::stage_bytes);        // [4][8][D] or [2][16][D], columns swizzled by row
     float2* ml = reinterpret_cast<float2*>(sm + ST * Cfg<D>::stage_bytes + Cfg<D>::red_bytes);  // [4][16] (m, l)
     float2* joint = ml + 64;                                                     // [16]
     uint64_t* bars = reinterpret_cast<uint64_t*>(joint + 16);                    // full[ST], empty[ST]
@@ -253,10 +257,12 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     // -------------------------------------------------------------- consumers
     const int g = lane >> 2, tq = lane & 3;
     bool dead = false;
-    // this lane's rows of the K fragments (keys (lane / 16) * 8 + lane % 8, 8 columns by bit 3)
-    // and of the V fragments (keys (bit 3) * 8 + lane % 8, 8 columns by lane / 16)
-    const int krow = warp * 16 + (lane >> 4) * 8 + (lane & 7), kcol = (lane >> 3) & 1;
-    const int vrow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), vcol = lane >> 4;
+    // rows and columns of the 8x8 blocks this lane addresses. K, keys as the product's rows: blocks
+    // (keys 0-7, 8-15) x (columns 0-7), then columns 8-15. V, transposed, columns as the product's
+    // rows: blocks (columns 0-7, 8-15) x (keys 0-7), then keys 8-15.
+    const int krow = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), kcol = lane >> 4;
+    const int vrow = warp * 16 + (lane >> 4) * 8 + (lane & 7), vcol = (lane >> 3) & 1;
+    constexpr int kRegions = 4 / NT;  // of `red`, 8 * NT rows each
     constexpr int64_t slot = 16 * (D + 2);  // floats of a partial result
     if (tid < 2) joins[tid] = make_int4(0, 0, 0, 0);  // (read after later barriers)
     const auto out_of = [&](int tok, int h) {
@@ -275,34 +281,43 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         }
     };
     const auto summed = [&](int row, int d) {
-        const int col = d ^ ((row & 3) * 8);
-        const float4 x = *reinterpret_cast<const float4*>(red + row * D + col),
-                     y = *reinterpret_cast<const float4*>(red + (16 + row) * D + col);
-        return make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        const int col = d ^ (((row >> 1) & 3) * 8);
+        float4 x = *reinterpret_cast<const float4*>(red + row * D + col);
+#pragma unroll
+        for (int i = 1; i < kRegions; ++i) {
+            const float4 y = *reinterpret_cast<const float4*>(red + (i * 8 * NT + row) * D + col);
+            x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+        }
+        return x;
     };
     for (int64_t u = u0; u < u1;) {
         const Piece pc = piece_at(a, sp, u, u1, base);
         const int h = pc.h, t0 = pc.t0, cnt = pc.cnt;
         if (cnt > 0) {
-        // the query heads as the products' rows g and g + 8; rows past G are zero
-        uint32_t qf[D / 16][4];
+        // the query heads as the products' columns; those past G are zero
+        uint32_t qf[D / 16][NT][2];
         {
             const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)e * a.q_token + (int64_t)(h * G) * a.q_head;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = g + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + 2 * tq;
-                    const uint16_t* x = q + (int64_t)r * a.q_head + col;
-                    qf[ks][i] = r >= G ? 0u
-                                : a.vec ? *reinterpret_cast<const uint32_t*>(x)
-                                        : (uint32_t)x[0] | ((uint32_t)x[1] << 16);
+                for (int i = 0; i < 2 * NT; ++i) {
+                    const int r = g + (i >> 1) * 8;
+                    const uint16_t* x = q + (int64_t)r * a.q_head + ks * 16 + (i & 1) * 8 + 2 * tq;
+                    qf[ks][i >> 1][i & 1] = r >= G ? 0u
+                                            : a.vec ? *reinterpret_cast<const uint32_t*>(x)
+                                                    : (uint32_t)x[0] | ((uint32_t)x[1] << 16);
                 }
         }
-        float o[D / 8][4];
+        // o[i][n]: columns 16 i + g and + 8 (by bit 1) of query heads 8 n + 2 tq and + 1 (by bit 0)
+        float o[D / 16][NT][4];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+        float m[2 * NT], l[2 * NT];
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) m[i] = -INFINITY, l[i] = 0.f;
         for (int t = t0; t < t0 + cnt; ++t) {
             // a warp whose wait gave up goes on without waiting (its results are void, the status
             // says so): the other warps still meet it at the barriers below
@@ -313,79 +328,83 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             }
             const uint32_t kb = ring + (uint32_t)stage * Cfg<D>::stage_bytes, vb = kb + (D / 64) * kHalf;
             // (two sums each, of the even and the odd steps: a shorter chain of products)
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, so[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            float s[NT][4], so[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] = so[n][i] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
                 uint32_t b[4];
                 const int c16 = (ks & 3) * 2 + kcol;
                 ldsm4<false>(b, kb + (ks >> 2) * kHalf + krow * 128 + ((c16 ^ (krow & 7)) << 4));
-                mma16<BF16>(ks & 1 ? so[0] : s[0], qf[ks], b[0], b[1]);
-                mma16<BF16>(ks & 1 ? so[1] : s[1], qf[ks], b[2], b[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16<BF16>(ks & 1 ? so[n] : s[n], b, qf[ks][n][0], qf[ks][n][1]);
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] += so[i >> 2][i & 3];
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + so[n][i]) * a.scale_log2;
             // positions that the token does not see: their scores are -inf and their V rows
             // are taken as zero, whatever their memory holds
             const int j0 = tile_at(sp, t) * kUnit;
             uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
-            const float sc = a.scale_log2;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s[i >> 2][i & 3] *= sc;
             if (j0 + kUnit > sp.n || (j0 < sp.lo && j0 + kUnit > sp.sinks)) {
-                const int j = j0 + warp * 16 + 2 * tq;
-                const bool s00 = visible(sp, j), s01 = visible(sp, j + 1), s10 = visible(sp, j + 8), s11 = visible(sp, j + 9);
-                keep0 = (s00 ? 0x0000FFFFu : 0u) | (s01 ? 0xFFFF0000u : 0u);
-                keep1 = (s10 ? 0x0000FFFFu : 0u) | (s11 ? 0xFFFF0000u : 0u);
-                if (!s00) s[0][0] = s[0][2] = -INFINITY;
-                if (!s01) s[0][1] = s[0][3] = -INFINITY;
-                if (!s10) s[1][0] = s[1][2] = -INFINITY;
-                if (!s11) s[1][1] = s[1][3] = -INFINITY;
-            }
-            float x0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-            float x1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-            x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-            x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-            // (with the exact maximum the largest weight is 1, which the cache's type holds exactly)
-            if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-                const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-                // (a row without a visible position stays at -inf; its sums are zero)
-                const float f0 = n0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 0.f : ex2(m1 - n1);
-                m0 = n0;
-                m1 = n1;
-                l0 *= f0;
-                l1 *= f1;
+                const int j = j0 + warp * 16;
+                keep0 = (visible(sp, j + 2 * tq) ? 0x0000FFFFu : 0u) | (visible(sp, j + 2 * tq + 1) ? 0xFFFF0000u : 0u);
+                keep1 = (visible(sp, j + 2 * tq + 8) ? 0x0000FFFFu : 0u) | (visible(sp, j + 2 * tq + 9) ? 0xFFFF0000u : 0u);
+                const bool see0 = visible(sp, j + g), see1 = visible(sp, j + g + 8);
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    o[i][0] *= f0;
-                    o[i][1] *= f0;
-                    o[i][2] *= f1;
-                    o[i][3] *= f1;
+                for (int n = 0; n < NT; ++n) {
+                    if (!see0) s[n][0] = s[n][1] = -INFINITY;
+                    if (!see1) s[n][2] = s[n][3] = -INFINITY;
                 }
             }
-            const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-            float p[2][4];
+            float x[2 * NT];
+            bool grows = false;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                p[i][0] = ex2(s[i][0] - z0);
-                p[i][1] = ex2(s[i][1] - z0);
-                p[i][2] = ex2(s[i][2] - z1);
-                p[i][3] = ex2(s[i][3] - z1);
-                l0 += p[i][0] + p[i][1];
-                l1 += p[i][2] + p[i][3];
+            for (int i = 0; i < 2 * NT; ++i) {
+                x[i] = fmaxf(s[i >> 1][i & 1], s[i >> 1][2 + (i & 1)]);
+#pragma unroll
+                for (int b = 4; b < 32; b <<= 1) x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], b));
+                grows |= x[i] > m[i];
             }
-            // P in the cache's type: a relative rounding of 2^-11 (f16) or 2^-8 (bf16) / 2 per
-            // weight, below the output's own; the sums l stay f32
-            const uint32_t pa[4] = {pack16<BF16>(p[0][0], p[0][1]), pack16<BF16>(p[0][2], p[0][3]),
-                                    pack16<BF16>(p[1][0], p[1][1]), pack16<BF16>(p[1][2], p[1][3])};
+            // (with the exact maximum the largest weight is 1, which the cache's type holds exactly)
+            if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                for (int i = 0; i < 2 * NT; ++i) {
+                    const float nm = fmaxf(m[i], x[i]);
+                    // (a query head without a visible position stays at -inf; its sums are zero)
+                    const float f = nm == -INFINITY ? 0.f : ex2(m[i] - nm);
+                    m[i] = nm;
+                    l[i] *= f;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        o[k][i >> 1][i & 1] *= f;
+                        o[k][i >> 1][2 + (i & 1)] *= f;
+                    }
+                }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float z0 = m[2 * n] == -INFINITY ? 0.f : m[2 * n], z1 = m[2 * n + 1] == -INFINITY ? 0.f : m[2 * n + 1];
+                const float p0 = ex2(s[n][0] - z0), p1 = ex2(s[n][1] - z1), p2 = ex2(s[n][2] - z0), p3 = ex2(s[n][3] - z1);
+                l[2 * n] += p0 + p2;
+                l[2 * n + 1] += p1 + p3;
+                // P in the cache's type: a relative rounding of 2^-11 (f16) or 2^-8 (bf16) a weight,
+                // below the output's own; the sums l stay f32. Transposed: keys as the product's depth.
+                pb[n][0] = transpose8(pack16<BF16>(p0, p1));
+                pb[n][1] = transpose8(pack16<BF16>(p2, p3));
+            }
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 uint32_t b[4];
                 const int c16 = (i & 3) * 2 + vcol;
                 ldsm4<true>(b, vb + (i >> 2) * kHalf + vrow * 128 + ((c16 ^ (vrow & 7)) << 4));
-                mma16<BF16>(o[2 * i], pa, b[0] & keep0, b[1] & keep1);
-                mma16<BF16>(o[2 * i + 1], pa, b[2] & keep0, b[3] & keep1);
+                const uint32_t va[4] = {b[0] & keep0, b[1] & keep0, b[2] & keep1, b[3] & keep1};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma16<BF16>(o[i][n], va, pb[n][0], pb[n][1]);
             }
             __syncwarp();
             if (lane == 0 && !dead) mbar_arrive(smem_u32(bars + ST + stage));
@@ -394,61 +413,57 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 phase ^= 1u;
             }
         }
-        // ---- the four warps' results into one: o[row][d] = red[0] + red[1], (m, l) in joint
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if (tq == 0) {
-            ml[warp * 16 + g] = make_float2(m0, l0);
-            ml[warp * 16 + g + 8] = make_float2(m1, l1);
+        // ---- the four warps' results into one: o[head][d] = the sum of red's regions, (m, l) in joint
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+#pragma unroll
+            for (int b = 4; b < 32; b <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], b);
+            if (g == 0) ml[warp * 16 + 8 * (i >> 1) + 2 * tq + (i & 1)] = make_float2(m[i], l[i]);
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
         {
-            float M0 = -INFINITY, M1 = -INFINITY, L0 = 0.f, L1 = 0.f;
 #pragma unroll
-            for (int i = 0; i < kConsumers; ++i) {
-                M0 = fmaxf(M0, ml[i * 16 + g].x);
-                M1 = fmaxf(M1, ml[i * 16 + g + 8].x);
-            }
+            for (int i = 0; i < 2 * NT; ++i) {
+                const int row = 8 * (i >> 1) + 2 * tq + (i & 1);
+                float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (int i = 0; i < kConsumers; ++i) {
-                const float2 v0 = ml[i * 16 + g], v1 = ml[i * 16 + g + 8];
-                L0 += v0.x == -INFINITY ? 0.f : v0.y * ex2(v0.x - M0);
-                L1 += v1.x == -INFINITY ? 0.f : v1.y * ex2(v1.x - M1);
-            }
-            const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M1);
-            if (warp == 0 && tq == 0) {
-                joint[g] = make_float2(M0, L0);
-                joint[g + 8] = make_float2(M1, L1);
-            }
-            float* r = red + (warp & 1) * 16 * D;
-            const int sw = (g & 3) * 8;  // columns of row g and g + 8 exchanged in blocks of 8: no bank twice
+                for (int k = 0; k < kConsumers; ++k) M = fmaxf(M, ml[k * 16 + row].x);
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                o[i][0] *= f0;
-                o[i][1] *= f0;
-                o[i][2] *= f1;
-                o[i][3] *= f1;
-                if (warp >= 2) {
-                    const int col = (8 * i + 2 * tq) ^ sw;
-                    *reinterpret_cast<float2*>(r + g * D + col) = make_float2(o[i][0], o[i][1]);
-                    *reinterpret_cast<float2*>(r + (g + 8) * D + col) = make_float2(o[i][2], o[i][3]);
+                for (int k = 0; k < kConsumers; ++k) {
+                    const float2 v = ml[k * 16 + row];
+                    L += v.x == -INFINITY ? 0.f : v.y * ex2(v.x - M);
+                }
+                if (warp == 0 && g == 0) joint[row] = make_float2(M, L);
+                const float f = m[i] == -INFINITY ? 0.f : ex2(m[i] - M);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    o[k][i >> 1][i & 1] *= f;
+                    o[k][i >> 1][2 + (i & 1)] *= f;
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (warp < 2) {
+            // rows 2 tq (+ 1) of a region, columns exchanged in blocks of 8 by tq: no bank twice
+            float* r = red + (warp % kRegions) * 8 * NT * D;
+            const auto cell = [&](int k, int n, int i) { return r + (8 * n + 2 * tq + (i & 1)) * D + ((16 * k + (i >> 1) * 8 + g) ^ (8 * tq)); };
+            if (warp >= kConsumers - kRegions) {
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const int col = (8 * i + 2 * tq) ^ sw;
-                    float2* a0 = reinterpret_cast<float2*>(r + g * D + col);
-                    float2* a1 = reinterpret_cast<float2*>(r + (g + 8) * D + col);
-                    const float2 v0 = *a0, v1 = *a1;
-                    *a0 = make_float2(o[i][0] + v0.x, o[i][1] + v0.y);
-                    *a1 = make_float2(o[i][2] + v1.x, o[i][3] + v1.y);
-                }
+                for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) *cell(k, n, i) = o[k][n][i];
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
+            if constexpr (kRegions < kConsumers) {
+                if (warp < kConsumers - kRegions) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) *cell(k, n, i) += o[k][n][i];
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
         }
         if (cnt == sp.tiles) {
             for (int i = tid; i < G * (D / 4); i += 32 * kConsumers) {
@@ -539,14 +554,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     }
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, int NT>
 cudaError_t launch(AttendArgs a, const CUtensorMap& kmap, const CUtensorMap& vmap, int n_sm, cudaStream_t s) {
     static thread_local int prepared = -1;  // the device whose attribute this thread has set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (prepared != dev) {
-        e = cudaFuncSetAttribute(decode_attend_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem);
+        e = cudaFuncSetAttribute(decode_attend_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem);
         if (e != cudaSuccess) return e;
         prepared = dev;
     }
@@ -558,7 +573,7 @@ cudaError_t launch(AttendArgs a, const CUtensorMap& kmap, const CUtensorMap& vma
     const int64_t cap = ((int64_t)a.c.max_pages << a.c.page_shift) / kUnit + 2 + a.over;
     const int64_t units = (int64_t)a.T * a.c.HK * cap;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((int64_t)n_sm * Cfg<D>::ctas, units));
-    return launch_in_turn(decode_attend_kernel<D, BF16>, grid, kThreads, Cfg<D>::smem, s, a, kmap, vmap);
+    return launch_in_turn(decode_attend_kernel<D, BF16, NT>, grid, kThreads, Cfg<D>::smem, s, a, kmap, vmap);
 }
 
 }  // namespace
@@ -568,11 +583,17 @@ size_t pages_decode_part_floats(int D, int n_sm) { return (size_t)pages_decode_m
 
 cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                 int n_sm, cudaStream_t s) {
+    const auto typed = [&](auto d, auto bf) {
+        constexpr int D = decltype(d)::value;
+        constexpr bool B = decltype(bf)::value;
+        return a.H / a.c.HK <= 8 ? launch<D, B, 1>(a, kmap, vmap, n_sm, s) : launch<D, B, 2>(a, kmap, vmap, n_sm, s);
+    };
+    const auto sized = [&](auto d) { return bf16 ? typed(d, std::true_type{}) : typed(d, std::false_type{}); };
     switch (a.c.D) {
-        case 64: return bf16 ? launch<64, true>(a, kmap, vmap, n_sm, s) : launch<64, false>(a, kmap, vmap, n_sm, s);
-        case 128: return bf16 ? launch<128, true>(a, kmap, vmap, n_sm, s) : launch<128, false>(a, kmap, vmap, n_sm, s);
-        case 192: return bf16 ? launch<192, true>(a, kmap, vmap, n_sm, s) : launch<192, false>(a, kmap, vmap, n_sm, s);
-        case 256: return bf16 ? launch<256, true>(a, kmap, vmap, n_sm, s) : launch<256, false>(a, kmap, vmap, n_sm, s);
+        case 64: return sized(std::integral_constant<int, 64>{});
+        case 128: return sized(std::integral_constant<int, 128>{});
+        case 192: return sized(std::integral_constant<int, 192>{});
+        case 256: return sized(std::integral_constant<int, 256>{});
     }
     return cudaErrorInvalidValue;
 }

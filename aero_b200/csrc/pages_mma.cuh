@@ -36,6 +36,13 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
                      : "memory");
 }
 
+// An 8x8 16-bit matrix transposed across the warp (the fragment of one register a lane).
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t t;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+    return t;
+}
+
 // D (16x8 f32) += A (16x16) x B (16x8), operands in the cache's type.
 template <bool BF16>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
