@@ -26,7 +26,10 @@
 // each, Q is read twice as often from shared memory, whose 128 bytes a cycle then bind: 1000.) One
 // row tile has two S buffers instead and writes P over S. O is rescaled only when a row's
 // maximum has grown by more than 2^8 since it was last: until then the weights are at most
-// 2^8, which f16, bf16 and the f32 sums hold as exactly as any.
+// 2^8, as exact as any in f16, bf16 and the f32 sums, but the largest is no longer 1, which those
+// types hold without rounding. In bf16 the output's distance from the exact one is 1.37 times that
+// of rounding the exact one; rescaled at every growth 1.14 times, for 10 % more time (four
+// windowed prompts 113 -> 124 us, 4096 tokens 131 -> 149 us), at growths past 2^3 1.23 times for 7 %.
 //
 // Few row tiles over a long cache: the positions of a row tile are split over several
 // CTAs that leave (o, m, l); the last to arrive joins them in order.
