@@ -49,7 +49,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     tmp = LIB + ".tmp"
     cmd = [nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-cudart", "static", "--expt-relaxed-constexpr", "-I", CSRC, "-I", INCLUDE,
+           "-cudart", "static", "--expt-relaxed-constexpr", "-t", "0", "-I", CSRC, "-I", INCLUDE,
            *sources(), "-o", tmp, "-lpthread"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
