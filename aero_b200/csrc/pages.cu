@@ -438,8 +438,8 @@ struct Pages {
     int n_sm = 148;
     PageView view{};
     BooksWork work{};
-    void *k = nullptr, *v = nullptr, *books = nullptr;
-    size_t pool_bytes = 0, books_bytes = 0;  // pool_bytes: K or V alone
+    void *k = nullptr, *v = nullptr, *books = nullptr;  // v: behind k, in one allocation
+    size_t pool_bytes = 0, books_bytes = 0;
     float *decode_part = nullptr, *prompt_part = nullptr;
     uint32_t *decode_count = nullptr, *prompt_count = nullptr;
     CUtensorMap kmap{}, vmap{};
@@ -462,7 +462,6 @@ struct Pages {
     ~Pages() {
         if (stream) cudaStreamSynchronize(stream);
         if (k) guarded_free(k, pool_bytes, kKVCache);
-        if (v) guarded_free(v, pool_bytes, kKVCache);
         if (books) guarded_free(books, books_bytes, kScratch);
         if (moved) cudaEventDestroy(moved);
         if (own_stream) cudaStreamDestroy(own_stream);
@@ -549,9 +548,10 @@ Pages* open_pages(const aero_cuda_pages_desc* desc, std::string* why) {
         delete g;
         return nullptr;
     };
-    if (guarded_malloc(&g->k, l.pool, kKVCache) != cudaSuccess) return refuse("device allocation for the K pages refused (memory guard budget or device memory)");
-    g->pool_bytes = l.pool;
-    if (guarded_malloc(&g->v, l.pool, kKVCache) != cudaSuccess) return refuse("device allocation for the V pages refused (memory guard budget or device memory)");
+    if (guarded_malloc(&g->k, 2 * l.pool, kKVCache) != cudaSuccess)
+        return refuse("device allocation for the pages refused (memory guard budget or device memory)");
+    g->pool_bytes = 2 * l.pool;
+    g->v = static_cast<char*>(g->k) + l.pool;  // (l.pool is a multiple of a page's kv head, 1 KB or more)
     if (guarded_malloc(&g->books, l.books, kScratch) != cudaSuccess) return refuse("device allocation for the books refused (memory guard budget or device memory)");
     g->books_bytes = l.books;
     if (cudaStreamCreate(&g->own_stream) != cudaSuccess ||
@@ -584,8 +584,7 @@ Pages* open_pages(const aero_cuda_pages_desc* desc, std::string* why) {
     g->decode_count = reinterpret_cast<uint32_t*>(b + l.dcount);
     g->prompt_part = reinterpret_cast<float*>(b + l.ppart);
     g->prompt_count = reinterpret_cast<uint32_t*>(b + l.pcount);
-    if (cudaMemsetAsync(g->k, 0, l.pool, g->stream) != cudaSuccess ||
-        cudaMemsetAsync(g->v, 0, l.pool, g->stream) != cudaSuccess ||
+    if (cudaMemsetAsync(g->k, 0, 2 * l.pool, g->stream) != cudaSuccess ||
         cudaMemsetAsync(g->books, 0, l.books, g->stream) != cudaSuccess ||
         cudaMemsetAsync(c.table, 0xFF, (size_t)desc->n_seq * desc->max_pages * 4, g->stream) != cudaSuccess ||
         cudaStreamSynchronize(g->stream) != cudaSuccess)
