@@ -40,6 +40,7 @@ struct BooksWork {
     PageJob* jobs;    // (max(n_page, n_seq))
     int32_t* n_jobs;
     int32_t* n_live;
+    int32_t* lowest;  // every page below it is held: where a scan for free ones begins
 };
 
 // Exclusive sum of v over the CTA; *total the whole sum. Every thread calls it.
@@ -85,10 +86,12 @@ __device__ __forceinline__ int4 refs4(const PageView& c, int p0) {
     return r;
 }
 
-// list[0 .. want) = the lowest free pages; false when there are fewer.
-__device__ bool lowest_free(const PageView& c, int want, int32_t* list) {
+// w.list[0 .. want) = the lowest free pages; false when there are fewer. (A full pool of 65536 pages
+// would take 16 steps from its beginning; a decode step's extend finds its pages in the first.)
+__device__ bool lowest_free(const PageView& c, const BooksWork& w, int want) {
+    int32_t* list = w.list;
     int found = 0;
-    for (int base = 0; base < c.n_page && found < want; base += 4 * (int)blockDim.x) {
+    for (int base = *w.lowest & ~3; base < c.n_page && found < want; base += 4 * (int)blockDim.x) {
         const int p0 = base + 4 * (int)threadIdx.x;
         const int4 r = refs4(c, p0);
         const int free4[4] = {r.x == 0, r.y == 0, r.z == 0, r.w == 0};
@@ -106,9 +109,10 @@ __device__ bool lowest_free(const PageView& c, int want, int32_t* list) {
     return found >= want;
 }
 
-__global__ void set_tables_kernel(PageView c, const int32_t* __restrict__ table, const int32_t* __restrict__ length,
+__global__ void set_tables_kernel(PageView c, BooksWork w, const int32_t* __restrict__ table, const int32_t* __restrict__ length,
                                   const int32_t* __restrict__ refs) {
     stream_turn();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *w.lowest = 0;
     const int64_t nt = (int64_t)c.n_seq * c.max_pages, all = nt + c.n_seq + c.n_page;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
         if (i < nt)
@@ -177,10 +181,11 @@ __global__ void __launch_bounds__(kBooksThreads) extend_kernel(PageView c, Books
     const auto pages = [&](int len) { return (int)(((int64_t)len + P - 1) >> c.page_shift); };
     const int want = place_needs(n, c.n_page, w.first,
                                  [&](int i) { return pages(w.len[i] + counts[i]) - pages(w.len[i]); });
-    if (!lowest_free(c, want, w.list)) {
+    if (!lowest_free(c, w, want)) {
         if (threadIdx.x == 0) pages_flag(c, AERO_CUDA_PAGES_NO_PAGES);
         return;
     }
+    if (threadIdx.x == 0 && want > 0) *w.lowest = w.list[want - 1] + 1;
     for (int i = threadIdx.x; i < want; i += blockDim.x) c.refs[w.list[i]] = 1;
     // a warp per entry
     for (int i = (int)threadIdx.x >> 5; i < n; i += (int)blockDim.x >> 5) {
@@ -226,10 +231,11 @@ __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWo
         return;
     }
     const int want = place_needs(n, c.n_page, w.first, [&](int i) { return (w.len[i] & (P - 1)) != 0; });
-    if (!lowest_free(c, want, w.list)) {
+    if (!lowest_free(c, w, want)) {
         if (threadIdx.x == 0) pages_flag(c, AERO_CUDA_PAGES_NO_PAGES);
         return;
     }
+    if (threadIdx.x == 0 && want > 0) *w.lowest = w.list[want - 1] + 1;
     if (threadIdx.x == 0) *w.n_jobs = want;
     for (int i = (int)threadIdx.x >> 5; i < n; i += (int)blockDim.x >> 5) {
         const int len = w.len[i], full = len >> c.page_shift, part = len & (P - 1), lane = (int)threadIdx.x & 31;
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWo
 
 // A CTA per listed sequence. The exchange of the length hands the sequence's pages to
 // one CTA even when the list names it twice.
-__global__ void __launch_bounds__(256) free_kernel(PageView c, const int32_t* __restrict__ seqs, int n) {
+__global__ void __launch_bounds__(256) free_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs, int n) {
     stream_turn();
     __shared__ int held;
     const int P = 1 << c.page_shift;
@@ -274,9 +280,14 @@ __global__ void __launch_bounds__(256) free_kernel(PageView c, const int32_t* __
         row[i] = -1;
         if (p < 0 || p >= c.n_page) {
             pages_flag(c, AERO_CUDA_PAGES_BAD_PAGE);
-        } else if (atomicSub(c.refs + p, 1) <= 0) {  // the books did not hold it
-            atomicAdd(c.refs + p, 1);
-            pages_flag(c, AERO_CUDA_PAGES_BAD_PAGE);
+        } else {
+            const int had = atomicSub(c.refs + p, 1);
+            if (had <= 0) {  // the books did not hold it
+                atomicAdd(c.refs + p, 1);
+                pages_flag(c, AERO_CUDA_PAGES_BAD_PAGE);
+            } else if (had == 1) {
+                atomicMin(w.lowest, p);
+            }
         }
     }
 }
@@ -334,6 +345,7 @@ __global__ void __launch_bounds__(kBooksThreads) compact_kernel(PageView c, Book
     if (threadIdx.x == 0) {
         *w.n_jobs = n;
         *w.n_live = L;
+        *w.lowest = L;
     }
 }
 
@@ -517,7 +529,7 @@ Layout layout(const aero_cuda_pages_desc& d, int n_sm) {
     l.first = take((size_t)d.n_seq * 4);
     l.len = take((size_t)d.n_seq * 4);
     l.jobs = take((size_t)std::max(d.n_page, d.n_seq) * sizeof(PageJob));
-    l.counts = take(8);
+    l.counts = take(12);
     l.dpart = take(pages_decode_part_floats(d.head_dim, n_sm) * 4);
     l.dcount = take((size_t)pages_decode_max_grid(n_sm) * 4);
     l.ppart = take(pages_prompt_part_floats(d.head_dim, n_sm) * 4);
@@ -580,6 +592,7 @@ Pages* open_pages(const aero_cuda_pages_desc* desc, std::string* why) {
     w.jobs = reinterpret_cast<PageJob*>(b + l.jobs);
     w.n_jobs = reinterpret_cast<int32_t*>(b + l.counts);
     w.n_live = w.n_jobs + 1;
+    w.lowest = w.n_jobs + 2;  // (zero at first: the books block is cleared)
     g->decode_part = reinterpret_cast<float*>(b + l.dpart);
     g->decode_count = reinterpret_cast<uint32_t*>(b + l.dcount);
     g->prompt_part = reinterpret_cast<float*>(b + l.ppart);
@@ -741,7 +754,7 @@ int aero_cuda_pages_set_tables(void* cache, const int32_t* table, const int32_t*
             return false;
         const int64_t all = (int64_t)g.d.n_seq * g.d.max_pages + g.d.n_seq + g.d.n_page;
         const unsigned grid = (unsigned)std::min<int64_t>((all + 255) / 256, (int64_t)g.n_sm * 8);
-        return g.ok(aero::launch_in_turn(aero::set_tables_kernel, grid, 256, 0, g.stream, g.view, table, length, refs), "set_tables");
+        return g.ok(aero::launch_in_turn(aero::set_tables_kernel, grid, 256, 0, g.stream, g.view, g.work, table, length, refs), "set_tables");
     });
 }
 
@@ -793,7 +806,7 @@ int aero_cuda_pages_free(void* cache, const int32_t* seqs, int n) {
     return aero::entry(cache, [&](Pages& g) {
         if (!aero::listed(g, seqs, "seqs", nullptr, "", n)) return false;
         if (n == 0) return true;
-        return g.ok(aero::launch_in_turn(aero::free_kernel, (unsigned)n, 256, 0, g.stream, g.view, seqs, n), "free");
+        return g.ok(aero::launch_in_turn(aero::free_kernel, (unsigned)n, 256, 0, g.stream, g.view, g.work, seqs, n), "free");
     });
 }
 

@@ -108,14 +108,16 @@ class PagedCache:
         return self._pool(self._ptr[1], layer)
 
     def tables(self):
-        """(table, length, refs): the books as tensors over the cache's own memory."""
+        """(table, length, refs): the books as tensors over the cache's own memory, to be read; they
+        are changed by the calls below (set_tables for books kept elsewhere)."""
         return (self._view(self._ptr[2], (self.n_seq, self.max_pages), "<i4"),
                 self._view(self._ptr[3], (self.n_seq,), "<i4"), self._view(self._ptr[4], (self.n_page,), "<i4"))
 
     # ---- streams and errors
     def set_stream(self, stream) -> None:
-        """Run on a cudaStream_t (int) or torch.cuda.Stream; None: on torch's current stream at
-        each call (the default)."""
+        """Run on a cudaStream_t (int) or torch.cuda.Stream, whatever torch's current one is (the
+        caller then orders tensors made or used on others); None: on torch's current stream
+        at each call (the default)."""
         self._follow = stream is None
         if stream is not None:
             self._use(getattr(stream, "cuda_stream", stream))

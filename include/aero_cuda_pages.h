@@ -70,7 +70,8 @@ void aero_cuda_pages_close(void* cache);
  * captured (synchronise before the capture). A stream given here must exist until
  * another one is set or the cache is closed. 0 / -1. */
 int aero_cuda_pages_set_stream(void* cache, void* stream);
-/* Device addresses of the pool and the books; any of them may be NULL. 0 / -1. */
+/* Device addresses of the pool and the books (the books to be read: they are changed
+ * by the calls below); any of them may be NULL. 0 / -1. */
 int aero_cuda_pages_buffers(void* cache, void** k, void** v, int32_t** table, int32_t** length, int32_t** refs);
 /* The first code recorded since the last status read (0: none), after
  * synchronising the handle's stream. */
