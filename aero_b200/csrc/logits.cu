@@ -39,6 +39,7 @@ struct LogitArgs {
     int vocab, slice;
     const int32_t* history;
     int64_t ld_history;
+    int history_width;  // entries of a row, however far apart the rows lie
     const int32_t *n_history, *n_prompt;
     const float *repetition, *frequency, *presence;
     const int32_t *bias_start, *bias_token;
@@ -67,7 +68,7 @@ __device__ __forceinline__ E from_f(float v) {
 }
 
 // NB: bits of a token's note, its count after the prompt below a bit that says the prompt holds
-// it: 16 for histories of at most 32767 tokens, else 32.
+// it: 16 for histories at most 32767 tokens wide, else 32.
 template <typename E, int NB>
 __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const LogitArgs a) {
     constexpr int V = 16 / (int)sizeof(E), U = kLogitBatch;
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
     const bool vec = (((uintptr_t)in | (uintptr_t)out) & 15) == 0;
     const uint32_t* bits = a.mask ? reinterpret_cast<const uint32_t*>(a.mask) + (int64_t)r * a.ld_mask : nullptr;
     stream_turn();
-    const int nh = a.history ? (int)min((int64_t)max(0, a.n_history[r]), a.ld_history) : 0;
+    const int nh = a.history ? min(max(0, a.n_history[r]), a.history_width) : 0;
     const int np = nh && a.n_prompt ? a.n_prompt[r] : 0;
     const int b0 = a.bias_start ? a.bias_start[r] : 0, b1 = a.bias_start ? a.bias_start[r + 1] : 0;
     const float rep = a.repetition ? a.repetition[r] : 1.f;
@@ -254,64 +255,88 @@ bool refuse(const char* what) {
 
 bool device_or_null(const void* p) { return !p || (is_device_ptr(p) && ((uintptr_t)p & 3) == 0); }
 
+bool adjust(const void* logits, int64_t ld, int dtype, int rows, int vocab, const int32_t* history, int64_t ld_history,
+            int history_width, const int32_t* n_history, const int32_t* n_prompt, const float* repetition,
+            const float* frequency, const float* presence, const int32_t* bias_start, const int32_t* bias_token,
+            const float* bias_value, const int32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream) {
+    if (dtype != AERO_CUDA_TYPE_F32 && dtype != AERO_CUDA_TYPE_F16 && dtype != AERO_CUDA_TYPE_BF16)
+        return refuse("logits are F32, F16 or BF16");
+    if (rows < 0 || rows > 65535 || vocab <= 0) return refuse("rows must be from 0 to 65535 and vocab positive");
+    if (rows == 0) return true;
+    if (ld < vocab || ld_out < vocab) return refuse("ld and ld_out must be at least vocab");
+    const uintptr_t size = dtype == AERO_CUDA_TYPE_F32 ? 4 : 2;
+    cudaPointerAttributes where{};
+    if (cudaPointerGetAttributes(&where, logits) != cudaSuccess) {
+        cudaGetLastError();
+        where.type = cudaMemoryTypeUnregistered;
+    }
+    if ((where.type != cudaMemoryTypeDevice && where.type != cudaMemoryTypeManaged) || !is_device_ptr(out)) return refuse("logits and out must be device memory");
+    if (((uintptr_t)logits | (uintptr_t)out) % size) return refuse("logits and out must be aligned to their type");
+    if (history && (ld_history < 0 || history_width < 1)) return refuse("ld_history must be >= 0 and the history's width positive");
+    if (history && !n_history) return refuse("a history needs n_history");
+    if (bias_start && (!bias_token || !bias_value)) return refuse("bias_start needs bias_token and bias_value");
+    if (mask && ld_mask != 0 && ld_mask < (vocab + 31) / 32) return refuse("ld_mask must be 0 or at least (vocab + 31) / 32");
+    const void* arrays[] = {history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask};
+    for (const void* p : arrays)
+        if (!device_or_null(p)) return refuse("histories, penalties, biases and masks must be device memory, aligned to 4 bytes");
+    OnDevice on(where.device);
+    if (!on.good) return refuse("cudaSetDevice failed");
+    LogitArgs a{logits, out, ld, ld_out, vocab, 0, history, ld_history, history ? history_width : 0, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask};
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int n_sm = 148;
+    cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, where.device);
+    // As many slices as leave two CTAs for each SM in one wave, none narrower than a CTA's first
+    // batch of loads (f32; 16-bit logits: half of it), none wider than the notes' place.
+    const int nb = a.history_width <= 32767 ? 16 : 32, widest = kNotesBytes / 4 * 32 / nb;
+    const int64_t fill = std::max(1, kLogitCtas * n_sm / rows), least = ((int64_t)vocab + widest - 1) / widest;
+    const int64_t most = std::max<int64_t>(least, vocab / (kLogitThreads * 4 * kLogitBatch) + 1);
+    const int64_t slices = std::min(std::max(fill, least), most);
+    a.slice = (int)std::min<int64_t>((((int64_t)vocab + slices - 1) / slices + 127) / 128 * 128, widest);
+    const auto typed = [&](auto zero) {
+        using E = decltype(zero);
+        return nb == 16 ? launch_adjust<E, 16>(a, rows, where.device, s) : launch_adjust<E, 32>(a, rows, where.device, s);
+    };
+    const cudaError_t e = dtype == AERO_CUDA_TYPE_F32   ? typed(float{})
+                          : dtype == AERO_CUDA_TYPE_F16 ? typed(__half{})
+                                                        : typed(__nv_bfloat16{});
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        set_free_error(std::string("logits_adjust: ") + cudaGetErrorString(e));
+        return false;
+    }
+    return true;
+}
+
 }  // namespace
 }  // namespace aero
 
-extern "C" int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype, int rows, int vocab,
-                                       const int32_t* history, int64_t ld_history, const int32_t* n_history,
-                                       const int32_t* n_prompt, const float* repetition, const float* frequency,
-                                       const float* presence, const int32_t* bias_start, const int32_t* bias_token,
-                                       const float* bias_value, const int32_t* mask, int64_t ld_mask, void* out,
-                                       int64_t ld_out, void* stream) {
-    using namespace aero;
+extern "C" {
+
+int aero_cuda_logits_adjust_views(const void* logits, int64_t ld, int dtype, int rows, int vocab, const int32_t* history,
+                                  int64_t ld_history, int history_width, const int32_t* n_history,
+                                  const int32_t* n_prompt, const float* repetition, const float* frequency,
+                                  const float* presence, const int32_t* bias_start, const int32_t* bias_token,
+                                  const float* bias_value, const int32_t* mask, int64_t ld_mask, void* out,
+                                  int64_t ld_out, void* stream) {
     try {
-        if (dtype != AERO_CUDA_TYPE_F32 && dtype != AERO_CUDA_TYPE_F16 && dtype != AERO_CUDA_TYPE_BF16)
-            return refuse("logits are F32, F16 or BF16"), -1;
-        if (rows < 0 || rows > 65535 || vocab <= 0) return refuse("rows must be from 0 to 65535 and vocab positive"), -1;
-        if (rows == 0) return 0;
-        if (ld < vocab || ld_out < vocab) return refuse("ld and ld_out must be at least vocab"), -1;
-        const uintptr_t size = dtype == AERO_CUDA_TYPE_F32 ? 4 : 2;
-        cudaPointerAttributes where{};
-        if (cudaPointerGetAttributes(&where, logits) != cudaSuccess) {
-            cudaGetLastError();
-            where.type = cudaMemoryTypeUnregistered;
-        }
-        if ((where.type != cudaMemoryTypeDevice && where.type != cudaMemoryTypeManaged) || !is_device_ptr(out)) return refuse("logits and out must be device memory"), -1;
-        if (((uintptr_t)logits | (uintptr_t)out) % size) return refuse("logits and out must be aligned to their type"), -1;
-        if (history && ld_history < 1) return refuse("ld_history must be positive"), -1;
-        if (history && !n_history) return refuse("a history needs n_history"), -1;
-        if (bias_start && (!bias_token || !bias_value)) return refuse("bias_start needs bias_token and bias_value"), -1;
-        if (mask && ld_mask < (vocab + 31) / 32) return refuse("ld_mask must be at least (vocab + 31) / 32"), -1;
-        const void* arrays[] = {history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask};
-        for (const void* p : arrays)
-            if (!device_or_null(p)) return refuse("histories, penalties, biases and masks must be device memory, aligned to 4 bytes"), -1;
-        OnDevice on(where.device);
-        if (!on.good) return refuse("cudaSetDevice failed"), -1;
-        LogitArgs a{logits, out, ld, ld_out, vocab, 0, history, ld_history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask};
-        const cudaStream_t s = static_cast<cudaStream_t>(stream);
-        int n_sm = 148;
-        cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, where.device);
-        // As many slices as leave two CTAs for each SM in one wave, none narrower than a CTA's first
-        // batch of loads (f32; 16-bit logits: half of it), none wider than the notes' place.
-        const int nb = ld_history <= 32767 ? 16 : 32, widest = kNotesBytes / 4 * 32 / nb;
-        const int64_t fill = std::max(1, kLogitCtas * n_sm / rows), least = ((int64_t)vocab + widest - 1) / widest;
-        const int64_t most = std::max<int64_t>(least, vocab / (kLogitThreads * 4 * kLogitBatch) + 1);
-        const int64_t slices = std::min(std::max(fill, least), most);
-        a.slice = (int)std::min<int64_t>((((int64_t)vocab + slices - 1) / slices + 127) / 128 * 128, widest);
-        const auto typed = [&](auto zero) {
-            using E = decltype(zero);
-            return nb == 16 ? launch_adjust<E, 16>(a, rows, where.device, s) : launch_adjust<E, 32>(a, rows, where.device, s);
-        };
-        const cudaError_t e = dtype == AERO_CUDA_TYPE_F32   ? typed(float{})
-                              : dtype == AERO_CUDA_TYPE_F16 ? typed(__half{})
-                                                            : typed(__nv_bfloat16{});
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            set_free_error(std::string("logits_adjust: ") + cudaGetErrorString(e));
-            return -1;
-        }
-        return 0;
+        return aero::adjust(logits, ld, dtype, rows, vocab, history, ld_history, history_width, n_history, n_prompt, repetition,
+                            frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask, out, ld_out, stream)
+                   ? 0
+                   : -1;
     } catch (...) {
         return -1;
     }
 }
+
+int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype, int rows, int vocab, const int32_t* history,
+                            int64_t ld_history, const int32_t* n_history, const int32_t* n_prompt,
+                            const float* repetition, const float* frequency, const float* presence,
+                            const int32_t* bias_start, const int32_t* bias_token, const float* bias_value,
+                            const int32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream) {
+    const int width = (int)std::max<int64_t>(0, std::min<int64_t>(ld_history, INT32_MAX));
+    return aero_cuda_logits_adjust_views(logits, ld, dtype, rows, vocab, history, ld_history, width, n_history, n_prompt,
+                                         repetition, frequency, presence, bias_start, bias_token, bias_value, mask,
+                                         ld_mask, out, ld_out, stream);
+}
+
+}  // extern "C"

@@ -23,9 +23,10 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
     """logits (rows, vocab), a CUDA tensor of float32, float16 or bfloat16; returns out (a new
     tensor, or the one given: it may be logits itself).
 
-    history (rows, length) int32 token ids, the first n_history[r] of row r counted, of
-    which the first n_prompt[r] are the prompt (the repetition penalty takes all of them,
-    the others what follows the prompt). repetition, frequency, presence: float32 (rows).
+    history (rows, length) int32 token ids, the first n_history[r] of row r counted (at most
+    length), of which the first n_prompt[r] are the prompt (the repetition penalty takes all of
+    them, the others what follows the prompt). History and mask may be views: slices of wider
+    tensors, or one row expanded over all. repetition, frequency, presence: float32 (rows).
     Biases: row r's entries are [bias_start[r], bias_start[r + 1]) of bias_token (int32)
     and bias_value (float32). mask: int32 (rows, at least (vocab + 31) // 32), bit token % 32 of
     word token // 32 set where the token is allowed. Runs on torch's current stream."""
@@ -50,14 +51,14 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
 
     def mat(t, name, width):
         if t is None:
-            return None, 0
+            return None, 0, 0
         shape = t.shape
         if t.dtype is not i32 or t.get_device() != index or len(shape) != 2 or shape[0] != rows or shape[1] < width:
             raise ValueError(f"{name} must be int32 ({rows}, at least {width}) on {logits.device}")
         stride, one = t.stride()
         if one != 1 and shape[1] > 1:
             raise ValueError(f"{name} must be contiguous along its rows")
-        return t.data_ptr(), stride if rows > 1 else max(shape[1], 1)
+        return t.data_ptr(), stride if rows > 1 else shape[1], shape[1]
 
     if (history is None) != (n_history is None):
         raise ValueError("history and n_history come together")
@@ -70,10 +71,10 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
             bias_start = bias_token = bias_value = None
     if history is not None and history.shape[-1] == 0:
         history = n_history = None
-    hp, hl = mat(history, "history", 0)
-    mp, mlw = mat(mask, "mask", (vocab + 31) // 32)
-    if L.aero_cuda_logits_adjust(
-            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kinds[logits.dtype], rows, vocab, hp, hl,
+    hp, hl, hw = mat(history, "history", 0)
+    mp, mlw, _ = mat(mask, "mask", (vocab + 31) // 32)
+    if L.aero_cuda_logits_adjust_views(
+            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kinds[logits.dtype], rows, vocab, hp, hl, hw,
             vec(n_history, "n_history", i32, rows), vec(n_prompt, "n_prompt", i32, rows),
             vec(repetition, "repetition", f32, rows), vec(frequency, "frequency", f32, rows),
             vec(presence, "presence", f32, rows), vec(bias_start, "bias_start", i32, rows + 1),
