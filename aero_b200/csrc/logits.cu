@@ -44,6 +44,7 @@ struct LogitArgs {
     const float *repetition, *frequency, *presence;
     const int32_t *bias_start, *bias_token;
     const float* bias_value;
+    int n_bias;  // entries of bias_token and bias_value
     const int32_t* mask;
     int64_t ld_mask;
 };
@@ -88,7 +89,9 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
     stream_turn();
     const int nh = a.history ? min(max(0, a.n_history[r]), a.history_width) : 0;
     const int np = nh && a.n_prompt ? a.n_prompt[r] : 0;
-    const int b0 = a.bias_start ? a.bias_start[r] : 0, b1 = a.bias_start ? a.bias_start[r + 1] : 0;
+    // whatever bias_start holds, nothing outside the list is read
+    const int b0 = a.bias_start ? min(max(a.bias_start[r], 0), a.n_bias) : 0;
+    const int b1 = a.bias_start ? min(max(a.bias_start[r + 1], b0), a.n_bias) : 0;
     const float rep = a.repetition ? a.repetition[r] : 1.f;
     const float per = 1.f / rep;  // x * (1 / rep) for x / rep: one f32 rounding more
     const float fr = a.frequency ? a.frequency[r] : 0.f, pr = a.presence ? a.presence[r] : 0.f;
@@ -258,7 +261,8 @@ bool device_or_null(const void* p) { return !p || (is_device_ptr(p) && ((uintptr
 bool adjust(const void* logits, int64_t ld, int dtype, int rows, int vocab, const int32_t* history, int64_t ld_history,
             int history_width, const int32_t* n_history, const int32_t* n_prompt, const float* repetition,
             const float* frequency, const float* presence, const int32_t* bias_start, const int32_t* bias_token,
-            const float* bias_value, const int32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream) {
+            const float* bias_value, int n_bias, const int32_t* mask, int64_t ld_mask, void* out, int64_t ld_out,
+            void* stream) {
     if (dtype != AERO_CUDA_TYPE_F32 && dtype != AERO_CUDA_TYPE_F16 && dtype != AERO_CUDA_TYPE_BF16)
         return refuse("logits are F32, F16 or BF16");
     if (rows < 0 || rows > 65535 || vocab <= 0) return refuse("rows must be from 0 to 65535 and vocab positive");
@@ -275,13 +279,14 @@ bool adjust(const void* logits, int64_t ld, int dtype, int rows, int vocab, cons
     if (history && (ld_history < 0 || history_width < 1)) return refuse("ld_history must be >= 0 and the history's width positive");
     if (history && !n_history) return refuse("a history needs n_history");
     if (bias_start && (!bias_token || !bias_value)) return refuse("bias_start needs bias_token and bias_value");
+    if (n_bias < 0) return refuse("n_bias must be >= 0");
     if (mask && ld_mask != 0 && ld_mask < (vocab + 31) / 32) return refuse("ld_mask must be 0 or at least (vocab + 31) / 32");
     const void* arrays[] = {history, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask};
     for (const void* p : arrays)
         if (!device_or_null(p)) return refuse("histories, penalties, biases and masks must be device memory, aligned to 4 bytes");
     OnDevice on(where.device);
     if (!on.good) return refuse("cudaSetDevice failed");
-    LogitArgs a{logits, out, ld, ld_out, vocab, 0, history, ld_history, history ? history_width : 0, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask};
+    LogitArgs a{logits, out, ld, ld_out, vocab, 0, history, ld_history, history ? history_width : 0, n_history, n_prompt, repetition, frequency, presence, bias_start, bias_token, bias_value, n_bias, mask, ld_mask};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     int n_sm = 148;
     cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, where.device);
@@ -316,11 +321,12 @@ int aero_cuda_logits_adjust_views(const void* logits, int64_t ld, int dtype, int
                                   int64_t ld_history, int history_width, const int32_t* n_history,
                                   const int32_t* n_prompt, const float* repetition, const float* frequency,
                                   const float* presence, const int32_t* bias_start, const int32_t* bias_token,
-                                  const float* bias_value, const int32_t* mask, int64_t ld_mask, void* out,
-                                  int64_t ld_out, void* stream) {
+                                  const float* bias_value, int n_bias, const int32_t* mask, int64_t ld_mask,
+                                  void* out, int64_t ld_out, void* stream) {
     try {
         return aero::adjust(logits, ld, dtype, rows, vocab, history, ld_history, history_width, n_history, n_prompt, repetition,
-                            frequency, presence, bias_start, bias_token, bias_value, mask, ld_mask, out, ld_out, stream)
+                            frequency, presence, bias_start, bias_token, bias_value, n_bias, mask, ld_mask, out, ld_out,
+                            stream)
                    ? 0
                    : -1;
     } catch (...) {
@@ -335,8 +341,8 @@ int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype, int rows,
                             const int32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream) {
     const int width = (int)std::max<int64_t>(0, std::min<int64_t>(ld_history, INT32_MAX));
     return aero_cuda_logits_adjust_views(logits, ld, dtype, rows, vocab, history, ld_history, width, n_history, n_prompt,
-                                         repetition, frequency, presence, bias_start, bias_token, bias_value, mask,
-                                         ld_mask, out, ld_out, stream);
+                                         repetition, frequency, presence, bias_start, bias_token, bias_value,
+                                         INT32_MAX, mask, ld_mask, out, ld_out, stream);
 }
 
 }  // extern "C"

@@ -28,8 +28,9 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
     them, the others what follows the prompt). History and mask may be views: slices of wider
     tensors, or one row expanded over all. repetition, frequency, presence: float32 (rows).
     Biases: row r's entries are [bias_start[r], bias_start[r + 1]) of bias_token (int32)
-    and bias_value (float32). mask: int32 (rows, at least (vocab + 31) // 32), bit token % 32 of
-    word token // 32 set where the token is allowed. Runs on torch's current stream."""
+    and bias_value (float32); what these name outside the two is passed over. mask: int32
+    (rows, at least (vocab + 31) // 32), bit token % 32 of word token // 32 set where the token
+    is allowed. Runs on torch's current stream."""
     import torch
     L, kinds = nc.lib(), _kinds()
     f32, i32 = torch.float32, torch.int32
@@ -78,7 +79,8 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
             vec(n_history, "n_history", i32, rows), vec(n_prompt, "n_prompt", i32, rows),
             vec(repetition, "repetition", f32, rows), vec(frequency, "frequency", f32, rows),
             vec(presence, "presence", f32, rows), vec(bias_start, "bias_start", i32, rows + 1),
-            vec(bias_token, "bias_token", i32, -1), vec(bias_value, "bias_value", f32, -1), mp, mlw, out.data_ptr(),
+            vec(bias_token, "bias_token", i32, -1), vec(bias_value, "bias_value", f32, -1),
+            0 if bias_token is None else bias_token.numel(), mp, mlw, out.data_ptr(),
             out.stride(0) if rows > 1 else vocab, torch._C._cuda_getCurrentRawStream(index) or None) != 0:
         raise ValueError(f"logits_adjust refused: {nc.last_error()}")
     return out

@@ -126,7 +126,8 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
  *   x = -infinity where bit (token % 32) of mask[r * ld_mask + token / 32] is 0
  * computed in f32. history, n_prompt (none), repetition (1), frequency (0), presence
  * (0), bias_start and mask may be NULL. ld_mask 0: one row of the mask for all rows.
- * Token ids outside [0, vocab) are passed over.
+ * Token ids outside [0, vocab) are passed over. bias_start ascends from 0 and its last entry is
+ * the number of entries of bias_token and bias_value: this form cannot check it.
  * 0, or -1 with the reason in aero_cuda_moe_last_error(NULL). */
 int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype, int rows, int vocab, const int32_t* history,
                             int64_t ld_history, const int32_t* n_history, const int32_t* n_prompt,
@@ -135,13 +136,14 @@ int aero_cuda_logits_adjust(const void* logits, int64_t ld, int dtype, int rows,
                             const int32_t* mask, int64_t ld_mask, void* out, int64_t ld_out, void* stream);
 /* The same for views: a history's rows hold history_width tokens each, of which at most that
  * many count, and lie ld_history apart, which may be less (rows that overlap) or 0 (one
- * history for all rows). */
+ * history for all rows); bias_token and bias_value hold n_bias entries, and what bias_start
+ * names outside them is passed over. */
 int aero_cuda_logits_adjust_views(const void* logits, int64_t ld, int dtype, int rows, int vocab, const int32_t* history,
                                   int64_t ld_history, int history_width, const int32_t* n_history,
                                   const int32_t* n_prompt, const float* repetition, const float* frequency,
                                   const float* presence, const int32_t* bias_start, const int32_t* bias_token,
-                                  const float* bias_value, const int32_t* mask, int64_t ld_mask, void* out,
-                                  int64_t ld_out, void* stream);
+                                  const float* bias_value, int n_bias, const int32_t* mask, int64_t ld_mask,
+                                  void* out, int64_t ld_out, void* stream);
 
 #ifdef __cplusplus
 }

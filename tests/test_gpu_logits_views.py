@@ -59,3 +59,19 @@ def test_shared_and_overlapping_rows():
     assert torch.equal(got, adjust(x, history=tokens.repeat(rows, 1), mask=bits.repeat(rows, 1), **kw))
     sliding = tokens[0].as_strided((rows, 6), (1, 1))
     assert torch.equal(adjust(x, history=sliding, **kw), adjust(x, history=torch.stack(list(sliding)), **kw))
+
+
+@pytest.mark.parametrize("start", [[0, 3, 9], [-4, 2, 5], [0, 5, 2**30], [4, 1, 5], [7, 9, 9], [-9, -3, 1], [-2**31, 2**31 - 1, 0]])
+def test_bias_offsets_outside_the_list(start):
+    """Offsets that begin before the list, end behind it or descend: what lies in the list counts, and
+    nothing beside it."""
+    from aero_b200.logits import adjust
+    rows, vocab, first, n = len(start) - 1, 50, 6, 5
+    x = torch.randn((rows, vocab), device="cuda")
+    token, value = torch.arange(20, dtype=torch.int32, device="cuda"), torch.full((20,), 8.0, device="cuda")
+    got = adjust(x, bias_start=i32(start), bias_token=token[first:first + n], bias_value=value[first:first + n])
+    want = x.clone()
+    for r in range(rows):
+        for i in range(max(start[r], 0), min(start[r + 1], n)):
+            want[r, first + i] += 8.0
+    assert torch.equal(got, want)
