@@ -436,6 +436,10 @@ __global__ void __launch_bounds__(256) append_kernel(PageView c, int layer, cons
             pages_flag(c, AERO_CUDA_PAGES_BAD_PAGE);
             continue;
         }
+        if (c.refs[page] > 1) {  // another sequence reads it
+            pages_flag(c, AERO_CUDA_PAGES_SHARED);
+            continue;
+        }
         const int64_t row = ((((int64_t)layer * c.n_page + page) * c.HK + h) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
         kp[row * rowp + d] = k[t * k_token + h * k_head + d];
         vp[row * rowp + d] = v[t * v_token + h * v_head + d];

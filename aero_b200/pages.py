@@ -33,6 +33,7 @@ STATUS = {
     5: "a page number outside the pool, or a position without a page",
     6: "q_start does not ascend from 0 to the tokens' number within the sequences' lengths",
     7: "a bounded device wait gave up",
+    8: "an append into a page that several sequences hold",
 }
 
 
@@ -192,7 +193,7 @@ class PagedCache:
 
     def append(self, layer: int, k, v, seqs, positions) -> None:
         """K and V rows (T, n_head_kv, head_dim) of T tokens into a layer: token t to position
-        positions[t] of sequence seqs[t]."""
+        positions[t] of sequence seqs[t], in a page that no other sequence holds."""
         self._on()
         T = k.shape[0]
         if v.shape != k.shape:

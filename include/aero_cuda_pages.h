@@ -12,7 +12,8 @@
  *   refs   (n_page)            sequences that hold the page; 0: free
  * The pages a call takes are the lowest-numbered free ones, in the order of its
  * list. Sequences share full pages only (a fork copies the last page when it is
- * partly filled), so rows are never appended to a page that another sequence reads.
+ * partly filled), so room taken by an extend is a sequence's own; an append to an earlier
+ * position, in a page that a fork shares, is refused.
  *
  * All arrays are device memory; every call enqueues its work on the handle's stream
  * and returns (0, or -1 with the reason in aero_cuda_pages_last_error), does not
@@ -46,6 +47,7 @@ extern "C" {
 #define AERO_CUDA_PAGES_BAD_PAGE 5   /* a page number outside [0, n_page), or a position without a page */
 #define AERO_CUDA_PAGES_BAD_ROWS 6   /* q_start does not ascend from 0 to T within the sequences' lengths */
 #define AERO_CUDA_PAGES_WAIT 7       /* a bounded device wait gave up */
+#define AERO_CUDA_PAGES_SHARED 8     /* an append into a page that several sequences hold */
 
 typedef struct aero_cuda_pages_desc {
     int32_t n_layer, n_page;
@@ -85,7 +87,7 @@ int aero_cuda_pages_set_tables(void* cache, const int32_t* table, const int32_t*
 int aero_cuda_pages_extend(void* cache, const int32_t* seqs, const int32_t* counts, int n);
 /* K and V rows of T tokens into `layer`: token t's head h at k + t * k_token + h *
  * k_head elements (head_dim contiguous values of the cache's type), to position
- * positions[t] < length of sequence seqs[t]. */
+ * positions[t] < length of sequence seqs[t], in a page that no other sequence holds. */
 int aero_cuda_pages_append(void* cache, int layer, const void* k, int64_t k_token, int64_t k_head, const void* v,
                            int64_t v_token, int64_t v_head, const int32_t* seqs, const int32_t* positions, int T);
 /* Sequence children[i] (empty, listed once) becomes a copy of parents[i]: full
