@@ -37,11 +37,13 @@
 // Positions that no token of the CTA sees are zeroed in the V tile (their memory may
 // hold anything, and 0 x NaN is NaN). A position that only some rows see (diagonal, ends of the
 // window) may hold values that are not finite; then the rows that do not see it come out not
-// finite too. So a row whose result is not finite is computed again in f32 by row_slow,
-// position by position over what it sees: one that sees such a value keeps its result.
+// finite too. So where a warp ends with such rows, it looks through the V rows that one of its rows
+// does not see and another of the CTA does, and computes the rows that do not see one that is not
+// finite again, by rows_slow. A row that sees all such values keeps its result.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "pages.h"
 #include "pages_mma.cuh"
@@ -224,40 +226,203 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     p1 = __uint_as_float(__float_as_uint(t1) + (__float_as_uint(r1) << 23));
 }
 
-// One row over the tiles [ta, tb), position by position in f32: 32 columns of o at a time to
-// put(d, o, l), then m to done(m, l). For rows that meet values that are not finite.
-template <int D, bool BF16, typename Put, typename Done>
-__device__ __noinline__ void row_slow(const AttendArgs& a, const Work& w, int h, const uint16_t* q, int pos, int ta,
-                                      int tb, const uint16_t* kp, const uint16_t* vp, Put put, Done done) {
-    const int P = 1 << a.c.page_shift;
-    const auto each = [&](auto f) {  // f(score, V row) for every position that the row sees
-        for (int t = ta; t < tb; ++t)
-            for (int i = 0; i < PCfg<D>::BN; ++i) {
-                const int j = tile_pos<PCfg<D>::BN>(w, t) + i;
-                if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) continue;
-                const int page = a.c.table[(int64_t)w.seq * a.c.max_pages + (j >> a.c.page_shift)];
-                if ((uint32_t)page >= (uint32_t)a.c.n_page) continue;
-                const int64_t row =
-                    ((((int64_t)a.layer * a.c.n_page + page) * a.c.HK + h) << a.c.page_shift) + (j & (P - 1));
-                float s = 0.f;
-                for (int d = 0; d < D; ++d) s = fmaf(to_f32<BF16>(q[d]), to_f32<BF16>(kp[row * D + d]), s);
-                f(s * a.scale_log2, vp + row * D);
-            }
-    };
-    float m = -INFINITY, l = 0.f;
-    each([&](float s, const uint16_t*) { m = fmaxf(m, s); });
-    const float z = m == -INFINITY ? 0.f : m;
-    each([&](float s, const uint16_t*) { l += ex2(s - z); });
-    for (int d0 = 0; d0 < D; d0 += 32) {
-        float o[32];
-        for (int d = 0; d < 32; ++d) o[d] = 0.f;
-        each([&](float s, const uint16_t* v) {
-            const float p = ex2(s - z);
-            for (int d = 0; d < 32; ++d) o[d] = fmaf(p, to_f32<BF16>(v[d0 + d]), o[d]);
-        });
-        put(d0, o, l);
+// The pool's row of position j, or -1 where its page is none.
+__device__ __forceinline__ int64_t pool_row(const AttendArgs& a, const Work& w, int h, int j) {
+    const int page = a.c.table[(int64_t)w.seq * a.c.max_pages + (j >> a.c.page_shift)];
+    if ((uint32_t)page >= (uint32_t)a.c.n_page) return -1;
+    return ((((int64_t)a.layer * a.c.n_page + page) * a.c.HK + h) << a.c.page_shift) + (j & ((1 << a.c.page_shift) - 1));
+}
+// Where piece c (16 bytes) of the CTA's row r lies in Q's place, as the products read it.
+template <int D>
+__device__ __forceinline__ uint32_t staged(int r, int c) {
+    return (uint32_t)((r >> 7) * PCfg<D>::q_bytes + (c >> 3) * (kTileRows * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+// 1 / sum of a row's weights: 0 for a row that sees nothing, and no number stays none.
+__device__ __forceinline__ float inverse(float sum) { return sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum; }
+
+// Does position j's V row hold a value that is not finite?
+template <int D, bool BF16>
+__device__ bool v_not_finite(const AttendArgs& a, const Work& w, int h, int j, const uint16_t* vp) {
+    constexpr uint32_t ones = BF16 ? 0x7F807F80u : 0x7C007C00u;  // an exponent of ones, in both halves
+    const int64_t row = pool_row(a, w, h, j);
+    if (row < 0) return false;
+    const uint4* v = reinterpret_cast<const uint4*>(vp + row * D);
+    uint32_t any = 0;
+#pragma unroll 4
+    for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = v[c];
+        any |= __vcmpeq2(x.x & ones, ones) | __vcmpeq2(x.y & ones, ones) | __vcmpeq2(x.z & ones, ones) | __vcmpeq2(x.w & ones, ones);
     }
-    done(m, l);
+    return any != 0;
+}
+
+// 8 values of a query row in f32.
+template <bool BF16>
+__device__ __forceinline__ void query8(const uint16_t* q, int vec, float (&f)[8]) {
+    uint32_t u[4];
+    if (vec) {
+        const uint4 x = *reinterpret_cast<const uint4*>(q);
+        u[0] = x.x, u[1] = x.y, u[2] = x.z, u[3] = x.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = q[2 * e] | (uint32_t)q[2 * e + 1] << 16;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = to_f32<BF16>((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
+}
+
+// kSlowRows rows over the tiles [ta, tb) in f32 by a whole warp: 32 positions' scores at a time, a lane
+// each, then the columns of o by lane, 2 (lane + 32 k) and the next in o[.][2 k] and o[.][2 k + 1]. What it
+// costs is the way to K and V, which the rows share. One V row in the middle of a
+// prompt of 4096, 32 query heads of 128 on 4 kv heads, infinite: 4.3 ms in place of 0.14; of 16384: 19 in
+// place of 1.7; every 40th of 4096: 20 ms. Rows that all see such a value take none of this.
+constexpr int kSlowRows = 4;
+template <int D, bool BF16>
+__device__ __noinline__ void rows_slow(const AttendArgs& a, const Work& w, int h, const uint16_t* const (&q)[kSlowRows],
+                                       const int (&pos)[kSlowRows], int ta, int tb, const uint16_t* kp, const uint16_t* vp,
+                                       float (&o)[kSlowRows][D / 32], float (&m)[kSlowRows], float (&l)[kSlowRows]) {
+    const int lane = (int)threadIdx.x & 31;
+#pragma unroll
+    for (int r = 0; r < kSlowRows; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) o[r][k] = 0.f;
+    }
+    for (int t = ta; t < tb; ++t)
+        for (int i0 = 0; i0 < PCfg<D>::BN; i0 += 32) {
+            const int j = tile_pos<PCfg<D>::BN>(w, t) + i0 + lane;
+            uint32_t seen[kSlowRows], by_any = 0;
+#pragma unroll
+            for (int r = 0; r < kSlowRows; ++r) {
+                seen[r] = __ballot_sync(0xffffffffu, j <= pos[r] && (!a.window || j > pos[r] - a.window || j < a.sinks));
+                by_any |= seen[r];
+            }
+            if (!by_any) continue;
+            const int64_t row = by_any >> lane & 1u ? pool_row(a, w, h, j) : -1;
+            float s[kSlowRows];
+#pragma unroll
+            for (int r = 0; r < kSlowRows; ++r) s[r] = 0.f;
+            if (row >= 0) {
+                const uint4* kr = reinterpret_cast<const uint4*>(kp + row * D);
+#pragma unroll 1
+                for (int c0 = 0; c0 < D / 8; c0 += 8) {
+                    uint4 x[8];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) x[c] = kr[c0 + c];
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const uint32_t u[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+                        for (int r = 0; r < kSlowRows; ++r) {
+                            float f[8];
+                            query8<BF16>(q[r] + (c0 + c) * 8, a.vec, f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) s[r] = fmaf(f[e], to_f32<BF16>((uint16_t)(u[e >> 1] >> (16 * (e & 1)))), s[r]);
+                        }
+                    }
+                }
+            }
+            float p[kSlowRows];
+#pragma unroll
+            for (int r = 0; r < kSlowRows; ++r) {
+                s[r] = row >= 0 && (seen[r] >> lane & 1u) ? s[r] * a.scale_log2 : -INFINITY;
+                float x = s[r];
+#pragma unroll
+                for (int b = 1; b < 32; b <<= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, b));
+                const float mn = max_nan(m[r], x), f = mn == -INFINITY ? 1.f : ex2(m[r] - mn), z = mn == -INFINITY ? 0.f : mn;
+                m[r] = mn;
+                p[r] = ex2(s[r] - z);
+                float sum = p[r];
+#pragma unroll
+                for (int b = 1; b < 32; b <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, b);
+                l[r] = fmaf(l[r], f, sum);
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) o[r][k] *= f;
+            }
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32; i0 += 8) {
+                uint32_t u[8][D / 64];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t from = (int64_t)((uint64_t)__shfl_sync(0xffffffffu, (uint32_t)((uint64_t)row >> 32), i0 + i) << 32 |
+                                                   __shfl_sync(0xffffffffu, (uint32_t)row, i0 + i));
+                    const uint32_t* v = reinterpret_cast<const uint32_t*>(vp + from * D) + lane;
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k) u[i][k] = from < 0 ? 0u : v[32 * k];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int r = 0; r < kSlowRows; ++r) {
+                        const float y = __shfl_sync(0xffffffffu, p[r], i0 + i);
+                        if (!(seen[r] >> (i0 + i) & 1u)) continue;  // (0 x infinity is no number)
+#pragma unroll
+                        for (int k = 0; k < D / 64; ++k) {
+                            o[r][2 * k] = fmaf(y, to_f32<BF16>((uint16_t)u[i][k]), o[r][2 * k]);
+                            o[r][2 * k + 1] = fmaf(y, to_f32<BF16>((uint16_t)(u[i][k] >> 16)), o[r][2 * k + 1]);
+                        }
+                    }
+            }
+        }
+}
+
+// Of a warp's rows (lane: row), those in doubt that do not see a V row which is not finite and which the
+// CTA's products read for another row: computed again, to where a row's result is kept (`parts`: the
+// CTA's partial results, else Q's place in shared memory). All lanes call it.
+template <int D, bool BF16>
+__device__ __noinline__ void rows_again(const AttendArgs& a, const Work& w, int h, int pos, bool doubt, int ta, int tb,
+                                        const uint16_t* kp, const uint16_t* vp, uint8_t* sm, float* parts, float& m, float& l) {
+    using C = PCfg<D>;
+    const int lane = (int)threadIdx.x & 31, lrow0 = (int)threadIdx.x & ~31, G = a.H / a.c.HK;
+    const int first = __shfl_sync(0xffffffffu, pos, 0), last = __reduce_max_sync(0xffffffffu, pos);
+    // the last such V row behind the warp's first position, and the first in front of its last row's window
+    const auto bad = [&](int j) {
+        const int t = w.first + j / C::BN - w.tile0;
+        return t >= ta && t < tb && v_not_finite<D, BF16>(a, w, h, j, vp);
+    };
+    int behind = -1, before = INT_MAX;
+    for (int j = first + 1 + lane; j <= w.p1; j += 32)
+        if (bad(j)) behind = j;
+    if (a.window)
+        for (int j = max(w.lo, a.sinks) + lane; j <= last - a.window; j += 32)
+            if (bad(j)) before = min(before, j);
+    behind = __reduce_max_sync(0xffffffffu, behind);
+    before = __reduce_min_sync(0xffffffffu, before);
+    uint32_t again = __ballot_sync(0xffffffffu, doubt && (behind > pos || (a.window && before <= pos - a.window)));
+    while (again) {
+        int which[kSlowRows], at[kSlowRows], some = 0;
+        const uint16_t* q[kSlowRows];
+#pragma unroll
+        for (int i = 0; i < kSlowRows; ++i) {
+            if (again) some = __ffs(again) - 1;  // (the last one again where there are no more)
+            again &= again - 1;
+            which[i] = some;
+            at[i] = __shfl_sync(0xffffffffu, pos, some);
+            const int row = w.row0 + lrow0 + some;
+            q[i] = static_cast<const uint16_t*>(a.q) + (int64_t)(w.q0 + row / G) * a.q_token + (int64_t)(h * G + row % G) * a.q_head;
+        }
+        float o[kSlowRows][D / 32], row_m[kSlowRows], row_l[kSlowRows];
+        rows_slow<D, BF16>(a, w, h, q, at, ta, tb, kp, vp, o, row_m, row_l);
+#pragma unroll
+        for (int i = 0; i < kSlowRows; ++i) {
+            const int lrow = lrow0 + which[i];
+            if (lane == which[i]) m = row_m[i], l = row_l[i];
+            const float inv = inverse(row_l[i]);
+#pragma unroll
+            for (int k = 0; k < D / 64; ++k) {
+                const int d = 2 * (lane + 32 * k);
+                if (parts) {
+                    float* to = parts + (int64_t)d * C::rows + lrow;
+                    to[0] = o[i][2 * k];
+                    to[C::rows] = o[i][2 * k + 1];
+                } else {
+                    *reinterpret_cast<uint32_t*>(sm + staged<D>(lrow, d >> 3) + (d & 7) * 2) =
+                        pack16<BF16>(o[i][2 * k] * inv, o[i][2 * k + 1] * inv);
+                }
+            }
+        }
+    }
 }
 
 template <int D, bool BF16>
@@ -509,16 +674,12 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         const bool real = row < w.rows && w.n_new <= w.len;
         const int tok = row / G, head = h * G + row % G;  // (used where real)
         const int pos = real ? w.len - w.n_new + tok : -1;
-        const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(w.q0 + tok) * a.q_token + (int64_t)head * a.q_head;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         // The warp's 32 rows, 16 bytes a lane, neighbouring lanes neighbouring pieces: piece x of the
         // x-th of 32 * D / 8, where it lies in shared memory (as the products read it), and the
         // offset of its row, which the row's own lane knows.
         constexpr int kPieces = D / 8;
-        const auto at = [&](int x) {
-            const int r = x / kPieces, c = x % kPieces;
-            return (uint32_t)(q * C::q_bytes + (c >> 3) * (kTileRows * 128) + ((warp & 3) * 32 + r) * 128 + (((c & 7) ^ (r & 7)) << 4));
-        };
+        const auto at = [&](int x) { return staged<D>(warp * 32 + x / kPieces, x % kPieces); };
         const auto of_row = [&](int64_t mine, int r) {
             const uint32_t low = __shfl_sync(0xffffffffu, (uint32_t)mine, r), high = __shfl_sync(0xffffffffu, (uint32_t)(mine >> 32), r);
             return (int64_t)((uint64_t)high << 32 | low);
@@ -674,21 +835,10 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         tc_fence_after();
         if (!good) give_up();
         const bool stores = row < w.rows;
-        const auto put_row = [&](int d0, const float* o, float k) {  // 32 columns of the row, to Q's place
-            for (int e = 0; e < 32; e += 8)
-                *reinterpret_cast<uint4*>(sm + at(lane * kPieces + (d0 + e) / 8)) =
-                    make_uint4(pack16<BF16>(o[e] * k, o[e + 1] * k), pack16<BF16>(o[e + 2] * k, o[e + 3] * k),
-                               pack16<BF16>(o[e + 4] * k, o[e + 5] * k), pack16<BF16>(o[e + 6] * k, o[e + 7] * k));
-        };
-        const auto inverse = [](float sum) { return sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum; };
         // partial results: columns in front of rows, so a warp's stores are contiguous
         constexpr int64_t slot_f = (int64_t)C::rows * (D + 2);
         const int64_t unit = (int64_t)(blockIdx.x) * splits;
         float* mine = a.part + (unit + part) * slot_f;
-        const auto put_part = [&](int d0, const float* o, int n) {
-            if (stores)
-                for (int e = 0; e < n; ++e) mine[(int64_t)(d0 + e) * C::rows + lrow] = o[e];
-        };
         const float k = inverse(l);
         const uint32_t ot = tmem + lanes + C::o_col0 + q * D;
         uint64_t zero = pair(0.f, 0.f);
@@ -706,10 +856,9 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             for (int e = 0; e < 32; e += 2)  // 0 x o is no number where o is infinite or none
                 zero = fma2(pair(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), pair(0.f, 0.f), zero);
             if (parts > 1) {
-                float f[32];
+                if (stores)
 #pragma unroll
-                for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(o[e]);
-                put_part(c * 32, f, 32);
+                    for (int e = 0; e < 32; ++e) mine[(int64_t)(c * 32 + e) * C::rows + lrow] = __uint_as_float(o[e]);
             } else {
                 // into Q's place, which no product reads any more
 #pragma unroll
@@ -725,17 +874,14 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         }
         float z0, z1;
         unpair(zero, z0, z1);
-        if (!(z0 + z1 == 0.f) && real && l == l)  // (a score that is no number leaves none in the whole row)
-            row_slow<D, BF16>(
-                a, w, h, qp, pos, ta, tb, kp, vp,
-                [&](int d0, const float* o, float sum) {
-                    if (parts > 1)
-                        put_part(d0, o, 32);
-                    else
-                        put_row(d0, o, inverse(sum));
-                },
-                [&](float slow_m, float slow_l) { m = slow_m, l = slow_l; });
         __syncwarp();
+        const bool doubt = !(z0 + z1 == 0.f) && real && l == l;  // (a score that is no number leaves none in the whole row)
+        if (__any_sync(0xffffffffu, doubt)) {
+            float m2 = m, l2 = l;
+            rows_again<D, BF16>(a, w, h, pos, doubt, ta, tb, kp, vp, sm, parts > 1 ? mine : nullptr, m2, l2);
+            m = m2, l = l2;
+            __syncwarp();
+        }
         if (parts == 1) {
             const int64_t to = stores ? (int64_t)(w.q0 + tok) * a.o_token + (int64_t)head * a.o_head : -1;
 #pragma unroll 1

@@ -7,6 +7,7 @@ import math
 import pytest
 
 from aero_b200 import native_cuda as nc
+from test_gpu_pages import close, join, open_cache, reference
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -51,3 +52,74 @@ def test_append_leaves_shared_pages_alone(D, shift):
     c.append(1, k[:1], v[:1], i32([0]), i32([3]))
     c.check()
     assert torch.equal(c.k(1)[table[0][0], :, 3], k[0]) and torch.equal(c.v(1)[table[0][0], :, 3], v[0])
+
+
+# ------------------------------------------------------------------ values that are not finite
+def poke(c, which, j, value, columns=slice(None), seq=0):
+    """Position j of a sequence: `columns` of its row in every kv head set to a value."""
+    P = c.page_size
+    which[int(c.tables()[0][seq, j // P]), :, j % P, columns] = value
+
+
+def test_value_that_all_later_rows_see_costs_no_more():
+    """A long prompt whose first V row is not finite in three columns: those columns of every row are
+    not finite either, the others come out to the bit, in about the same time."""
+    T, H, HK, D = 4096, 32, 4, 128
+    c, _, _ = open_cache([T], 64, HK, D, F16)
+    q = (2 * torch.randn((T, H, D), device="cuda")).half()
+    out = torch.empty_like(q)
+
+    def timed():
+        best = math.inf
+        for _ in range(4):
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            e0.record()
+            c.attend(0, q, i32([0]), start, out=out)
+            e1.record()
+            torch.cuda.synchronize()
+            best = min(best, e0.elapsed_time(e1))
+        return best, out.clone()
+
+    start = i32([0, T])
+    clean, want = timed()
+    poke(c, c.v(0), 0, math.nan, slice(5, 8))
+    took, got = timed()
+    c.check()
+    assert torch.isnan(got[..., 5:8]).all()
+    assert torch.equal(got[..., :5], want[..., :5]) and torch.equal(got[..., 8:], want[..., 8:])
+    assert took < 3 * clean, (took, clean)
+
+
+@pytest.mark.parametrize("n,T,P,HK,G,D,dtype,window,sinks,bad", [
+    (500, 300, 16, 2, 3, 64, F16, 0, 0, [0, 250, 333, 499]),
+    (500, 300, 64, 1, 8, 128, BF16, 0, 0, [201, 202, 203, 320, 450]),
+    (900, 400, 16, 2, 4, 128, F16, 130, 5, [2, 4, 5, 480, 600, 633, 764]),
+    (900, 300, 8, 1, 2, 192, BF16, 100, 129, [128, 129, 501, 700, 801, 802]),
+    (700, 200, 32, 1, 5, 256, F16, 0, 0, [499, 500, 620, 699]),
+    (4000, 40, 64, 1, 4, 64, BF16, 0, 0, [100, 3970, 3999]),    # split over CTAs and joined
+    (3000, 260, 16, 1, 1, 256, F16, 700, 40, [39, 40, 2050, 2100, 2800, 2999])])
+def test_rows_beside_values_that_are_not_finite(n, T, P, HK, G, D, dtype, window, sinks, bad):
+    """V rows not finite in some columns, seen by some rows of a tile and not by others: a row that
+    does not see them comes out as without them, one that does has no finite value there alone."""
+    c, K, V = open_cache([n], P, HK, D, dtype)
+    q = (2 * torch.randn((T, HK * G, D), device="cuda")).to(dtype)
+    columns = [d for d in range(D) if d % 7 == 3]
+    for i, j in enumerate(bad):
+        poke(c, c.v(0), j, (math.inf, math.nan, -math.inf)[i % 3], columns)
+    got = c.attend(0, q, i32([0]), i32([0, T]), window=window, sinks=sinks)
+    c.check()
+    pos = [n - T + t for t in range(T)]
+    sees = [any(j <= p and (not window or j > p - window or j < sinks) for j in bad) for p in pos]
+    pick = sorted({t for j in bad for t in range(j - n + T - 3, j - n + T + 4)} |
+                  {t for j in bad for t in range(j - n + T + window - 3, j - n + T + window + 4)} | set(range(0, T, 41)))
+    pick = [t for t in pick if 0 <= t < T]
+    ref = reference(q[pick], K[0], V[0], [pos[t] for t in pick], window, sinks, 1 / math.sqrt(D))
+    some = torch.tensor([sees[t] for t in pick], device="cuda")
+    fine = torch.ones(D, dtype=torch.bool, device="cuda")
+    fine[columns] = False
+    mine = got[pick]
+    assert not torch.isfinite(mine[some][..., ~fine]).any()
+    close(mine[..., fine], tuple(x[..., fine] for x in ref), dtype)
+    if not all(sees[t] for t in pick):
+        close(mine[~some], tuple(x[~some] for x in ref), dtype)
+    assert torch.equal(got.nan_to_num(0, 1, -1), c.attend(0, q, i32([0]), i32([0, T]), window=window, sinks=sinks).nan_to_num(0, 1, -1))
