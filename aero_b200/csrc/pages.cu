@@ -258,19 +258,40 @@ __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWo
     }
 }
 
-// A CTA per listed sequence. The exchange of the length hands the sequence's pages to
-// one CTA even when the list names it twice.
-__global__ void __launch_bounds__(256) free_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs, int n) {
+// The list of a free, for lists longer than a CTA of free_kernel can look over by itself.
+__global__ void __launch_bounds__(kBooksThreads) free_check_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs, int n) {
+    stream_turn();
+    const bool good = distinct_seqs(c, seqs, n, w.mark);
+    if (threadIdx.x == 0) *w.n_jobs = good;
+    if (!good && threadIdx.x == 0) pages_flag(c, AERO_CUDA_PAGES_BAD_SEQ);
+}
+
+constexpr int kFreeThreads = 256;  // and the longest list that free_kernel checks itself
+
+// A CTA per listed sequence. Each looks over the whole list first (`checked`: free_check_kernel has), so
+// that a list with a fault in it changes nothing.
+__global__ void __launch_bounds__(kFreeThreads) free_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs, int n, int checked) {
     stream_turn();
     __shared__ int held;
+    __shared__ int list[kFreeThreads];
     const int P = 1 << c.page_shift;
-    const int s = seqs[blockIdx.x];
-    if (s < 0 || s >= c.n_seq) {
-        if (threadIdx.x == 0) pages_flag(c, AERO_CUDA_PAGES_BAD_SEQ);
-        return;
+    if (checked) {
+        if (!*w.n_jobs) return;
+    } else {
+        const int i = (int)threadIdx.x, mine = i < n ? seqs[i] : 0;
+        list[i] = mine;
+        __syncthreads();
+        bool bad = i < n && (mine < 0 || mine >= c.n_seq);
+        for (int j = 0; j < n; ++j) bad |= j < i && i < n && list[j] == mine;
+        if (__syncthreads_or(bad)) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) pages_flag(c, AERO_CUDA_PAGES_BAD_SEQ);
+            return;
+        }
     }
+    const int s = seqs[blockIdx.x];
     if (threadIdx.x == 0) {
-        const int64_t len = max(0, atomicExch(c.length + s, 0));
+        const int64_t len = max(0, c.length[s]);
+        c.length[s] = 0;
         held = (int)min((int64_t)c.max_pages, (len + P - 1) >> c.page_shift);
     }
     __syncthreads();
@@ -810,7 +831,9 @@ int aero_cuda_pages_free(void* cache, const int32_t* seqs, int n) {
     return aero::entry(cache, [&](Pages& g) {
         if (!aero::listed(g, seqs, "seqs", nullptr, "", n)) return false;
         if (n == 0) return true;
-        return g.ok(aero::launch_in_turn(aero::free_kernel, (unsigned)n, 256, 0, g.stream, g.view, g.work, seqs, n), "free");
+        const int checked = n > aero::kFreeThreads;
+        return (!checked || g.ok(aero::launch_in_turn(aero::free_check_kernel, 1, aero::kBooksThreads, 0, g.stream, g.view, g.work, seqs, n), "free")) &&
+               g.ok(aero::launch_in_turn(aero::free_kernel, (unsigned)n, aero::kFreeThreads, 0, g.stream, g.view, g.work, seqs, n, checked), "free");
     });
 }
 

@@ -212,7 +212,7 @@ class PagedCache:
             self._refused("fork")
 
     def free(self, seqs) -> None:
-        """The sequences give up their pages and become empty."""
+        """The sequences (each listed once) give up their pages and become empty."""
         self._on()
         if self._lib.aero_cuda_pages_free(self.handle, self._i32(seqs, "seqs"), seqs.numel()) != 0:
             self._refused("free")

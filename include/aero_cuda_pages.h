@@ -93,8 +93,8 @@ int aero_cuda_pages_append(void* cache, int layer, const void* k, int64_t k_toke
 /* Sequence children[i] (empty, listed once) becomes a copy of parents[i]: full
  * pages are shared, a partly filled last page is copied in every layer. */
 int aero_cuda_pages_fork(void* cache, const int32_t* parents, const int32_t* children, int n);
-/* The sequences give up their pages and become empty; pages that no sequence holds
- * any more are free. */
+/* The sequences (each listed once) give up their pages and become empty; pages that no
+ * sequence holds any more are free. */
 int aero_cuda_pages_free(void* cache, const int32_t* seqs, int n);
 /* Pages dst[i] = src[i] in every layer (whole pages; no dst among the src or twice). */
 int aero_cuda_pages_copy(void* cache, const int32_t* src, const int32_t* dst, int n);

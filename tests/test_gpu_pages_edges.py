@@ -54,6 +54,24 @@ def test_append_leaves_shared_pages_alone(D, shift):
     assert torch.equal(c.k(1)[table[0][0], :, 3], k[0]) and torch.equal(c.v(1)[table[0][0], :, 3], v[0])
 
 
+@pytest.mark.parametrize("n", [3, 256, 257, 1200])
+def test_free_of_a_bad_list_changes_nothing(n):
+    """Lists with a number outside the cache, or one twice, on both sides of the length that takes a
+    check of its own."""
+    from aero_b200.pages import PagedCache
+    c = PagedCache(1, 2 * n, 8, 1, 64, n, 3, dtype=F16)
+    c.extend(i32(range(n)), i32([1 + s % 16 for s in range(n)]))
+    before = [t.clone() for t in c.tables()]
+    for bad in ([n] + list(range(1, n)), list(range(n - 1)) + [-1], list(range(n - 1)) + [0], [1, 1], [n]):
+        c.free(i32(bad))
+        assert c.status() == 1, bad[:3]
+        assert all(torch.equal(x, y) for x, y in zip(before, c.tables()))
+    c.free(i32(range(n - 1, -1, -1)))
+    c.check()
+    table, length, refs = c.tables()
+    assert (table == -1).all() and not length.any() and not refs.any()
+
+
 # ------------------------------------------------------------------ values that are not finite
 def poke(c, which, j, value, columns=slice(None), seq=0):
     """Position j of a sequence: `columns` of its row in every kv head set to a value."""
