@@ -503,10 +503,10 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         // ------------------------------------------------------------ K and V tiles by TMA
         const int P = 1 << a.c.page_shift, box = min(P, 64), boxes = BN / box;
         bool good = true;
-        // this lane's box of tile i: the pool's row, or -1
+        // this lane's box of tile i, if a row sees a position in it: the pool's row, or -1
         const auto find = [&](int i) {
             const int j0 = tile_pos<BN>(w, ta + i) + lane * box;
-            if (i >= nt || lane >= boxes || j0 > w.p1) return -1;
+            if (i >= nt || lane >= boxes || j0 > w.p1 || (j0 + box <= w.lo && j0 >= w.sinks)) return -1;
             const int page = a.c.table[(int64_t)w.seq * a.c.max_pages + (j0 >> a.c.page_shift)];
             if ((uint32_t)page >= (uint32_t)a.c.n_page) {
                 pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);

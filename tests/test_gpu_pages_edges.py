@@ -141,3 +141,29 @@ def test_rows_beside_values_that_are_not_finite(n, T, P, HK, G, D, dtype, window
     if not all(sees[t] for t in pick):
         close(mine[~some], tuple(x[~some] for x in ref), dtype)
     assert torch.equal(got.nan_to_num(0, 1, -1), c.attend(0, q, i32([0]), i32([0, T]), window=window, sinks=sinks).nan_to_num(0, 1, -1))
+
+
+# ------------------------------------------------------------------ tables with holes
+def holes(c, pages, seq=0):
+    """The books with these places of a sequence's row empty, as a keeper of books elsewhere may have them."""
+    table, length, refs = (t.clone() for t in c.tables())
+    for i in pages:
+        refs[int(table[seq, i])] -= 1
+        table[seq, i] = -1
+    c.set_tables(table, length, refs)
+
+
+@pytest.mark.parametrize("P,T,window,sinks", [(16, 60, 100, 5), (8, 40, 33, 0), (64, 100, 70, 64), (128, 300, 200, 0), (16, 20, 100, 5)])
+@pytest.mark.parametrize("D", [64, 192])
+def test_pages_before_the_window_need_not_be_there(P, T, window, sinks, D):
+    """A sequence that gave up the pages that its new tokens no longer see: no code, the same bits."""
+    n = 900
+    c, K, V = open_cache([n], P, 1, D, F16)
+    q = torch.randn((T, 4, D), device="cuda").half()
+    ask = [(q, i32([0]), i32([0, T])), (q[-1:], i32([0]))]
+    want = [c.attend(0, *x, window=window, sinks=sinks) for x in ask]
+    first = (n - T - window + 1) // P  # the first page that a token's window reaches
+    holes(c, range(-(-sinks // P), first))
+    got = [c.attend(0, *x, window=window, sinks=sinks) for x in ask]
+    c.check()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
