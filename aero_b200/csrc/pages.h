@@ -126,6 +126,9 @@ size_t pages_decode_part_floats(int D, int n_sm);
 size_t pages_prompt_part_floats(int D, int n_sm);
 int pages_decode_max_grid(int n_sm);
 int pages_prompt_max_grid(int n_sm);
+// A box of rows of a visible position without a page starts here: wholly outside the pool, so the
+// copy fills it with zeros.
+constexpr int kNoPageRow = -64;
 // kmap / vmap: (n_layer * n_page * HK * page rows, D) with boxes of min(page, 64)
 // rows by 64 columns, 128-byte swizzle.
 cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,

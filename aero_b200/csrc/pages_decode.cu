@@ -205,14 +205,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             for (int t = t0; t < t0 + cnt; ++t) {
                 // lane i brings box i, if a position in it is visible
                 const int j0 = tile_at(sp, t) * kUnit + lane * rows;
-                bool want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
+                const bool want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
                 int page = 0;
                 if (want) {
                     page = a.c.table[(int64_t)s * a.c.max_pages + (j0 >> a.c.page_shift)];
-                    if ((uint32_t)page >= (uint32_t)a.c.n_page) {
-                        pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
-                        want = false;
-                    }
+                    if ((uint32_t)page >= (uint32_t)a.c.n_page) pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
                 }
                 if (!warp_wait(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
                     good = false;
@@ -229,7 +226,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 __syncwarp();
                 if (want) {
                     const int64_t row0 = (((int64_t)a.layer * a.c.n_page + page) * HK + h) << a.c.page_shift;
-                    const int row = (int)row0 + (j0 & (P - 1));  // < 2^31: checked when the cache was opened
+                    // < 2^31: checked when the cache was opened
+                    const int row = (uint32_t)page < (uint32_t)a.c.n_page ? (int)row0 + (j0 & (P - 1)) : kNoPageRow;
                     const uint32_t dst = ring + (uint32_t)stage * Cfg<D>::stage_bytes + (uint32_t)(lane * rows * 128);
 #pragma unroll
                     for (int c = 0; c < D / 64; ++c) tma_load_2d(dst + c * kHalf, &kmap, c * 64, row, full);

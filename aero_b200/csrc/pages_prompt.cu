@@ -326,7 +326,7 @@ __device__ __noinline__ void rows_slow(const AttendArgs& a, const Work& w, int h
             float p[kSlowRows];
 #pragma unroll
             for (int r = 0; r < kSlowRows; ++r) {
-                s[r] = row >= 0 && (seen[r] >> lane & 1u) ? s[r] * a.scale_log2 : -INFINITY;
+                s[r] = seen[r] >> lane & 1u ? s[r] * a.scale_log2 : -INFINITY;  // (0 without a page)
                 float x = s[r];
 #pragma unroll
                 for (int b = 1; b < 32; b <<= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, b));
@@ -503,20 +503,20 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
         // ------------------------------------------------------------ K and V tiles by TMA
         const int P = 1 << a.c.page_shift, box = min(P, 64), boxes = BN / box;
         bool good = true;
-        // this lane's box of tile i, if a row sees a position in it: the pool's row, or -1
+        // this lane's box of tile i, if a row sees a position in it: the pool's row, kNoPageRow, or -1
         const auto find = [&](int i) {
             const int j0 = tile_pos<BN>(w, ta + i) + lane * box;
             if (i >= nt || lane >= boxes || j0 > w.p1 || (j0 + box <= w.lo && j0 >= w.sinks)) return -1;
             const int page = a.c.table[(int64_t)w.seq * a.c.max_pages + (j0 >> a.c.page_shift)];
             if ((uint32_t)page >= (uint32_t)a.c.n_page) {
                 pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
-                return -1;
+                return kNoPageRow;
             }
             // < 2^31: checked when the cache was opened
             return (int)(((((int64_t)a.layer * a.c.n_page + page) * HK + h) << a.c.page_shift) + (j0 & (P - 1)));
         };
         const auto load = [&](const CUtensorMap& map, uint32_t tile, int row, int full) {
-            if (row < 0) return;
+            if (row == -1) return;
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) tma_load_2d(tile + lane * box * 128 + c * C::half, &map, c * 64, row, bar(full));
         };
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             }
             __syncwarp();
         };
-        const auto count = [&](int row) { return __popc(__ballot_sync(0xffffffffu, row >= 0)); };
+        const auto count = [&](int row) { return __popc(__ballot_sync(0xffffffffu, row != -1)); };
         // rows of the tiles i .. i + SA - 1, whose K is on its way
         int row[SA + 1];
 #pragma unroll

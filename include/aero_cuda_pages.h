@@ -112,7 +112,8 @@ int aero_cuda_pages_compact(void* cache);
  * (window == 0 or j > p - window or j < sinks); where none is visible (an empty
  * sequence) its output is 0. scores = scale * q . k with a positive, finite scale; softmax statistics and sums
  * are f32, the probabilities meet V in the cache's type. Values of positions past a
- * sequence's length are never used. */
+ * sequence's length are never used; a visible position without a page is recorded and
+ * counts as a key and a value of zeros. */
 int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
                            const int32_t* seqs, const int32_t* q_start, int n, float scale, int window, int sinks,
                            void* out, int64_t o_token, int64_t o_head);

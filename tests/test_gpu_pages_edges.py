@@ -167,3 +167,34 @@ def test_pages_before_the_window_need_not_be_there(P, T, window, sinks, D):
     got = [c.attend(0, *x, window=window, sinks=sinks) for x in ask]
     c.check()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("P,D,dtype,window", [(8, 64, F16, 0), (16, 128, BF16, 0), (64, 128, F16, 300), (128, 192, F16, 0), (256, 256, BF16, 0)])
+def test_visible_positions_without_a_page_count_as_zeros(P, D, dtype, window):
+    """In both forms, beside other sequences and after calls that left other rows in the CTAs' memory:
+    the result with zeros there, and the code."""
+    n, T, HK = 700, 120, 2
+    c, K, V = open_cache([n, 300], P, HK, D, dtype)
+    q = (2 * torch.randn((T, 2 * HK, D), device="cuda")).to(dtype)
+    gone = [0, 1, (n - 1) // P] if P < 128 else [1, (n - 1) // P]
+    holes(c, gone)
+    K, V = K[0].clone(), V[0].clone()
+    for i in gone:
+        K[i * P:(i + 1) * P] = 0
+        V[i * P:(i + 1) * P] = 0
+    c.status()
+    many = c.attend(0, q, i32([0, 1]), i32([0, T, T]), window=window)
+    assert c.status() == 5
+    one = c.attend(0, q[:2], i32([0, 1]), window=window)
+    assert c.status() == 5
+    pick = [0, 1, 31, 60, T - 2, T - 1]
+    sc = 1 / math.sqrt(D)
+    close(many[pick], reference(q[pick], K, V, [n - T + t for t in pick], window, 0, sc), dtype)
+    close(one[:1], reference(q[:1], K, V, [n - 1], window, 0, sc), dtype)
+    # and where a value that is not finite lies beside them
+    j = n - 40 if (n - 40) // P not in gone else (n - 1) // P * P - 10
+    poke(c, c.v(0), j, math.inf)
+    many = c.attend(0, q, i32([0, 1]), i32([0, T, T]), window=window)
+    pick = [t for t in (0, 5, j - n + T - 2, j - n + T - 1) if 0 <= t < j - n + T]
+    if pick:
+        close(many[pick], reference(q[pick], K, V, [n - T + t for t in pick], window, 0, sc), dtype)
