@@ -43,6 +43,7 @@ class PagedDecoder:
             m.set_stream(self.stream)
         # rotary angles of half the head
         self.freq = 1e4 ** (-torch.arange(D // 2, device="cuda") / (D // 2))
+        self.stream.wait_stream(torch.cuda.current_stream())  # the weights above are made on the caller's stream
 
     def _norm(self, x):
         return x * self.torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-6)
