@@ -75,3 +75,63 @@ def test_bias_offsets_outside_the_list(start):
         for i in range(max(start[r], 0), min(start[r + 1], n)):
             want[r, first + i] += 8.0
     assert torch.equal(got, want)
+
+
+def long_lists(rows, vocab, per_row, dtype, seed, spread=1):
+    """Lists of per_row biases a row, most tokens more than once, with histories and a mask."""
+    import numpy as np
+    r = np.random.default_rng(seed)
+    x = torch.randn((rows, vocab), device="cuda", generator=torch.Generator("cuda").manual_seed(seed)).mul_(4).to(dtype)
+    history = r.integers(0, vocab, (rows, 300)).astype(np.int32)
+    token = r.integers(-2, vocab // spread + 2, rows * per_row).astype(np.int32)
+    value = r.normal(size=rows * per_row).astype(np.float32)
+    mask = r.integers(-2**31, 2**31, (rows, (vocab + 31) // 32)).astype(np.int32)
+    return x, dict(history=history, n_history=np.full(rows, 300, np.int32), n_prompt=np.full(rows, 100, np.int32),
+                   repetition=np.full(rows, 1.25, np.float32), frequency=np.full(rows, 0.25, np.float32),
+                   presence=np.full(rows, 0.5, np.float32), bias_start=np.arange(rows + 1, dtype=np.int32) * per_row,
+                   bias_token=token, bias_value=value, mask=mask)
+
+
+@pytest.mark.parametrize("rows,vocab,per_row,dtype,spread", [
+    (1, 9000, 513, torch.float32, 8), (2, 9001, 2000, torch.float16, 2), (3, 5003, 12000, torch.float32, 1),
+    (2, 40001, 3000, torch.bfloat16, 400), (1, 700, 9000, torch.float32, 1)])
+def test_long_bias_lists_match_plain(rows, vocab, per_row, dtype, spread):
+    """More biases in a slice than its place in shared memory holds. Tolerance as in test_gpu_logits.py:
+    f32 sums of the values met, one rounding an addition, then the type's own."""
+    import numpy as np
+
+    from aero_b200.logits import adjust
+    from test_gpu_logits import U, plain
+    x, kw = long_lists(rows, vocab, per_row, dtype, 3, spread)
+    dev = {k: torch.from_numpy(v).cuda() for k, v in kw.items()}
+    got = adjust(x, **dev)
+    want, mag = plain(x, kw["history"], kw["n_history"], kw["n_prompt"], kw["repetition"], kw["frequency"], kw["presence"],
+                      kw["bias_start"], kw["bias_token"], kw["bias_value"], kw["mask"])
+    g, off = got.double().cpu().numpy(), np.isinf(want)
+    assert np.array_equal(np.isneginf(g), off)
+    most = np.bincount(kw["bias_token"][kw["bias_token"] >= 0]).max()
+    tol = U[dtype] * np.abs(want[~off]) + 8 * 2.0**-24 * (mag[~off] + 1) * (1 + most)
+    assert (np.abs(g[~off] - want[~off]) <= tol).all()
+    again = x.clone()
+    assert adjust(again, out=again, **dev) is again and torch.equal(again, got)  # in place
+
+
+def test_dense_biases_take_time_in_proportion():
+    """A bias for every token of a vocabulary, against one for every eighth: no more than 16 times as long
+    (each token searching the whole list takes 64 times as long)."""
+    from aero_b200.logits import adjust
+    took = []
+    for per_row in (5000, 40000):
+        x, kw = long_lists(4, 40000, per_row, torch.float32, 5)
+        kw["bias_token"] = torch.arange(40000).repeat(4)[::40000 // per_row].int().numpy()
+        dev = {k: torch.from_numpy(v).cuda() for k, v in kw.items()}
+        best = 1e9
+        for _ in range(4):
+            e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            e0.record()
+            adjust(x, **dev)
+            e1.record()
+            torch.cuda.synchronize()
+            best = min(best, e0.elapsed_time(e1))
+        took.append(best)
+    assert took[1] < 16 * took[0] + 0.1
