@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 for (int b = 4; b < 32; b <<= 1) x[i] = fmaxf(x[i], __shfl_xor_sync(0xffffffffu, x[i], b));
                 grows |= x[i] > m[i];
             }
-            // (with the exact maximum the largest weight is 1, which the cache's type holds exactly)
+            // (with the exact maximum the largest weight is a power of two, which the cache's type holds exactly)
             if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                 for (int i = 0; i < 2 * NT; ++i) {
@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             uint32_t pb[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float z0 = m[2 * n] == -INFINITY ? 0.f : m[2 * n], z1 = m[2 * n + 1] == -INFINITY ? 0.f : m[2 * n + 1];
+                const float z0 = m[2 * n] == -INFINITY ? 0.f : lifted<BF16>(m[2 * n], 0.f);
+                const float z1 = m[2 * n + 1] == -INFINITY ? 0.f : lifted<BF16>(m[2 * n + 1], 0.f);
                 const float p0 = ex2(s[n][0] - z0), p1 = ex2(s[n][1] - z1), p2 = ex2(s[n][2] - z0), p3 = ex2(s[n][3] - z1);
                 l[2 * n] += p0 + p2;
                 l[2 * n + 1] += p1 + p3;

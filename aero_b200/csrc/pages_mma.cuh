@@ -56,6 +56,16 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// What a row's weights are multiplied by, as a power of two, so that the largest of them is at most 2^15.
+// f16 has no number below 2^-24 and full precision only from 2^-14 on: with a largest weight of 1 the
+// many small ones of a long sequence would be lost to V's product while their sum l has them
+// (65536 positions of weight 2^-25 beside one of 1: 0.2 %). bf16 reaches as far down as f32. The factor
+// is in o and l alike, of all parts of a row, and leaves with their quotient.
+template <bool BF16>
+__device__ __forceinline__ float lifted(float m, float top) {
+    return BF16 ? m : m - (15.f - top);  // top: how far above 2^0 a weight may lie beside a maximum of m
+}
+
 // Bounded wait of a whole warp for a phase of an mbarrier: true in every lane, or false in every
 // lane after kWaitNs or when another warp has given up. Lanes may leave the polling at different
 // tries; the vote brings them together again, as the .aligned instructions that follow need.

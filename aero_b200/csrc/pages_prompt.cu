@@ -57,6 +57,8 @@ constexpr int kTileRows = 128;
 // joins the reading of rows * D sums. A tile takes about as long as the sums of kJoinRows
 // rows, so nt / parts + parts * rows / kJoinRows is least at sqrt(nt * kJoinRows / rows) parts.
 constexpr float kJoinRows = 220.f;
+// O is rescaled when a row's maximum has grown by more than this power of two since it was last.
+constexpr float kLazy = 8.f;
 // Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly), to
 // relieve the special-function pipe. Head size 64, 8192 tokens: none 393 us, every 8th pair 374,
 // every 4th 371; head size 128: alike within 1 %, more of them cost power.
@@ -330,7 +332,7 @@ __device__ __noinline__ void rows_slow(const AttendArgs& a, const Work& w, int h
                 float x = s[r];
 #pragma unroll
                 for (int b = 1; b < 32; b <<= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, b));
-                const float mn = max_nan(m[r], x), f = mn == -INFINITY ? 1.f : ex2(m[r] - mn), z = mn == -INFINITY ? 0.f : mn;
+                const float mn = max_nan(m[r], x), f = mn == -INFINITY ? 1.f : ex2(m[r] - mn), z = mn == -INFINITY ? 0.f : lifted<BF16>(mn, kLazy);
                 m[r] = mn;
                 p[r] = ex2(s[r] - z);
                 float sum = p[r];
@@ -770,7 +772,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             }
             if (i == 0) {
                 m = mt;
-            } else if (__any_sync(0xffffffffu, !(mt <= m + 8.f) && mt != -INFINITY)) {
+            } else if (__any_sync(0xffffffffu, !(mt <= m + kLazy) && mt != -INFINITY)) {
                 const float mn = max_nan(m, mt);
                 const float f = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
@@ -796,7 +798,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
             }
             // (m + (m - m) is m, or no number where m is infinite or none: then the whole row is
             // none, as its formula says, and ex2_poly's result does not matter)
-            const float z = m == -INFINITY ? 0.f : m + (m - m);
+            const float z = m == -INFINITY ? 0.f : lifted<BF16>(m + (m - m), kLazy);
             const uint64_t sc2 = pair(sc, sc), nz2 = pair(-z, -z);
             uint64_t sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll

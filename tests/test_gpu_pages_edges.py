@@ -198,3 +198,35 @@ def test_visible_positions_without_a_page_count_as_zeros(P, D, dtype, window):
     pick = [t for t in (0, 5, j - n + T - 2, j - n + T - 1) if 0 <= t < j - n + T]
     if pick:
         close(many[pick], reference(q[pick], K, V, [n - T + t for t in pick], window, 0, sc), dtype)
+
+
+# ------------------------------------------------------------------ many small weights
+@pytest.mark.parametrize("form", ["one", "many", "tiles", "beside"])
+@pytest.mark.parametrize("D,dtype", [(64, F16), (128, F16), (256, F16), (64, BF16)])
+def test_many_small_weights_are_not_lost(form, D, dtype):
+    """65535 positions, each of 2^-25.2 of the weight of one: together 0.17 % of all. All V rows are 1
+    but that one's, which is 0, so the output is their share. Tolerance: the weights' rounding in the
+    cache's type u = 2^-11 (f16) or 2^-8 (bf16), the same for the output, and 2^-14 for f32 scores,
+    exponentials and sums, all relative to the output."""
+    from aero_b200.pages import PagedCache
+    n, P, T = 65536, 256, {"one": 1, "many": 5, "tiles": 64, "beside": 64}[form]
+    c = PagedCache(1, n // P, P, 1, D, 1, n // P, dtype=dtype)
+    c.extend(i32([0]), i32([n]))
+    c.v().fill_(1.0)
+    score = torch.tensor(25.2 * math.log(2), dtype=dtype, device="cuda")
+    page = int(c.tables()[0][0, 11])  # the heavy one somewhere in the first tiles
+    c.k(0)[page, 0, 77, 0] = score
+    c.v(0)[page, 0, 77] = 0.0
+    q = torch.zeros((T, 2, D), dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    if form == "beside":  # rows beside a value that is not finite, computed again
+        poke(c, c.v(0), n - 1, math.inf)
+    out = c.attend(0, q, i32([0]), None if form == "one" else i32([0, T]), scale=1.0)
+    c.check()
+    if form == "beside":
+        out = out[:-1]
+    seen = torch.arange(n - T, n, device="cuda", dtype=torch.float64)[:out.shape[0]]  # light ones that a row sees
+    want = (seen / (seen + torch.exp(score.double())))[:, None, None].expand(out.shape)
+    assert 0.001 < float(want.min()) < 0.002
+    u = 2.0**-11 if dtype == F16 else 2.0**-8
+    assert ((out.double() - want).abs() <= (2 * u + 2.0**-14) * want).all(), float((out.double() / want - 1).abs().max())
