@@ -21,6 +21,19 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     }
 }
 
+// A value of the cache's type in f32, and the low half of a pair of them.
+template <bool BF16>
+__device__ __forceinline__ float to_f32(uint16_t v) {
+    if constexpr (BF16)
+        return __uint_as_float((uint32_t)v << 16);
+    else
+        return __half2float(__ushort_as_half(v));
+}
+template <bool BF16>
+__device__ __forceinline__ float low16(uint32_t pair) {
+    return to_f32<BF16>((uint16_t)pair);
+}
+
 // Four 8x8 16-bit matrices from shared memory (lane i addresses row i % 8 of matrix i / 8).
 template <bool TRANS>
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {

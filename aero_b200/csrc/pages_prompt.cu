@@ -170,14 +170,6 @@ __device__ __forceinline__ uint32_t idesc16(int N, bool bn) {
 // The lowest n bits set (none for n <= 0, all for n >= 32).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
-template <bool BF16>
-__device__ __forceinline__ float to_f32(uint16_t v) {
-    if constexpr (BF16)
-        return __uint_as_float((uint32_t)v << 16);
-    else
-        return __half2float(__ushort_as_half(v));
-}
-
 // Pairs of f32 in a 64-bit register, and their packed arithmetic.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t v;

@@ -111,7 +111,9 @@ int aero_cuda_pages_compact(void* cache);
  * listed more than once. A token at position p sees position j when j <= p and
  * (window == 0 or j > p - window or j < sinks); where none is visible (an empty
  * sequence) its output is 0. scores = scale * q . k with a positive, finite scale; softmax statistics and sums
- * are f32, the probabilities meet V in the cache's type. Values of positions past a
+ * are f32. The probabilities meet V as two values of the cache's type where tokens go one
+ * by one (q_start NULL, at most 32 tokens, or fewer than two a sequence), so the output is as
+ * exact as its own rounding; else as one value. Values of positions past a
  * sequence's length are never used; a visible position without a page is recorded and
  * counts as a key and a value of zeros. */
 int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,

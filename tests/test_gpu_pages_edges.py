@@ -230,3 +230,25 @@ def test_many_small_weights_are_not_lost(form, D, dtype):
     assert 0.001 < float(want.min()) < 0.002
     u = 2.0**-11 if dtype == F16 else 2.0**-8
     assert ((out.double() - want).abs() <= (2 * u + 2.0**-14) * want).all(), float((out.double() / want - 1).abs().max())
+
+
+@pytest.mark.parametrize("G", [1, 8, 16])
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, BF16), (128, F16), (192, F16), (256, BF16)])
+def test_single_tokens_are_as_exact_as_their_type(D, dtype, G):
+    """Token by token, weights lose nothing that the output's type could show. Tolerance: the output's own
+    rounding u|o| (u = 2^-11 in f16, 2^-8 in bf16), the weights' two values u^2 sum w|v|, and 2^-14 sum w|v|
+    for f32 scores, exponentials and sums."""
+    lens = [3000, 200, 64, 1]
+    c, K, V = open_cache(lens, 32, 2, D, dtype)
+    q = torch.randn((len(lens), 2 * G, D), device="cuda").to(dtype)
+    u = 2.0**-11 if dtype == F16 else 2.0**-8
+    few = c.attend(0, q[:3], i32([0, 1]), i32([0, 2, 3]))
+    for got, refs in (
+            (c.attend(0, q, i32(range(4))), [reference(q[s:s + 1], K[s], V[s], [lens[s] - 1], 0, 0, 1 / math.sqrt(D)) for s in range(4)]),
+            (few, [reference(q[:2], K[0], V[0], [2998, 2999], 0, 0, 1 / math.sqrt(D)),
+                   reference(q[2:3], K[1], V[1], [199], 0, 0, 1 / math.sqrt(D))])):
+        out, mag, _ = join(refs)
+        tol = u * out.abs() + (u * u + 2.0**-14) * mag + 2.0**-25
+        err = (got.double() - out).abs()
+        assert (err <= tol).all(), f"worst {float((err / tol).max()):.3f} of the tolerance"
+    c.check()
