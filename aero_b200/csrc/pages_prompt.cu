@@ -59,9 +59,9 @@ constexpr int kTileRows = 128;
 constexpr float kJoinRows = 220.f;
 // O is rescaled when a row's maximum has grown by more than this power of two since it was last.
 constexpr float kLazy = 8.f;
-// Of every so many pairs of exponentials one is computed on the multiply-add pipe (ex2_poly), to
-// relieve the special-function pipe. Head size 64, 8192 tokens: none 393 us, every 8th pair 374,
-// every 4th 371; head size 128: alike within 1 %, more of them cost power.
+// At head size 64, where exponentials bind, one of every so many pairs of them is computed on the
+// multiply-add pipe (ex2_poly), to relieve the special-function pipe: 8192 tokens, 32 heads, none 404 us,
+// every 8th pair 380. Wider heads (4096 tokens, 128, 192 and 256) take the same time without.
 constexpr int kPolyEvery = 8;
 
 template <int D>
@@ -200,8 +200,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // 2^x of a pair on the multiply-add pipe: x = n + f with n the nearest integer and |f| <= 1/2,
-// 2^f by a polynomial of degree 4 (least largest relative error with a constant term of 1,
-// fitted over [-1/2, 1/2]: 3e-6), n added to the exponent. Below -127, -inf among them,
+// 2^f by a polynomial of degree 5 (least largest relative error with a constant term of 1,
+// fitted over [-1/2, 1/2]: 1.1e-7, half of what ex2 may have), n added to the exponent. Below -127, -inf among them,
 // exactly 0; x at most 127 and no NaN.
 __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     float a, b;
@@ -209,9 +209,10 @@ __device__ __forceinline__ void ex2_poly(uint64_t x, float& p0, float& p1) {
     x = pair(fmaxf(a, -127.f), fmaxf(b, -127.f));
     const uint64_t r = add2(x, pair(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's last bits are n
     const uint64_t f = fma2(add2(r, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
-    uint64_t t = fma2(f, pair(0.009585382416844368f, 0.009585382416844368f), pair(0.05590662732720375f, 0.05590662732720375f));
-    t = fma2(t, f, pair(0.24024038016796112f, 0.24024038016796112f));
-    t = fma2(t, f, pair(0.6931241750717163f, 0.6931241750717163f));
+    uint64_t t = fma2(f, pair(0.001326472731307149f, 0.001326472731307149f), pair(0.009671512991189957f, 0.009671512991189957f));
+    t = fma2(t, f, pair(0.05550733581185341f, 0.05550733581185341f));
+    t = fma2(t, f, pair(0.24022242426872253f, 0.24022242426872253f));
+    t = fma2(t, f, pair(0.6931470036506653f, 0.6931470036506653f));
     t = fma2(t, f, pair(1.f, 1.f));
     float t0, t1, r0, r1;
     unpair(t, t0, t1);
@@ -800,7 +801,7 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                 for (int e = 0; e < 16; ++e) {
                     const uint64_t y = fma2(pair(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])), sc2, nz2);
                     float p0, p1;
-                    if (e % kPolyEvery == kPolyEvery - 1) {
+                    if (D == 64 && e % kPolyEvery == kPolyEvery - 1) {
                         ex2_poly(y, p0, p1);
                     } else {
                         unpair(y, p0, p1);
