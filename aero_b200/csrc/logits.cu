@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
         for (int k = 0; k < U; ++k) {
             const int i = base + (k * kLogitThreads + tid) * V;
             // the bits of tokens v0 + i .. + V: of one word, since V divides 32 and S is a multiple of 32
-            allow[k] = bits && i < nv ? __ldg(bits + ((v0 + i) >> 5)) >> ((v0 + i) & 31) : 0xFFFFFFFFu;
+            allow[k] = bits && i < nv ? __ldca(bits + ((v0 + i) >> 5)) >> ((v0 + i) & 31) : 0xFFFFFFFFu;
             E* x = reinterpret_cast<E*>(raw + k);
             if (vec && i + V <= nv) {
                 raw[k] = __ldcs(reinterpret_cast<const uint4*>(in + i));
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
                     const int i = i0 + 4 * kLogitThreads * k;
-                    t[k] = i < whole ? __ldg(reinterpret_cast<const int4*>(h + i)) : make_int4(-1, -1, -1, -1);
+                    t[k] = i < whole ? __ldcg(reinterpret_cast<const int4*>(h + i)) : make_int4(-1, -1, -1, -1);
                 }
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kLogitThreads, kLogitCtas) adjust_kernel(const
             if (nh > 0) n = NB == 16 ? notes[t >> 1] >> 16 * (t & 1) & 0xFFFFu : notes[t];
             const float y = penalised(to_f(out[t]), n) + sums[t - t0];
             const int v = v0 + t;
-            out[t] = from_f<E>(!bits || __ldg(bits + (v >> 5)) >> (v & 31) & 1u ? y : -INFINITY);
+            out[t] = from_f<E>(!bits || bits[v >> 5] >> (v & 31) & 1u ? y : -INFINITY);
         }
     }
 }

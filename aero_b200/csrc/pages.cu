@@ -109,8 +109,8 @@ __device__ bool lowest_free(const PageView& c, const BooksWork& w, int want) {
     return found >= want;
 }
 
-__global__ void set_tables_kernel(PageView c, BooksWork w, const int32_t* __restrict__ table, const int32_t* __restrict__ length,
-                                  const int32_t* __restrict__ refs) {
+__global__ void set_tables_kernel(PageView c, BooksWork w, const int32_t* table, const int32_t* length,
+                                  const int32_t* refs) {
     stream_turn();
     if (blockIdx.x == 0 && threadIdx.x == 0) *w.lowest = 0;
     const int64_t nt = (int64_t)c.n_seq * c.max_pages, all = nt + c.n_seq + c.n_page;
@@ -160,8 +160,8 @@ __device__ int place_needs(int n, int n_page, int32_t* first, F need) {
     return min(total, n_page + 1);
 }
 
-__global__ void __launch_bounds__(kBooksThreads) extend_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs,
-                                                               const int32_t* __restrict__ counts, int n) {
+__global__ void __launch_bounds__(kBooksThreads) extend_kernel(PageView c, BooksWork w, const int32_t* seqs,
+                                                               const int32_t* counts, int n) {
     stream_turn();
     const int P = 1 << c.page_shift;
     if (!distinct_seqs(c, seqs, n, w.mark)) {
@@ -198,8 +198,8 @@ __global__ void __launch_bounds__(kBooksThreads) extend_kernel(PageView c, Books
 
 // Also writes the copies of partly filled last pages as jobs for move_kernel.
 __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWork w,
-                                                             const int32_t* __restrict__ parents,
-                                                             const int32_t* __restrict__ children, int n) {
+                                                             const int32_t* parents,
+                                                             const int32_t* children, int n) {
     stream_turn();
     const int P = 1 << c.page_shift;
     if (threadIdx.x == 0) *w.n_jobs = 0;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kBooksThreads) fork_kernel(PageView c, BooksWo
 }
 
 // The list of a free, for lists longer than a CTA of free_kernel can look over by itself.
-__global__ void __launch_bounds__(kBooksThreads) free_check_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs, int n) {
+__global__ void __launch_bounds__(kBooksThreads) free_check_kernel(PageView c, BooksWork w, const int32_t* seqs, int n) {
     stream_turn();
     const bool good = distinct_seqs(c, seqs, n, w.mark);
     if (threadIdx.x == 0) *w.n_jobs = good;
@@ -270,7 +270,7 @@ constexpr int kFreeThreads = 256;  // and the longest list that free_kernel chec
 
 // A CTA per listed sequence. Each looks over the whole list first (`checked`: free_check_kernel has), so
 // that a list with a fault in it changes nothing.
-__global__ void __launch_bounds__(kFreeThreads) free_kernel(PageView c, BooksWork w, const int32_t* __restrict__ seqs, int n, int checked) {
+__global__ void __launch_bounds__(kFreeThreads) free_kernel(PageView c, BooksWork w, const int32_t* seqs, int n, int checked) {
     stream_turn();
     __shared__ int held;
     __shared__ int list[kFreeThreads];
@@ -370,8 +370,8 @@ __global__ void __launch_bounds__(kBooksThreads) compact_kernel(PageView c, Book
     }
 }
 
-__global__ void copy_jobs_kernel(PageView c, BooksWork w, const int32_t* __restrict__ src,
-                                 const int32_t* __restrict__ dst, int n) {
+__global__ void copy_jobs_kernel(PageView c, BooksWork w, const int32_t* src,
+                                 const int32_t* dst, int n) {
     stream_turn();
     const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
     if (i == 0) *w.n_jobs = n;
@@ -390,7 +390,7 @@ constexpr int kMoveUnit = 256 * kMoveVec;
 // The jobs' rows, in every layer and kv head of K and V: a page of a layer is HK * P * D
 // contiguous values; a unit is 16 KB of one. With `retable`, the table's entries
 // from n_live on follow their pages.
-__global__ void __launch_bounds__(256) move_kernel(PageView c, BooksWork w, uint4* __restrict__ k, uint4* __restrict__ v,
+__global__ void __launch_bounds__(256) move_kernel(PageView c, BooksWork w, uint4* k, uint4* v,
                                                    int retable) {
     stream_turn();
     const int P = 1 << c.page_shift, row_vec = c.D / 8;
@@ -431,11 +431,11 @@ __global__ void __launch_bounds__(256) move_kernel(PageView c, BooksWork w, uint
 // K and V rows of T tokens. VEC: 16 bytes a thread, else one value (rows that do not
 // start on 16 bytes).
 template <typename E>
-__global__ void __launch_bounds__(256) append_kernel(PageView c, int layer, const E* __restrict__ k, int64_t k_token,
-                                                     int64_t k_head, const E* __restrict__ v, int64_t v_token,
-                                                     int64_t v_head, const int32_t* __restrict__ seqs,
-                                                     const int32_t* __restrict__ positions, int T, E* __restrict__ kp,
-                                                     E* __restrict__ vp) {
+__global__ void __launch_bounds__(256) append_kernel(PageView c, int layer, const E* k, int64_t k_token,
+                                                     int64_t k_head, const E* v, int64_t v_token,
+                                                     int64_t v_head, const int32_t* seqs,
+                                                     const int32_t* positions, int T, E* kp,
+                                                     E* vp) {
     stream_turn();
     // E counts in pieces of the row: strides and D come in those
     constexpr int PER = sizeof(E) / 2;
@@ -446,14 +446,16 @@ __global__ void __launch_bounds__(256) append_kernel(PageView c, int layer, cons
         const int64_t th = i / rowp;
         const int h = (int)(th % c.HK);
         const int64_t t = th / c.HK;
+        // (the rows on their way while the page is looked for)
+        const E x = __ldcs(k + t * k_token + h * k_head + d), y = __ldcs(v + t * v_token + h * v_head + d);
         const int s = seqs[t], p = positions[t];
         if (s < 0 || s >= c.n_seq) {
             pages_flag(c, AERO_CUDA_PAGES_BAD_SEQ);
             continue;
         }
-        int page = -1;
-        if (p >= 0 && p < pages_length(c, s)) page = c.table[(int64_t)s * c.max_pages + (p >> c.page_shift)];
-        if ((uint32_t)page >= (uint32_t)c.n_page) {
+        const int held = pages_length(c, s);
+        const int page = p >= 0 && p >> c.page_shift < c.max_pages ? c.table[(int64_t)s * c.max_pages + (p >> c.page_shift)] : -1;
+        if (p >= held || (uint32_t)page >= (uint32_t)c.n_page) {
             pages_flag(c, AERO_CUDA_PAGES_BAD_PAGE);
             continue;
         }
@@ -462,8 +464,8 @@ __global__ void __launch_bounds__(256) append_kernel(PageView c, int layer, cons
             continue;
         }
         const int64_t row = ((((int64_t)layer * c.n_page + page) * c.HK + h) << c.page_shift) + (p & ((1 << c.page_shift) - 1));
-        kp[row * rowp + d] = k[t * k_token + h * k_head + d];
-        vp[row * rowp + d] = v[t * v_token + h * v_head + d];
+        kp[row * rowp + d] = x;
+        vp[row * rowp + d] = y;
     }
 }
 

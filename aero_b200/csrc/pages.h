@@ -26,7 +26,9 @@ struct OnDevice {
 };
 
 // Launches a kernel that begins while the one before it in the stream ends: such a kernel calls
-// stream_turn() before it touches any memory that another kernel may have written or reads.
+// stream_turn() before it touches any memory that another kernel may have written or reads, and reads it
+// by ordinary loads (or __ldcs and the like): those of the read-only path (__ldg, const __restrict__) are
+// for memory that nothing writes while the kernel runs, and it runs before its turn.
 template <typename... P, typename... A>
 cudaError_t launch_in_turn(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A&&... args) {
     cudaLaunchAttribute at{};

@@ -423,8 +423,8 @@ __device__ __noinline__ void rows_again(const AttendArgs& a, const Work& w, int 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(PCfg<D>::threads, 1)
     prompt_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
-                         const __grid_constant__ CUtensorMap vmap, const uint16_t* __restrict__ kp,
-                         const uint16_t* __restrict__ vp, int n_slot, int splits) {
+                         const __grid_constant__ CUtensorMap vmap, const uint16_t* kp,
+                         const uint16_t* vp, int n_slot, int splits) {
     using C = PCfg<D>;
     constexpr int NQ = C::NQ, BN = C::BN, SA = C::SA, PH = C::PH, ST = C::stages, SW = 4 * NQ;  // SW: softmax warps
     extern __shared__ __align__(1024) uint8_t sm[];
