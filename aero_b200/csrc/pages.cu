@@ -734,12 +734,15 @@ int aero_cuda_pages_set_stream(void* cache, void* stream) {
         // a captured stream cannot wait for work outside its graph, nor other work for it: who
         // captures has waited for what went before
         cudaStreamCaptureStatus was = cudaStreamCaptureStatusNone, is = cudaStreamCaptureStatusNone;
-        if (!g.ok(cudaStreamIsCapturing(g.stream, &was), "set_stream") || !g.ok(cudaStreamIsCapturing(to, &is), "set_stream"))
-            return false;
-        if (was != cudaStreamCaptureStatusNone || is != cudaStreamCaptureStatusNone) {
+        const cudaError_t e0 = cudaStreamIsCapturing(g.stream, &was), e1 = cudaStreamIsCapturing(to, &is);
+        if (e0 != cudaSuccess || e1 != cudaSuccess) cudaGetLastError();
+        if ((e0 == cudaSuccess && was != cudaStreamCaptureStatusNone) || (e1 == cudaSuccess && is != cudaStreamCaptureStatusNone)) {
             g.stream = to;
             return true;
         }
+        // (the legacy default stream cannot be asked while a blocking stream is captured: that is no
+        // matter where the other of the two is the one, and an error where it is neither)
+        if (!g.ok(e0, "set_stream") || !g.ok(e1, "set_stream")) return false;
         if (!g.ok(cudaEventRecord(g.moved, g.stream), "set_stream") ||
             !g.ok(cudaStreamWaitEvent(to, g.moved, 0), "set_stream"))
             return false;

@@ -252,3 +252,24 @@ def test_single_tokens_are_as_exact_as_their_type(D, dtype, G):
         err = (got.double() - out).abs()
         assert (err <= tol).all(), f"worst {float((err / tol).max()):.3f} of the tolerance"
     c.check()
+
+
+# ------------------------------------------------------------------ streams
+def test_capture_on_a_blocking_stream_after_the_default_one():
+    """A stream of cudaStreamCreate, which waits for the default stream and the other way round, captured
+    when the cache last ran on the default stream; then calls there again."""
+    import ctypes
+    raw = ctypes.c_void_p()
+    assert int(torch.cuda.cudart().cudaStreamCreate(ctypes.addressof(raw))) == 0
+    s = torch.cuda.ExternalStream(raw.value)
+    c, K, V = open_cache([100, 40], 16, 2, 64, F16)
+    q, seqs = torch.randn((2, 4, 64), device="cuda").half(), i32([0, 1])
+    want = c.attend(0, q, seqs)
+    out = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        c.attend(0, q, seqs, out=out)
+    g.replay()
+    assert torch.equal(out, want) and torch.equal(c.attend(0, q, seqs), want)
+    c.check()
+    torch.cuda.synchronize()
