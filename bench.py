@@ -40,7 +40,8 @@ between steps.
 
 --impl reference times the reference's own CPU block (oracle/_ref) on rank 0
 with all host threads, on the same workload and config, with weights from the
-host generator (no GPU and none of this package's native code on that arm).
+host generator (no GPU and none of this package's native code on that arm);
+where that block is not built it prints {"impl": "reference", "unavailable": why}.
 --profile runs a few layer calls with device-resident inputs and prints the
 per-stage device times: the command the profile summaries are captured from.
 """
@@ -308,7 +309,15 @@ def run_reference(args, ws, wl):
     host generator, so nothing on this arm uses the GPU or this package's
     native library."""
     from aero_b200 import synth
+    sys.path.insert(0, os.path.join(ROOT, "oracle"))
+    import oracle as O
     spec, T = wl.spec, wl.T
+    # the restatement in oracle/ is not the reference: without the reference's own block there is no such arm
+    why = "the reference's own block is not built (oracle/_ref needs the reference's sources)" if not O.ref_available() else \
+        "the reference's block has no shared expert of another width" if spec.Fs and spec.Fs != spec.F else None
+    if why:
+        print(json.dumps({"impl": "reference", "unavailable": why}), flush=True)
+        return
     x = synth.make_x(T * wl.calls, spec.d, 0, bf16=wl.bf16_x)
     layer = synth.make_layer(spec, 0, host_parallel=True)
     if wl.zipf_s:
