@@ -14,7 +14,8 @@ sequence numbers, counts and positions int32. Calls run on torch's current strea
 (or the one given to `set_stream`), enqueue their work and return; they do not
 synchronise and can be captured in a CUDA graph. What only the device knows (lengths,
 free pages) is checked there: `status()` returns the first code recorded, `check()`
-raises it.
+raises it. A cache's calls share its books and workspace: whoever replays graphs that hold them
+orders the replays, among one another and with calls, and a cache is not for two threads at once.
 """
 
 from __future__ import annotations

@@ -22,6 +22,11 @@
  * device: a call that fails there changes nothing (append and copy skip the rows and
  * pages at fault) and records a code for aero_cuda_pages_status. There is no CPU
  * path.
+ *
+ * The calls of a cache share its books and its workspace, so their work runs one call after
+ * another: set_stream orders calls on different streams; replays of graphs that hold calls
+ * of the cache are ordered by their caller, among one another and with calls. A handle is not
+ * for two threads at once.
  */
 #ifndef AERO_CUDA_PAGES_H
 #define AERO_CUDA_PAGES_H

@@ -135,3 +135,69 @@ def test_dense_biases_take_time_in_proportion():
             best = min(best, e0.elapsed_time(e1))
         took.append(best)
     assert took[1] < 16 * took[0] + 0.1
+
+
+def exact_adjust(x, kw):
+    """The definition in 64 bits on the GPU: the adjusted logits, and the largest values met on the way."""
+    rows, vocab = x.shape
+    y = x.double()
+    at = torch.arange(kw["history"].shape[1], device="cuda")[None, :]
+    ids = kw["history"].long()
+    inside = (at < kw["n_history"][:, None]) & (ids >= 0) & (ids < vocab)
+
+    def counted(keep):
+        return torch.zeros((rows, vocab), dtype=torch.float64, device="cuda").scatter_add_(1, ids.clamp(0, vocab - 1), keep.double())
+
+    there, c = counted(inside) > 0, counted(inside & (at >= kw["n_prompt"][:, None]))
+    rep, fr, pr = (kw[n].double()[:, None] for n in ("repetition", "frequency", "presence"))
+    mag = y.abs() * torch.maximum(rep, 1 / rep)
+    y = torch.where(there, torch.where(y > 0, y / rep, y * rep), y)
+    y = torch.where(c > 0, y - fr * c - pr, y)
+    mag = mag + fr.abs() * c + pr.abs()
+    most = 1
+    for r in range(rows):
+        t = kw["bias_token"][int(kw["bias_start"][r]):int(kw["bias_start"][r + 1])].long()
+        v = kw["bias_value"][int(kw["bias_start"][r]):int(kw["bias_start"][r + 1])].double()
+        t, v = t[(t >= 0) & (t < vocab)], v[(t >= 0) & (t < vocab)]
+        y[r].scatter_add_(0, t, v)
+        mag[r].scatter_add_(0, t, v.abs())
+        most = max(most, int(torch.bincount(t).max()) if t.numel() else 0)
+    bit = torch.arange(vocab, device="cuda")
+    allowed = (kw["mask"][:, bit // 32] >> (bit % 32).int()) & 1
+    return torch.where(allowed.bool(), y, torch.full_like(y, -float("inf"))), mag, most
+
+
+@pytest.mark.parametrize("rows,vocab,width,per_row,dtype", [
+    (64, 151937, 300, 8, torch.float32), (64, 151937, 300, 8, torch.bfloat16), (40, 100001, 2000, 64, torch.float16),
+    (70, 152064, 40000, 5, torch.float32), (3, 50001, 70000, 600, torch.bfloat16), (1, 33, 33000, 40, torch.float16),
+    (2, 262145, 50, 0, torch.float32)])
+def test_large_calls_match_plain(rows, vocab, width, per_row, dtype):
+    """Slices of several trips with a remainder, vocabularies that are no multiple of a vector, notes of 32
+    bits (histories wider than 32767, one token repeated more often than 16 bits count), more rows than
+    slices. Tolerance as in test_gpu_logits.py."""
+    from aero_b200.logits import adjust
+    from test_gpu_logits import U
+    g = torch.Generator("cuda").manual_seed(vocab + width)
+    x = torch.randn((rows, vocab), device="cuda", generator=g).mul_(4).to(dtype)
+    history = torch.randint(-2, vocab + 2, (rows, width), device="cuda", generator=g, dtype=torch.int32)
+    if width > 32767:
+        history[:, 100:34000] = vocab // 3  # (33900 times)
+        history[-1, :200] = vocab - 1
+    n = torch.randint(width // 2, width + 1, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    n[0] = width
+    kw = dict(history=history, n_history=n, n_prompt=torch.div(n, 3, rounding_mode="floor").int(),
+              repetition=0.8 + 0.7 * torch.rand(rows, device="cuda", generator=g),
+              frequency=torch.rand(rows, device="cuda", generator=g) / 64, presence=torch.rand(rows, device="cuda", generator=g),
+              bias_start=torch.arange(rows + 1, device="cuda", dtype=torch.int32) * per_row,
+              bias_token=torch.randint(-1, vocab + 1, (rows * per_row,), device="cuda", generator=g, dtype=torch.int32),
+              bias_value=torch.randn(rows * per_row, device="cuda", generator=g),
+              mask=torch.randint(-2**31, 2**31, (rows, (vocab + 31) // 32), device="cuda", generator=g).int())
+    got = adjust(x, **kw)
+    want, mag, most = exact_adjust(x, kw)
+    off = torch.isinf(want)
+    assert torch.equal(torch.isneginf(got), off) and bool(off.any())
+    err = (got.double() - want).abs()[~off]
+    tol = (U[dtype] * want.abs() + 8 * 2.0**-24 * (mag + 1) * (1 + most))[~off]
+    assert (err <= tol).all(), float((err / tol).max())
+    again = x.clone()
+    assert adjust(again, out=again, **kw) is again and torch.equal(again, got)

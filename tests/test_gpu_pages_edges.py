@@ -273,3 +273,89 @@ def test_capture_on_a_blocking_stream_after_the_default_one():
     assert torch.equal(out, want) and torch.equal(c.attend(0, q, seqs), want)
     c.check()
     torch.cuda.synchronize()
+
+
+def test_explicit_stream_and_back():
+    """set_stream with a torch stream and with a raw one: calls run there whatever torch's current stream
+    is, behind what the cache did before; None follows torch's again."""
+    c, K, V = open_cache([100, 40], 16, 2, 64, F16)
+    q, seqs = torch.randn((2, 4, 64), device="cuda").half(), i32([0, 1])
+    k, v = (torch.randn((2, 2, 64), device="cuda").half() for _ in range(2))
+    one, pos = i32([1, 1]), i32([100, 40])
+    out = torch.empty_like(q)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(int(1e8))  # the cache's calls below wait for this one's stream
+        c.extend(seqs, one)
+    c.set_stream(b)
+    c.append(0, k, v, seqs, pos)
+    busy = not b.query()
+    c.set_stream(a.cuda_stream)
+    c.attend(0, q, seqs, out=out)
+    a.synchronize()
+    assert busy
+    want = join([reference(q[i:i + 1], torch.cat([K[i], k[i:i + 1]]), torch.cat([V[i], v[i:i + 1]]), [n], 0, 0, 0.125)
+                 for i, n in enumerate((100, 40))])
+    close(out, want, F16)
+    c.set_stream(None)
+    assert torch.equal(c.attend(0, q, seqs), out)
+    c.check()
+
+
+def test_every_call_in_a_capture():
+    """One graph of all calls (which a call that allocated or synchronised would end), the split form of
+    attend among them, replayed on new data; eager calls on a twin give the same books, pages and outputs."""
+    from aero_b200.logits import adjust
+    from aero_b200.pages import PagedCache
+
+    def setup(seed):
+        c = PagedCache(1, 80, 16, 1, 128, 6, 40, dtype=F16)
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        c.k().normal_(generator=g)
+        c.v().normal_(generator=g)
+        c.extend(i32([0, 1]), i32([600, 37]))
+        return c
+
+    q = torch.randn((40, 8, 128), device="cuda").half()
+    k = torch.randn((3, 1, 128), device="cuda").half()
+    x = torch.randn((2, 1000), device="cuda")
+    outs = [torch.zeros_like(q) for _ in range(2)] + [torch.zeros_like(q[:3]), torch.zeros_like(x)]
+    ids = {n: i32(v) for n, v in dict(s=[0, 1], n=[1, 1], rs=[0, 1, 0], rp=[600, 37, 599], par=[0, 1], kid=[2, 3], gone=[1, 3],
+                                       start=[0, 36, 40], src=[0], dst=[79], three=[0, 2, 0]).items()}
+    hist, hn = i32(range(20)).reshape(2, 10), i32([10, 4])
+
+    def step(c, outs):
+        c.extend(ids["s"], ids["n"])
+        c.append(0, k, k, ids["rs"], ids["rp"])
+        c.attend(0, q, ids["s"], ids["start"], out=outs[0])
+        c.fork(ids["par"], ids["kid"])
+        c.attend(0, q, ids["s"], ids["start"], window=100, sinks=3, out=outs[1])
+        c.free(ids["gone"])
+        c.copy(ids["src"], ids["dst"])
+        c.compact()
+        c.attend(0, q[:3], ids["three"], out=outs[2])
+        adjust(x, history=hist, n_history=hn, repetition=rep, out=outs[3])
+
+    rep = torch.full((2,), 1.5, device="cuda")
+    step(setup(0), [o.clone() for o in outs])  # kernels loaded
+    c, twin = setup(1), setup(1)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        step(c, outs)
+    q.normal_()
+    k.normal_()
+    x.normal_()
+    torch.cuda.synchronize()
+    g.replay()
+    torch.cuda.synchronize()
+    mine = [o.clone() for o in outs]
+    step(twin, outs)
+    assert all(torch.equal(a, b) for a, b in zip(mine, outs)) and mine[0].abs().max() > 0
+    assert all(torch.equal(a, b) for a, b in zip(c.tables(), twin.tables()))
+    assert torch.equal(c.k(), twin.k()) and torch.equal(c.v(), twin.v())
+    c.check()
+    twin.check()
