@@ -8,7 +8,7 @@
 // slice. Slices are as wide as shared memory allows and the number of rows asks for, so that all
 // CTAs run at once and a history is read few times: with slices of 8192 tokens every CTA of the
 // 19 of a row read it, and three waves of CTAs each waited for it (64 rows of 151936 with 8192
-// tokens of history: 31 us). Counts are integer sums, so their order does not matter; the
+// tokens of history: 31 us; as it is 21 us, of which HBM's share is 12.6). Counts are integer sums, so their order does not matter; the
 // biases of one token are added by its own thread in the list's order. A slice that more of them
 // name (the list's place holds kBiasList) is streamed with the biased tokens left as they are, and those
 // are adjusted after it: for 2 kBiasList tokens at a time a warp adds the row's list up in the list's

@@ -86,8 +86,10 @@ __device__ __forceinline__ int4 refs4(const PageView& c, int p0) {
     return r;
 }
 
-// w.list[0 .. want) = the lowest free pages; false when there are fewer. (A full pool of 65536 pages
-// would take 16 steps from its beginning; a decode step's extend finds its pages in the first.)
+// w.list[0 .. want) = the lowest free pages; false when there are fewer. The scan begins at w.lowest, 4096
+// pages a step, so a decode step's extend finds its pages in the first steps where they lie just above
+// it; where they do not, it walks the held pages between (a pool of 2^20 pages with one free: at its
+// beginning 8 us, in its middle 124, at its end 238, once).
 __device__ bool lowest_free(const PageView& c, const BooksWork& w, int want) {
     int32_t* list = w.list;
     int found = 0;
@@ -897,10 +899,12 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
         a.vec = aero::vec16(q, q_token, q_head) && aero::vec16(out, o_token, o_head);
         const bool bf16 = g.d.dtype == AERO_CUDA_TYPE_BF16;
         // Few tokens, or hardly more than one a sequence, go token by token: a tile of 128 rows
-        // would be mostly empty, and its CTA costs some 15 us before it is done (B200, 4 x 8 heads of
-        // 128, tokens against tiles: 16 tokens over 4096 positions 27 / 34 us, 32 of 16 sequences
-        // over 2000 28 / 33, 64 of 64 over 2000 57 / 82; but 64 of one over 4096 61 / 47, 128 of 64
-        // over 2000 95 / 84).
+        // would be mostly empty, and its CTA costs some 12 us before it is done (B200, 4 x 8 heads of
+        // 128, tokens against tiles: 8 tokens over 1000 positions 12 / 15 us, 16 over 4096 22 / 25, 32 of
+        // 16 sequences over 2000 23 / 26, 64 of 64 over 2000 53 / 79; but 64 of one over 4096 48 / 38, 128
+        // of 64 over 2000 91 / 80). The lengths, which the host does not know, would move the line: each
+        // token reads its sequence again (8 of one over 32768 47 / 43, 32 of one 148 / 71, 32 of 8 over 8000
+        // 51 / 44), and a batch of one prompt and many single tokens is not divided.
         const bool by_token = !q_start || T <= 32 || T < 2 * (int64_t)n;
         if (!by_token) {
             a.part = g.prompt_part;

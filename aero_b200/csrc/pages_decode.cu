@@ -6,8 +6,8 @@
 // and two partial results join by the same rule.
 //
 // Bound by HBM: every visible K and V row is read once (up to 16 query heads share it,
-// at most 16 operations a byte). Measured: 48 sequences of 8192 to 32768 positions, 32 query
-// heads on 4 kv heads of 128, 279 us (1.85 GB: 6.6 TB/s); one sequence of 4096 12.6 us, of 20 5.4 us,
+// at most 16 operations a byte). Measured, time on the GPU: 48 sequences of 8192 to 32768 positions, 32
+// query heads on 4 kv heads of 128, 281 us (1.85 GB: 6.6 TB/s); one sequence of 4096 13.6 us, of 20 5.3 us,
 // where a launch, the chain from lengths to pages to rows, and the join set the time.
 //
 // Split: the work of the call is one line of units, unit = 64 positions of one
@@ -21,11 +21,11 @@
 // rows per head; a box of min(page, 64) rows by 64 columns, swizzled), four consumer warps
 // take 16 positions of each unit as S^T = K Q^T and O^T += V^T P^T in m16n8k16 products, the kv
 // head's query heads as the 8 or 16 columns (as rows they would be padded to 16, with twice the
-// products and sums: 13.6 against 12.6 us for one sequence of 4096, 288 against 279 us for the long
-// ones), each warp with its own m, l, o until the segment's end. The consumers never wait for one
-// another within a segment. An SM's share of HBM takes 1400 cycles for a unit's 32 KB (head size
-// 128), a warp's part of it some 800: the unit's bytes, not its products, set the time, so
-// tcgen05's 128 rows would not help.
+// products and sums: 8 % more for one sequence of 4096, 3 % for the long ones), each warp with its own
+// m, l, o until the segment's end. The consumers never wait for one another within a segment. An SM's
+// share of HBM takes 1400 cycles for a unit's 32 KB (head size 128); the matrix pipe is active for 15 %
+// of them, issue slots for 21 %: the unit's bytes, not its products, set the time, so tcgen05's 128
+// rows would not help.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -84,7 +84,7 @@ __device__ __forceinline__ bool visible(const Span& p, int j) { return j < p.n &
 // (sequence, head)s of up to kWhole units are left whole: joining parts costs more than those few
 // units one after another. Longer ones are cut into about kParts parts, as many as a join reads at
 // once, of 2 to 4 units, if possible an even cut, so that no part holds the end of one and the
-// beginning of the next (one sequence of 4096, 64 units: parts of 3 15.0 us, of 4 12.6 us).
+// beginning of the next (one sequence of 4096, 64 units: parts of 3 take 2.4 us more than of 4).
 __device__ __forceinline__ int64_t piece_length(int64_t total, int64_t segments) {
     const int64_t each = (total + segments - 1) / segments, share = (total + gridDim.x - 1) / gridDim.x;
     if (each <= kWhole) return max(each, share);

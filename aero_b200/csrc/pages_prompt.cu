@@ -6,8 +6,9 @@
 // Bound by the tensor cores and, as much, by the exponentials: a step of two row tiles of 128
 // rows by 128 positions at head size 128 is 4 x 2.1 M multiply-adds (2048 cycles of an SM's
 // tcgen05 pipe) and 2 x 16384 exponentials (2048 cycles at 16 a cycle). Measured: 2600 cycles a
-// step; a prompt of 4096 tokens of 32 query heads on 4 kv heads 134 us (1020 TFLOP/s of the causal
-// half), of 16384 tokens 1.75 ms cold (1257), 1.9 ms in a row under the power cap.
+// step; a prompt of 4096 tokens of 32 query heads on 4 kv heads 126 us (1090 TFLOP/s of the causal
+// half), of 16384 tokens 1.66 ms cold (1330), 1.81 ms in a row under the power cap. Head size 64, 8192
+// tokens: 379 us (725); 256, 16 query heads on 2, 8192 tokens: 514 us (1070).
 //
 // Layout: a row is one (token, query head); the rows of a sequence's kv head, its group of
 // query heads innermost, are cut into tiles of 128, so a K/V tile in shared memory serves
@@ -24,12 +25,17 @@
 // other's softmax. (With an S of its own for each, which P then overwrites, the two fall into
 // step and wait together: 881 against 1100 TFLOP/s at 16384 tokens; with two S of 64 positions
 // each, Q is read twice as often from shared memory, whose 128 bytes a cycle then bind: 1000.) One
-// row tile has two S buffers instead and writes P over S. O is rescaled only when a row's
-// maximum has grown by more than 2^8 since it was last: until then the weights are at most
-// 2^8, as exact as any in f16, bf16 and the f32 sums, but the largest is no longer 1, which those
-// types hold without rounding. In bf16 the output's distance from the exact one is 1.37 times that
-// of rounding the exact one; rescaled at every growth 1.14 times, for 10 % more time (four
-// windowed prompts 113 -> 124 us, 4096 tokens 131 -> 149 us), at growths past 2^3 1.23 times for 7 %.
+// row tile has two S buffers instead and writes P over S.
+//
+// Exactness: scores, m, l and O are f32. A weight meets V rounded to the cache's type, which moves the
+// output about as far as its own rounding does, so it comes out up to 1.4 times as far from the exact one
+// as rounding that would be (four windowed prompts in bf16 0.0023 against 0.0017 of the output's norm,
+// 16384 tokens in f16 0.00027 against 0.00020). Weights as two values of the type, as for single tokens,
+// would be half as many products again, and products bind here. O is rescaled only when a row's maximum
+// has grown by more than 2^8 since it was last: the weights are as exact relative to their size, but the
+// largest is no longer a power of two, which would not round. Rescaled at every growth: 0.0019 and
+// 0.00023, for 108 -> 119 us, 1.81 -> 2.11 ms, 4096 tokens 126 -> 148 us and at head size 256 149 -> 239 us;
+// with the sum of the rounded weights for l: 0.0021 and 0.00026, for 108 -> 111 us and 1.81 -> 1.96 ms.
 //
 // Few row tiles over a long cache: the positions of a row tile are split over several
 // CTAs that leave (o, m, l); the last to arrive joins them in order.
@@ -809,8 +815,8 @@ __global__ void __launch_bounds__(PCfg<D>::threads, 1)
                         p1 = ex2(p1);
                     }
                     sum[e & 1] = add2(sum[e & 1], pair(p0, p1));
-                    // the weights meet V in its type: a relative rounding of 2^-11 (f16) or 2^-8
-                    // (bf16) each, below the output's own; their sum l stays f32
+                    // the weights meet V in its type: a relative rounding of up to 2^-11 (f16) or 2^-8 (bf16)
+                    // each, as much as the output's own; their sum l stays f32
                     p[e] = pack16<BF16>(p0, p1);
                 }
                 tmem_st16(pt + c * 16, p);

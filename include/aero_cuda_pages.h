@@ -20,8 +20,8 @@
  * allocate and does not synchronise, so calls can be captured in a CUDA graph. What
  * the host cannot see (sequence numbers, lengths, free pages) is checked on the
  * device: a call that fails there changes nothing (append and copy skip the rows and
- * pages at fault) and records a code for aero_cuda_pages_status. There is no CPU
- * path.
+ * pages at fault, free the places of a sequence's row that hold no page) and records a
+ * code for aero_cuda_pages_status. There is no CPU path.
  *
  * The calls of a cache share its books and its workspace, so their work runs one call after
  * another: set_stream orders calls on different streams; replays of graphs that hold calls
@@ -118,8 +118,10 @@ int aero_cuda_pages_compact(void* cache);
  * sequence) its output is 0. scores = scale * q . k with a positive, finite scale; softmax statistics and sums
  * are f32. The probabilities meet V as two values of the cache's type where tokens go one
  * by one (q_start NULL, at most 32 tokens, or fewer than two a sequence), so the output is as
- * exact as its own rounding; else as one value. Values of positions past a
- * sequence's length are never used; a visible position without a page is recorded and
+ * exact as its own rounding; else as one value, which leaves it up to 1.4 times as far from
+ * the exact one. A column of V that is not finite where a token sees it leaves that column
+ * of the token's output not finite (infinite or no number), and nothing else. Values of
+ * positions past a sequence's length are never used; a visible position without a page is recorded and
  * counts as a key and a value of zeros. */
 int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
                            const int32_t* seqs, const int32_t* q_start, int n, float scale, int window, int sinks,

@@ -286,7 +286,7 @@ def test_explicit_stream_and_back():
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
     torch.cuda.synchronize()
     with torch.cuda.stream(a):
-        torch.cuda._sleep(int(1e8))  # the cache's calls below wait for this one's stream
+        torch.cuda._sleep(int(4e8))  # the cache's calls below wait for this one's stream
         c.extend(seqs, one)
     c.set_stream(b)
     c.append(0, k, v, seqs, pos)
