@@ -386,7 +386,7 @@ __device__ __noinline__ void rows_again(const AttendArgs& a, const Work& w, int 
     for (int j = first + 1 + lane; j <= w.p1; j += 32)
         if (bad(j)) behind = j;
     if (a.window)
-        for (int j = max(w.lo, a.sinks) + lane; j <= last - a.window; j += 32)
+        for (int j = max(w.lo, min(a.sinks, w.p1 + 1)) + lane; j <= last - a.window; j += 32)
             if (bad(j)) before = min(before, j);
     behind = __reduce_max_sync(0xffffffffu, behind);
     before = __reduce_min_sync(0xffffffffu, before);

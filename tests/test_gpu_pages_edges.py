@@ -143,6 +143,23 @@ def test_rows_beside_values_that_are_not_finite(n, T, P, HK, G, D, dtype, window
     assert torch.equal(got.nan_to_num(0, 1, -1), c.attend(0, q, i32([0]), i32([0, T]), window=window, sinks=sinks).nan_to_num(0, 1, -1))
 
 
+@pytest.mark.parametrize("window,sinks", [(100, 2**31 - 1), (2**31 - 1, 3), (2**31 - 1, 2**31 - 1), (1, 2**31 - 1)])
+def test_largest_windows_and_sinks_beside_bad_values(window, sinks):
+    """As many first tokens or as wide a window as 32 bits hold: plain causal attention, also where rows
+    are computed again."""
+    c, K, V = open_cache([500], 16, 1, 64, F16)
+    q = torch.randn((300, 4, 64), device="cuda").half()
+    poke(c, c.v(0), 333, math.inf)
+    want = c.attend(0, q, i32([0]), i32([0, 300]))
+    got = c.attend(0, q, i32([0]), i32([0, 300]), window=window, sinks=sinks)
+    c.check()
+    pick = [0, 5, 130, 131, 132]
+    close(got[pick], reference(q[pick], K[0], V[0], [200 + t for t in pick], 0, 0, 0.125), F16)
+    assert not torch.isfinite(got[133:]).any() and not torch.isfinite(want[133:]).any()
+    one = c.attend(0, q[:1], i32([0]), window=window, sinks=sinks)
+    assert not torch.isfinite(one).any()
+
+
 # ------------------------------------------------------------------ tables with holes
 def holes(c, pages, seq=0):
     """The books with these places of a sequence's row empty, as a keeper of books elsewhere may have them."""
