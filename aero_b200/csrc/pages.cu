@@ -390,8 +390,8 @@ constexpr int kMoveVec = 4;  // 16-byte pieces a thread moves per unit, all load
 constexpr int kMoveUnit = 256 * kMoveVec;
 
 // The jobs' rows, in every layer and kv head of K and V: a page of a layer is HK * P * D
-// contiguous values; a unit is 16 KB of one. With `retable`, the table's entries
-// from n_live on follow their pages.
+// contiguous values; a unit is 16 KB of one. Then the pages' bounds, where they are kept: HK * 2 * D
+// values of a page. With `retable`, the table's entries from n_live on follow their pages.
 __global__ void __launch_bounds__(256) move_kernel(PageView c, BooksWork w, uint4* k, uint4* v,
                                                    int retable) {
     stream_turn();
@@ -407,21 +407,25 @@ __global__ void __launch_bounds__(256) move_kernel(PageView c, BooksWork w, uint
             if (p >= L && p < c.n_page) c.table[i] = w.to[p];
         }
     }
-    const int64_t per_job = (int64_t)c.n_layer * 2 * pieces;
+    const int bound_vec = c.bounds ? c.HK * 2 * row_vec : 0, bound_pieces = (bound_vec + kMoveUnit - 1) / kMoveUnit;
+    const int64_t per_job = (int64_t)c.n_layer * (2 * pieces + bound_pieces);
     const int64_t units = (int64_t)*w.n_jobs * per_job;
     for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
         const PageJob j = w.jobs[u / per_job];
         const int r = (int)(u % per_job);  // n_layer * 2 * pieces fits: the host checks
-        const int layer = r / (2 * pieces), kv = (r / pieces) & 1, piece = r % pieces;
-        uint4* pool = kv ? v : k;
-        const uint4* s = pool + ((int64_t)layer * c.n_page + j.src) * page_vec;
-        uint4* d = pool + ((int64_t)layer * c.n_page + j.dst) * page_vec;
+        const bool rows = r < c.n_layer * 2 * pieces;
+        const int rb = r - c.n_layer * 2 * pieces;  // (of the bounds)
+        const int layer = rows ? r / (2 * pieces) : rb / bound_pieces, piece = rows ? r % pieces : rb % bound_pieces;
+        uint4* pool = !rows ? reinterpret_cast<uint4*>(c.bounds) : (r / pieces) & 1 ? v : k;
+        const int vecs = rows ? page_vec : j.rows ? bound_vec : 0;
+        const uint4* s = pool + ((int64_t)layer * c.n_page + j.src) * (rows ? page_vec : bound_vec);
+        uint4* d = pool + ((int64_t)layer * c.n_page + j.dst) * (rows ? page_vec : bound_vec);
         uint4 x[kMoveVec];
         bool on[kMoveVec];
 #pragma unroll
         for (int i = 0; i < kMoveVec; ++i) {
             const int at = piece * kMoveUnit + i * 256 + (int)threadIdx.x;
-            on[i] = at < page_vec && ((at / row_vec) & (P - 1)) < j.rows;
+            on[i] = at < vecs && (!rows || ((at / row_vec) & (P - 1)) < j.rows);
             if (on[i]) x[i] = __ldcs(s + at);
         }
 #pragma unroll
@@ -480,7 +484,7 @@ struct Pages {
     PageView view{};
     BooksWork work{};
     void *k = nullptr, *v = nullptr, *books = nullptr;  // v: behind k, in one allocation
-    size_t pool_bytes = 0, books_bytes = 0;
+    size_t pool_bytes = 0, books_bytes = 0, bounds_bytes = 0;
     float *decode_part = nullptr, *prompt_part = nullptr;
     uint32_t *decode_count = nullptr, *prompt_count = nullptr;
     CUtensorMap kmap{}, vmap{};
@@ -504,6 +508,7 @@ struct Pages {
         if (stream) cudaStreamSynchronize(stream);
         if (k) guarded_free(k, pool_bytes, kKVCache);
         if (books) guarded_free(books, books_bytes, kScratch);
+        if (view.bounds) guarded_free(view.bounds, bounds_bytes, kKVCache);
         if (moved) cudaEventDestroy(moved);
         if (own_stream) cudaStreamDestroy(own_stream);
     }
@@ -531,6 +536,11 @@ const char* bad_desc(const aero_cuda_pages_desc& d) {
     if ((double)d.n_seq * d.max_pages > 1073741824.0 || (double)d.max_pages * d.page_size > 1073741824.0)
         return "n_seq * max_pages and max_pages * page_size must be at most 2^30";
     return nullptr;
+}
+
+// Bytes of the pages' bounds.
+size_t bounds_size(const aero_cuda_pages_desc& d) {
+    return (size_t)d.n_layer * d.n_page * d.n_head_kv * 2 * d.head_dim * 2;
 }
 
 struct Layout {
@@ -671,7 +681,8 @@ bool listed(Pages& g, const void* a, const char* an, const void* b, const char* 
 cudaError_t launch_move(Pages& g, int64_t max_jobs, int retable) {
     const PageView& c = g.view;
     const int64_t page_vec = (int64_t)c.HK * (c.D / 8) << c.page_shift;
-    const int64_t units = max_jobs * c.n_layer * 2 * ((page_vec + kMoveUnit - 1) / kMoveUnit);
+    const int64_t bound_vec = c.bounds ? (int64_t)c.HK * 2 * (c.D / 8) : 0;
+    const int64_t units = max_jobs * c.n_layer * (2 * ((page_vec + kMoveUnit - 1) / kMoveUnit) + (bound_vec + kMoveUnit - 1) / kMoveUnit);
     const int64_t books = retable ? ((int64_t)c.n_seq * c.max_pages + 255) / 256 : 0;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(std::max(units, books), (int64_t)g.n_sm * 8));
     return launch_in_turn(move_kernel, grid, 256, 0, g.stream, c, g.work, static_cast<uint4*>(g.k), static_cast<uint4*>(g.v),
@@ -686,6 +697,46 @@ bool layer_ok(Pages& g, int layer) {
 bool vec16(const void* p, int64_t token, int64_t head) {
     return ((uintptr_t)p & 15) == 0 && token % 8 == 0 && head % 8 == 0;
 }
+
+// What the calls that take queries ask of their numbers, and of their arrays.
+bool tokens_ok(Pages& g, int layer, int T, int n_head, const int32_t* q_start, int n) {
+    if (!layer_ok(g, layer)) return false;
+    const int HK = g.d.n_head_kv;
+    if (n_head <= 0 || n_head % HK || n_head / HK > 16)
+        return g.fail("n_head must be a multiple of n_head_kv = %d, at most 16 times it; got %d", HK, n_head);
+    if (T < 0 || n < 0 || T > (1 << 24) || n > (1 << 20)) return g.fail("T must be from 0 to 2^24, n from 0 to 2^20");
+    if (!q_start && T != n) return g.fail("without q_start T must be n, one token per sequence (T %d, n %d)", T, n);
+    if (q_start && T > 0 && n == 0) return g.fail("%d tokens of no sequence", T);
+    return true;
+}
+bool query_ok(Pages& g, const void* q, const int32_t* seqs, const int32_t* q_start) {
+    if (!is_device_ptr(q)) return g.fail("q must be device memory");
+    if ((uintptr_t)q & 1) return g.fail("q must be aligned to its type");
+    return device_i32(g, seqs, "seqs") && (!q_start || device_i32(g, q_start, "q_start"));
+}
+bool attend_args(Pages& g, AttendArgs& a, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
+                 const int32_t* seqs, const int32_t* q_start, int n, float scale, void* out, int64_t o_token, int64_t o_head) {
+    if (!is_device_ptr(q) || !is_device_ptr(out)) return g.fail("q and out must be device memory");
+    if (((uintptr_t)q | (uintptr_t)out) & 1) return g.fail("q and out must be aligned to their type");
+    if (!query_ok(g, q, seqs, q_start)) return false;
+    a.c = g.view;
+    a.q = q;
+    a.q_token = q_token;
+    a.q_head = q_head;
+    a.out = out;
+    a.o_token = o_token;
+    a.o_head = o_head;
+    a.seqs = seqs;
+    a.q_start = q_start;
+    a.layer = layer;
+    a.T = T;
+    a.n = n;
+    a.H = n_head;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.vec = vec16(q, q_token, q_head) && vec16(out, o_token, o_head);
+    return true;
+}
+bool bounds_ok(Pages& g) { return g.view.bounds || g.fail("the cache keeps no bounds (aero_cuda_pages_keep_bounds)"); }
 
 }  // namespace
 }  // namespace aero
@@ -819,7 +870,9 @@ int aero_cuda_pages_append(void* cache, int layer, const void* k, int64_t k_toke
                                         k_token / per, k_head / per, static_cast<const E*>(v), v_token / per, v_head / per,
                                         seqs, positions, T, static_cast<E*>(g.k), static_cast<E*>(g.v));
         };
-        return g.ok(vec ? launch(uint4{}) : launch(uint16_t{}), "append");
+        return g.ok(vec ? launch(uint4{}) : launch(uint16_t{}), "append") &&
+               (!g.view.bounds || g.ok(aero::launch_append_bounds(g.view, g.d.dtype == AERO_CUDA_TYPE_BF16, layer, g.k, seqs, positions,
+                                                                  T, g.n_sm, g.stream), "append"));
     });
 }
 
@@ -866,37 +919,14 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
                            const int32_t* seqs, const int32_t* q_start, int n, float scale, int window, int sinks,
                            void* out, int64_t o_token, int64_t o_head) {
     return aero::entry(cache, [&](Pages& g) {
-        if (!aero::layer_ok(g, layer)) return false;
-        const int HK = g.d.n_head_kv;
-        if (n_head <= 0 || n_head % HK || n_head / HK > 16)
-            return g.fail("n_head must be a multiple of n_head_kv = %d, at most 16 times it; got %d", HK, n_head);
-        if (T < 0 || n < 0 || T > (1 << 24) || n > (1 << 20)) return g.fail("T must be from 0 to 2^24, n from 0 to 2^20");
-        if (!q_start && T != n) return g.fail("without q_start T must be n, one token per sequence (T %d, n %d)", T, n);
-        if (q_start && T > 0 && n == 0) return g.fail("%d tokens of no sequence", T);
+        if (!aero::tokens_ok(g, layer, T, n_head, q_start, n)) return false;
         if (window < 0 || sinks < 0) return g.fail("window and sinks must be >= 0");
         if (!(scale > 0.f) || !(scale < 1e30f)) return g.fail("scale must be positive and finite");
         if (T == 0) return true;
-        if (!aero::is_device_ptr(q) || !aero::is_device_ptr(out)) return g.fail("q and out must be device memory");
-        if (((uintptr_t)q | (uintptr_t)out) & 1) return g.fail("q and out must be aligned to their type");
-        if (!aero::device_i32(g, seqs, "seqs") || (q_start && !aero::device_i32(g, q_start, "q_start"))) return false;
         aero::AttendArgs a{};
-        a.c = g.view;
-        a.q = q;
-        a.q_token = q_token;
-        a.q_head = q_head;
-        a.out = out;
-        a.o_token = o_token;
-        a.o_head = o_head;
-        a.seqs = seqs;
-        a.q_start = q_start;
-        a.layer = layer;
-        a.T = T;
-        a.n = n;
-        a.H = n_head;
+        if (!aero::attend_args(g, a, layer, q, q_token, q_head, T, n_head, seqs, q_start, n, scale, out, o_token, o_head)) return false;
         a.window = window;
         a.sinks = window ? sinks : 0;
-        a.scale_log2 = scale * 1.4426950408889634f;
-        a.vec = aero::vec16(q, q_token, q_head) && aero::vec16(out, o_token, o_head);
         const bool bf16 = g.d.dtype == AERO_CUDA_TYPE_BF16;
         // Few tokens, or hardly more than one a sequence, go token by token: a tile of 128 rows
         // would be mostly empty, and its CTA costs some 12 us before it is done (B200, 4 x 8 heads of
@@ -914,6 +944,94 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
         a.part = g.decode_part;
         a.counters = g.decode_count;
         return g.ok(aero::launch_pages_decode(a, bf16, g.kmap, g.vmap, g.n_sm, g.stream), "attend");
+    });
+}
+
+int64_t aero_cuda_pages_bounds_bytes(const aero_cuda_pages_desc* desc) {
+    return !desc || aero::bad_desc(*desc) ? -1 : (int64_t)aero::bounds_size(*desc);
+}
+
+int aero_cuda_pages_keep_bounds(void* cache) {
+    return aero::entry(cache, [&](Pages& g) {
+        if (g.view.bounds) return true;
+        const size_t bytes = aero::bounds_size(g.d);
+        void* p = nullptr;
+        if (aero::guarded_malloc(&p, bytes, aero::kKVCache) != cudaSuccess) {
+            cudaGetLastError();
+            return g.fail("device allocation for the bounds refused (memory guard budget or device memory)");
+        }
+        if (!g.ok(cudaMemsetAsync(p, 0, bytes, g.stream), "keep_bounds") || !g.ok(cudaStreamSynchronize(g.stream), "keep_bounds")) {
+            aero::guarded_free(p, bytes, aero::kKVCache);
+            return false;
+        }
+        g.view.bounds = static_cast<uint16_t*>(p);
+        g.bounds_bytes = bytes;
+        return true;
+    });
+}
+
+void* aero_cuda_pages_bounds(void* cache) {
+    auto* g = static_cast<Pages*>(cache);
+    return g ? g->view.bounds : nullptr;
+}
+
+int aero_cuda_pages_set_bounds(void* cache, int layer, const int32_t* seqs, int n) {
+    return aero::entry(cache, [&](Pages& g) {
+        if (!aero::layer_ok(g, layer) || !aero::bounds_ok(g) || !aero::listed(g, seqs, "seqs", nullptr, "", n)) return false;
+        if (n == 0) return true;
+        return g.ok(aero::launch_set_bounds(g.view, g.d.dtype == AERO_CUDA_TYPE_BF16, layer, g.k, seqs, n, g.n_sm, g.stream), "set_bounds");
+    });
+}
+
+int aero_cuda_pages_select(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
+                           const int32_t* seqs, const int32_t* q_start, int n, int first, int recent, int n_blocks,
+                           int32_t* blocks) {
+    return aero::entry(cache, [&](Pages& g) {
+        if (!aero::bounds_ok(g) || !aero::tokens_ok(g, layer, T, n_head, q_start, n)) return false;
+        if (first < 0 || recent < 1) return g.fail("first must be >= 0 and recent >= 1");
+        if ((int64_t)first + recent > n_blocks || n_blocks > (1 << 27))
+            return g.fail("n_blocks must be from first + recent = %lld to 2^27, got %d", (long long)first + recent, n_blocks);
+        if (g.d.max_pages > aero::kSelectPages)
+            return g.fail("select serves sequences of up to %d pages, the cache's are of up to %d", aero::kSelectPages, g.d.max_pages);
+        if ((int64_t)T * g.d.n_head_kv > (1 << 24)) return g.fail("T * n_head_kv must be at most 2^24");
+        if (T == 0) return true;
+        aero::SelectArgs a{};
+        if (!aero::query_ok(g, q, seqs, q_start) || !aero::device_i32(g, blocks, "blocks")) return false;
+        a.c = g.view;
+        a.q = q;
+        a.q_token = q_token;
+        a.q_head = q_head;
+        a.seqs = seqs;
+        a.q_start = q_start;
+        a.layer = layer;
+        a.T = T;
+        a.n = n;
+        a.H = n_head;
+        a.first = first;
+        a.recent = recent;
+        a.width = n_blocks;
+        a.out = blocks;
+        return g.ok(aero::launch_select(a, g.d.dtype == AERO_CUDA_TYPE_BF16, g.n_sm, g.stream), "select");
+    });
+}
+
+int aero_cuda_pages_attend_blocks(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
+                                  const int32_t* seqs, const int32_t* q_start, int n, const int32_t* blocks, int n_blocks,
+                                  float scale, void* out, int64_t o_token, int64_t o_head) {
+    return aero::entry(cache, [&](Pages& g) {
+        if (!aero::tokens_ok(g, layer, T, n_head, q_start, n)) return false;
+        if (!(scale > 0.f) || !(scale < 1e30f)) return g.fail("scale must be positive and finite");
+        if (n_blocks < 1 || n_blocks > (1 << 27)) return g.fail("n_blocks must be from 1 to 2^27, got %d", n_blocks);
+        if (T == 0) return true;
+        aero::AttendArgs a{};
+        if (!aero::attend_args(g, a, layer, q, q_token, q_head, T, n_head, seqs, q_start, n, scale, out, o_token, o_head) ||
+            !aero::device_i32(g, blocks, "blocks"))
+            return false;
+        a.blocks = blocks;
+        a.width = n_blocks;
+        a.part = g.decode_part;
+        a.counters = g.decode_count;
+        return g.ok(aero::launch_pages_decode(a, g.d.dtype == AERO_CUDA_TYPE_BF16, g.kmap, g.vmap, g.n_sm, g.stream), "attend_blocks");
     });
 }
 

@@ -1,6 +1,7 @@
 // The paged key/value cache (include/aero_cuda_pages.h): what its translation
 // units share. pages.cu owns the handle and the books, pages_decode.cu the
-// attention of single tokens, pages_prompt.cu that of several tokens a sequence.
+// attention of single tokens, over all positions or over listed blocks, pages_prompt.cu that of
+// several tokens a sequence, pages_select.cu the bounds of pages and the choice of blocks.
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -51,6 +52,7 @@ struct PageView {
     int32_t* refs;    // (n_page)
     int32_t* status;  // first code recorded, 0: none
     int32_t n_page, page_shift, HK, D, n_seq, max_pages, n_layer;
+    uint16_t* bounds;  // (n_layer, n_page, HK, 2, D) smallest and largest key values; null: not kept
 };
 
 #if defined(__CUDACC__)
@@ -87,11 +89,25 @@ struct AttendArgs {
     int over;           // places of pages_decode.cu's line that stand for a beginning and an end
     float* part;        // partial results of units that several CTAs share
     uint32_t* counters; // arrivals per shared unit; zero between launches
+    const int32_t* blocks;  // (T, HK, width) blocks that a token's kv head attends to; null: all positions
+    int width;
+};
+
+// One choice of blocks.
+struct SelectArgs {
+    PageView c;
+    const void* q;
+    int64_t q_token, q_head;
+    const int32_t* seqs;
+    const int32_t* q_start;
+    int layer, T, n, H, first, recent, width;
+    int32_t* out;  // (T, HK, width)
 };
 
 #if defined(__CUDACC__)
 // By one CTA of a launch: q_start ascends from 0 to T.
-__device__ __forceinline__ void check_q_start(const AttendArgs& a) {
+template <typename A>
+__device__ __forceinline__ void check_q_start(const A& a) {
     bool bad = false;
     for (int i = threadIdx.x; i < a.n; i += blockDim.x) bad |= a.q_start[i] > a.q_start[i + 1];
     if (threadIdx.x == 0) bad |= a.q_start[0] != 0 || a.q_start[a.n] != a.T;
@@ -99,7 +115,8 @@ __device__ __forceinline__ void check_q_start(const AttendArgs& a) {
 }
 // Which sequence token t is of, and how many of its positions the token sees at most
 // (its own position + 1). q_start is searched within its n + 1 entries whatever they hold.
-__device__ __forceinline__ void token_rows(const AttendArgs& a, int t, int& seq, int& n) {
+template <typename A>
+__device__ __forceinline__ void token_rows(const A& a, int t, int& seq, int& n) {
     if (!a.q_start) {
         seq = a.seqs[t];
         n = pages_length(a.c, seq);
@@ -138,5 +155,13 @@ cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMa
 // k, v: the pool itself.
 cudaError_t launch_pages_prompt(const AttendArgs& a, bool bf16, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                 const void* k, const void* v, int n_sm, cudaStream_t s);
+// Bounds of the pages that n sequences hold, and of the pages that an append of T tokens wrote to.
+cudaError_t launch_set_bounds(const PageView& c, bool bf16, int layer, const void* k, const int32_t* seqs, int n, int n_sm,
+                              cudaStream_t s);
+cudaError_t launch_append_bounds(const PageView& c, bool bf16, int layer, const void* k, const int32_t* seqs,
+                                 const int32_t* positions, int T, int n_sm, cudaStream_t s);
+// Pages a sequence may hold at most for launch_select.
+constexpr int kSelectPages = 131072;
+cudaError_t launch_select(const SelectArgs& a, bool bf16, int n_sm, cudaStream_t s);
 
 }  // namespace aero

@@ -43,6 +43,7 @@ constexpr int kConsumers = 4;      // warps; each takes 16 positions of a unit
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kWhole = 8, kParts = 16;  // see piece_length
 constexpr int kHalf = kUnit * 128; // bytes of a unit's 64-column half
+constexpr int kNowhere = 1 << 30;  // a position that no token sees (sequences hold at most 2^30)
 
 template <int D>
 struct Cfg {
@@ -66,10 +67,20 @@ struct Span {
     int tiles;  // at least 1: an empty sequence has a unit that writes zeros
 };
 
+// Over listed blocks (SEL) a kv head's units are the list's: 64 positions of it in its order, `first`
+// entries of it at all. No list has more blocks that the token sees than there are, so of a
+// longer one the entries behind that many are not looked at.
+template <bool SEL>
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int e) {
     Span p;
     token_rows(a, e, p.seq, p.n);
     if (p.seq < 0 || p.seq >= a.c.n_seq) pages_flag(a.c, AERO_CUDA_PAGES_BAD_SEQ);
+    if constexpr (SEL) {
+        p.lo = p.sinks = p.tile0 = 0;
+        p.first = p.n > 0 ? min(a.width, ((p.n - 1) >> a.c.page_shift) + 1) : 0;
+        p.tiles = p.n > 0 ? (int)((((int64_t)p.first << a.c.page_shift) + kUnit - 1) / kUnit) : 1;
+        return p;
+    }
     p.lo = a.window && p.n > a.window ? p.n - a.window : 0;
     p.sinks = min(a.sinks, p.lo);
     p.tile0 = p.lo / kUnit;
@@ -112,8 +123,8 @@ __device__ __forceinline__ Piece piece_at(const AttendArgs& a, const Span& p, in
     return c;
 }
 
-// NT: tiles of 8 query heads (a kv head's group is up to 8 or up to 16 of them).
-template <int D, bool BF16, int NT>
+// NT: tiles of 8 query heads (a kv head's group is up to 8 or up to 16 of them). SEL: over listed blocks.
+template <int D, bool BF16, int NT, bool SEL>
 __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     decode_attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap) {
@@ -127,6 +138,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     int4* joins = reinterpret_cast<int4*>(begin_s + 2);                          // [2]: parts to join (or 0), first CTA, token, head
     int* misc = reinterpret_cast<int*>(joins + 2);                               // entry, abort
     Span* span_s = reinterpret_cast<Span*>(misc + 2);                            // the first entry's
+    int* box_at = reinterpret_cast<int*>(span_s + 1);                            // [ST][8]: SEL: a box's first position
+    static_assert((64 + 16) * 8 + 2 * ST * 8 + 16 + 32 + 8 + sizeof(Span) + ST * 32 <= 1024, "the last 1024 bytes hold these");
     volatile int* abort_flag = misc + 1;
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int HK = a.c.HK, G = a.H / HK;
@@ -148,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         const int per = (a.T + kThreads - 1) / kThreads;
         const int e0 = min(a.T, tid * per), e1 = min(a.T, e0 + per);
         int64_t mine = 0;
-        for (int e = e0; e < e1; ++e) mine += span_of(a, e).tiles + a.over;
+        for (int e = e0; e < e1; ++e) mine += span_of<SEL>(a, e).tiles + a.over;
         int64_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -170,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             int e = e0;
             Span at;
             for (;; ++e) {
-                at = span_of(a, e);
+                at = span_of<SEL>(a, e);
                 const int64_t next = base + (int64_t)(at.tiles + a.over) * HK;
                 if (u0 < next) break;
                 base = next;
@@ -204,8 +217,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             const int s = sp.seq;
             for (int t = t0; t < t0 + cnt; ++t) {
                 // lane i brings box i, if a position in it is visible
-                const int j0 = tile_at(sp, t) * kUnit + lane * rows;
-                const bool want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
+                int j0;
+                bool want;
+                if constexpr (SEL) {
+                    const int64_t at = (int64_t)t * kUnit + lane * rows;  // in the list's positions
+                    const int i = (int)(at >> a.c.page_shift);
+                    const int block = lane < boxes && i < sp.first ? a.blocks[((int64_t)e * HK + h) * a.width + i] : -1;
+                    want = block >= 0 && block <= (sp.n - 1) >> a.c.page_shift;
+                    j0 = want ? (block << a.c.page_shift) + (int)(at & (P - 1)) : kNowhere;
+                    want = j0 < sp.n;
+                    if (!want) j0 = kNowhere;
+                } else {
+                    j0 = tile_at(sp, t) * kUnit + lane * rows;
+                    want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
+                }
                 int page = 0;
                 if (want) {
                     page = a.c.table[(int64_t)s * a.c.max_pages + (j0 >> a.c.page_shift)];
@@ -216,6 +241,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                     break;
                 }
                 const uint32_t full = smem_u32(bars + stage);
+                if constexpr (SEL) {
+                    if (lane < 8) box_at[stage * 8 + lane] = j0;
+                    __syncwarp();  // before lane 0's arrival
+                }
                 const int n_box = __popc(__ballot_sync(0xffffffffu, want));
                 if (lane == 0) {
                     if (n_box)
@@ -244,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             u += pc.line;
             if (u == base + (int64_t)(sp.tiles + a.over) * HK && u < u1) {
                 base = u;
-                sp = span_of(a, ++e);
+                sp = span_of<SEL>(a, ++e);
             }
         }
         if (!good) {
@@ -352,13 +381,24 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                 for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + so[n][i]) * a.scale_log2;
             // positions that the token does not see: their scores are -inf and their V rows
             // are taken as zero, whatever their memory holds
-            const int j0 = tile_at(sp, t) * kUnit;
+            int j, j8;  // positions of the warp's first and ninth row (boxes are of 8 rows or more)
+            bool partly;
+            if constexpr (SEL) {
+                const int rows = min(1 << a.c.page_shift, kUnit), r = warp * 16;
+                j = box_at[stage * 8 + r / rows] + (r & (rows - 1));
+                j8 = box_at[stage * 8 + (r + 8) / rows] + ((r + 8) & (rows - 1));
+                partly = j + 8 > sp.n || j8 + 8 > sp.n;
+            } else {
+                const int j0 = tile_at(sp, t) * kUnit;
+                j = j0 + warp * 16;
+                j8 = j + 8;
+                partly = j0 + kUnit > sp.n || (j0 < sp.lo && j0 + kUnit > sp.sinks);
+            }
             uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
-            if (j0 + kUnit > sp.n || (j0 < sp.lo && j0 + kUnit > sp.sinks)) {
-                const int j = j0 + warp * 16;
+            if (partly) {
                 keep0 = (visible(sp, j + 2 * tq) ? 0x0000FFFFu : 0u) | (visible(sp, j + 2 * tq + 1) ? 0xFFFF0000u : 0u);
-                keep1 = (visible(sp, j + 2 * tq + 8) ? 0x0000FFFFu : 0u) | (visible(sp, j + 2 * tq + 9) ? 0xFFFF0000u : 0u);
-                const bool see0 = visible(sp, j + g), see1 = visible(sp, j + g + 8);
+                keep1 = (visible(sp, j8 + 2 * tq) ? 0x0000FFFFu : 0u) | (visible(sp, j8 + 2 * tq + 1) ? 0xFFFF0000u : 0u);
+                const bool see0 = visible(sp, j + g), see1 = visible(sp, j8 + g);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (!see0) s[n][0] = s[n][1] = -INFINITY;
@@ -510,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         u += pc.line;
         if (u == base + (int64_t)(sp.tiles + a.over) * HK && u < u1) {
             base = u;
-            sp = span_of(a, ++e);
+            sp = span_of<SEL>(a, ++e);
         }
     }
     // ---- joins of the (at most two) shared (sequence, head)s whose last part this CTA wrote; here,
@@ -567,14 +607,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     }
 }
 
-template <int D, bool BF16, int NT>
+template <int D, bool BF16, int NT, bool SEL>
 cudaError_t launch(AttendArgs a, const CUtensorMap& kmap, const CUtensorMap& vmap, int n_sm, cudaStream_t s) {
     static thread_local int prepared = -1;  // the device whose attribute this thread has set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (prepared != dev) {
-        e = cudaFuncSetAttribute(decode_attend_kernel<D, BF16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem);
+        e = cudaFuncSetAttribute(decode_attend_kernel<D, BF16, NT, SEL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::smem);
         if (e != cudaSuccess) return e;
         prepared = dev;
     }
@@ -583,10 +623,10 @@ cudaError_t launch(AttendArgs a, const CUtensorMap& kmap, const CUtensorMap& vma
     // are split over all CTAs that would only shift the cuts (one sequence of 4096: 12.9 -> 14.5 us).
     a.over = (int64_t)a.T * a.c.HK >= 32 ? 3 : 0;
     // no more CTAs than units the tables can hold
-    const int64_t cap = ((int64_t)a.c.max_pages << a.c.page_shift) / kUnit + 2 + a.over;
+    const int64_t cap = ((int64_t)(SEL ? std::min(a.width, a.c.max_pages) : a.c.max_pages) << a.c.page_shift) / kUnit + 2 + a.over;
     const int64_t units = (int64_t)a.T * a.c.HK * cap;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((int64_t)n_sm * Cfg<D>::ctas, units));
-    return launch_in_turn(decode_attend_kernel<D, BF16, NT>, grid, kThreads, Cfg<D>::smem, s, a, kmap, vmap);
+    return launch_in_turn(decode_attend_kernel<D, BF16, NT, SEL>, grid, kThreads, Cfg<D>::smem, s, a, kmap, vmap);
 }
 
 }  // namespace
@@ -599,7 +639,9 @@ cudaError_t launch_pages_decode(const AttendArgs& a, bool bf16, const CUtensorMa
     const auto typed = [&](auto d, auto bf) {
         constexpr int D = decltype(d)::value;
         constexpr bool B = decltype(bf)::value;
-        return a.H / a.c.HK <= 8 ? launch<D, B, 1>(a, kmap, vmap, n_sm, s) : launch<D, B, 2>(a, kmap, vmap, n_sm, s);
+        const bool few = a.H / a.c.HK <= 8;
+        if (a.blocks) return few ? launch<D, B, 1, true>(a, kmap, vmap, n_sm, s) : launch<D, B, 2, true>(a, kmap, vmap, n_sm, s);
+        return few ? launch<D, B, 1, false>(a, kmap, vmap, n_sm, s) : launch<D, B, 2, false>(a, kmap, vmap, n_sm, s);
     };
     const auto sized = [&](auto d) { return bf16 ? typed(d, std::true_type{}) : typed(d, std::false_type{}); };
     switch (a.c.D) {

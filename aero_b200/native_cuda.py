@@ -129,6 +129,13 @@ SYMBOLS = [
     ("aero_cuda_pages_compact", c_int, [_P]),
     ("aero_cuda_pages_attend", c_int, [_P, c_int, _P, c_int64, c_int64, c_int, c_int, _P, _P, c_int, c_float, c_int,
                                        c_int, _P, c_int64, c_int64]),
+    ("aero_cuda_pages_bounds_bytes", c_int64, [POINTER(PagesDesc)]),
+    ("aero_cuda_pages_keep_bounds", c_int, [_P]),
+    ("aero_cuda_pages_bounds", c_void_p, [_P]),
+    ("aero_cuda_pages_set_bounds", c_int, [_P, c_int, _P, c_int]),
+    ("aero_cuda_pages_select", c_int, [_P, c_int, _P, c_int64, c_int64, c_int, c_int, _P, _P, c_int, c_int, c_int, c_int, _P]),
+    ("aero_cuda_pages_attend_blocks", c_int, [_P, c_int, _P, c_int64, c_int64, c_int, c_int, _P, _P, c_int, _P, c_int, c_float,
+                                              _P, c_int64, c_int64]),
     ("aero_cuda_logits_adjust_views", c_int, [_P, c_int64, c_int, c_int, c_int, _P, c_int64, c_int, _P, _P, _P, _P, _P, _P,
                                               _P, _P, c_int, _P, c_int64, _P, c_int64, _P]),
     ("aero_cuda_logits_adjust", c_int, [_P, c_int64, c_int, c_int, c_int, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P,

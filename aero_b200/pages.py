@@ -9,6 +9,12 @@ pages hold which sequence. A serving step over a batch:
     out = cache.attend(layer, q, seqs)              # one new token per sequence
     out = cache.attend(layer, q, seqs, q_start)     # or several (prompts, drafts)
 
+or, in a cache that keeps the bounds of its pages' keys (`bounds=True`), over the blocks of a sequence
+(a page's positions each) that these bounds say matter most to a token:
+
+    blocks = cache.select(layer, q, seqs, n_blocks=64)
+    out = cache.attend_blocks(layer, q, seqs, blocks)
+
 and between steps `fork`, `free`, `copy` and `compact`. Arrays are CUDA torch tensors,
 sequence numbers, counts and positions int32. Calls run on torch's current stream
 (or the one given to `set_stream`), enqueue their work and return; they do not
@@ -53,20 +59,23 @@ def _dtypes():
 
 
 def plan_bytes(n_layer: int, n_page: int, page_size: int, n_head_kv: int, head_dim: int, n_seq: int, max_pages: int,
-               device: int = 0) -> dict:
+               device: int = 0, bounds: bool = False) -> dict:
     """Device bytes a cache of this shape allocates, as the memory guard charges them."""
     d = nc.PagesDesc(n_layer, n_page, page_size, n_head_kv, head_dim, n_seq, max_pages, nc.TYPE_F16, device, 0)
     by = (ctypes.c_int64 * 2)()
     if nc.lib().aero_cuda_pages_plan_bytes(ctypes.byref(d), by) < 0:
         raise ValueError("invalid cache description")
+    if bounds:
+        by[0] += nc.lib().aero_cuda_pages_bounds_bytes(ctypes.byref(d))
     return {"kv_cache": int(by[0]), "scratch": int(by[1]), "total": int(by[0]) + int(by[1])}
 
 
 class PagedCache:
     def __init__(self, n_layer: int, n_page: int, page_size: int, n_head_kv: int, head_dim: int, n_seq: int,
-                 max_pages: int, dtype=None, device: int = 0) -> None:
+                 max_pages: int, dtype=None, device: int = 0, bounds: bool = False) -> None:
         """n_page pages of page_size positions in each of n_layer layers, for n_seq sequences of at
-        most max_pages pages; dtype torch.float16 (default) or torch.bfloat16."""
+        most max_pages pages; dtype torch.float16 (default) or torch.bfloat16. bounds: keep the bounds of
+        the pages' keys, for `select`."""
         import torch
         self.handle = None
         self._lib = nc.lib()
@@ -92,6 +101,13 @@ class PagedCache:
         p = [ctypes.c_void_p() for _ in range(5)]
         self._lib.aero_cuda_pages_buffers(h, *(ctypes.byref(x) for x in p))
         self._ptr = [x.value for x in p]
+        self._bounds = None
+        if bounds:
+            if self._lib.aero_cuda_pages_keep_bounds(h) != 0:
+                why = self.last_error()
+                self.close()
+                raise RuntimeError(f"paged cache open: {why}")
+            self._bounds = self._lib.aero_cuda_pages_bounds(h)
 
     # ---- memory
     def _view(self, ptr, shape, typestr):
@@ -108,6 +124,15 @@ class PagedCache:
 
     def v(self, layer: Optional[int] = None):
         return self._pool(self._ptr[1], layer)
+
+    def bounds(self, layer: Optional[int] = None):
+        """The bounds of the pages' keys as a tensor over the cache's own memory: (n_layer, n_page,
+        n_head_kv, 2, head_dim), the smallest and the largest value of each column, or one layer's. A page's are
+        set by an append to it and by `set_bounds`."""
+        if self._bounds is None:
+            raise ValueError("the cache keeps no bounds (PagedCache(..., bounds=True))")
+        t = self._view(self._bounds, (self.n_layer, self.n_page, self.n_head_kv, 2, self.head_dim), "<i2").view(self.dtype)
+        return t if layer is None else t[layer]
 
     def tables(self):
         """(table, length, refs): the books as tensors over the cache's own memory, to be read; they
@@ -232,6 +257,18 @@ class PagedCache:
             self._refused("compact")
 
     # ---- attention
+    def _out(self, q, q_token, q_head, out):
+        """(out, its address and strides): a new tensor of q's shape, or the one given."""
+        if out is None:
+            if q.is_contiguous():
+                out, o_token, o_head = self._torch.empty_like(q), q_token, q_head
+            else:
+                out, o_token, o_head = q.new_empty(q.shape), q.shape[1] * self.head_dim, self.head_dim
+            return out, out.data_ptr(), o_token, o_head
+        if out.shape != q.shape:
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {tuple(q.shape)}")
+        return out, *self._rows(out, "out", q.shape[1])
+
     def attend(self, layer: int, q, seqs, q_start=None, *, window: int = 0, sinks: int = 0,
                scale: Optional[float] = None, out=None):
         """Attention of new tokens q (T, n_head, head_dim) over a layer's pages, causal; with a
@@ -242,22 +279,60 @@ class PagedCache:
         self._on()
         qp, q_token, q_head = self._rows(q, "q", None)
         T, H, _ = q.shape
-        if out is None:
-            if q.is_contiguous():
-                out, o_token, o_head = self._torch.empty_like(q), q_token, q_head
-            else:
-                out, o_token, o_head = q.new_empty(q.shape), H * self.head_dim, self.head_dim
-            op = out.data_ptr()
-        else:
-            if out.shape != q.shape:
-                raise ValueError(f"out has shape {tuple(out.shape)}, expected {tuple(q.shape)}")
-            op, o_token, o_head = self._rows(out, "out", H)
+        out, op, o_token, o_head = self._out(q, q_token, q_head, out)
         n = seqs.numel()
         if self._lib.aero_cuda_pages_attend(
                 self.handle, layer, qp, q_token, q_head, T, H, self._i32(seqs, "seqs"),
                 None if q_start is None else self._i32(q_start, "q_start", n + 1), n,
                 self._scale if scale is None else scale, window, sinks, op, o_token, o_head) != 0:
             self._refused("attend")
+        return out
+
+    # ---- attention over selected blocks
+    def set_bounds(self, layer: int, seqs) -> None:
+        """The bounds of every page of the sequences, from the pool's K rows: after set_tables, or after K
+        rows were written other than by append."""
+        self._on()
+        if self._lib.aero_cuda_pages_set_bounds(self.handle, layer, self._i32(seqs, "seqs"), seqs.numel()) != 0:
+            self._refused("set_bounds")
+
+    def select(self, layer: int, q, seqs, q_start=None, *, n_blocks: int, first: int = 1, recent: int = 1, out=None):
+        """For each token of q (T, n_head, head_dim; q_start as for `attend`) and each kv head the numbers of
+        the blocks to attend to, int32 (T, n_head_kv, n_blocks), ascending, -1 behind the last: the first `first`
+        and the last `recent` of the blocks it sees, and of the others those whose bounds allow the largest product
+        with one of the kv head's queries (equal ones: the lower number)."""
+        self._on()
+        qp, q_token, q_head = self._rows(q, "q", None)
+        T, H, _ = q.shape
+        if out is None:
+            out = self._torch.empty((T, self.n_head_kv, max(n_blocks, 0)), dtype=self._i32_type, device=self.device)
+        elif out.shape != (T, self.n_head_kv, n_blocks):
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {(T, self.n_head_kv, n_blocks)}")
+        n = seqs.numel()
+        if self._lib.aero_cuda_pages_select(
+                self.handle, layer, qp, q_token, q_head, T, H, self._i32(seqs, "seqs"),
+                None if q_start is None else self._i32(q_start, "q_start", n + 1), n, first, recent, n_blocks,
+                self._i32(out, "out")) != 0:
+            self._refused("select")
+        return out
+
+    def attend_blocks(self, layer: int, q, seqs, blocks, q_start=None, *, scale: Optional[float] = None, out=None):
+        """Attention as `attend`'s, token by token, over the positions in the listed blocks: blocks (T, n_head_kv, any
+        number) int32 block numbers, in any order; negative ones and those past the token's own are passed over, one
+        listed twice counts twice, and no more entries are looked at than the token has blocks. A token
+        without a listed position has an output of zeros."""
+        self._on()
+        qp, q_token, q_head = self._rows(q, "q", None)
+        T, H, _ = q.shape
+        if blocks.dim() != 3 or blocks.shape[0] != T or blocks.shape[1] != self.n_head_kv:
+            raise ValueError(f"blocks must be ({T}, {self.n_head_kv}, any), got {tuple(blocks.shape)}")
+        out, op, o_token, o_head = self._out(q, q_token, q_head, out)
+        n = seqs.numel()
+        if self._lib.aero_cuda_pages_attend_blocks(
+                self.handle, layer, qp, q_token, q_head, T, H, self._i32(seqs, "seqs"),
+                None if q_start is None else self._i32(q_start, "q_start", n + 1), n, self._i32(blocks, "blocks"),
+                blocks.shape[2], self._scale if scale is None else scale, op, o_token, o_head) != 0:
+            self._refused("attend_blocks")
         return out
 
     # ---- end

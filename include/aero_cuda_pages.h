@@ -127,6 +127,43 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
                            const int32_t* seqs, const int32_t* q_start, int n, float scale, int window, int sinks,
                            void* out, int64_t o_token, int64_t o_head);
 
+/* Attention over selected blocks. Block i of a sequence is its i-th page's positions, [i * page_size,
+ * (i + 1) * page_size). Beside its pages a cache may keep their bounds, (n_layer, n_page, n_head_kv, 2,
+ * head_dim) in the cache's type: the smallest and the largest value of each column of a page's keys
+ * below the sequence's length (infinities count as the type's largest values, what is no
+ * number is passed over, a column of nothing else has bounds 0). From keep_bounds on an append sets the bounds of
+ * the pages that it writes to, a fork, a copy and a compaction move them with their pages, and
+ * set_bounds makes them from the pool. */
+
+/* Device bytes of the bounds. -1 for an invalid description. */
+int64_t aero_cuda_pages_bounds_bytes(const aero_cuda_pages_desc* desc);
+/* Allocate the bounds (zeros, charged to the memory guard as the pool is) and keep them from now on. Call it before
+ * the cache's calls: graphs captured before do not keep them. It synchronises. 0 / -1. */
+int aero_cuda_pages_keep_bounds(void* cache);
+/* The bounds' device address; NULL where they are not kept. */
+void* aero_cuda_pages_bounds(void* cache);
+/* The bounds of every page of n sequences in `layer`, from the rows that the pool holds. */
+int aero_cuda_pages_set_bounds(void* cache, int layer, const int32_t* seqs, int n);
+/* For each of T tokens (as for attend) and each kv head h the blocks it should attend to, into
+ * blocks (T, n_head_kv, n_blocks), ascending, -1 behind the last. Of the blocks that hold a position the
+ * token sees, the first `first` and the last `recent` (1 or more: the token's own among them) are
+ * chosen always, and of the others those with the highest score, equal ones by the lower number, until there
+ * are n_blocks (first + recent or more). score = the largest, over the kv head's query heads g, of sum_d max(q_gd *
+ * lo_d, q_gd * hi_d): no key between the bounds has a larger product with g's query. Scores are summed
+ * in 64 bits; one that is no number counts as +infinity. A block without a page is recorded and has bounds
+ * 0. An empty sequence has no blocks. For caches of max_pages at most 131072. */
+int aero_cuda_pages_select(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
+                           const int32_t* seqs, const int32_t* q_start, int n, int first, int recent, int n_blocks,
+                           int32_t* blocks);
+/* Attention as attend's, token by token and exact as there, of kv head h's query heads of token t over the
+ * positions up to the token's own in the blocks listed in blocks (T, n_head_kv, n_blocks), in any order.
+ * Entries below 0 and past the token's own block are passed over, and of a list longer than the
+ * number of the token's blocks only that many entries are looked at. A block listed twice counts twice. A
+ * token none of whose positions is listed has an output of 0. */
+int aero_cuda_pages_attend_blocks(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
+                                  const int32_t* seqs, const int32_t* q_start, int n, const int32_t* blocks, int n_blocks,
+                                  float scale, void* out, int64_t o_token, int64_t o_head);
+
 /* Adjusts `rows` rows of `vocab` logits (type dtype, row stride ld elements) into out
  * (same type, row stride ld_out; may be logits itself), on `stream`. Per row r, with
  * its history's first n_history[r] token ids (row stride ld_history; at most ld_history count) of which the
