@@ -1,5 +1,6 @@
 """Logits of a batch adjusted before sampling (aero_cuda_logits_adjust,
-include/aero_cuda_pages.h): penalties for repeated tokens, biases, grammar masks.
+include/aero_cuda_pages.h): penalties for repeated tokens, biases, grammar masks; and
+tokens drawn from them (aero_cuda_logits_sample): temperature, top-k, top-p, min-p.
 """
 
 from __future__ import annotations
@@ -84,3 +85,43 @@ def adjust(logits, *, history=None, n_history=None, n_prompt=None, repetition=No
             out.stride(0) if rows > 1 else vocab, torch._C._cuda_getCurrentRawStream(index) or None) != 0:
         raise ValueError(f"logits_adjust refused: {nc.last_error()}")
     return out
+
+
+def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, logprob=False, out=None):
+    """A token from each row of logits (rows, vocab), a CUDA tensor of float32, float16 or bfloat16, with the
+    random numbers u (rows) float32 in [0, 1): int32 (rows), a new tensor or `out`; with logprob also the logs of the
+    probabilities they were drawn with, float32 (rows).
+
+    In falling order of the logits (equal ones: the lower token) with weights exp((x - largest) / temperature), kept are the
+    first top_k; of those the ones up to where the running sum reaches top_p of the whole; of those the ones with
+    at least min_p of the largest weight. Drawn is the first whose running sum exceeds u times the sum of the kept.
+    temperature, top_p, min_p: float32 (rows), top_k: int32 (rows); None, or a row's top_k of 0 or less, top_p of 1 or
+    more, min_p of 0 or less: no such limit; a row's temperature of 0 or less: the largest logit. Logits of -infinity and
+    those that are no number are never drawn; -1 for a row of nothing else. Runs on torch's current stream."""
+    import torch
+    L, kinds = nc.lib(), _kinds()
+    index = logits.get_device()
+    if logits.dim() != 2 or logits.dtype not in kinds or index < 0 or logits.stride(1) != 1:
+        raise ValueError("logits must be a (rows, vocab) CUDA tensor of float32, float16 or bfloat16, contiguous along vocab")
+    rows, vocab = logits.shape
+
+    def vec(t, name, dtype):
+        if t is None:
+            return None
+        if t.dtype is not dtype or t.get_device() != index or t.numel() != rows or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dtype}, {rows} entries, on {logits.device}")
+        return t.data_ptr()
+
+    f32, i32 = torch.float32, torch.int32
+    if u is None:
+        raise ValueError("u is required")
+    if out is None:
+        out = torch.empty(rows, dtype=i32, device=logits.device)
+    logs = torch.empty(rows, dtype=f32, device=logits.device) if logprob else None
+    if L.aero_cuda_logits_sample(
+            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kinds[logits.dtype], rows, vocab, vec(u, "u", f32),
+            vec(temperature, "temperature", f32), vec(top_k, "top_k", i32), vec(top_p, "top_p", f32),
+            vec(min_p, "min_p", f32), vec(out, "out", i32), None if logs is None else logs.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(index) or None) != 0:
+        raise ValueError(f"logits_sample refused: {nc.last_error()}")
+    return (out, logs) if logprob else out

@@ -138,6 +138,7 @@ SYMBOLS = [
                                               _P, c_int64, c_int64]),
     ("aero_cuda_logits_adjust_views", c_int, [_P, c_int64, c_int, c_int, c_int, _P, c_int64, c_int, _P, _P, _P, _P, _P, _P,
                                               _P, _P, c_int, _P, c_int64, _P, c_int64, _P]),
+    ("aero_cuda_logits_sample", c_int, [_P, c_int64, c_int, c_int, c_int, _P, _P, _P, _P, _P, _P, _P, _P]),
     ("aero_cuda_logits_adjust", c_int, [_P, c_int64, c_int, c_int, c_int, _P, c_int64, _P, _P, _P, _P, _P, _P, _P, _P,
                                         _P, c_int64, _P, c_int64, _P]),
     ("aero_cuda_moe_forward", c_int, [_P, c_int, _P, c_int, c_int, _P]),

@@ -1,7 +1,7 @@
 /*
  * aero_cuda_pages — a paged key/value cache on one B200, the attention that reads
- * it, and the adjustment of a batch's logits, plain C ABI (same library as
- * aero_cuda_moe.h).
+ * it, over all positions or over selected blocks, the adjustment of a batch's logits and the
+ * tokens drawn from them, plain C ABI (same library as aero_cuda_moe.h).
  *
  * A cache holds n_page pages of page_size positions for every layer: K and V as
  * (n_layer, n_page, n_head_kv, page_size, head_dim) f16 or bf16. Its books are
@@ -193,6 +193,25 @@ int aero_cuda_logits_adjust_views(const void* logits, int64_t ld, int dtype, int
                                   const float* presence, const int32_t* bias_start, const int32_t* bias_token,
                                   const float* bias_value, int n_bias, const int32_t* mask, int64_t ld_mask,
                                   void* out, int64_t ld_out, void* stream);
+
+/* Draws a token from each of `rows` rows of `vocab` logits (type dtype, row stride ld elements, 0: one row for
+ * all) with the random number u[r] in [0, 1), on `stream`. In falling order of the logits, equal ones by the lower number,
+ * token j has the weight exp((x_j - largest) / temperature[r]). Of that order the tokens are kept that
+ *   are among the first top_k[r] (0 or less: all),
+ *   then, of those, up to the first whose running sum of weights reaches top_p[r] times their sum (1 or more, or
+ *   no number: all),
+ *   then have at least min_p[r] times the first one's weight (0 or less, or no number: all),
+ * the first one always. tokens[r] = the first whose running sum exceeds u[r] times the sum of those kept, logprob[r] (may
+ * be NULL) = the log of its weight's share of that sum. temperature[r] of 0 or less, or no number: the first of the
+ * order. Logits of -infinity and those that are no number are never drawn; a row of nothing else gives -1 and
+ * -infinity. With a logit of +infinity all others have weight 0. temperature (1), top_k, top_p and min_p may
+ * be NULL. Weights are computed in 64 bits and summed as multiples of 2^-b of the largest, b = 62 less the bits of
+ * vocab (48 at most, 44 for 2^18), so a weight below half of that is never drawn; the
+ * result does not depend on timing. vocab is at most 2^22.
+ * 0, or -1 with the reason in aero_cuda_moe_last_error(NULL). */
+int aero_cuda_logits_sample(const void* logits, int64_t ld, int dtype, int rows, int vocab, const float* u,
+                            const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                            int32_t* tokens, float* logprob, void* stream);
 
 #ifdef __cplusplus
 }
