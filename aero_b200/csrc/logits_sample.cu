@@ -36,7 +36,7 @@ using u64 = unsigned long long;
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleCluster = 8;
-constexpr int kBins = 4 * kSampleThreads, kLast = kBins - 1;
+constexpr int kBins = 4 * kSampleThreads, kLast = kBins - 1, kGroups = kBins / 32;
 constexpr int kMembers = 2048;
 constexpr int kFew = kSampleThreads / 4;  // members put in order by counting
 constexpr int kMostVocab = 1 << 22;
@@ -86,27 +86,28 @@ __device__ __forceinline__ float value_in(uint32_t w, int j) {
 struct Row {
     float m;             // the largest logit
     float half_m, scale; // slice = (m / 2 - x / 2) * scale (halves: the difference of any two numbers is one)
+    float grid;          // step / T, of 13 bits: a slice's number times it is exact
+    float floor;         // below the last slice's beginning, above -infinity; -infinity: there is no such number
     double per_t;        // 1 / T
-    double grid;         // step / T
-    double least;        // min_p 2^B
     double lift;         // 2^B
+    u64 least;           // min_p 2^B
     // (as a number beside 2^23, for comparisons)
     __device__ __forceinline__ float slice(float x) const { return fminf(fmaf(x, -0.5f, half_m) * scale, (float)kLast) + 8388608.f; }
     __device__ __forceinline__ int bin(float x) const { return (int)(__float_as_uint(slice(x)) & (kBins - 1)); }
-    // 2^B e^((x - m) / T) in 64 bits, for slices but the last: with y = (x - m) / T + b step / T, at most 0.009 either way, the
-    // table's value e^(-b step / T) 2^B times e^y by its series, whose first term left out is below 10^-15
-    __device__ __forceinline__ double weight(float x, int b, const double* table) const {
-        const double t = (double)x - (double)m;
-        const double y = fma(t, per_t, (__hiloint2double(0x43300000, b) - kTwo52) * grid);
+    // 2^52 + 2^B e^((x - m) / T), which leaves the weight's nearest whole number in the low bits (2^B is at most 2^48), for
+    // slices but the last: with y = (x - m) / T + b step / T, at most 0.009 either way, the table's value e^(-b step / T) 2^B
+    // times e^y by its series, whose first term left out is below 10^-15
+    __device__ __forceinline__ double beside(float x, float slice, const double* table) const {
+        const double y = fma((double)x - (double)m, per_t, (double)((slice - 8388608.f) * grid));
         double p = fma(y, 1.0 / 120, 1.0 / 24);
         p = fma(p, y, 1.0 / 6);
         p = fma(p, y, 0.5);
         p = fma(p, y, 1.0);
         p = fma(p, y, 1.0);
-        return p * table[b];
+        return fma(p, table[__float_as_uint(slice) & (kBins - 1)], kTwo52);
     }
-    // the nearest whole number (2^B is at most 2^48)
-    static __device__ __forceinline__ u64 whole(double w) { return (u64)__double_as_longlong(w + kTwo52) & 0xFFFFFFFFFFFFFull; }
+    static __device__ __forceinline__ u64 whole(double beside) { return (u64)__double_as_longlong(beside) & 0xFFFFFFFFFFFFFull; }
+    __device__ __forceinline__ u64 weight(float x, const double* table) const { return whole(beside(x, slice(x), table)); }
 };
 
 // what the cluster does next
@@ -124,6 +125,7 @@ struct Search {
     int shift;           // kDivide: slice = (hi - key) >> shift
     int b0, b1, b2;      // kGather: slices [b0, b1] and b2
     int last;            // kGather: the members have the answer for certain; -1: a slice has too many
+    int by_count;        // kBoth: the first is what top_k keeps
     uint32_t nth;        // kTies: which of the tokens with key lo, from 1
     float logprob;       // kTies
     uint32_t count_before;         // tokens before the slice in hand
@@ -132,14 +134,26 @@ struct Search {
     u64 total, kept, likely;       // sums: of the row, of the kept, of those that min_p keeps
 };
 
+// A CTA's histogram of its tokens: sums as two words, numbers.
+struct Histogram {
+    uint32_t low[kBins], high[kBins], count[kBins];
+};
+// Sums over 32 slices each.
+struct Groups {
+    u64 mass[kGroups];
+    uint32_t count[kGroups];
+};
+
 struct Shared {
     double table[kBins];
-    u64 first_mass[kBins];    // the row's first histogram: sums, and first_count
-    u64 more_mass[kBins];     // the row's histogram of a slice; the members' weights
+    Histogram first;          // of Row's slices
+    Histogram more;           // of one slice's keys, or of members' keys; the place of members on their way; else zero
     u64 member[kMembers];     // key, then all ones less the token's number (in the first CTA)
-    uint32_t own_low[kBins], own_high[kBins], own_count[kBins];  // this CTA's histogram: sums, numbers; zero when not in use
-    uint32_t first_count[kBins], more_count[kBins];
+    u64 weight[kMembers];     // (in the first CTA)
+    Groups from[kSampleCluster];         // what the CTAs' histograms hold
+    Groups first_groups, more_groups;    // the row's
     u64 set_member[kFew], set_weight[kFew];
+    int set_slice[kFew];
     double coarse[kBins / 32], fine[32];
     u64 warp_mass[kSampleWarps];
     uint32_t warp_count[kSampleWarps], warp_lo[kSampleWarps], warp_hi[kSampleWarps];
@@ -151,9 +165,9 @@ struct Shared {
     Search find;
     float u, p, min_p;
     int k, few, table_made, fresh;
-    int at[2];
-    u64 at_mass[2], at_own[2], at_one;
-    uint32_t at_count[2], at_members[2];
+    int at[3];
+    u64 at_mass[3], at_own[3], at_one;
+    uint32_t at_count[3], at_members[3];
 };
 static_assert(sizeof(Shared) <= 113 * 1024, "two CTAs an SM");
 
@@ -175,9 +189,9 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
     return v;
 }
 
-__device__ __forceinline__ void clear(Shared& s) {
+__device__ __forceinline__ void clear(Histogram& h) {
 #pragma unroll 1
-    for (int i = (int)threadIdx.x; i < 3 * kBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(s.own_low)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = (int)threadIdx.x; i < 3 * kBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(h.low)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // u S as the running sum to be reached: the first above it.
@@ -223,53 +237,86 @@ __device__ __noinline__ uint32_t lowest_key(int b) {
 // (hi - lo) >> shift < kBins = 2^11
 __device__ __forceinline__ int shift_of(uint32_t span) { return max(0, 21 - __clz((int)span)); }
 
-// A thread's four slices of a histogram and what lies before them.
-struct Slices {
-    u64 mass, mass4[4];
-    uint32_t count, count4[4];
-    // mass, count: of all before the histogram's first; every thread calls it
-    __device__ __forceinline__ void scan(Shared& s, u64 mass_before, uint32_t count_before) {
-        const int lane = (int)threadIdx.x & 31, warp = (int)threadIdx.x >> 5;
-        const u64 m0 = mass4[0] + mass4[1] + mass4[2] + mass4[3];
-        const uint32_t c0 = count4[0] + count4[1] + count4[2] + count4[3];
-        u64 m = m0;
-        uint32_t c = c0;
-#pragma unroll 1
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 x = __shfl_up_sync(0xffffffffu, m, o);
-            const uint32_t y = __shfl_up_sync(0xffffffffu, c, o);
-            if (lane >= o) m += x, c += y;
-        }
-        if (lane == 31) s.warp_mass[warp] = m, s.warp_count[warp] = c;
-        __syncthreads();
-        mass = m - m0 + mass_before;
-        count = c - c0 + count_before;
-#pragma unroll 1
-        for (int i = 0; i < warp; ++i) mass += s.warp_mass[i], count += s.warp_count[i];
-    }
-    // the slice that holds the answer to a limit into at[j]
-    __device__ __forceinline__ void pick(Shared& s, bool by_count, int j, u64 limit) const {
-        u64 m = mass;
-        uint32_t c = count;
+// A histogram's groups; every thread calls it. Four slices a thread, eight threads a group.
+__device__ __forceinline__ void group(const Histogram& h, Groups& g) {
+    const int t = (int)threadIdx.x;
+    const uint4 low = reinterpret_cast<const uint4*>(h.low)[t], high = reinterpret_cast<const uint4*>(h.high)[t];
+    const uint4 count = reinterpret_cast<const uint4*>(h.count)[t];
+    u64 m = (u64)low.x + low.y + low.z + low.w + (((u64)high.x + high.y + high.z + high.w) << 32);
+    uint32_t c = count.x + count.y + count.z + count.w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const u64 had = by_count ? c : m, has = by_count ? c + count4[i] : m + mass4[i];
-            if (had < limit && limit <= has) {
-                s.at[j] = 4 * (int)threadIdx.x + i;
-                s.at_mass[j] = m;
-                s.at_own[j] = mass4[i];
-                s.at_count[j] = c;
-                s.at_members[j] = count4[i];
+    for (int o = 1; o < 8; o <<= 1) {
+        m += __shfl_xor_sync(0xffffffffu, m, o);
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+    }
+    if (t % 8 == 0) g.mass[t / 8] = m, g.count[t / 8] = c;
+}
+
+template <typename V>
+__device__ __forceinline__ V scanned(V v) {
+    const int lane = (int)threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
+// By a warp: the slice of a histogram (C CTAs' together) that holds the answer to a limit into at[j], with what lies before it
+// and what it holds (numbers before it: only where the limit is one). Reads of other CTAs' memory are slow: groups first, then 32
+// slices.
+__device__ __noinline__ void find(int j, const Groups& g, const Histogram& h, int C, u64 mass_before, uint32_t count_before, bool by_count,
+                                  u64 limit) {
+    Shared& s = shared();
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int lane = (int)threadIdx.x & 31;
+    int b = 0;
+    // groups 0 to 31 and 32 to 63, as far as the one with the answer; then its 32 slices
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+        u64 m0 = 0;
+        uint32_t c0 = 0;
+        if (step < 2) {
+            m0 = g.mass[32 * step + lane];
+            c0 = g.count[32 * step + lane];
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < C; ++i) {
+                const Histogram* o = C > 1 ? cluster.map_shared_rank(const_cast<Histogram*>(&h), i) : &h;
+                m0 += (u64)o->low[b + lane] + ((u64)o->high[b + lane] << 32);
+                c0 += o->count[b + lane];
             }
-            m += mass4[i];
-            c += count4[i];
+        }
+        const u64 m = scanned(m0);
+        const uint32_t c = by_count ? scanned(c0) : 0;
+        const int at = __popc(__ballot_sync(0xffffffffu, (by_count ? (u64)count_before + c : mass_before + m) < limit));
+        if (step == 0 && at == 32) {
+            mass_before += __shfl_sync(0xffffffffu, m, 31);
+            count_before += __shfl_sync(0xffffffffu, c, 31);
+            continue;
+        }
+        const int in = min(at, 31);
+        if (step < 2) {
+            mass_before += __shfl_sync(0xffffffffu, m - m0, in);
+            count_before += by_count ? __shfl_sync(0xffffffffu, c - c0, in) : 0;
+            b = 32 * (32 * step + in);
+            step = 1;
+        } else if (lane == in) {
+            s.at[j] = b + in;
+            s.at_mass[j] = mass_before + m - m0;
+            s.at_own[j] = m0;
+            s.at_count[j] = count_before + (by_count ? c - c0 : 0);
+            s.at_members[j] = c0;
         }
     }
-};
+    __syncwarp();
+}
+static_assert(kGroups == 64, "two steps of groups");
 
-// f(four values, the first one's token) for a CTA's tokens; values past the last one are -infinity. Two 16-byte pieces a
-// thread are on their way while two are looked at.
-template <typename E, typename F>
+// f(four values, the first one's token) for a CTA's tokens; values past the last one are -infinity. U 16-byte pieces a
+// thread are on their way while as many are looked at.
+template <typename E, int U = 2, typename F>
 __device__ __forceinline__ void each(const E* in, int v0, int nv, F f) {
     constexpr int PER = 4 / (int)sizeof(E), V = 4 * PER;
     const int tid = (int)threadIdx.x, vecs = ((uintptr_t)in & 15) == 0 ? nv / V : 0;
@@ -284,16 +331,20 @@ __device__ __forceinline__ void each(const E* in, int v0, int nv, F f) {
             f(x, v0 + i * V + j);
         }
     };
-    uint4 one = make_uint4(0u, 0u, 0u, 0u), two = one;
-    if (tid < vecs) one = v[tid];
-    if (tid + kSampleThreads < vecs) two = v[tid + kSampleThreads];
+    uint4 next[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) next[k] = tid + k * kSampleThreads < vecs ? v[tid + k * kSampleThreads] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
-    for (int i = tid; i < vecs; i += 2 * kSampleThreads) {
-        const uint4 now = one, then = two;
-        if (i + 2 * kSampleThreads < vecs) one = v[i + 2 * kSampleThreads];
-        if (i + 3 * kSampleThreads < vecs) two = v[i + 3 * kSampleThreads];
-        piece(now, i);
-        if (i + kSampleThreads < vecs) piece(then, i + kSampleThreads);
+    for (int i = tid; i < vecs; i += U * kSampleThreads) {
+        uint4 now[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            now[k] = next[k];
+            if (i + (U + k) * kSampleThreads < vecs) next[k] = v[i + (U + k) * kSampleThreads];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            if (i + k * kSampleThreads < vecs) piece(now[k], i + k * kSampleThreads);
     }
 #pragma unroll 1
     for (int i = vecs * V + 4 * tid; i < nv; i += 4 * kSampleThreads) {
@@ -304,15 +355,16 @@ __device__ __forceinline__ void each(const E* in, int v0, int nv, F f) {
     }
 }
 
-// Four weights into this CTA's histogram: a 64-bit sum as two of 32 bits.
-__device__ __forceinline__ void add4(Shared& s, const int (&b)[4], const u64 (&n)[4]) {
+// Four weights (as Row::beside) into this CTA's histogram: a 64-bit sum as two of 32 bits.
+__device__ __forceinline__ void add4(Histogram& h, const int (&b)[4], const double (&w)[4]) {
     uint32_t was[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) was[e] = atomicAdd(&s.own_low[b[e]], (uint32_t)n[e]);
+    for (int e = 0; e < 4; ++e) was[e] = atomicAdd(&h.low[b[e]], (uint32_t)__double2loint(w[e]));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t high = (uint32_t)(n[e] >> 32) + (was[e] + (uint32_t)n[e] < was[e]);
-        if (high) atomicAdd(&s.own_high[b[e]], high);
+        const uint32_t low = (uint32_t)__double2loint(w[e]);
+        const uint32_t high = (uint32_t)__double2hiint(w[e]) - 0x43300000u + (was[e] + low < low);
+        if (high) atomicAdd(&h.high[b[e]], high);
     }
 }
 
@@ -322,11 +374,11 @@ __device__ __noinline__ void numbers_pass(const E* in, int nv) {
     const Row r = s.row;
     each<E>(in, 0, nv, [&](const float (&x)[4], int) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) atomicAdd(&s.own_count[r.bin(x[e])], 1u);
+        for (int e = 0; e < 4; ++e) atomicAdd(&s.first.count[r.bin(x[e])], 1u);
     });
 }
 
-// FULL: numbers too, and returns the sum of this thread's weights that min_p keeps.
+// FULL: numbers too, values down to the least of all numbers, and returns the sum of this thread's weights that min_p keeps.
 template <typename E, bool FULL>
 __device__ __noinline__ u64 sums_pass(const E* in, int nv) {
     Shared& s = shared();
@@ -334,18 +386,22 @@ __device__ __noinline__ u64 sums_pass(const E* in, int nv) {
     u64 likely = 0;
     each<E>(in, 0, nv, [&](const float (&x)[4], int) {
         int b[4];
-        u64 n[4];
+        double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            b[e] = r.bin(x[e]);
-            const double w = r.weight(x[e], b[e], s.table);
-            n[e] = b[e] == kLast ? 0 : Row::whole(w);
+            // (what is below the last slice's beginning, or no number, is there: the table's last value is 0)
+            const float y = FULL ? x[e] : fmaxf(x[e], r.floor);
+            const float at = r.slice(y);
+            b[e] = (int)(__float_as_uint(at) & (kBins - 1));
+            w[e] = r.beside(y, at, s.table);
             if (FULL) {
-                if (w >= r.least && b[e] != kLast) likely += n[e];
-                atomicAdd(&s.own_count[b[e]], 1u);
+                if (b[e] == kLast) w[e] = kTwo52;
+                const u64 n = Row::whole(w[e]);
+                if (n >= r.least) likely += n;
+                atomicAdd(&s.first.count[b[e]], 1u);
             }
         }
-        add4(s, b, n);
+        add4(s.first, b, w);
     });
     return likely;
 }
@@ -358,29 +414,29 @@ __device__ __noinline__ void divide_pass(const E* in, int nv) {
     const int shift = s.find.shift;
     each<E>(in, 0, nv, [&](const float (&x)[4], int) {
         int b[4];
-        u64 n[4];
+        double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t key = key_of(x[e]);
             const bool is = key >= lo && key <= hi;
-            const int from = r.bin(x[e]);
+            const float at = r.slice(x[e]);
             b[e] = is ? (int)((hi - key) >> shift) : 0;
-            n[e] = is && from != kLast ? Row::whole(r.weight(x[e], from, s.table)) : 0;
-            if (is) atomicAdd(&s.own_count[b[e]], 1u);
+            w[e] = is && at < 8388608.f + (float)kLast ? r.beside(x[e], at, s.table) : kTwo52;
+            if (is) atomicAdd(&s.more.count[b[e]], 1u);
         }
-        add4(s, b, n);
+        add4(s.more, b, w);
     });
 }
 
-// The members into this CTA's memory (its histogram's place).
+// The members into this CTA's memory (a histogram's place).
 template <typename E, bool KEYS>
 __device__ __noinline__ void gather_pass(const E* in, int v0, int nv) {
     Shared& s = shared();
     const Row r = s.row;
     const uint32_t lo = s.find.lo, hi = s.find.hi;
     const float f0 = 8388608.f + (float)s.find.b0, f1 = 8388608.f + (float)s.find.b1, f2 = 8388608.f + (float)s.find.b2;
-    u64* const stage = reinterpret_cast<u64*>(s.own_low);
-    each<E>(in, v0, nv, [&](const float (&x)[4], int token) {
+    u64* const stage = reinterpret_cast<u64*>(s.more.low);
+    each<E, 4 / (4 / (int)sizeof(E))>(in, v0, nv, [&](const float (&x)[4], int token) {
         uint32_t is = 0;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -482,151 +538,152 @@ __device__ __noinline__ void nth_token(const SampleArgs& a, int row, const E* in
         }
 }
 
-// The CTAs' histograms into the row's, each CTA a part of it for all; and cleared.
-__device__ __noinline__ void collect(bool first, bool sums, bool numbers) {
+// What the CTAs' histograms hold, to all of them.
+__device__ __noinline__ void collect(const Histogram& h, Groups& to, int C, int rank) {
     Shared& s = shared();
     cg::cluster_group cluster = cg::this_cluster();
-    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    uint32_t* const counts = first ? s.first_count : s.more_count;
-    u64* const masses = first ? s.first_mass : s.more_mass;
-    cluster.sync();
-#pragma unroll 1
-    for (int b = rank * (kBins / C) + (int)threadIdx.x; b < (rank + 1) * (kBins / C); b += kSampleThreads) {
-        uint32_t c = 0;
-        u64 m = 0;
-#pragma unroll 4
-        for (int i = 0; i < C; ++i) {
-            const Shared* o = cluster.map_shared_rank(&s, i);
-            if (numbers) c += o->own_count[b];
-            if (sums) m += (u64)o->own_low[b] + ((u64)o->own_high[b] << 32);
-        }
-#pragma unroll 4
-        for (int i = 0; i < C; ++i) {
-            if (numbers) *cluster.map_shared_rank(counts + b, i) = c;
-            if (sums) *cluster.map_shared_rank(masses + b, i) = m;
-        }
+    const int tid = (int)threadIdx.x;
+    __syncthreads();
+    if (C == 1) {
+        group(h, to);
+        __syncthreads();
+        return;
+    }
+    Groups& own = s.from[rank];
+    group(h, own);
+    __syncthreads();
+    static_assert(kGroups * kSampleCluster == kSampleThreads, "a thread a group and CTA");
+    const int g = tid % kGroups, c = tid / kGroups;
+    if (c < C && c != rank) {
+        Groups* const there = cluster.map_shared_rank(&own, c);
+        there->mass[g] = own.mass[g];
+        there->count[g] = own.count[g];
     }
     cluster.sync();
-    clear(s);
+    if (tid < kGroups) {
+        u64 m = 0;
+        uint32_t n = 0;
+#pragma unroll 4
+        for (int i = 0; i < C; ++i) m += s.from[i].mass[tid], n += s.from[i].count[tid];
+        to.mass[tid] = m;
+        to.count[tid] = n;
+    }
+    __syncthreads();
 }
 
-// The slice of a histogram that holds the answer, and what to do with it. Every CTA works this out for itself.
+// The slice of a histogram that holds the answer, and what to do with it. Every CTA works this out for itself, in its first warp.
 __device__ __noinline__ void look(bool first, bool sums, int C) {
     Shared& s = shared();
     Search& f = s.find;
-    const int tid = (int)threadIdx.x, k = s.k;
-    Slices t;
-    {
-        const uint32_t* counts = first ? s.first_count : s.more_count;
-        const u64* masses = first ? s.first_mass : s.more_mass;
-        const bool numbers = !first || k > 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            t.mass4[i] = sums ? masses[4 * tid + i] : 0;
-            t.count4[i] = numbers ? counts[4 * tid + i] : 0;
+    const int lane = (int)threadIdx.x & 31, k = s.k;
+    const int warp = (int)threadIdx.x >> 5;
+    if (warp == 0) {
+        if (s.fresh) {
+            const u64 total = warp_sum(s.first_groups.mass[lane] + s.first_groups.mass[lane + 32]);
+            const uint32_t count = __reduce_add_sync(0xffffffffu, s.first_groups.count[lane] + s.first_groups.count[lane + 32]);
+            if (lane == 0) {
+                u64 likely = 0;
+                for (int i = 0; sums && i < C; ++i) likely += s.likely[i];
+                f.total = total;
+                // (the first of the order is kept whatever min_p is)
+                f.likely = s.row.least ? max(likely, (u64)s.row.lift) : total;
+                f.goal = kTopK;
+                f.last = 0;
+                s.fresh = 0;
+                // (count: with those of the last slice that are never drawn)
+                if (k > 1 && (s.few || (uint32_t)k < count))
+                    f.limit = min((uint32_t)k, count);
+                else
+                    next_goal(total);
+            }
+            __syncwarp();
         }
-        t.scan(s, first ? 0 : f.mass_before, first ? 0 : f.count_before);
-        if (s.fresh && tid == kSampleThreads - 1) {
-            u64 likely = 0;
-            f.total = t.mass + t.mass4[0] + t.mass4[1] + t.mass4[2] + t.mass4[3];
-            for (int i = 0; sums && i < C; ++i) likely += s.likely[i];
-            // (the first of the order is kept whatever min_p is)
-            f.likely = s.row.least > 0.0 ? max(likely, (u64)s.row.lift) : f.total;
-            f.goal = kTopK;
-            f.last = 0;
-            const u64 all = t.count + t.count4[0] + t.count4[1] + t.count4[2] + t.count4[3];  // (the last slice's never drawn too)
-            if (k > 1 && (s.few || (u64)k < all))
-                f.limit = min((u64)k, all);
-            else
-                next_goal(f.total);
-        }
-        __syncthreads();
+        find(0, first ? s.first_groups : s.more_groups, first ? s.first : s.more, C, first ? 0 : f.mass_before, first ? 0 : f.count_before,
+             f.goal == kTopK, f.limit);
     }
-    const int goal = f.goal;
-    const bool by_key = f.last < 0;
-    t.pick(s, goal == kTopK, 0, f.limit);
     __syncthreads();
-    const int b = s.at[0];
-    if (first && goal == kTopP && !by_key) {
-        // and the slices that can hold the token, as the kept ones end somewhere in slice b
-        const u64 front = s.at_mass[0], own = s.at_own[0], likely = f.likely;
-        const float u = s.u;
-        __syncthreads();
-#pragma unroll 1
-        for (int j = 0; j < 2; ++j) t.pick(s, false, j, drawn(u, min(j ? front + own : front + 1, likely)));
-        __syncthreads();
-        if (tid == 0) {
+    const int goal = f.goal, b = s.at[0];
+    const bool by_key = f.last < 0;
+    const u64 front = s.at_mass[0], own = s.at_own[0];
+    const uint32_t before = s.at_count[0], members = s.at_members[0];
+    const bool both = first && !by_key && (goal == kTopP || (goal == kTopK && sums && b != kLast && !(s.p < 1.f)));
+    // (the end of what is kept lies in slice b: and the slices that can hold the token)
+    if (both && warp < 2) find(1 + warp, s.first_groups, s.first, C, 0, 0, false, drawn(s.u, min(warp ? front + own : front + 1, f.likely)));
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        if (both) {
             f.op = kGather;
-            f.b0 = s.at[0];
-            f.b1 = s.at[1];
+            f.b0 = s.at[1];
+            f.b1 = s.at[2];
             f.b2 = b;
+            f.by_count = goal == kTopK;
             f.goal = kBoth;
-            f.mass_before = s.at_mass[0];
+            f.mass_before = s.at_mass[1];
             f.more_before = front;
+            f.count_before = before;
             // no slice has more members than its sum has least weights of its (and half a unit each)
-            const auto most = [&](u64 sum, int slice) { return (double)sum / fmax(s.table[slice] * 0.98 - 1.0, 1e-9); };
-            const u64 middle = f.b1 < b ? s.at_mass[1] + s.at_own[1] - s.at_mass[0] : front - s.at_mass[0];
-            f.last = most(middle, min(f.b1, b)) + most(own, b) <= (double)kMembers;
-        }
-    } else if (tid == 0) {
-        const uint32_t before = s.at_count[0], members = s.at_members[0];
-        uint32_t lo = 0, hi = 0;
-        bool into = false;
-        if (!first) {
-            hi = f.hi - ((uint32_t)b << f.shift);
-            const uint32_t span = (1u << f.shift) - 1;
-            lo = hi - f.lo > span ? hi - span : f.lo;
-            into = true;
-        } else if (goal == kTopK && s.few && (b == kLast ? before : before + members) <= (uint32_t)kMembers) {
-            // the kept ones and no more than kMembers in all (those of the last slice have no weight)
-            f.goal = kPrefix;
-            f.limit = b == kLast ? min(f.limit, (u64)before) : f.limit;
-            f.op = kGather;
-            f.b0 = 0;
-            f.b1 = f.b2 = b == kLast ? b - 1 : b;
-            f.last = 1;
-        } else if (!sums) {
-            f.op = kSums;
-        } else if (goal == kTopK && b == kLast) {
-            next_goal(f.total);
-        } else if (goal == kDraw && !by_key) {
-            f.mass_before = s.at_mass[0];
-            f.op = kGather;
-            f.b0 = f.b1 = f.b2 = b;
-            f.last = (double)s.at_own[0] <= (double)kMembers * (s.table[b] * 0.98 - 1.0);
+            const auto most = [&](u64 sum, int slice) { return __fdividef((float)sum, fmaxf((float)s.table[slice] * 0.97f - 1.f, 1e-9f)); };
+            const u64 middle = f.b1 < b ? s.at_mass[2] + s.at_own[2] - s.at_mass[1] : front - s.at_mass[1];
+            f.last = most(middle, min(f.b1, b)) + (k > 1 ? (float)members : most(own, b)) <= (float)kMembers;
         } else {
-            lo = lowest_key(b);
-            hi = b ? lowest_key(b - 1) - 1 : key_of(s.row.m);
-            into = true;
-        }
-        if (into) {
-            f.mass_before = s.at_mass[0];
-            f.count_before = s.at_count[0];
-            f.lo = lo;
-            f.hi = hi;
-            f.last = 0;
-            if ((!first || k > 1) && members <= (uint32_t)kMembers) {
-                f.op = kGatherKeys;
-            } else if (lo < hi) {
-                f.op = kDivide;
-                f.shift = shift_of(hi - lo);
+            uint32_t lo = 0, hi = 0;
+            bool into = false;
+            if (!first) {
+                hi = f.hi - ((uint32_t)b << f.shift);
+                const uint32_t span = (1u << f.shift) - 1;
+                lo = hi - f.lo > span ? hi - span : f.lo;
+                into = true;
+            } else if (goal == kTopK && s.few && (b == kLast ? before : before + members) <= (uint32_t)kMembers) {
+                // the kept ones and no more than kMembers in all (those of the last slice have no weight)
+                f.goal = kPrefix;
+                f.limit = b == kLast ? min(f.limit, (u64)before) : f.limit;
+                f.op = kGather;
+                f.b0 = 0;
+                f.b1 = f.b2 = b == kLast ? b - 1 : b;
+                f.last = 1;
+            } else if (!sums) {
+                f.op = kSums;
+            } else if (goal == kTopK && b == kLast) {
+                next_goal(f.total);
+            } else if (!by_key && (goal == kDraw || members <= (uint32_t)kMembers)) {
+                f.mass_before = front;
+                f.count_before = before;
+                f.op = kGather;
+                f.b0 = f.b1 = f.b2 = b;
+                f.last = goal == kDraw && (float)own <= (float)kMembers * ((float)s.table[b] * 0.97f - 1.f);
             } else {
-                // equal keys
-                const Row r = s.row;
-                const float x = value_of(lo);
-                const u64 w = Row::whole(r.weight(x, r.bin(x), s.table));
-                const u64 nth = goal == kTopK ? f.limit - f.count_before : (f.limit - f.mass_before + w - 1) / max(w, 1ull);
-                if (goal == kDraw) {
-                    f.op = kTies;
-                    f.nth = (uint32_t)nth;
-                    f.logprob = logprob_of(r, x, f.kept);
+                lo = lowest_key(b);
+                hi = b ? lowest_key(b - 1) - 1 : key_of(s.row.m);
+                into = true;
+            }
+            if (into) {
+                f.mass_before = front;
+                f.count_before = before;
+                f.lo = lo;
+                f.hi = hi;
+                f.last = 0;
+                if ((!first || k > 1) && members <= (uint32_t)kMembers) {
+                    f.op = kGatherKeys;
+                } else if (lo < hi) {
+                    f.op = kDivide;
+                    f.shift = shift_of(hi - lo);
                 } else {
-                    next_goal(f.mass_before + nth * w);
+                    // equal keys
+                    const Row r = s.row;
+                    const float x = value_of(lo);
+                    const u64 w = r.weight(x, s.table);
+                    const u64 nth = goal == kTopK ? f.limit - f.count_before : (f.limit - f.mass_before + w - 1) / max(w, 1ull);
+                    if (goal == kDraw) {
+                        f.op = kTies;
+                        f.nth = (uint32_t)nth;
+                        f.logprob = logprob_of(r, x, f.kept);
+                    } else {
+                        next_goal(f.mass_before + nth * w);
+                    }
                 }
             }
         }
     }
-    s.fresh = 0;
     __syncthreads();
 }
 
@@ -636,8 +693,13 @@ __device__ __noinline__ u64 reach(int lo, int hi, u64 before, uint32_t number, b
     Shared& s = shared();
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31, n = (int)s.members;
     const Row r = s.row;
-    const u64* const weight = s.more_mass;
+    const u64* const weight = s.weight;
     uint32_t klo = 0, khi = ~0u;
+    int part = -1;  // of the set, first divided into kSampleThreads parts by its place among the slices
+    const float begin = (float)lo - 0.5f, scale = (float)kSampleThreads / (float)(hi - lo + 1);
+    const auto part_of = [&](float x) {
+        return (int)fminf(fmaxf((fmaf(x, -0.5f, r.half_m) * r.scale - begin) * scale, 0.f), (float)(kSampleThreads - 1));
+    };
     // f(index, key) for this thread's members of the set; returns the set's size
     const auto members = [&](auto f) {
         int size = 0;
@@ -647,22 +709,54 @@ __device__ __noinline__ u64 reach(int lo, int hi, u64 before, uint32_t number, b
             const uint32_t key = i < n ? (uint32_t)(s.member[i] >> 32) : 0u;
             bool is = i < n && key >= klo && key <= khi;
             if (is) {
-                const int b = r.bin(value_of(key));
-                is = b >= lo && b <= hi;
+                const float x = value_of(key);
+                const int b = r.bin(x);
+                is = b >= lo && b <= hi && (part < 0 || part_of(x) == part);
             }
             if (is) f(i, key);
             size += __syncthreads_count(is);
         }
         return size;
     };
-    uint32_t least = ~0u, most = 0;
-    int size = members([&](int, uint32_t key) {
-        least = min(least, key);
-        most = max(most, key);
-    });
+    const auto note = [&](int to, u64 w) {
+        atomicAdd(&s.more.count[to], 1u);
+        const uint32_t was = atomicAdd(&s.more.low[to], (uint32_t)w);
+        atomicAdd(&s.more.high[to], (uint32_t)(w >> 32) + (was + (uint32_t)w < was));
+    };
+    int size = members([&](int i, uint32_t key) { note(part_of(value_of(key)), weight[i]); });
+    {
+        const u64 m0 = (u64)s.more.low[tid] + ((u64)s.more.high[tid] << 32);
+        const uint32_t c0 = s.more.count[tid];
+        const u64 m = scanned(m0);
+        const uint32_t c = scanned(c0);
+        if (lane == 31) s.warp_mass[warp] = m, s.warp_count[warp] = c;
+        __syncthreads();
+        u64 mass = before + m - m0;
+        uint32_t count = number + c - c0;
+#pragma unroll 4
+        for (int i = 0; i < warp; ++i) mass += s.warp_mass[i], count += s.warp_count[i];
+        const u64 had = by_count ? count : mass, has = by_count ? count + c0 : mass + m0;
+        if (had < limit && limit <= has) {
+            s.at[0] = tid;
+            s.at_mass[0] = mass;
+            s.at_count[0] = count;
+            s.at_members[0] = c0;
+        }
+        s.more.low[tid] = s.more.high[tid] = s.more.count[tid] = 0;
+        __syncthreads();
+        part = s.at[0];
+        before = s.at_mass[0];
+        number = s.at_count[0];
+        size = (int)s.at_members[0];
+    }
 #pragma unroll 1
     while (size > kFew) {
         // the set's keys from lowest to highest, divided
+        uint32_t least = ~0u, most = 0;
+        members([&](int, uint32_t key) {
+            least = min(least, key);
+            most = max(most, key);
+        });
         least = __reduce_min_sync(0xffffffffu, least);
         most = __reduce_max_sync(0xffffffffu, most);
         if (lane == 0) s.warp_lo[warp] = least, s.warp_hi[warp] = most;
@@ -671,33 +765,18 @@ __device__ __noinline__ u64 reach(int lo, int hi, u64 before, uint32_t number, b
         khi = __reduce_max_sync(0xffffffffu, s.warp_hi[lane % kSampleWarps]);
         if (klo == khi) break;
         const int shift = shift_of(khi - klo);
-        members([&](int i, uint32_t key) {
-            const int to = (int)((khi - key) >> shift);
-            const u64 w = weight[i];
-            atomicAdd(&s.own_count[to], 1u);
-            const uint32_t was = atomicAdd(&s.own_low[to], (uint32_t)w);
-            atomicAdd(&s.own_high[to], (uint32_t)(w >> 32) + (was + (uint32_t)w < was));
-        });
-        Slices t;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            t.mass4[i] = (u64)s.own_low[4 * tid + i] + ((u64)s.own_high[4 * tid + i] << 32);
-            t.count4[i] = s.own_count[4 * tid + i];
-        }
-        t.scan(s, before, number);
-        t.pick(s, by_count, 0, limit);
+        members([&](int i, uint32_t key) { note((int)((khi - key) >> shift), weight[i]); });
+        group(s.more, s.more_groups);
+        __syncthreads();
+        if (warp == 0) find(0, s.more_groups, s.more, 1, before, number, by_count, limit);
         __syncthreads();
         before = s.at_mass[0];
         number = s.at_count[0];
+        size = (int)s.at_members[0];
         const uint32_t top = khi - ((uint32_t)s.at[0] << shift), span = (1u << shift) - 1;
         klo = top - klo > span ? top - span : klo;
         khi = top;
-        clear(s);
-        least = ~0u, most = 0;
-        size = members([&](int, uint32_t key) {
-            least = min(least, key);
-            most = max(most, key);
-        });
+        clear(s.more);
     }
     if (tid == 0) s.staged = 0;
     __syncthreads();
@@ -767,10 +846,9 @@ __device__ __noinline__ void settle(const SampleArgs& a, int row) {
 #pragma unroll 1
         for (int i = tid; i < n; i += kSampleThreads) {
             const float x = value_of((uint32_t)(s.member[i] >> 32));
-            const double y = table ? r.weight(x, r.bin(x), s.table) : exp_of(((double)x - (double)r.m) * r.per_t) * r.lift;
-            const u64 w = Row::whole(y);
-            s.more_mass[i] = w;
-            if (y >= r.least) likely += w;
+            const u64 w = table ? r.weight(x, s.table) : Row::whole(exp_of(((double)x - (double)r.m) * r.per_t) * r.lift + kTwo52);
+            s.weight[i] = w;
+            if (w >= r.least) likely += w;
         }
     }
     if (goal == kPrefix) {
@@ -784,39 +862,99 @@ __device__ __noinline__ void settle(const SampleArgs& a, int row) {
     __syncthreads();
     const float p = s.p, u = s.u;
     u64 kept = s.find.kept, answer = 0;
-    const int questions = goal == kPrefix ? 3 : goal == kBoth ? 2 : 1;
-#pragma unroll 1
-    for (int q = 0; q < questions; ++q) {
-        int lo = 0, hi = kLast;
-        u64 before = s.find.mass_before, limit = s.find.limit;
-        uint32_t number = 0;
-        bool by_count = false;
-        if (goal == kPrefix) {
-            before = 0;
-            by_count = q == 0;
-            if (q == 1) {
-                if (!(p < 1.f)) continue;
-                limit = nucleus(p, kept);
+    if (n <= kFew) {
+        // a few members: four threads each find how many are before it and their sum, then a warp asks
+        const int e = min(tid / 4, n - 1);
+        const u64 mine = s.member[e], own = s.weight[e];
+        u64 sum = 0;
+        int place = 0;
+#pragma unroll 4
+        for (int i = tid % 4; i < n; i += 4)
+            if (s.member[i] > mine) {
+                ++place;
+                sum += s.weight[i];
             }
-            if (q == 2) {
-                kept = min(kept, likely);
-                limit = drawn(u, kept);
-            }
-        } else if (goal == kBoth) {
-            if (q == 0) {
-                lo = hi = s.find.b2;
-                before = s.find.more_before;
-            } else {
-                hi = s.find.b1;
-                kept = min(kept, s.find.likely);
-                limit = drawn(u, kept);
-            }
-        } else if (goal == kTopK) {
-            by_count = true;
-            number = s.find.count_before;
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            place += __shfl_xor_sync(0xffffffffu, place, o);
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        answer = reach(lo, hi, before, number, by_count, limit);
-        if (q + 1 < questions) kept = answer;
+        if (tid % 4 == 0 && tid / 4 < n) {
+            s.set_member[place] = mine;
+            s.set_weight[place] = sum + own;  // the running sum
+            s.set_slice[place] = Row(s.row).bin(value_of((uint32_t)(mine >> 32)));
+        }
+        __syncthreads();
+        if (warp != 0) return;
+        // the first place in [from, n) whose running sum and `more` reach the limit
+        const auto seek = [&](int from, u64 more, u64 limit) {
+            int at = from;
+#pragma unroll 1
+            for (int i = lane; i - lane < n; i += 32) at += __popc(__ballot_sync(0xffffffffu, i >= from && i < n && s.set_weight[i] + more < limit));
+            return min(at, n - 1);
+        };
+        int at = 0;
+        if (goal == kPrefix) {
+            kept = s.set_weight[s.find.limit - 1];
+            if (p < 1.f) kept = s.set_weight[seek(0, 0, nucleus(p, kept))];
+            kept = min(kept, likely);
+            at = seek(0, 0, drawn(u, kept));
+        } else if (goal == kBoth) {
+            // (members of slices before b2, then those of b2, which others lie in front of)
+            int ahead = 0;
+            for (int i = lane; i - lane < n; i += 32) ahead += __popc(__ballot_sync(0xffffffffu, i < n && s.set_slice[i] < s.find.b2));
+            const u64 more = s.find.more_before - (ahead ? s.set_weight[ahead - 1] : 0);
+            at = s.find.by_count ? ahead + (int)(s.find.limit - s.find.count_before) - 1 : seek(ahead, more, s.find.limit);
+            kept = min(s.set_weight[at] + more, s.find.likely);
+            at = seek(0, s.find.mass_before, drawn(u, kept));
+        } else if (goal == kTopK) {
+            at = (int)(s.find.limit - s.find.count_before) - 1;
+        } else {
+            at = seek(0, s.find.mass_before, s.find.limit);
+        }
+        answer = s.find.mass_before + s.set_weight[at];
+        if (lane == 0) s.at_one = s.set_member[at];
+        __syncwarp();
+    } else {
+        const int questions = goal == kPrefix ? 3 : goal == kBoth ? 2 : 1;
+#pragma unroll 1
+        for (int q = 0; q < questions; ++q) {
+            int lo = 0, hi = kLast;
+            u64 before = s.find.mass_before, limit = s.find.limit;
+            uint32_t number = 0;
+            bool by_count = false;
+            if (goal == kPrefix) {
+                before = 0;
+                by_count = q == 0;
+                hi = s.find.b1;
+                if (q == 1) {
+                    if (!(p < 1.f)) continue;
+                    limit = nucleus(p, kept);
+                }
+                if (q == 2) {
+                    kept = min(kept, likely);
+                    limit = drawn(u, kept);
+                }
+            } else if (goal == kBoth) {
+                if (q == 0) {
+                    lo = hi = s.find.b2;
+                    before = s.find.more_before;
+                    by_count = s.find.by_count;
+                    number = s.find.count_before;
+                } else {
+                    lo = s.find.b0;
+                    hi = s.find.b1;
+                    kept = min(kept, s.find.likely);
+                    limit = drawn(u, kept);
+                }
+            } else {
+                if (s.find.op == kGather) lo = s.find.b0, hi = s.find.b1;
+                by_count = goal == kTopK;
+                number = s.find.count_before;
+            }
+            answer = reach(lo, hi, before, number, by_count, limit);
+            if (q + 1 < questions) kept = answer;
+        }
     }
     if (tid != 0) return;
     if (goal == kTopK || goal == kTopP) {
@@ -838,7 +976,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const int v0 = min(a.vocab, rank * a.slice), nv = min(a.vocab - v0, a.slice);
     const E* in = static_cast<const E*>(a.in) + (int64_t)row * a.ld + v0;
     Shared* const head = cluster.map_shared_rank(&s, 0);
-    clear(s);
+    clear(s.first);
+    clear(s.more);
     stream_turn();
     const float T0 = a.temperature ? a.temperature[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
     const int k = a.top_k ? a.top_k[row] : 0;
@@ -851,6 +990,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         s.min_p = min_p;
         s.table_made = 0;
         s.fresh = 1;
+        s.row.per_t = 1.0 / (double)fmaxf(T0, 7.8886091e-31f);  // 2^-100: what follows stays within f32's range
     }
     // ---- the largest and the smallest
     {
@@ -892,15 +1032,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         // the first of the order; or, beside +infinity, only what is: tokens of equal weights
         op = !(T0 > 0.f) || k == 1 ? kTies : r.m == INFINITY ? kCrowd : k > 1 && k <= kMembers ? kNumbers : kSums;
         if (tid == 0) {
-            const float T = fmaxf(T0, 7.8886091e-31f);  // 2^-100: what follows stays within f32's range
+            const float T = fmaxf(T0, 7.8886091e-31f);
             r.half_m = 0.5f * r.m;
-            r.per_t = 1.0 / (double)T;
+            r.per_t = s.row.per_t;
             r.lift = __longlong_as_double((long long)(1023 + a.bits) << 52);
-            r.least = min_p > 0.f ? (double)min_p * r.lift : 0.0;
+            r.least = min_p > 0.f ? min_p <= 1.f ? (u64)ceil((double)min_p * r.lift) : ~0ull : 0;
             // half of the range that the first histogram divides: all values, or those with a weight
             const float range = fminf(fmaf(least, -0.5f, r.half_m), 18.f * T);
             r.scale = range > 0.f ? fminf((float)(kLast - 1) / range, 1e35f) : 0.f;
-            r.grid = r.scale > 0.f ? 2.0 / (double)r.scale * r.per_t : 0.0;
+            // step / T rounded up to 13 bits, and the scale to match it (where T is without end there is neither)
+            const float per_t = (float)r.per_t, grid = r.scale > 0.f ? 2.f / r.scale * per_t : 0.f;
+            r.grid = grid > 1e-30f && grid < 1.f ? __uint_as_float((__float_as_uint(grid * 1.000001f) + 0x7FFu) & ~0x7FFu) : 0.f;
+            if (r.grid > 0.f) r.scale = 2.f * per_t / r.grid;
+            const float step = r.scale > 0.f ? 2.f / r.scale : 0.f;
+            r.floor = r.m - (float)(kBins + 1) * step;
+            if (!(r.scale > 0.f) || !(fabsf(r.m) < 1e30f) || !(r.floor > -1e30f) || r.bin(r.floor) != kLast) r.floor = -INFINITY;
             s.row = r;
             s.find.lo = key_of(r.m);
             s.find.nth = 1;
@@ -928,18 +1074,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             if (tid == 0) s.base = atomicAdd(&head->members, staged);
             __syncthreads();
             const uint32_t base = s.base;
-            const u64* const stage = reinterpret_cast<const u64*>(s.own_low);
+            const u64* const stage = reinterpret_cast<const u64*>(s.more.low);
 #pragma unroll 1
             for (uint32_t i = tid; i < staged && base + i < (uint32_t)kMembers; i += kSampleThreads) head->member[base + i] = stage[i];
             __syncthreads();
-            clear(s);
+            clear(s.more);
             cluster.sync();
             if (last && rank != 0) return;
             if (rank == 0) {
                 if (s.members > (uint32_t)kMembers) {
                     // (a slice whose tokens were not counted has more than that: by its keys)
                     if (tid == 0) {
-                        if (s.find.goal == kBoth) s.find.goal = kTopP;
+                        if (s.find.goal == kBoth) s.find.goal = s.find.by_count ? kTopK : kTopP;
                         s.find.op = kLook;
                         s.find.last = -1;
                     }
@@ -958,23 +1104,29 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             if (op == kDone) return;
         }
         if (op == kDivide) {
+            cluster.sync();  // what the histograms before held is read by all
             divide_pass<E>(in, nv);
         } else if (op == kNumbers) {
             numbers_pass<E>(in, nv);
         } else if (op == kSums) {
+            if (k > 1 && k <= kMembers) {
+                // (the numbers there are first: read by all, then cleared)
+                cluster.sync();
+                clear(s.first);
+            }
             if (tid < kBins / 32 + 32) {
                 const int i = tid < kBins / 32 ? 32 * tid : tid - kBins / 32;
-                const double e = exp_of(-i * s.row.grid);
+                const double e = exp_of(-i * (double)s.row.grid);
                 if (tid < kBins / 32)
                     s.coarse[tid] = e * s.row.lift;
                 else
                     s.fine[tid - kBins / 32] = e;
             }
             __syncthreads();
-            for (int i = tid; i < kBins; i += kSampleThreads) s.table[i] = s.coarse[i / 32] * s.fine[i % 32];
+            for (int i = tid; i < kBins; i += kSampleThreads) s.table[i] = i == kLast ? 0.0 : s.coarse[i / 32] * s.fine[i % 32];
             if (tid == 0) s.table_made = s.fresh = 1;
             __syncthreads();
-            if (k > 1 || s.row.least > 0.0) {
+            if (k > 1 || s.row.least || s.row.floor == -INFINITY) {
                 const u64 likely = warp_sum(sums_pass<E, true>(in, nv));
                 if (lane == 0) s.warp_mass[warp] = likely;
                 __syncthreads();
@@ -987,8 +1139,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 sums_pass<E, false>(in, nv);
             }
         }
-        if (op != kLook) collect(op != kDivide, op != kNumbers, op != kSums || k > 1);
+        if (op == kDivide)
+            collect(s.more, s.more_groups, C, rank);
+        else if (op != kLook)
+            collect(s.first, s.first_groups, C, rank);
         look(op != kDivide, op != kNumbers, C);
+        if (op == kDivide) {
+            cluster.sync();  // read by all, then cleared
+            clear(s.more);
+            __syncthreads();
+        }
         op = s.find.op;
     }
 }
