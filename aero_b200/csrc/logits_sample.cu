@@ -36,7 +36,8 @@ using u64 = unsigned long long;
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleCluster = 8;
-constexpr int kBins = 4 * kSampleThreads, kLast = kBins - 1, kGroups = kBins / 32;
+constexpr int kBins = 8 * kSampleThreads, kLast = kBins - 1, kGroups = 64;
+constexpr int kParts = 4 * kSampleThreads;  // of a slice's keys
 constexpr int kMembers = 2048;
 constexpr int kFew = kSampleThreads / 4;  // members put in order by counting
 constexpr int kMostVocab = 1 << 22;
@@ -80,34 +81,42 @@ __device__ __forceinline__ float value_in(uint32_t w, int j) {
         return __uint_as_float(j ? w & 0xFFFF0000u : w << 16);
 }
 
-// What all threads know of a row. Its values are divided into kBins slices, slice b around m - b step; the last one holds
-// what lies 36 T and more below m, whose weights (e^-36 < 2^-51) are 0 as multiples of 2^-48 or more, and what is never
-// drawn (-infinity and no numbers).
+// What all threads know of a row. Its values are divided into kBins slices below m, 64 to each halving of the weights; the last
+// one holds what lies 63.99 halvings and more below m, whose weights are 0 as multiples of 2^-48 or more, and what is
+// never drawn (-infinity and no numbers).
 struct Row {
     float m;             // the largest logit
     float half_m, scale; // slice = (m / 2 - x / 2) * scale (halves: the difference of any two numbers is one)
-    float grid;          // step / T, of 13 bits: a slice's number times it is exact
-    float floor;         // below the last slice's beginning, above -infinity; -infinity: there is no such number
-    double per_t;        // 1 / T
+    float step;          // a slice's width; infinity: m is too large for sums and differences of slices' ends
+    float floor;         // a value of the last slice, next to its middle; -infinity: there is none
+    double per_t;        // 16 log2(e) / T
     double lift;         // 2^B
     u64 least;           // min_p 2^B
+    __device__ __forceinline__ float open_place(float x) const { return fmaf(x, -0.5f, half_m) * scale; }
+    __device__ __forceinline__ float place(float x) const { return fminf(open_place(x), (float)kLast); }
     // (as a number beside 2^23, for comparisons)
-    __device__ __forceinline__ float slice(float x) const { return fminf(fmaf(x, -0.5f, half_m) * scale, (float)kLast) + 8388608.f; }
+    __device__ __forceinline__ float slice(float x) const { return place(x) + 8388608.f; }
     __device__ __forceinline__ int bin(float x) const { return (int)(__float_as_uint(slice(x)) & (kBins - 1)); }
     // 2^52 + 2^B e^((x - m) / T), which leaves the weight's nearest whole number in the low bits (2^B is at most 2^48), for
-    // slices but the last: with y = (x - m) / T + b step / T, at most 0.009 either way, the table's value e^(-b step / T) 2^B
-    // times e^y by its series, whose first term left out is below 10^-15
-    __device__ __forceinline__ double beside(float x, float slice, const double* table) const {
-        const double y = fma((double)x - (double)m, per_t, (double)((slice - 8388608.f) * grid));
-        double p = fma(y, 1.0 / 120, 1.0 / 24);
-        p = fma(p, y, 1.0 / 6);
-        p = fma(p, y, 0.5);
-        p = fma(p, y, 1.0);
-        p = fma(p, y, 1.0);
-        return fma(p, table[__float_as_uint(slice) & (kBins - 1)], kTwo52);
+    // slices but the last. at = place(x). In sixteenths of a halving x lies z = 16 log2(e) (x - m) / T above m; with i the whole number
+    // next to -z and r = z + i, at most a half either way, the weight is 2^-(i / 16) 2^(r / 16): a table's value (2^B's sixteen parts,
+    // the halvings taken off its exponent) times the series of 2^(r / 16) to r^5, whose term in r^6 is made up for by Chebyshev's
+    // polynomial; what is left out is below 2^-46.
+    __device__ __forceinline__ double beside(float x, float at, const double* table) const {
+        constexpr double L = 0.6931471805599453 / 16, h2 = 0.25, a5 = L * L * L * L * L * L / 720;
+        const float i = fmaf(at, 0.25f, 8388608.f);
+        const double z = fma((double)x - (double)m, per_t, (double)(i - 8388608.f));
+        double p = fma(z, L * L * L * L * L / 120, L * L * L * L / 24 + 1.25 * h2 * a5);
+        p = fma(p, z, L * L * L / 6);
+        p = fma(p, z, L * L / 2 - 0.3125 * h2 * h2 * a5);
+        p = fma(p, z, L);
+        p = fma(p, z, 1.0);
+        const uint32_t n = __float_as_uint(i);
+        const double t = table[n & 15u];
+        return fma(p, __hiloint2double(__double2hiint(t) - (int)((n & ~15u) * 65536u), __double2loint(t)), kTwo52);
     }
     static __device__ __forceinline__ u64 whole(double beside) { return (u64)__double_as_longlong(beside) & 0xFFFFFFFFFFFFFull; }
-    __device__ __forceinline__ u64 weight(float x, const double* table) const { return whole(beside(x, slice(x), table)); }
+    __device__ __forceinline__ u64 weight(float x, const double* table) const { return whole(beside(x, place(x), table)); }
 };
 
 // what the cluster does next
@@ -126,6 +135,8 @@ struct Search {
     int b0, b1, b2;      // kGather: slices [b0, b1] and b2
     int last;            // kGather: the members have the answer for certain; -1: a slice has too many
     int by_count;        // kBoth: the first is what top_k keeps
+    int k_slice;         // the slice that holds the k-th, or -1: top_k keeps all
+    uint32_t k_before, k_members;  // tokens before it and in it
     uint32_t nth;        // kTies: which of the tokens with key lo, from 1
     float logprob;       // kTies
     uint32_t count_before;         // tokens before the slice in hand
@@ -134,37 +145,39 @@ struct Search {
     u64 total, kept, likely;       // sums: of the row, of the kept, of those that min_p keeps
 };
 
-// A CTA's histogram of its tokens: sums as two words, numbers.
-struct Histogram {
-    uint32_t low[kBins], high[kBins], count[kBins];
+// A CTA's histogram of its tokens: sums as two words (or numbers, as the low one), numbers.
+struct Slices {
+    uint32_t low[kBins], high[kBins];
 };
-// Sums over 32 slices each.
+struct Parts {
+    uint32_t low[kParts], high[kParts], count[kParts];
+};
+// Sums over a 64th of a histogram each.
 struct Groups {
     u64 mass[kGroups];
     uint32_t count[kGroups];
 };
 
 struct Shared {
-    double table[kBins];
-    Histogram first;          // of Row's slices
-    Histogram more;           // of one slice's keys, or of members' keys; the place of members on their way; else zero
+    double table[16];
+    Slices first;             // of Row's slices
+    Parts more;               // of one slice's keys, or of members' keys; the place of members on their way; else zero
     u64 member[kMembers];     // key, then all ones less the token's number (in the first CTA)
     u64 weight[kMembers];     // (in the first CTA)
     Groups from[kSampleCluster];         // what the CTAs' histograms hold
     Groups first_groups, more_groups;    // the row's
     u64 set_member[kFew], set_weight[kFew];
     int set_slice[kFew];
-    double coarse[kBins / 32], fine[32];
     u64 warp_mass[kSampleWarps];
     uint32_t warp_count[kSampleWarps], warp_lo[kSampleWarps], warp_hi[kSampleWarps];
-    float2 ends[kSampleCluster], warp_ends[kSampleWarps];  // largest and smallest of the CTAs, of the warps
+    float ends[kSampleCluster], warp_ends[kSampleWarps];  // the largest of the CTAs, of the warps
     u64 likely[kSampleCluster];
     uint32_t ties[kSampleCluster];
     uint32_t members, staged, base;
     Row row;
     Search find;
     float u, p, min_p;
-    int k, few, table_made, fresh;
+    int k, few, fresh;
     int at[3];
     u64 at_mass[3], at_own[3], at_one;
     uint32_t at_count[3], at_members[3];
@@ -177,10 +190,9 @@ __device__ __forceinline__ Shared& shared() {
     extern __shared__ __align__(16) uint8_t smem[];
     return *reinterpret_cast<Shared*>(smem);
 }
-__device__ __noinline__ double exp_of(double x) { return exp(x); }
 __device__ __noinline__ double log_of(double x) { return log(x); }
 __device__ __forceinline__ float logprob_of(const Row& r, float x, u64 kept) {
-    return (float)(((double)x - (double)r.m) * r.per_t - log_of((double)kept / r.lift));
+    return (float)(((double)x - (double)r.m) * r.per_t * (0.6931471805599453 / 16) - log_of((double)kept / r.lift));
 }
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -189,9 +201,10 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
     return v;
 }
 
-__device__ __forceinline__ void clear(Histogram& h) {
+template <typename H>
+__device__ __forceinline__ void clear(H& h) {
 #pragma unroll 1
-    for (int i = (int)threadIdx.x; i < 3 * kBins / 4; i += kSampleThreads) reinterpret_cast<uint4*>(h.low)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = (int)threadIdx.x; i < (int)sizeof(H) / 16; i += kSampleThreads) reinterpret_cast<uint4*>(&h)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
 // u S as the running sum to be reached: the first above it.
@@ -234,11 +247,23 @@ __device__ __noinline__ uint32_t lowest_key(int b) {
     return lo;
 }
 
-// (hi - lo) >> shift < kBins = 2^11
+// (hi - lo) >> shift < kParts = 2^11
 __device__ __forceinline__ int shift_of(uint32_t span) { return max(0, 21 - __clz((int)span)); }
 
-// A histogram's groups; every thread calls it. Four slices a thread, eight threads a group.
-__device__ __forceinline__ void group(const Histogram& h, Groups& g) {
+// A histogram's groups; every thread calls it: eight threads a group.
+__device__ __forceinline__ void group(const Slices& h, Groups& g) {
+    const int t = (int)threadIdx.x;
+    u64 m = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint4 low = reinterpret_cast<const uint4*>(h.low)[2 * t + i], high = reinterpret_cast<const uint4*>(h.high)[2 * t + i];
+        m += (u64)low.x + low.y + low.z + low.w + (((u64)high.x + high.y + high.z + high.w) << 32);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    if (t % 8 == 0) g.mass[t / 8] = m;
+}
+__device__ __forceinline__ void group(const Parts& h, Groups& g) {
     const int t = (int)threadIdx.x;
     const uint4 low = reinterpret_cast<const uint4*>(h.low)[t], high = reinterpret_cast<const uint4*>(h.high)[t];
     const uint4 count = reinterpret_cast<const uint4*>(h.count)[t];
@@ -251,6 +276,7 @@ __device__ __forceinline__ void group(const Histogram& h, Groups& g) {
     }
     if (t % 8 == 0) g.mass[t / 8] = m, g.count[t / 8] = c;
 }
+static_assert(kSampleThreads == 8 * kGroups, "eight threads a group");
 
 template <typename V>
 __device__ __forceinline__ V scanned(V v) {
@@ -263,33 +289,76 @@ __device__ __forceinline__ V scanned(V v) {
     return v;
 }
 
-// By a warp: the slice of a histogram (C CTAs' together) that holds the answer to a limit into at[j], with what lies before it
-// and what it holds (numbers before it: only where the limit is one). Reads of other CTAs' memory are slow: groups first, then 32
-// slices.
-__device__ __noinline__ void find(int j, const Groups& g, const Histogram& h, int C, u64 mass_before, uint32_t count_before, bool by_count,
-                                  u64 limit) {
+// By a warp: the slice of the first histogram (C CTAs' together) that holds the answer to a limit into at[j], with what lies
+// before it and what it holds; or, of slice b, the last two. Reads of other CTAs' memory are slow: groups first, then 64 slices.
+__device__ __noinline__ void find(int j, int C, u64 limit, int b) {
+    Shared& s = shared();
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int lane = (int)threadIdx.x & 31;
+    const u64 g0 = s.first_groups.mass[2 * lane], g1 = s.first_groups.mass[2 * lane + 1];
+    const u64 g = scanned(g0 + g1);
+    // which group: 2 lane or 2 lane + 1 of the lane that the limit lies in
+    int group;
+    if (b < 0) {
+        const int in = min(__popc(__ballot_sync(0xffffffffu, g < limit)), 31);
+        group = 2 * in + (__shfl_sync(0xffffffffu, g - g1, in) < limit);
+    } else {
+        group = b / 64;
+    }
+    const u64 to_odd = __shfl_sync(0xffffffffu, g - g1, group / 2), to_even = __shfl_sync(0xffffffffu, g - g1 - g0, group / 2);
+    const u64 before = group & 1 ? to_odd : to_even;
+    u64 m0 = 0, m1 = 0;
+    const int at = 64 * group + 2 * lane;
+#pragma unroll 4
+    for (int i = 0; i < C; ++i) {
+        const Slices* o = C > 1 ? cluster.map_shared_rank(&s.first, i) : &s.first;
+        const uint2 low = *reinterpret_cast<const uint2*>(o->low + at), high = *reinterpret_cast<const uint2*>(o->high + at);
+        m0 += (u64)low.x + ((u64)high.x << 32);
+        m1 += (u64)low.y + ((u64)high.y << 32);
+    }
+    const u64 m = before + scanned(m0 + m1);
+    bool odd;
+    int in;
+    if (b < 0) {
+        in = min(__popc(__ballot_sync(0xffffffffu, m < limit)), 31);
+        odd = m - m1 < limit;
+    } else {
+        in = b % 64 / 2;
+        odd = b & 1;
+    }
+    if (lane == in) {
+        s.at[j] = at + odd;
+        s.at_mass[j] = odd ? m - m1 : m - m1 - m0;
+        s.at_own[j] = odd ? m1 : m0;
+    }
+    __syncwarp();
+}
+
+// By a warp: the part of a slice's histogram (C CTAs' together) that holds the answer to a limit into at[0], with what lies before it and
+// what it holds.
+__device__ __noinline__ void find_part(int C, u64 mass_before, uint32_t count_before, bool by_count, u64 limit) {
     Shared& s = shared();
     const cg::cluster_group cluster = cg::this_cluster();
     const int lane = (int)threadIdx.x & 31;
     int b = 0;
-    // groups 0 to 31 and 32 to 63, as far as the one with the answer; then its 32 slices
+    // groups 0 to 31 and 32 to 63, as far as the one with the answer; then its 32 parts
 #pragma unroll 1
     for (int step = 0; step < 3; ++step) {
         u64 m0 = 0;
         uint32_t c0 = 0;
         if (step < 2) {
-            m0 = g.mass[32 * step + lane];
-            c0 = g.count[32 * step + lane];
+            m0 = s.more_groups.mass[32 * step + lane];
+            c0 = s.more_groups.count[32 * step + lane];
         } else {
-#pragma unroll 4
+#pragma unroll 1
             for (int i = 0; i < C; ++i) {
-                const Histogram* o = C > 1 ? cluster.map_shared_rank(const_cast<Histogram*>(&h), i) : &h;
+                const Parts* o = C > 1 ? cluster.map_shared_rank(&s.more, i) : &s.more;
                 m0 += (u64)o->low[b + lane] + ((u64)o->high[b + lane] << 32);
                 c0 += o->count[b + lane];
             }
         }
         const u64 m = scanned(m0);
-        const uint32_t c = by_count ? scanned(c0) : 0;
+        const uint32_t c = scanned(c0);
         const int at = __popc(__ballot_sync(0xffffffffu, (by_count ? (u64)count_before + c : mass_before + m) < limit));
         if (step == 0 && at == 32) {
             mass_before += __shfl_sync(0xffffffffu, m, 31);
@@ -299,20 +368,19 @@ __device__ __noinline__ void find(int j, const Groups& g, const Histogram& h, in
         const int in = min(at, 31);
         if (step < 2) {
             mass_before += __shfl_sync(0xffffffffu, m - m0, in);
-            count_before += by_count ? __shfl_sync(0xffffffffu, c - c0, in) : 0;
+            count_before += __shfl_sync(0xffffffffu, c - c0, in);
             b = 32 * (32 * step + in);
             step = 1;
         } else if (lane == in) {
-            s.at[j] = b + in;
-            s.at_mass[j] = mass_before + m - m0;
-            s.at_own[j] = m0;
-            s.at_count[j] = count_before + (by_count ? c - c0 : 0);
-            s.at_members[j] = c0;
+            s.at[0] = b + in;
+            s.at_mass[0] = mass_before + m - m0;
+            s.at_own[0] = m0;
+            s.at_count[0] = count_before + c - c0;
+            s.at_members[0] = c0;
         }
     }
     __syncwarp();
 }
-static_assert(kGroups == 64, "two steps of groups");
 
 // f(four values, the first one's token) for a CTA's tokens; values past the last one are -infinity. U 16-byte pieces a
 // thread are on their way while as many are looked at.
@@ -331,21 +399,30 @@ __device__ __forceinline__ void each(const E* in, int v0, int nv, F f) {
             f(x, v0 + i * V + j);
         }
     };
-    uint4 next[U];
+    int i = tid;
+    if (i + (2 * U - 1) * kSampleThreads < vecs) {
+        const uint4* q = v + tid;
+        uint4 next[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) next[k] = tid + k * kSampleThreads < vecs ? v[tid + k * kSampleThreads] : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 1
-    for (int i = tid; i < vecs; i += U * kSampleThreads) {
-        uint4 now[U];
+        for (int k = 0; k < U; ++k) next[k] = q[k * kSampleThreads];
+        do {
+            uint4 now[U];
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            now[k] = next[k];
-            if (i + (U + k) * kSampleThreads < vecs) next[k] = v[i + (U + k) * kSampleThreads];
-        }
+            for (int k = 0; k < U; ++k) {
+                now[k] = next[k];
+                next[k] = q[(U + k) * kSampleThreads];
+            }
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (i + k * kSampleThreads < vecs) piece(now[k], i + k * kSampleThreads);
+            for (int k = 0; k < U; ++k) piece(now[k], i + k * kSampleThreads);
+            q += U * kSampleThreads;
+            i += U * kSampleThreads;
+        } while (i + (2 * U - 1) * kSampleThreads < vecs);
+#pragma unroll
+        for (int k = 0; k < U; ++k) piece(next[k], i + k * kSampleThreads);
+        i += U * kSampleThreads;
     }
+#pragma unroll 1
+    for (; i < vecs; i += kSampleThreads) piece(v[i], i);
 #pragma unroll 1
     for (int i = vecs * V + 4 * tid; i < nv; i += 4 * kSampleThreads) {
         float x[4];
@@ -355,16 +432,28 @@ __device__ __forceinline__ void each(const E* in, int v0, int nv, F f) {
     }
 }
 
-// Four weights (as Row::beside) into this CTA's histogram: a 64-bit sum as two of 32 bits.
-__device__ __forceinline__ void add4(Histogram& h, const int (&b)[4], const double (&w)[4]) {
-    uint32_t was[4];
+// Four weights (as Row::beside) into this CTA's histogram: a 64-bit sum as two of 32 bits. b: the slices, beside 2^23 as f32's bits
+// (what lies above them leaves by overflow when they become addresses).
+template <typename H>
+__device__ __forceinline__ void add4(H& h, const uint32_t (&b)[4], const double (&w)[4]) {
+    constexpr uint32_t kBeside = 0x4B000000u;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(h.low) - (kBeside << 2);
+    uint32_t was[4], high[4], any = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) was[e] = atomicAdd(&h.low[b[e]], (uint32_t)__double2loint(w[e]));
+    for (int e = 0; e < 4; ++e)
+        asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(was[e]) : "r"(to + (b[e] << 2)), "r"(__double2loint(w[e])) : "memory");
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const uint32_t low = (uint32_t)__double2loint(w[e]);
-        const uint32_t high = (uint32_t)__double2hiint(w[e]) - 0x43300000u + (was[e] + low < low);
-        if (high) atomicAdd(&h.high[b[e]], high);
+        uint32_t sum;
+        asm("add.cc.u32 %0, %2, %3;\n\taddc.u32 %1, %4, 0xBCD00000;"  // (less the high word of 2^52)
+            : "=r"(sum), "=r"(high[e])
+            : "r"(was[e]), "r"(__double2loint(w[e])), "r"(__double2hiint(w[e])));
+        any |= high[e];
+    }
+    if (any) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (high[e]) atomicAdd(&h.high[b[e] - kBeside], high[e]);
     }
 }
 
@@ -374,31 +463,29 @@ __device__ __noinline__ void numbers_pass(const E* in, int nv) {
     const Row r = s.row;
     each<E>(in, 0, nv, [&](const float (&x)[4], int) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) atomicAdd(&s.first.count[r.bin(x[e])], 1u);
+        for (int e = 0; e < 4; ++e) atomicAdd(&s.first.low[r.bin(x[e])], 1u);
     });
 }
 
-// FULL: numbers too, values down to the least of all numbers, and returns the sum of this thread's weights that min_p keeps.
+// FULL: values down to the least of all numbers, and returns the sum of this thread's weights that min_p keeps.
 template <typename E, bool FULL>
 __device__ __noinline__ u64 sums_pass(const E* in, int nv) {
     Shared& s = shared();
     const Row r = s.row;
     u64 likely = 0;
     each<E>(in, 0, nv, [&](const float (&x)[4], int) {
-        int b[4];
+        uint32_t b[4];
         double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            // (what is below the last slice's beginning, or no number, is there: the table's last value is 0)
-            const float y = FULL ? x[e] : fmaxf(x[e], r.floor);
-            const float at = r.slice(y);
-            b[e] = (int)(__float_as_uint(at) & (kBins - 1));
+            // (what is below the last slice's beginning, or no number, is there, and its weight is less than a half)
+            const float y = FULL ? x[e] : fmaxf(x[e], r.floor), at = FULL ? r.place(y) : r.open_place(y);
+            b[e] = __float_as_uint(at + 8388608.f);
             w[e] = r.beside(y, at, s.table);
             if (FULL) {
-                if (b[e] == kLast) w[e] = kTwo52;
+                if (at > (float)kLast - 0.5f) w[e] = kTwo52;
                 const u64 n = Row::whole(w[e]);
                 if (n >= r.least) likely += n;
-                atomicAdd(&s.first.count[b[e]], 1u);
             }
         }
         add4(s.first, b, w);
@@ -413,16 +500,17 @@ __device__ __noinline__ void divide_pass(const E* in, int nv) {
     const uint32_t lo = s.find.lo, hi = s.find.hi;
     const int shift = s.find.shift;
     each<E>(in, 0, nv, [&](const float (&x)[4], int) {
-        int b[4];
+        uint32_t b[4];
         double w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t key = key_of(x[e]);
             const bool is = key >= lo && key <= hi;
-            const float at = r.slice(x[e]);
-            b[e] = is ? (int)((hi - key) >> shift) : 0;
-            w[e] = is && at < 8388608.f + (float)kLast ? r.beside(x[e], at, s.table) : kTwo52;
-            if (is) atomicAdd(&s.more.count[b[e]], 1u);
+            const float at = r.place(x[e]);
+            const uint32_t to = is ? (hi - key) >> shift : 0u;
+            b[e] = 0x4B000000u + to;
+            w[e] = is && r.bin(x[e]) != kLast ? r.beside(x[e], at, s.table) : kTwo52;
+            if (is) atomicAdd(&s.more.count[to], 1u);
         }
         add4(s.more, b, w);
     });
@@ -434,7 +522,10 @@ __device__ __noinline__ void gather_pass(const E* in, int v0, int nv) {
     Shared& s = shared();
     const Row r = s.row;
     const uint32_t lo = s.find.lo, hi = s.find.hi;
-    const float f0 = 8388608.f + (float)s.find.b0, f1 = 8388608.f + (float)s.find.b1, f2 = 8388608.f + (float)s.find.b2;
+    const int b0 = s.find.b0, b1 = s.find.b1, b2 = s.find.b2;
+    // values that the slices lie between, a slice more on either side
+    const auto end_of = [&](int b, float off) { return r.step < INFINITY ? fmaf(-((float)b + off), r.step, r.m) : -off * INFINITY; };
+    const float lo1 = end_of(b1, 1.5f), hi1 = end_of(b0, -1.5f), lo2 = end_of(b2, 1.5f), hi2 = end_of(b2, -1.5f);
     u64* const stage = reinterpret_cast<u64*>(s.more.low);
     each<E, 4 / (4 / (int)sizeof(E))>(in, v0, nv, [&](const float (&x)[4], int token) {
         uint32_t is = 0;
@@ -444,14 +535,15 @@ __device__ __noinline__ void gather_pass(const E* in, int v0, int nv) {
                 const uint32_t key = key_of(x[e]);
                 if (key >= lo && key <= hi) is |= 1u << e;
             } else {
-                const float at = r.slice(x[e]);
-                if ((at >= f0 && at <= f1) || at == f2) is |= 1u << e;
+                if ((x[e] >= lo1 && x[e] <= hi1) || (x[e] >= lo2 && x[e] <= hi2)) is |= 1u << e;
             }
         }
         if (is) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (is >> e & 1u) {
+                    const int b = r.bin(x[e]);
+                    if (!KEYS && !((b >= b0 && b <= b1) || b == b2)) continue;
                     const uint32_t at = atomicAdd(&s.staged, 1u);
                     if (at < (uint32_t)kMembers) stage[at] = (u64)key_of(x[e]) << 32 | (uint32_t)~(token + e);
                 }
@@ -459,16 +551,12 @@ __device__ __noinline__ void gather_pass(const E* in, int v0, int nv) {
     });
 }
 
-// The largest and the smallest but -infinity, of this thread's values.
+// The largest of this thread's values.
 template <typename E>
-__device__ __noinline__ float2 ends_pass(const E* in, int nv) {
+__device__ __noinline__ float most_pass(const E* in, int nv) {
     constexpr int PER = 4 / (int)sizeof(E), V = 4 * PER, U = 4;  // (from HBM: more on their way)
     const int tid = (int)threadIdx.x, vecs = ((uintptr_t)in & 15) == 0 ? nv / V : 0;
-    float most = -INFINITY, least = INFINITY;
-    const auto see = [&](float x) {
-        most = fmaxf(most, x);
-        least = fminf(least, x > -INFINITY ? x : INFINITY);
-    };
+    float most = -INFINITY;
 #pragma unroll 1
     for (int i = tid; i < vecs; i += U * kSampleThreads) {
         uint4 raw[U];
@@ -478,12 +566,12 @@ __device__ __noinline__ float2 ends_pass(const E* in, int nv) {
         for (int j = 0; j < U; ++j) {
             const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
-            for (int e = 0; e < V; ++e) see(value_in<E>(w[e / PER], e % PER));
+            for (int e = 0; e < V; ++e) most = fmaxf(most, value_in<E>(w[e / PER], e % PER));
         }
     }
 #pragma unroll 1
-    for (int i = vecs * V + tid; i < nv; i += kSampleThreads) see(to_f(in[i]));
-    return make_float2(most, least);
+    for (int i = vecs * V + tid; i < nv; i += kSampleThreads) most = fmaxf(most, to_f(in[i]));
+    return most;
 }
 
 // The nth token with key find.lo, or (crowd) the one drawn among all with it: a warp's in their order, then the warps', then the CTAs'.
@@ -539,7 +627,8 @@ __device__ __noinline__ void nth_token(const SampleArgs& a, int row, const E* in
 }
 
 // What the CTAs' histograms hold, to all of them.
-__device__ __noinline__ void collect(const Histogram& h, Groups& to, int C, int rank) {
+template <typename H>
+__device__ __noinline__ void collect(const H& h, Groups& to, int C, int rank) {
     Shared& s = shared();
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = (int)threadIdx.x;
@@ -557,7 +646,7 @@ __device__ __noinline__ void collect(const Histogram& h, Groups& to, int C, int 
     if (c < C && c != rank) {
         Groups* const there = cluster.map_shared_rank(&own, c);
         there->mass[g] = own.mass[g];
-        there->count[g] = own.count[g];
+        if (sizeof(H) == sizeof(Parts)) there->count[g] = own.count[g];
     }
     cluster.sync();
     if (tid < kGroups) {
@@ -571,6 +660,11 @@ __device__ __noinline__ void collect(const Histogram& h, Groups& to, int C, int 
     __syncthreads();
 }
 
+// No slice has more members than its sum has least weights of its (and half a unit each).
+__device__ __forceinline__ float most_members(u64 sum, int slice) {
+    return __fdividef((float)sum, fmaxf((float)shared().row.lift * exp2f(-(float)(slice + 1) / 64.f) * 0.97f - 1.f, 1e-9f));
+}
+
 // The slice of a histogram that holds the answer, and what to do with it. Every CTA works this out for itself, in its first warp.
 __device__ __noinline__ void look(bool first, bool sums, int C) {
     Shared& s = shared();
@@ -580,35 +674,36 @@ __device__ __noinline__ void look(bool first, bool sums, int C) {
     if (warp == 0) {
         if (s.fresh) {
             const u64 total = warp_sum(s.first_groups.mass[lane] + s.first_groups.mass[lane + 32]);
-            const uint32_t count = __reduce_add_sync(0xffffffffu, s.first_groups.count[lane] + s.first_groups.count[lane + 32]);
             if (lane == 0) {
-                u64 likely = 0;
-                for (int i = 0; sums && i < C; ++i) likely += s.likely[i];
-                f.total = total;
-                // (the first of the order is kept whatever min_p is)
-                f.likely = s.row.least ? max(likely, (u64)s.row.lift) : total;
                 f.goal = kTopK;
                 f.last = 0;
                 s.fresh = 0;
-                // (count: with those of the last slice that are never drawn)
-                if (k > 1 && (s.few || (uint32_t)k < count))
-                    f.limit = min((uint32_t)k, count);
-                else
-                    next_goal(total);
+                if (!sums) {
+                    // (total: of the tokens' number, with those of the last slice that are never drawn)
+                    f.limit = min((u64)k, total);
+                } else {
+                    u64 likely = 0;
+                    for (int i = 0; i < C; ++i) likely += s.likely[i];
+                    f.total = total;
+                    // (the first of the order is kept whatever min_p is)
+                    f.likely = s.row.least ? max(likely, (u64)s.row.lift) : total;
+                    if (f.k_slice < 0) next_goal(total);
+                }
             }
             __syncwarp();
         }
-        find(0, first ? s.first_groups : s.more_groups, first ? s.first : s.more, C, first ? 0 : f.mass_before, first ? 0 : f.count_before,
-             f.goal == kTopK, f.limit);
+        if (first)
+            find(0, C, f.limit, sums && f.goal == kTopK ? f.k_slice : -1);
+        else
+            find_part(C, f.mass_before, f.count_before, f.goal == kTopK, f.limit);
     }
     __syncthreads();
     const int goal = f.goal, b = s.at[0];
     const bool by_key = f.last < 0;
     const u64 front = s.at_mass[0], own = s.at_own[0];
-    const uint32_t before = s.at_count[0], members = s.at_members[0];
-    const bool both = first && !by_key && (goal == kTopP || (goal == kTopK && sums && b != kLast && !(s.p < 1.f)));
+    const bool both = first && sums && !by_key && (goal == kTopP || (goal == kTopK && !(s.p < 1.f)));
     // (the end of what is kept lies in slice b: and the slices that can hold the token)
-    if (both && warp < 2) find(1 + warp, s.first_groups, s.first, C, 0, 0, false, drawn(s.u, min(warp ? front + own : front + 1, f.likely)));
+    if (both && warp < 2) find(1 + warp, C, drawn(s.u, min(warp ? front + own : front + 1, f.likely)), -1);
     __syncthreads();
     if (threadIdx.x == 0) {
         if (both) {
@@ -620,49 +715,52 @@ __device__ __noinline__ void look(bool first, bool sums, int C) {
             f.goal = kBoth;
             f.mass_before = s.at_mass[1];
             f.more_before = front;
-            f.count_before = before;
-            // no slice has more members than its sum has least weights of its (and half a unit each)
-            const auto most = [&](u64 sum, int slice) { return __fdividef((float)sum, fmaxf((float)s.table[slice] * 0.97f - 1.f, 1e-9f)); };
+            f.count_before = f.k_before;
             const u64 middle = f.b1 < b ? s.at_mass[2] + s.at_own[2] - s.at_mass[1] : front - s.at_mass[1];
-            f.last = most(middle, min(f.b1, b)) + (k > 1 ? (float)members : most(own, b)) <= (float)kMembers;
+            f.last = most_members(middle, min(f.b1, b)) + (goal == kTopK ? (float)f.k_members : most_members(own, b)) <= (float)kMembers;
         } else {
-            uint32_t lo = 0, hi = 0;
+            uint32_t lo = 0, hi = 0, members = first ? goal == kTopK && sums ? f.k_members : ~0u : s.at_members[0];
             bool into = false;
             if (!first) {
                 hi = f.hi - ((uint32_t)b << f.shift);
                 const uint32_t span = (1u << f.shift) - 1;
                 lo = hi - f.lo > span ? hi - span : f.lo;
+                f.count_before = s.at_count[0];
                 into = true;
-            } else if (goal == kTopK && s.few && (b == kLast ? before : before + members) <= (uint32_t)kMembers) {
-                // the kept ones and no more than kMembers in all (those of the last slice have no weight)
-                f.goal = kPrefix;
-                f.limit = b == kLast ? min(f.limit, (u64)before) : f.limit;
-                f.op = kGather;
-                f.b0 = 0;
-                f.b1 = f.b2 = b == kLast ? b - 1 : b;
-                f.last = 1;
             } else if (!sums) {
-                f.op = kSums;
-            } else if (goal == kTopK && b == kLast) {
-                next_goal(f.total);
+                // front and own are numbers of tokens
+                if (s.few && (b == kLast ? front : front + own) <= (u64)kMembers) {
+                    // the kept ones and no more than kMembers in all (those of the last slice have no weight)
+                    f.goal = kPrefix;
+                    f.limit = b == kLast ? min(f.limit, front) : f.limit;
+                    f.op = kGather;
+                    f.b0 = 0;
+                    f.b1 = f.b2 = b == kLast ? b - 1 : b;
+                    f.last = 1;
+                } else {
+                    f.op = kSums;
+                    f.k_slice = b == kLast ? -1 : b;
+                    f.k_before = (uint32_t)front;
+                    f.k_members = (uint32_t)own;
+                }
             } else if (!by_key && (goal == kDraw || members <= (uint32_t)kMembers)) {
                 f.mass_before = front;
-                f.count_before = before;
+                f.count_before = f.k_before;
                 f.op = kGather;
                 f.b0 = f.b1 = f.b2 = b;
-                f.last = goal == kDraw && (float)own <= (float)kMembers * ((float)s.table[b] * 0.97f - 1.f);
+                f.last = goal == kDraw && most_members(own, b) <= (float)kMembers;
             } else {
                 lo = lowest_key(b);
                 hi = b ? lowest_key(b - 1) - 1 : key_of(s.row.m);
+                f.count_before = f.k_before;
                 into = true;
             }
             if (into) {
                 f.mass_before = front;
-                f.count_before = before;
                 f.lo = lo;
                 f.hi = hi;
                 f.last = 0;
-                if ((!first || k > 1) && members <= (uint32_t)kMembers) {
+                if (members <= (uint32_t)kMembers) {
                     f.op = kGatherKeys;
                 } else if (lo < hi) {
                     f.op = kDivide;
@@ -698,7 +796,7 @@ __device__ __noinline__ u64 reach(int lo, int hi, u64 before, uint32_t number, b
     int part = -1;  // of the set, first divided into kSampleThreads parts by its place among the slices
     const float begin = (float)lo - 0.5f, scale = (float)kSampleThreads / (float)(hi - lo + 1);
     const auto part_of = [&](float x) {
-        return (int)fminf(fmaxf((fmaf(x, -0.5f, r.half_m) * r.scale - begin) * scale, 0.f), (float)(kSampleThreads - 1));
+        return (int)fminf(fmaxf((r.place(x) - begin) * scale, 0.f), (float)(kSampleThreads - 1));
     };
     // f(index, key) for this thread's members of the set; returns the set's size
     const auto members = [&](auto f) {
@@ -768,7 +866,7 @@ __device__ __noinline__ u64 reach(int lo, int hi, u64 before, uint32_t number, b
         members([&](int i, uint32_t key) { note((int)((khi - key) >> shift), weight[i]); });
         group(s.more, s.more_groups);
         __syncthreads();
-        if (warp == 0) find(0, s.more_groups, s.more, 1, before, number, by_count, limit);
+        if (warp == 0) find_part(1, before, number, by_count, limit);
         __syncthreads();
         before = s.at_mass[0];
         number = s.at_count[0];
@@ -842,11 +940,10 @@ __device__ __noinline__ void settle(const SampleArgs& a, int row) {
     u64 likely = 0;
     {
         const Row r = s.row;
-        const bool table = s.table_made;
 #pragma unroll 1
         for (int i = tid; i < n; i += kSampleThreads) {
             const float x = value_of((uint32_t)(s.member[i] >> 32));
-            const u64 w = table ? r.weight(x, s.table) : Row::whole(exp_of(((double)x - (double)r.m) * r.per_t) * r.lift + kTwo52);
+            const u64 w = r.weight(x, s.table);
             s.weight[i] = w;
             if (w >= r.least) likely += w;
         }
@@ -978,6 +1075,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     Shared* const head = cluster.map_shared_rank(&s, 0);
     clear(s.first);
     clear(s.more);
+    const double lift = __longlong_as_double((long long)(1023 + a.bits) << 52);
+    if (tid < 16) s.table[tid] = exp2(-tid / 16.0) * lift;
     stream_turn();
     const float T0 = a.temperature ? a.temperature[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
     const int k = a.top_k ? a.top_k[row] : 0;
@@ -988,27 +1087,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         s.p = a.top_p ? a.top_p[row] : 1.f;
         s.u = a.u[row];
         s.min_p = min_p;
-        s.table_made = 0;
         s.fresh = 1;
-        s.row.per_t = 1.0 / (double)fmaxf(T0, 7.8886091e-31f);  // 2^-100: what follows stays within f32's range
+        s.row.per_t = 23.083120654223414 / (double)fmaxf(T0, 7.8886091e-31f);  // 2^-100: what follows stays within f32's range
+        s.find.k_slice = -1;
+        s.find.k_before = s.find.k_members = 0;
     }
-    // ---- the largest and the smallest
+    // ---- the largest
     {
-        float2 e = ends_pass<E>(in, nv);
+        float e = most_pass<E>(in, nv);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            e.x = fmaxf(e.x, __shfl_xor_sync(0xffffffffu, e.x, o));
-            e.y = fminf(e.y, __shfl_xor_sync(0xffffffffu, e.y, o));
-        }
+        for (int o = 1; o < 32; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, o));
         if (lane == 0) s.warp_ends[warp] = e;
         __syncthreads();
         if (warp == 0) {
             e = s.warp_ends[lane % kSampleWarps];
 #pragma unroll
-            for (int o = 1; o < kSampleWarps; o <<= 1) {
-                e.x = fmaxf(e.x, __shfl_xor_sync(0xffffffffu, e.x, o));
-                e.y = fminf(e.y, __shfl_xor_sync(0xffffffffu, e.y, o));
-            }
+            for (int o = 1; o < kSampleWarps; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, o));
             if (lane < C) cluster.map_shared_rank(&s, lane)->ends[rank] = e;
         }
         cluster.sync();
@@ -1016,12 +1110,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     int op;
     {
         Row r;
-        float least = INFINITY;
         r.m = -INFINITY;
-        for (int i = 0; i < C; ++i) {
-            r.m = fmaxf(r.m, s.ends[i].x);
-            least = fminf(least, s.ends[i].y);
-        }
+        for (int i = 0; i < C; ++i) r.m = fmaxf(r.m, s.ends[i]);
         if (r.m == -INFINITY) {
             if (rank == 0 && tid == 0) {
                 a.token[row] = -1;
@@ -1030,23 +1120,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             return;
         }
         // the first of the order; or, beside +infinity, only what is: tokens of equal weights
-        op = !(T0 > 0.f) || k == 1 ? kTies : r.m == INFINITY ? kCrowd : k > 1 && k <= kMembers ? kNumbers : kSums;
+        op = !(T0 > 0.f) || k == 1 ? kTies : r.m == INFINITY ? kCrowd : k > 1 && k < a.vocab ? kNumbers : kSums;
         if (tid == 0) {
-            const float T = fmaxf(T0, 7.8886091e-31f);
             r.half_m = 0.5f * r.m;
             r.per_t = s.row.per_t;
-            r.lift = __longlong_as_double((long long)(1023 + a.bits) << 52);
-            r.least = min_p > 0.f ? min_p <= 1.f ? (u64)ceil((double)min_p * r.lift) : ~0ull : 0;
-            // half of the range that the first histogram divides: all values, or those with a weight
-            const float range = fminf(fmaf(least, -0.5f, r.half_m), 18.f * T);
-            r.scale = range > 0.f ? fminf((float)(kLast - 1) / range, 1e35f) : 0.f;
-            // step / T rounded up to 13 bits, and the scale to match it (where T is without end there is neither)
-            const float per_t = (float)r.per_t, grid = r.scale > 0.f ? 2.f / r.scale * per_t : 0.f;
-            r.grid = grid > 1e-30f && grid < 1.f ? __uint_as_float((__float_as_uint(grid * 1.000001f) + 0x7FFu) & ~0x7FFu) : 0.f;
-            if (r.grid > 0.f) r.scale = 2.f * per_t / r.grid;
-            const float step = r.scale > 0.f ? 2.f / r.scale : 0.f;
-            r.floor = r.m - (float)(kBins + 1) * step;
-            if (!(r.scale > 0.f) || !(fabsf(r.m) < 1e30f) || !(r.floor > -1e30f) || r.bin(r.floor) != kLast) r.floor = -INFINITY;
+            r.lift = lift;
+            r.least = min_p > 0.f ? min_p <= 1.f ? (u64)ceil((double)min_p * lift) : ~0ull : 0;
+            r.scale = (float)(8.0 * r.per_t);  // (64 slices to 16 sixteenths, for halves)
+            const float step = 0.25f / (float)r.per_t;
+            // (m a few million slices from 0 at most: sums and differences of slices' ends are off by a small part of one)
+            const bool near = fabsf(r.m) < 4194304.f * step && step < 1e24f;
+            r.step = near ? step : INFINITY;
+            r.floor = near ? r.m - (float)kLast * step : -INFINITY;
             s.row = r;
             s.find.lo = key_of(r.m);
             s.find.nth = 1;
@@ -1109,24 +1194,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         } else if (op == kNumbers) {
             numbers_pass<E>(in, nv);
         } else if (op == kSums) {
-            if (k > 1 && k <= kMembers) {
+            if (k > 1 && k < a.vocab) {
                 // (the numbers there are first: read by all, then cleared)
                 cluster.sync();
                 clear(s.first);
+                if (tid == 0) s.fresh = 1;
+                __syncthreads();
             }
-            if (tid < kBins / 32 + 32) {
-                const int i = tid < kBins / 32 ? 32 * tid : tid - kBins / 32;
-                const double e = exp_of(-i * (double)s.row.grid);
-                if (tid < kBins / 32)
-                    s.coarse[tid] = e * s.row.lift;
-                else
-                    s.fine[tid - kBins / 32] = e;
-            }
-            __syncthreads();
-            for (int i = tid; i < kBins; i += kSampleThreads) s.table[i] = i == kLast ? 0.0 : s.coarse[i / 32] * s.fine[i % 32];
-            if (tid == 0) s.table_made = s.fresh = 1;
-            __syncthreads();
-            if (k > 1 || s.row.least || s.row.floor == -INFINITY) {
+            if (s.row.least || s.row.floor == -INFINITY) {
                 const u64 likely = warp_sum(sums_pass<E, true>(in, nv));
                 if (lane == 0) s.warp_mass[warp] = likely;
                 __syncthreads();
