@@ -1010,6 +1010,7 @@ int aero_cuda_pages_select(void* cache, int layer, const void* q, int64_t q_toke
         a.first = first;
         a.recent = recent;
         a.width = n_blocks;
+        a.vec = aero::vec16(q, q_token, q_head);
         a.out = blocks;
         return g.ok(aero::launch_select(a, g.d.dtype == AERO_CUDA_TYPE_BF16, g.n_sm, g.stream), "select");
     });

@@ -101,6 +101,7 @@ struct SelectArgs {
     const int32_t* seqs;
     const int32_t* q_start;
     int layer, T, n, H, first, recent, width;
+    int vec;       // q's rows may be read 16 bytes at a time
     int32_t* out;  // (T, HK, width)
 };
 

@@ -6,9 +6,12 @@
 // Choice. score(b) = max over the kv head's query heads g of sum_d max(q_gd lo_bd, q_gd hi_bd): no key
 // between the bounds has a larger product with any of these heads' queries. As one product with
 // depth 2 D: max(q lo, q hi) = q+ hi + q- lo, where q+ and q- are q's positive and negative parts (the
-// bounds are finite, so the part that is zero adds nothing). A wrong order of two scores is a wrong
-// block, so they are summed in 64 bits (the products of 16-bit values are exact): m8n8k4 products, 8
-// query heads by 8 blocks.
+// bounds are finite, so the part that is zero adds nothing). A wrong order of two scores is a wrong block, so what is
+// chosen has to follow from sums in 64 bits; those cost 64 products a cycle and SM at best (m8n8k4 products: 48
+// sequences of up to 512 blocks, 32 query heads, 16 us of scores). So every score is computed first in f32 (m16n8k16
+// products, the operands as they are), off by at most e = 2^-14 max_g sum_d |q_gd| max |bounds|: 32 sums of 17 terms, each
+// off by at most 2^-19 of their terms' sum. Only the blocks whose score lies within 2 e of where the least chosen one can
+// be are computed again in 64 bits, a handful; where they are many (blocks alike) all are.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -190,9 +193,28 @@ __device__ __forceinline__ u64 key_of(double score) {
 }
 
 template <int D, int NT>
-constexpr int query_bytes() {  // of the query heads' fragments
+constexpr int query_bytes() {  // of the query heads' fragments in 64 bits
     return NT * 8 * 2 * D * 8;
 }
+
+constexpr int kNear = 64;  // blocks of a CTA whose scores are computed again
+
+// Keys of scores in f32.
+__device__ __forceinline__ uint32_t key32_of(float score) {
+    const uint32_t b = __float_as_uint(score + 0.f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float score32_of(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7FFFFFFFu : ~key); }
+constexpr uint32_t kAlways32 = ~0u;
+
+// What a CTA of the cluster tells the others.
+struct Told {
+    uint32_t lo, hi;    // keys
+    float most;         // the largest bound
+    int chosen, sure, near;
+    u64 near_key[kNear];
+    int near_block[kNear];
+};
 
 // NT: tiles of 8 query heads.
 template <int D, bool BF16, int NT>
@@ -203,8 +225,11 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
     double* qf = reinterpret_cast<double*>(smem);                                          // [NT][2][KS][8][32]
     uint32_t* hist = reinterpret_cast<uint32_t*>(smem + query_bytes<D, NT>());             // [2][kBins]
     u64* keys = reinterpret_cast<u64*>(smem + query_bytes<D, NT>() + 2 * kBins * 4);
-    __shared__ u64 least[kSelWarps], most[kSelWarps], range[2];
+    __shared__ u64 least[kSelWarps], most64[kSelWarps], range[2];
     __shared__ uint32_t sums[kSelWarps], found[3], mine[1];
+    __shared__ float sizes[NT * 8], bounds_of[kSelWarps];
+    __shared__ Told told[kSelCluster];
+    __shared__ int near;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -217,20 +242,299 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
     if (tid == 0 && (seq < 0 || seq >= a.c.n_seq)) pages_flag(a.c, AERO_CUDA_PAGES_BAD_SEQ);
     const int W = a.width, nb = n > 0 ? (n + P - 1) >> a.c.page_shift : 0;
     int32_t* list = a.out + (int64_t)pair * W;
-    // the blocks that are chosen always: [0, f1) and [r0, nb)
-    const int f1 = min(a.first, nb), r0 = max(nb - a.recent, f1);
-    int need = W - (f1 + nb - r0);
+    // the blocks that are chosen always: [0, f1) and [r0_, nb)
+    const int f1 = min(a.first, nb), r0_ = max(nb - a.recent, f1);
+    int need = W - (f1 + nb - r0_);
     if (nb <= W || need <= 0) {
         // all of them, or no others
         for (int i = rank * kSelThreads + tid; i < W; i += C * kSelThreads)
-            list[i] = nb <= W ? (i < nb ? i : -1) : i < f1 ? i : r0 + i - f1;
+            list[i] = nb <= W ? (i < nb ? i : -1) : i < f1 ? i : r0_ + i - f1;
         return;
     }
     const int per = ((nb + C - 1) / C + 15) & ~15;
     const int b0 = min(nb, rank * per), b1 = min(nb, b0 + per);
+    const uint16_t* const q = static_cast<const uint16_t*>(a.q) + (int64_t)t * a.q_token + (int64_t)(h * G) * a.q_head;
+    const uint16_t* const bounds = a.c.bounds + (int64_t)h * 2 * D;
+    const auto page_of = [&](int b) { return b < b1 ? a.c.table[(int64_t)seq * a.c.max_pages + b] : -1; };
+    const auto row_of = [&](int page) { return bounds + ((int64_t)a.layer * a.c.n_page + page) * HK * 2 * D; };
+    // an entry's place among the CTA's, and all of them, of 256 small numbers a thread each
+    const auto scan = [&](uint32_t v, uint32_t& all) {
+        uint32_t incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        __syncthreads();
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        uint32_t before = 0;
+        all = 0;
+#pragma unroll
+        for (int i = 0; i < kSelWarps; ++i) {
+            before += i < warp ? sums[i] : 0;
+            all += sums[i];
+        }
+        return before + incl - v;
+    };
+    if (a.vec) {
+        // ---- scores in f32. The query heads' parts as the products' columns: a warp a head
+        uint2* const frag = reinterpret_cast<uint2*>(smem);  // [NT][2][KS][2][32]
+        uint32_t* const keys32 = reinterpret_cast<uint32_t*>(keys);
+        for (int i = tid; i < 2 * kBins; i += kSelThreads) hist[i] = 0;
+        for (int head = warp; head < NT * 8; head += kSelWarps) {
+            float size = 0.f;
+            if (lane < D / 8) {
+                const uint4 x = *reinterpret_cast<const uint4*>(q + (int64_t)(head % G) * a.q_head + lane * 8);  // (heads past G: the first ones again)
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                uint32_t neg[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    neg[j] = w[j] & ((w[j] >> 15 & 0x10001u) * 0xFFFFu);
+                    size += fabsf(low16<BF16>(w[j])) + fabsf(low16<BF16>(w[j] >> 16));
+                }
+                uint2* to = frag + ((head / 8 * 2) * KS + lane / 4) * 64 + (head % 8) * 4 + lane % 4;
+                to[0] = make_uint2(neg[0], neg[1]);  // with the lower bounds
+                to[32] = make_uint2(neg[2], neg[3]);
+                to[KS * 64] = make_uint2(w[0] ^ neg[0], w[1] ^ neg[1]);  // with the upper ones
+                to[KS * 64 + 32] = make_uint2(w[2] ^ neg[2], w[3] ^ neg[3]);
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) size += __shfl_xor_sync(0xffffffffu, size, o);
+            if (lane == 0) sizes[head] = size;
+        }
+        __syncthreads();
+        uint32_t lo = ~0u, hi = 0, most = 0;
+        for (int base = b0 + warp * 16; base < b1; base += kSelWarps * 16) {
+            const int p0 = page_of(base + lane / 4), p1 = page_of(base + 8 + lane / 4);
+            const bool g0 = (uint32_t)p0 < (uint32_t)a.c.n_page, g1 = (uint32_t)p1 < (uint32_t)a.c.n_page;
+            if ((!g0 && base + lane / 4 < b1) || (!g1 && base + 8 + lane / 4 < b1)) pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
+            const uint4 *r0 = reinterpret_cast<const uint4*>(row_of(p0)) + lane % 4, *r1 = reinterpret_cast<const uint4*>(row_of(p1)) + lane % 4;
+            float acc[NT][4];
+#pragma unroll
+            for (int m = 0; m < NT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+            constexpr int PH = D <= 128 ? 1 : 2;  // wide heads: the lower bounds first, then the upper ones
+#pragma unroll
+            for (int half = 0; half < PH; ++half) {
+                constexpr int N = 2 * KS / PH;
+                uint4 x[N], y[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    x[i] = g0 ? __ldcg(r0 + 4 * (half * N + i)) : make_uint4(0u, 0u, 0u, 0u);
+                    y[i] = g1 ? __ldcg(r1 + 4 * (half * N + i)) : make_uint4(0u, 0u, 0u, 0u);
+                }
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    constexpr uint32_t kSize = 0x7FFF7FFFu;
+                    most = max2<BF16>(most, max2<BF16>(max2<BF16>(x[i].x & kSize, x[i].y & kSize), max2<BF16>(x[i].z & kSize, x[i].w & kSize)));
+                    most = max2<BF16>(most, max2<BF16>(max2<BF16>(y[i].x & kSize, y[i].y & kSize), max2<BF16>(y[i].z & kSize, y[i].w & kSize)));
+#pragma unroll
+                    for (int m = 0; m < NT; ++m) {
+                        const uint2* f = frag + ((m * 2) * KS + half * N + i) * 64 + lane;
+                        const uint2 f0 = f[0], f1 = f[32];
+                        const uint32_t a0[4] = {x[i].x, y[i].x, x[i].y, y[i].y}, a1[4] = {x[i].z, y[i].z, x[i].w, y[i].w};
+                        mma16<BF16>(acc[m], a0, f0.x, f0.y);
+                        mma16<BF16>(acc[m], a1, f1.x, f1.y);
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float v = fmaxf(acc[0][2 * e], acc[0][2 * e + 1]);
+#pragma unroll
+                for (int m = 1; m < NT; ++m) v = fmaxf(v, fmaxf(acc[m][2 * e], acc[m][2 * e + 1]));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+                const int b = base + 8 * e + lane / 4;
+                if (lane % 4 == 0 && b < b1) {
+                    const bool always = b < f1 || b >= r0_;
+                    const uint32_t k = key32_of(v);
+                    keys32[b - b0] = always ? kAlways32 : k;
+                    if (!always) {
+                        lo = min(lo, k);
+                        hi = max(hi, k);
+                    }
+                }
+            }
+        }
+        // ---- all CTAs' ends, and how far the scores may be off
+        float bound = fmaxf(low16<BF16>(most), low16<BF16>(most >> 16));
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+        if (lane == 0) least[warp] = lo, most64[warp] = hi, bounds_of[warp] = bound;
+        __syncthreads();
+        if (tid < C) {
+            for (int i = 0; i < kSelWarps; ++i) {
+                lo = min(lo, (uint32_t)least[i]);
+                hi = max(hi, (uint32_t)most64[i]);
+                bound = fmaxf(bound, bounds_of[i]);
+            }
+            Told& to = cluster.map_shared_rank(told, tid)[rank];
+            to.lo = lo;
+            to.hi = hi;
+            to.most = bound;
+        }
+        cluster.sync();
+        lo = ~0u, hi = 0, bound = 0.f;
+        for (int i = 0; i < C; ++i) {
+            lo = min(lo, told[i].lo);
+            hi = max(hi, told[i].hi);
+            bound = fmaxf(bound, told[i].most);
+        }
+        float size = 0.f;
+        bool number = true;
+        for (int i = 0; i < NT * 8; ++i) {
+            number &= sizes[i] < INFINITY;
+            size = fmaxf(size, sizes[i]);
+        }
+        const float off = size * bound * 1.25e-4f;  // 2 e, rounded up
+        if (number && off < 1e30f) {
+            // ---- an interval that holds the least chosen score: a few blocks' or narrower than what they may be off
+            int left = need;
+            for (int level = 0; lo != hi; ++level) {
+                const int shift = max(0, 22 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins = 2^10
+                uint32_t* own = hist + (level & 1) * kBins;
+                for (int i = tid; i < b1 - b0; i += kSelThreads) {
+                    const uint32_t k = keys32[i];
+                    if (k >= lo && k <= hi && k != kAlways32) atomicAdd(own + ((hi - k) >> shift), 1u);
+                }
+                cluster.sync();
+                // the other histogram, read by all before this barrier, is the next one's
+                reinterpret_cast<uint4*>(hist + (~level & 1) * kBins)[tid] = make_uint4(0u, 0u, 0u, 0u);
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 4
+                for (int i = 0; i < C; ++i) {
+                    const uint4 x = reinterpret_cast<const uint4*>(C > 1 ? cluster.map_shared_rank(own, i) : own)[tid];
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                }
+                uint32_t all;
+                uint32_t before = scan(v.x + v.y + v.z + v.w, all);
+                if (before < (uint32_t)left && (uint32_t)left <= before + v.x + v.y + v.z + v.w) {
+                    const uint32_t c4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (before < (uint32_t)left && (uint32_t)left <= before + c4[e]) {
+                            found[0] = (uint32_t)(4 * tid + e);
+                            found[1] = before;
+                            found[2] = c4[e];
+                        }
+                        before += c4[e];
+                    }
+                }
+                __syncthreads();
+                const uint32_t top = hi - (found[0] << shift), span = (1u << shift) - 1;
+                left -= (int)found[1];
+                hi = top;
+                lo = top - lo > span ? top - span : lo;
+                if (found[2] <= 8 || score32_of(hi) - score32_of(lo) <= off) break;
+            }
+            // ---- blocks above what that leaves open are chosen, those within it computed again
+            const uint32_t open_lo = key32_of(score32_of(lo) - off * 1.001f), open_hi = min(key32_of(score32_of(hi) + off * 1.001f), kAlways32 - 1);
+            Told& mine = told[rank];
+            if (tid == 0) near = 0;
+            __syncthreads();
+            uint32_t chosen = 0, sure = 0;
+            for (int i = tid; i < b1 - b0; i += kSelThreads) {
+                const uint32_t k = keys32[i];
+                chosen += k > open_hi;
+                sure += k > open_hi && k != kAlways32;
+                if (k >= open_lo && k <= open_hi) {
+                    const int at = atomicAdd(&near, 1);
+                    if (at < kNear) mine.near_block[at] = b0 + i;
+                }
+            }
+            uint32_t both;
+            scan(chosen | sure << 16, both);
+            const int n = near;
+            for (int i = warp; i < min(n, kNear); i += kSelWarps) {
+                // a warp a block: its columns over the lanes, head by head
+                const int page = page_of(mine.near_block[i]);
+                const bool good = (uint32_t)page < (uint32_t)a.c.n_page;
+                const uint16_t* row = row_of(page);
+                u64 k = 0;
+                for (int g = 0; g < G; ++g) {
+                    double sum = 0.0;
+#pragma unroll
+                    for (int d = 0; d < D / 64; ++d) {
+                        const int at = 64 * d + 2 * lane;
+                        const uint32_t x = *reinterpret_cast<const uint32_t*>(q + (int64_t)g * a.q_head + at);
+                        const uint32_t l = good ? __ldcg(reinterpret_cast<const uint32_t*>(row + at)) : 0u, u = good ? __ldcg(reinterpret_cast<const uint32_t*>(row + D + at)) : 0u;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 16) {
+                            const float y = low16<BF16>(x >> e);
+                            sum = fma((double)y, (double)low16<BF16>((y < 0.f ? l : u) >> e), sum);
+                        }
+                    }
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    k = max(k, key_of(sum));
+                }
+                if (lane == 0) mine.near_key[i] = k;
+            }
+            __syncthreads();
+            for (int i = tid; i < C * kNear; i += kSelThreads) {
+                const int c = i / kNear, e = i % kNear;
+                Told& to = C > 1 ? cluster.map_shared_rank(told, c)[rank] : mine;
+                if (c != rank && e < min(n, kNear)) {
+                    to.near_key[e] = mine.near_key[e];
+                    to.near_block[e] = mine.near_block[e];
+                }
+                if (e == 0) {
+                    to.chosen = (int)(both & 0xFFFFu);
+                    to.sure = (int)(both >> 16);
+                    to.near = n;
+                }
+            }
+            cluster.sync();
+            bool few = true;
+            int open = need, base = 0;
+            for (int i = 0; i < C; ++i) {
+                few &= told[i].near <= kNear;
+                open -= told[i].sure;
+                base += i < rank ? told[i].chosen : 0;
+            }
+            if (few) {
+                // of all CTAs' the `open` highest, equal ones by their number
+                if (tid < 2) found[tid] = 0;  // this CTA's, and those before it
+                __syncthreads();
+                for (int i = tid; i < C * kNear; i += kSelThreads) {
+                    const int c = i / kNear, e = i % kNear;
+                    if (c > rank || e >= told[c].near) continue;
+                    const u64 k = told[c].near_key[e];
+                    const int b = told[c].near_block[e];
+                    int before = 0;
+                    for (int j = 0; j < C; ++j)
+                        for (int o = 0; o < told[j].near; ++o) {
+                            const u64 other = told[j].near_key[o];
+                            before += other > k || (other == k && told[j].near_block[o] < b);
+                        }
+                    if (before < open) {
+                        if (c == rank)
+                            keys32[b - b0] = kAlways32;
+                        else
+                            atomicAdd(found + 1, 1u);
+                    }
+                }
+                __syncthreads();
+                base += (int)found[1];
+                // ---- the chosen ones, in order: each thread a run of blocks
+                const int run = (per + kSelThreads - 1) / kSelThreads;
+                const int i0 = min(b1 - b0, tid * run), i1 = min(b1 - b0, i0 + run);
+                uint32_t count = 0, all;
+                for (int i = i0; i < i1; ++i) count += keys32[i] > open_hi;
+                int at = base + (int)scan(count, all);
+                for (int i = i0; i < i1; ++i)
+                    if (keys32[i] > open_hi) list[at++] = b0 + i;
+                return;
+            }
+        }
+    }
+    // ---- scores in 64 bits, all of them
+    cluster.sync();  // (the memory that others may be reading is written again)
     // ---- the query heads' positive and negative parts, as the products' fragments; heads past G are the first ones again
     {
-        const uint16_t* q = static_cast<const uint16_t*>(a.q) + (int64_t)t * a.q_token + (int64_t)(h * G) * a.q_head;
         for (int i = tid; i < NT * 8 * D; i += kSelThreads) {
             const int head = i / D, d = i % D, c16 = d / 8;
             const float x = to_f32<BF16>(q[(int64_t)(head % G) * a.q_head + d]);
@@ -243,16 +547,15 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
     __syncthreads();
     // ---- scores
     u64 lo = kAlways, hi = 0;
-    const uint16_t* bounds = a.c.bounds + (int64_t)h * 2 * D;
     for (int base = b0 + warp * 8 * NU; base < b1; base += kSelWarps * 8 * NU) {
         uint4 x[NU][2][KS];
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int b = base + u * 8 + lane / 4;
-            const int page = b < b1 ? a.c.table[(int64_t)seq * a.c.max_pages + b] : -1;
+            const int page = page_of(b);
             const bool good = (uint32_t)page < (uint32_t)a.c.n_page;
             if (b < b1 && !good) pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
-            const uint16_t* row = bounds + ((int64_t)a.layer * a.c.n_page + page) * HK * 2 * D;
+            const uint16_t* row = row_of(page);
 #pragma unroll
             for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -294,7 +597,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
                 for (int o = 4; o < 32; o <<= 1) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
                 const int b = base + u * 8 + 2 * (lane & 3) + e;
                 if (lane < 4 && b < b1) {
-                    const bool always = b < f1 || b >= r0;
+                    const bool always = b < f1 || b >= r0_;
                     keys[b - b0] = always ? kAlways : k;
                     if (!always) {
                         lo = min(lo, k);
@@ -309,12 +612,12 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
         lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    if (lane == 0) least[warp] = lo, most[warp] = hi;
+    if (lane == 0) least[warp] = lo, most64[warp] = hi;
     __syncthreads();
     if (tid == 0) {
         for (int i = 1; i < kSelWarps; ++i) {
             lo = min(lo, least[i]);
-            hi = max(hi, most[i]);
+            hi = max(hi, most64[i]);
         }
         range[0] = lo;
         range[1] = hi;
@@ -416,7 +719,7 @@ template <int D, bool BF16, int NT>
 cudaError_t launch(const SelectArgs& a, int n_sm, cudaStream_t s) {
     static thread_local int prepared = -1;  // the device whose attribute this thread has set
     constexpr int kFixed = query_bytes<D, NT>() + 2 * kBins * 4;
-    static_assert(kFixed + kMostKeys * 8 <= 226 * 1024, "shared memory of a CTA");
+    static_assert(kFixed + kMostKeys * 8 + kSelCluster * sizeof(Told) + 512 <= 226 * 1024, "shared memory of a CTA");
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;

@@ -482,3 +482,36 @@ def test_refusals():
     assert c.attend_blocks(0, q[:0], one[:0], lists[:0]).shape == (0, 4, 64)
     c.set_bounds(0, one[:0])
     c.check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("alike", [5, 40, 400])
+def test_select_scores_next_to_one_another(dtype, alike):
+    """Blocks whose scores differ by less than sums in f32 resolve, a few of them, more than a CTA's list, all."""
+    P, HK, D, blocks = 8, 1, 256, 600
+    values = few_bits((blocks, 1, D), 11) * 4
+    values[100:100 + alike] = values[100].abs() + 20  # alike, and high
+    step = {F16: 2.0**-10, BF16: 2.0**-7}[dtype]
+    which = torch.randperm(alike, generator=torch.Generator().manual_seed(1))
+    for i in range(alike):  # then each a few of the last bits of its columns more, in no order
+        values[100 + i, 0, :min(D, int(which[i]) % 200)] *= 1 + step
+    keys = values.repeat_interleave(P, 0).to(dtype)
+    c, K, _ = open_cache([P * blocks], P, HK, D, dtype, values=keys)
+    q = torch.rand((1, 8, D), device="cuda", generator=gen(12)).mul_(0.001).add_(1).to(dtype)
+    for W in (3, 4, 30, 300):
+        got = c.select(0, q, i32([0]), n_blocks=W).cpu().numpy()
+        c.check()
+        assert (got[0] == plain_select(q[0], plain_bounds(K[0], P), P * blocks, P, W, 1, 1)).all()
+
+
+def test_select_of_wide_rows_of_queries():
+    """A batch with rows of zeros and of infinities beside ordinary ones, long and short sequences, over 16 query heads."""
+    lens, P, HK, G, D = [3000, 5, 1111, 2048, 3000], 8, 2, 16, 192
+    c, K, _ = open_cache(lens, P, HK, D, F16)
+    q = torch.randn((5, HK * G, D), device="cuda", generator=gen(13)).half()
+    q[0] = 0
+    q[3, 5] = math.inf
+    q[4] *= 1e-4
+    got = c.select(0, q, i32([0, 1, 2, 3, 4]), n_blocks=20, first=2, recent=3).cpu().numpy()
+    for s, n in enumerate(lens):
+        assert (got[s] == plain_select(q[s], plain_bounds(K[s], P), n, P, 20, 2, 3)).all()
