@@ -169,11 +169,11 @@ __global__ void __launch_bounds__(kBoundThreads, 4) append_bounds_kernel(PageVie
 // ------------------------------------------------------------------ the choice of blocks
 // A cluster of CTAs per (token, kv head), each with an even share of its blocks in their order. Scores become
 // 64-bit keys that order as they do and stay in shared memory; the least chosen key is found by histograms over
-// the interval that holds it, narrowed by a factor of kBins each time (a cluster barrier each, two
-// or three times for scores of a few thousand blocks); then each CTA writes its chosen blocks in order behind
+// the interval that holds it, narrowed by a factor of kBins each time (a cluster barrier each, once
+// or twice for scores of a few thousand blocks); then each CTA writes its chosen blocks in order behind
 // those of the CTAs before it. Counts are integers and ties go to the lowest block, so timing changes nothing.
-constexpr int kSelThreads = 256, kSelWarps = kSelThreads / 32;
-constexpr int kBins = 4 * kSelThreads;
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
+constexpr int kBins = kSelThreads;  // (reads of peers' memory are slow: two or three levels of 512 rather than of 2048)
 constexpr int kSelCluster = 8;
 constexpr int kMostKeys = kSelectPages / kSelCluster;
 constexpr unsigned long long kAlways = ~0ull;  // the key of a block that is chosen whatever its score (no score has it)
@@ -218,7 +218,7 @@ struct Told {
 
 // NT: tiles of 8 query heads.
 template <int D, bool BF16, int NT>
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs a) {
     constexpr int KS = D / 32;             // 16-byte pieces of a bound's row a lane takes
     constexpr int NU = D <= 128 ? 2 : 1;   // tiles of 8 blocks a warp has in hand
     extern __shared__ __align__(16) uint8_t smem[];
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
             float acc[NT][4];
 #pragma unroll
             for (int m = 0; m < NT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-            constexpr int PH = D <= 128 ? 1 : 2;  // wide heads: the lower bounds first, then the upper ones
+            constexpr int PH = D / 64;  // (four pieces of each row at a time, so that two CTAs fit an SM)
 #pragma unroll
             for (int half = 0; half < PH; ++half) {
                 constexpr int N = 2 * KS / PH;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
             // ---- an interval that holds the least chosen score: a few blocks' or narrower than what they may be off
             int left = need;
             for (int level = 0; lo != hi; ++level) {
-                const int shift = max(0, 22 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins = 2^10
+                const int shift = max(0, 23 - __clz((int)(hi - lo)));  // (hi - lo) >> shift < kBins = 2^9
                 uint32_t* own = hist + (level & 1) * kBins;
                 for (int i = tid; i < b1 - b0; i += kSelThreads) {
                     const uint32_t k = keys32[i];
@@ -402,38 +402,28 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
                 }
                 cluster.sync();
                 // the other histogram, read by all before this barrier, is the next one's
-                reinterpret_cast<uint4*>(hist + (~level & 1) * kBins)[tid] = make_uint4(0u, 0u, 0u, 0u);
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 4
-                for (int i = 0; i < C; ++i) {
-                    const uint4 x = reinterpret_cast<const uint4*>(C > 1 ? cluster.map_shared_rank(own, i) : own)[tid];
-                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-                }
-                uint32_t all;
-                uint32_t before = scan(v.x + v.y + v.z + v.w, all);
-                if (before < (uint32_t)left && (uint32_t)left <= before + v.x + v.y + v.z + v.w) {
-                    const uint32_t c4[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (before < (uint32_t)left && (uint32_t)left <= before + c4[e]) {
-                            found[0] = (uint32_t)(4 * tid + e);
-                            found[1] = before;
-                            found[2] = c4[e];
-                        }
-                        before += c4[e];
-                    }
+                hist[(~level & 1) * kBins + tid] = 0;
+                uint32_t v = 0, all;
+#pragma unroll 8
+                for (int i = 0; i < C; ++i) v += (C > 1 ? cluster.map_shared_rank(own, i) : own)[tid];
+                const uint32_t before = scan(v, all);
+                if (before < (uint32_t)left && (uint32_t)left <= before + v) {
+                    found[0] = (uint32_t)tid;
+                    found[1] = before;
+                    found[2] = v;
                 }
                 __syncthreads();
                 const uint32_t top = hi - (found[0] << shift), span = (1u << shift) - 1;
                 left -= (int)found[1];
                 hi = top;
                 lo = top - lo > span ? top - span : lo;
-                if (found[2] <= 8 || score32_of(hi) - score32_of(lo) <= off) break;
+                if (found[2] <= 8u * (uint32_t)C || score32_of(hi) - score32_of(lo) <= off) break;
             }
             // ---- blocks above what that leaves open are chosen, those within it computed again
             const uint32_t open_lo = key32_of(score32_of(lo) - off * 1.001f), open_hi = min(key32_of(score32_of(hi) + off * 1.001f), kAlways32 - 1);
             Told& mine = told[rank];
             if (tid == 0) near = 0;
+            if (tid < kNear) mine.near_key[tid] = 0;
             __syncthreads();
             uint32_t chosen = 0, sure = 0;
             for (int i = tid; i < b1 - b0; i += kSelThreads) {
@@ -448,30 +438,27 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
             uint32_t both;
             scan(chosen | sure << 16, both);
             const int n = near;
-            for (int i = warp; i < min(n, kNear); i += kSelWarps) {
-                // a warp a block: its columns over the lanes, head by head
+            for (int item = warp; item < min(n, kNear) * G; item += kSelWarps) {
+                // a warp a block and query head, columns over the lanes
+                const int i = item / G, g = item % G;
                 const int page = page_of(mine.near_block[i]);
                 const bool good = (uint32_t)page < (uint32_t)a.c.n_page;
                 const uint16_t* row = row_of(page);
-                u64 k = 0;
-                for (int g = 0; g < G; ++g) {
-                    double sum = 0.0;
+                double sum = 0.0;
 #pragma unroll
-                    for (int d = 0; d < D / 64; ++d) {
-                        const int at = 64 * d + 2 * lane;
-                        const uint32_t x = *reinterpret_cast<const uint32_t*>(q + (int64_t)g * a.q_head + at);
-                        const uint32_t l = good ? __ldcg(reinterpret_cast<const uint32_t*>(row + at)) : 0u, u = good ? __ldcg(reinterpret_cast<const uint32_t*>(row + D + at)) : 0u;
+                for (int d = 0; d < D / 64; ++d) {
+                    const int at = 64 * d + 2 * lane;
+                    const uint32_t x = *reinterpret_cast<const uint32_t*>(q + (int64_t)g * a.q_head + at);
+                    const uint32_t l = good ? __ldcg(reinterpret_cast<const uint32_t*>(row + at)) : 0u, u = good ? __ldcg(reinterpret_cast<const uint32_t*>(row + D + at)) : 0u;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 16) {
-                            const float y = low16<BF16>(x >> e);
-                            sum = fma((double)y, (double)low16<BF16>((y < 0.f ? l : u) >> e), sum);
-                        }
+                    for (int e = 0; e < 32; e += 16) {
+                        const float y = low16<BF16>(x >> e);
+                        sum = fma((double)y, (double)low16<BF16>((y < 0.f ? l : u) >> e), sum);
                     }
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    k = max(k, key_of(sum));
                 }
-                if (lane == 0) mine.near_key[i] = k;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == 0) atomicMax(&mine.near_key[i], key_of(sum));
             }
             __syncthreads();
             for (int i = tid; i < C * kNear; i += kSelThreads) {
@@ -633,7 +620,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
     u64 edge = lo;
     int ties = need;
     for (int level = 0; lo != hi; ++level) {
-        const int shift = max(0, 54 - __clzll((long long)(hi - lo)));  // (hi - lo) >> shift < kBins = 2^10
+        const int shift = max(0, 55 - __clzll((long long)(hi - lo)));  // (hi - lo) >> shift < kBins = 2^9
         uint32_t* own = hist + (level & 1) * kBins;
         for (int i = tid; i < b1 - b0; i += kSelThreads) {
             const u64 k = keys[i];
@@ -641,30 +628,14 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
         }
         cluster.sync();
         // the other histogram, read by all before this barrier, is the next one's
-        reinterpret_cast<uint4*>(hist + (~level & 1) * kBins)[tid] = make_uint4(0u, 0u, 0u, 0u);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        for (int i = 0; i < C; ++i) {
-            const uint4 x = reinterpret_cast<const uint4*>(cluster.map_shared_rank(own, i))[tid];
-            v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
-        }
-        const uint32_t four = v.x + v.y + v.z + v.w;
-        uint32_t incl = four;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
-        }
-        if (lane == 31) sums[warp] = incl;
-        __syncthreads();
-        for (int i = 0; i < warp; ++i) incl += sums[i];
-        uint32_t before = incl - four;
-        if (before < (uint32_t)need && (uint32_t)need <= incl) {
-            const uint32_t c4[4] = {v.x, v.y, v.z, v.w};
-            int e = 0;
-            while (before + c4[e] < (uint32_t)need) before += c4[e++];
-            found[0] = (uint32_t)(4 * tid + e);
+        hist[(~level & 1) * kBins + tid] = 0;
+        uint32_t v = 0, all;
+        for (int i = 0; i < C; ++i) v += cluster.map_shared_rank(own, i)[tid];
+        const uint32_t before = scan(v, all);
+        if (before < (uint32_t)need && (uint32_t)need <= before + v) {
+            found[0] = (uint32_t)tid;
             found[1] = before;
-            found[2] = c4[e];
+            found[2] = v;
         }
         __syncthreads();
         const u64 top = hi - ((u64)found[0] << shift), span = (1ull << shift) - 1;
@@ -684,19 +655,11 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectArgs a)
     const int i0 = min(b1 - b0, tid * run), i1 = min(b1 - b0, i0 + run);
     uint32_t count = 0;  // above the edge; in the high half, on it
     for (int i = i0; i < i1; ++i) count += (keys[i] > edge) + ((uint32_t)(keys[i] == edge) << 16);
-    uint32_t incl = count;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = incl;
-    __syncthreads();
-    for (int i = 0; i < warp; ++i) incl += sums[i];
-    if (tid == kSelThreads - 1) mine[0] = incl;
+    uint32_t all;
+    const uint32_t before = scan(count, all);
+    if (tid == 0) mine[0] = all;
     cluster.sync();
-    int above = (int)((incl - count) & 0xFFFFu), on = (int)((incl - count) >> 16);
+    int above = (int)(before & 0xFFFFu), on = (int)(before >> 16);
     for (int i = 0; i < rank; ++i) {
         const uint32_t x = *cluster.map_shared_rank(mine, i);
         above += (int)(x & 0xFFFFu);
