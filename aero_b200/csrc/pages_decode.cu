@@ -215,26 +215,41 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             const Piece pc = piece_at(a, sp, u, u1, base);
             const int h = pc.h, t0 = pc.t0, cnt = pc.cnt;
             const int s = sp.seq;
+            // SEL: a box's first position and page for each lane, 32 boxes at once (the list and then the table are
+            // two reads one after another; for each unit anew they held the first stages up)
+            int at32 = kNowhere, page32 = 0;
             for (int t = t0; t < t0 + cnt; ++t) {
                 // lane i brings box i, if a position in it is visible
                 int j0;
                 bool want;
+                int page = 0;
                 if constexpr (SEL) {
-                    const int64_t at = (int64_t)t * kUnit + lane * rows;  // in the list's positions
-                    const int i = (int)(at >> a.c.page_shift);
-                    const int block = lane < boxes && i < sp.first ? a.blocks[((int64_t)e * HK + h) * a.width + i] : -1;
-                    want = block >= 0 && block <= (sp.n - 1) >> a.c.page_shift;
-                    j0 = want ? (block << a.c.page_shift) + (int)(at & (P - 1)) : kNowhere;
-                    want = j0 < sp.n;
-                    if (!want) j0 = kNowhere;
+                    const int slot = (t - t0) * boxes & 31;
+                    if (slot == 0) {
+                        const int64_t at = (int64_t)t * kUnit + lane * rows;  // in the list's positions
+                        const int i = (int)(at >> a.c.page_shift);
+                        // (beyond the piece: a box that no unit here takes)
+                        const int block = i < sp.first && lane < (t0 + cnt - t) * boxes ? a.blocks[((int64_t)e * HK + h) * a.width + i] : -1;
+                        at32 = kNowhere;
+                        if (block >= 0 && block <= (sp.n - 1) >> a.c.page_shift) {
+                            const int j = (block << a.c.page_shift) + (int)(at & (P - 1));
+                            if (j < sp.n) {
+                                at32 = j;
+                                page32 = a.c.table[(int64_t)s * a.c.max_pages + block];
+                                if ((uint32_t)page32 >= (uint32_t)a.c.n_page) pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
+                            }
+                        }
+                    }
+                    j0 = __shfl_sync(0xffffffffu, at32, slot + (lane & (boxes - 1)));
+                    page = __shfl_sync(0xffffffffu, page32, slot + (lane & (boxes - 1)));
+                    want = lane < boxes && j0 != kNowhere;
                 } else {
                     j0 = tile_at(sp, t) * kUnit + lane * rows;
                     want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
-                }
-                int page = 0;
-                if (want) {
-                    page = a.c.table[(int64_t)s * a.c.max_pages + (j0 >> a.c.page_shift)];
-                    if ((uint32_t)page >= (uint32_t)a.c.n_page) pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
+                    if (want) {
+                        page = a.c.table[(int64_t)s * a.c.max_pages + (j0 >> a.c.page_shift)];
+                        if ((uint32_t)page >= (uint32_t)a.c.n_page) pages_flag(a.c, AERO_CUDA_PAGES_BAD_PAGE);
+                    }
                 }
                 if (!warp_wait(smem_u32(bars + ST + stage), phase ^ 1u, abort_flag)) {
                     good = false;
