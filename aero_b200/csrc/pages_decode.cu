@@ -91,18 +91,24 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int e) {
 __device__ __forceinline__ int tile_at(const Span& p, int t) { return t < p.first ? t : p.tile0 + t - p.first; }
 __device__ __forceinline__ bool visible(const Span& p, int j) { return j < p.n && (j >= p.lo || j < p.sinks); }
 
+// a / b of numbers >= 0: in 32 bits where they fit (a division in 64 costs some 200 cycles, and those
+// of a CTA's beginning were most of its 5000 before the first copy).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 // Places of the line that a CTA takes: an equal share, but at least what is worth a part of its own.
 // (sequence, head)s of up to kWhole units are left whole: joining parts costs more than those few
 // units one after another. Longer ones are cut into about kParts parts, as many as a join reads at
 // once, of 2 to 4 units, if possible an even cut, so that no part holds the end of one and the
 // beginning of the next (one sequence of 4096, 64 units: parts of 3 take 2.4 us more than of 4).
 __device__ __forceinline__ int64_t piece_length(int64_t total, int64_t segments) {
-    const int64_t each = (total + segments - 1) / segments, share = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t each = quotient(total + segments - 1, segments), share = quotient(total + gridDim.x - 1, gridDim.x);
     if (each <= kWhole) return max(each, share);
     const int least = (int)min((int64_t)4, max((int64_t)2, (each + kParts - 1) / kParts));
     int w = least;
     for (int c = 2 * least - 1; c >= least; --c)
-        if (each % c == 0) w = c;
+        if (each - quotient(each, c) * c == 0) w = c;
     return max((int64_t)w, share);
 }
 
@@ -115,8 +121,8 @@ __device__ __forceinline__ Piece piece_at(const AttendArgs& a, const Span& p, in
     const int line = p.tiles + a.over;
     const int64_t in = u - base;
     Piece c;
-    c.h = (int)(in / line);
-    const int at = (int)(in % line);
+    c.h = (int)quotient(in, line);
+    const int at = (int)(in - (int64_t)c.h * line);
     c.line = (int)min((int64_t)(line - at), u1 - u);
     c.t0 = max(at - a.over, 0);
     c.cnt = max(at + c.line - a.over, 0) - c.t0;
@@ -134,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     float2* ml = reinterpret_cast<float2*>(sm + ST * Cfg<D>::stage_bytes + Cfg<D>::red_bytes);  // [4][16] (m, l)
     float2* joint = ml + 64;                                                     // [16]
     uint64_t* bars = reinterpret_cast<uint64_t*>(joint + 16);                    // full[ST], empty[ST]
-    int64_t* begin_s = reinterpret_cast<int64_t*>(bars + 2 * ST);                // entry base, total
+    int64_t* begin_s = reinterpret_cast<int64_t*>(bars + 2 * ST);                // entry base
     int4* joins = reinterpret_cast<int4*>(begin_s + 2);                          // [2]: parts to join (or 0), first CTA, token, head
     int* misc = reinterpret_cast<int*>(joins + 2);                               // entry, abort
     Span* span_s = reinterpret_cast<Span*>(misc + 2);                            // the first entry's
@@ -156,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
     stream_turn();
     if (blockIdx.x == 0 && a.q_start) check_q_start(a);
     // ---- this CTA's piece of the line of units
+    int64_t total, w;
     {
         int64_t* sums = reinterpret_cast<int64_t*>(red);  // [kThreads / 32]
         const int per = (a.T + kThreads - 1) / kThreads;
@@ -170,13 +177,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         }
         if (lane == 31) sums[warp] = incl;
         __syncthreads();
-        int64_t before = incl - mine, total = 0;
+        int64_t before = incl - mine;
+        total = 0;
         for (int i = 0; i < kThreads / 32; ++i) {
             if (i < warp) before += sums[i];
             total += sums[i];
         }
         total *= HK;
-        const int64_t w = piece_length(total, (int64_t)a.T * HK);
+        w = piece_length(total, (int64_t)a.T * HK);
         const int64_t u0 = w * blockIdx.x;
         if (u0 >= before * HK && u0 < (before + mine) * HK) {
             int64_t base = before * HK;
@@ -192,11 +200,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             misc[0] = e;
             *span_s = at;
         }
-        if (tid == 0) begin_s[1] = total;
         __syncthreads();
     }
-    const int64_t total = begin_s[1];
-    const int64_t w = piece_length(total, (int64_t)a.T * HK);
     const int64_t u0 = w * blockIdx.x, u1 = min(total, u0 + w);
     if (u0 >= u1) return;
 
@@ -550,8 +555,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             }
             if (tid < G) *reinterpret_cast<float2*>(mine + 16 * D + 2 * tid) = joint[tid];
             const int64_t seg0 = base + (int64_t)h * (sp.tiles + a.over) + a.over;  // its units: [seg0, seg0 + tiles)
-            const int64_t c0 = seg0 / w;
-            const int parts = (int)((seg0 + sp.tiles - 1) / w - c0) + 1;
+            const int64_t c0 = quotient(seg0, w);
+            const int parts = (int)(quotient(seg0 + sp.tiles - 1, w) - c0) + 1;
             asm volatile("bar.sync 1, 128;" ::: "memory");
             if (tid == 0) {
                 __threadfence();  // the CTA's stores, ordered before by the barrier
