@@ -1,14 +1,15 @@
 """A batch served over the paged cache: prompts, parallel samples, penalties, a grammar.
 
-    python -m aero_b200.serve_example [--steps 32]
+    python -m aero_b200.serve_example [--steps 32] [--temperature 0.8 --top-p 0.9] [--blocks 4]
 
 A small decoder with random weights (embedding, per layer grouped-query attention over
 `PagedCache` and the MoE block of `CudaMoeLayer`, a head) serves three prompts: one
 call takes all prompt tokens, every prompt is forked into parallel samples, each
 decode step takes one token of every sample and adjusts its logits (`logits.adjust`:
 penalties from its history, a bias against the end token, a mask of allowed tokens)
-before the largest is taken. Samples that end are freed and the pool is compacted. Odd
-layers attend within a window, with the first tokens kept visible.
+before the next one is drawn (`logits.sample`: the largest, unless a temperature is given). Samples
+that end are freed and the pool is compacted. Odd layers attend within a window, with the first tokens kept
+visible; with `blocks`, decode steps of the even layers attend to that many blocks that `select` chooses.
 """
 
 from __future__ import annotations
@@ -20,12 +21,13 @@ import math
 class PagedDecoder:
     """The decoder: random weights of a seed, f16 activations in attention, f32 elsewhere."""
 
-    def __init__(self, cache, n_head: int, d: int, vocab: int, window: int = 0, sinks: int = 0, seed: int = 0) -> None:
+    def __init__(self, cache, n_head: int, d: int, vocab: int, window: int = 0, sinks: int = 0, seed: int = 0,
+                 blocks: int = 0) -> None:
         import torch
         from . import synth
         from .quant import DTYPE_Q8_0
         self.torch, self.cache, self.H, self.d, self.vocab = torch, cache, n_head, d, vocab
-        self.window, self.sinks = window, sinks
+        self.window, self.sinks, self.blocks = window, sinks, blocks
         g = torch.Generator(device="cuda")
         g.manual_seed(seed)
 
@@ -64,7 +66,11 @@ class PagedDecoder:
             y = (self._norm(x) @ qkv.T).view(T, self.H + 2 * HK, D)
             q, k = self._rotate(self._norm(y[:, :self.H]), positions), self._rotate(self._norm(y[:, self.H:-HK]), positions)
             c.append(i, k.to(c.dtype), y[:, -HK:].to(c.dtype), row_seq, positions)
-            a = c.attend(i, q.to(c.dtype), seqs, q_start, window=self.window if i % 2 else 0, sinks=self.sinks)
+            q = q.to(c.dtype)
+            if self.blocks and q_start is None and i % 2 == 0:
+                a = c.attend_blocks(i, q, seqs, c.select(i, q, seqs, n_blocks=self.blocks))
+            else:
+                a = c.attend(i, q, seqs, q_start, window=self.window if i % 2 else 0, sinks=self.sinks)
             x = x + a.reshape(T, -1).float() @ o.T
             x = x + self.moe[i].forward(self._norm(x))
         last = x if q_start is None else x[(q_start[1:] - 1).long()]
@@ -91,16 +97,20 @@ def mask_of(allowed, vocab: int, rows: int):
     return torch.from_numpy(words).cuda().expand(rows, -1).contiguous()
 
 
-def serve(steps: int = 32, samples: int = 2, seed: int = 0, d: int = 256, vocab: int = 1000, layers: int = 2) -> dict:
-    """Serves three prompts with `samples` samples each; returns their tokens and the cache's state."""
+def serve(steps: int = 32, samples: int = 2, seed: int = 0, d: int = 256, vocab: int = 1000, layers: int = 2,
+          temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, blocks: int = 0) -> dict:
+    """Serves three prompts with `samples` samples each; returns their tokens and the cache's state. The largest
+    logit is taken, or with a temperature a token is drawn; blocks: see the top."""
     import torch
-    from .logits import adjust
+    from .logits import adjust, sample
     from .pages import PagedCache
     prompts = [[(7 * i + j * j) % vocab for j in range(n)] for i, n in enumerate((5, 70, 33))]
     P, n_seq, end = 16, len(prompts) * (samples + 1), vocab - 1
     longest = max(map(len, prompts)) + steps
-    cache = PagedCache(layers, n_seq * (longest // P + 2), P, 2, 64, n_seq, longest // P + 2, dtype=torch.float16)
-    net = PagedDecoder(cache, 8, d, vocab, window=32, sinks=4, seed=seed)
+    cache = PagedCache(layers, n_seq * (longest // P + 2), P, 2, 64, n_seq, longest // P + 2, dtype=torch.float16,
+                       bounds=blocks > 0)
+    net = PagedDecoder(cache, 8, d, vocab, window=32, sinks=4, seed=seed, blocks=blocks)
+    numbers = torch.Generator(device="cuda").manual_seed(seed)  # the random numbers that tokens are drawn with
     with torch.cuda.stream(net.stream):
         # all prompts in one call
         roots = list(range(len(prompts)))
@@ -139,7 +149,9 @@ def serve(steps: int = 32, samples: int = 2, seed: int = 0, d: int = 256, vocab:
                    presence=torch.full((B,), 0.2, device="cuda"), bias_start=i32(list(range(B + 1))),
                    bias_token=i32([end] * B), bias_value=torch.full((B,), -1.0, device="cuda"),
                    mask=mask_of(allowed, vocab, B), out=logits)
-            nxt = logits.argmax(1).int()
+            nxt = sample(logits, torch.rand(B, device="cuda", generator=numbers), temperature=torch.full((B,), temperature, device="cuda"),
+                         top_k=i32([top_k] * B), top_p=torch.full((B,), top_p, device="cuda"),
+                         min_p=torch.full((B,), min_p, device="cuda"))
             history[rows, held.long()] = nxt
             for s in live:
                 n[s] += 1
@@ -166,8 +178,13 @@ def main() -> None:
     p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     p.add_argument("--steps", type=int, default=32)
     p.add_argument("--samples", type=int, default=2)
+    p.add_argument("--temperature", type=float, default=0.0, help="0: the largest logit")
+    p.add_argument("--top-k", type=int, default=0)
+    p.add_argument("--top-p", type=float, default=1.0)
+    p.add_argument("--min-p", type=float, default=0.0)
+    p.add_argument("--blocks", type=int, default=0, help="blocks that a decode step's even layers attend to; 0: all")
     a = p.parse_args()
-    r = serve(a.steps, a.samples)
+    r = serve(a.steps, a.samples, temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, blocks=a.blocks)
     for row, n in enumerate(r["n"]):
         if n:
             print(f"sequence {row}: {r['history'][row, :n].tolist()}")
