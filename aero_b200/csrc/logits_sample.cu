@@ -598,7 +598,7 @@ __device__ __noinline__ void nth_token(const SampleArgs& a, int row, const E* in
         all += s.warp_count[i];
     }
     if (tid < C) cluster.map_shared_rank(&s, tid)->ties[rank] = all;
-    cluster.sync();
+    cluster_barrier(C);
     all = 0;
     for (int i = 0; i < C; ++i) {
         before += i < rank ? s.ties[i] : 0;
@@ -648,7 +648,7 @@ __device__ __noinline__ void collect(const H& h, Groups& to, int C, int rank) {
         there->mass[g] = own.mass[g];
         if (sizeof(H) == sizeof(Parts)) there->count[g] = own.count[g];
     }
-    cluster.sync();
+    cluster_barrier(C);
     if (tid < kGroups) {
         u64 m = 0;
         uint32_t n = 0;
@@ -1105,7 +1105,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             for (int o = 1; o < kSampleWarps; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, o));
             if (lane < C) cluster.map_shared_rank(&s, lane)->ends[rank] = e;
         }
-        cluster.sync();
+        cluster_barrier(C);
     }
     int op;
     {
@@ -1139,8 +1139,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         }
         __syncthreads();
     }
+    // (a row takes two or three rounds, with equal keys by the thousand some more; none takes as many as this)
 #pragma unroll 1
-    for (;;) {
+    for (int round = 0; round < 64; ++round) {
         if (op == kTies || op == kCrowd) {
             nth_token<E>(a, row, in, v0, nv, op == kCrowd);
             return;
@@ -1164,7 +1165,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             for (uint32_t i = tid; i < staged && base + i < (uint32_t)kMembers; i += kSampleThreads) head->member[base + i] = stage[i];
             __syncthreads();
             clear(s.more);
-            cluster.sync();
+            cluster_barrier(C);
             if (last && rank != 0) return;
             if (rank == 0) {
                 if (s.members > (uint32_t)kMembers) {
@@ -1182,21 +1183,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 if (tid == 0) s.members = 0;
             }
             // what it found, to all
-            cluster.sync();
+            cluster_barrier(C);
             if (rank != 0 && tid == 0) s.find = head->find;
-            cluster.sync();
+            cluster_barrier(C);
             op = s.find.op;
             if (op == kDone) return;
         }
         if (op == kDivide) {
-            cluster.sync();  // what the histograms before held is read by all
+            cluster_barrier(C);  // what the histograms before held is read by all
             divide_pass<E>(in, nv);
         } else if (op == kNumbers) {
             numbers_pass<E>(in, nv);
         } else if (op == kSums) {
             if (k > 1 && k < a.vocab) {
                 // (the numbers there are first: read by all, then cleared)
-                cluster.sync();
+                cluster_barrier(C);
                 clear(s.first);
                 if (tid == 0) s.fresh = 1;
                 __syncthreads();
@@ -1220,12 +1221,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             collect(s.first, s.first_groups, C, rank);
         look(op != kDivide, op != kNumbers, C);
         if (op == kDivide) {
-            cluster.sync();  // read by all, then cleared
+            cluster_barrier(C);  // read by all, then cleared
             clear(s.more);
             __syncthreads();
         }
         op = s.find.op;
     }
+    if (rank == 0 && tid == 0) {
+        a.token[row] = -1;
+        if (a.logprob) a.logprob[row] = -INFINITY;
+    }
+    cluster_barrier(C);  // no CTA ends while another reads its memory
 }
 
 template <typename E>

@@ -62,6 +62,15 @@ __device__ __forceinline__ void stream_turn() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+// A barrier of a cluster of C CTAs; of one CTA an ordinary one, which costs a third.
+__device__ __forceinline__ void cluster_barrier(int C) {
+    if (C == 1) {
+        __syncthreads();
+        return;
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void pages_flag(const PageView& c, int code) { atomicCAS(c.status, 0, code); }
 // Length of sequence s as kernels may use it: 0 for a number outside the table,
 // never past what its row of the table can hold.

@@ -9,8 +9,8 @@
 // bounds are finite, so the part that is zero adds nothing). A wrong order of two scores is a wrong block, so what is
 // chosen has to follow from sums in 64 bits; those cost 64 products a cycle and SM at best (m8n8k4 products: 48
 // sequences of up to 512 blocks, 32 query heads, 16 us of scores). So every score is computed first in f32 (m16n8k16
-// products, the operands as they are), off by at most e = 2^-14 max_g sum_d |q_gd| max |bounds|: 32 sums of 17 terms, each
-// off by at most 2^-19 of their terms' sum. Only the blocks whose score lies within 2 e of where the least chosen one can
+// products, the operands as they are), off by at most e = 2^-13 max_g sum_d |q_gd| max |bounds|: 32 sums of 17 terms, each
+// term cut at 2^-23 of the largest. Only the blocks whose score lies within 2 e of where the least chosen one can
 // be are computed again in 64 bits, a handful; where they are many (blocks alike) all are.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             to.hi = hi;
             to.most = bound;
         }
-        cluster.sync();
+        cluster_barrier(C);
         lo = ~0u, hi = 0, bound = 0.f;
         for (int i = 0; i < C; ++i) {
             lo = min(lo, told[i].lo);
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             number &= sizes[i] < INFINITY;
             size = fmaxf(size, sizes[i]);
         }
-        const float off = size * bound * 1.25e-4f;  // 2 e, rounded up
+        const float off = size * bound * 2.5e-4f;  // 2 e, rounded up
         if (number && off < 1e30f) {
             // ---- an interval that holds the least chosen score: a few blocks' or narrower than what they may be off
             int left = need;
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
                     const uint32_t k = keys32[i];
                     if (k >= lo && k <= hi && k != kAlways32) atomicAdd(own + ((hi - k) >> shift), 1u);
                 }
-                cluster.sync();
+                cluster_barrier(C);
                 // the other histogram, read by all before this barrier, is the next one's
                 hist[(~level & 1) * kBins + tid] = 0;
                 uint32_t v = 0, all;
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
                     to.near = n;
                 }
             }
-            cluster.sync();
+            cluster_barrier(C);
             bool few = true;
             int open = need, base = 0;
             for (int i = 0; i < C; ++i) {
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
         }
     }
     // ---- scores in 64 bits, all of them
-    cluster.sync();  // (the memory that others may be reading is written again)
+    cluster_barrier(C);  // (the memory that others may be reading is written again)
     // ---- the query heads' positive and negative parts, as the products' fragments; heads past G are the first ones again
     {
         for (int i = tid; i < NT * 8 * D; i += kSelThreads) {
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
         range[0] = lo;
         range[1] = hi;
     }
-    cluster.sync();
+    cluster_barrier(C);
     lo = kAlways, hi = 0;
     for (int i = 0; i < C; ++i) {
         const u64* r = cluster.map_shared_rank(range, i);
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             const u64 k = keys[i];
             if (k >= lo && k <= hi) atomicAdd(own + (uint32_t)((hi - k) >> shift), 1u);
         }
-        cluster.sync();
+        cluster_barrier(C);
         // the other histogram, read by all before this barrier, is the next one's
         hist[(~level & 1) * kBins + tid] = 0;
         uint32_t v = 0, all;
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
     uint32_t all;
     const uint32_t before = scan(count, all);
     if (tid == 0) mine[0] = all;
-    cluster.sync();
+    cluster_barrier(C);
     int above = (int)(before & 0xFFFFu), on = (int)(before >> 16);
     for (int i = 0; i < rank; ++i) {
         const uint32_t x = *cluster.map_shared_rank(mine, i);
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             ++on;
         }
     }
-    cluster.sync();  // no CTA ends while another reads its memory
+    cluster_barrier(C);  // no CTA ends while another reads its memory
 }
 
 template <int D, bool BF16, int NT>

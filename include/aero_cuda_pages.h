@@ -203,7 +203,7 @@ int aero_cuda_logits_adjust_views(const void* logits, int64_t ld, int dtype, int
  *   then have at least min_p[r] times the first one's weight (0 or less, or no number: all),
  * the first one always. tokens[r] = the first whose running sum exceeds u[r] times the sum of those kept, logprob[r] (may
  * be NULL) = the log of its weight's share of that sum. temperature[r] of 0 or less, or no number: the first of the
- * order. Logits of -infinity and those that are no number are never drawn; a row of nothing else gives -1 and
+ * order (below 2^-100: as 2^-100). Logits of -infinity and those that are no number are never drawn; a row of nothing else gives -1 and
  * -infinity. With a logit of +infinity all others have weight 0. temperature (1), top_k, top_p and min_p may
  * be NULL. Weights are computed in 64 bits and summed as multiples of 2^-b of the largest, b = 62 less the bits of
  * vocab (48 at most, 44 for 2^18), so a weight below half of that is never drawn; the

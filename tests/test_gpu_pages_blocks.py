@@ -225,12 +225,12 @@ def test_select_ties_and_values_that_are_no_numbers():
         assert got[0].tolist() == sorted([0, *others, 298, 299])
 
 
-@pytest.mark.parametrize("width", [700, 7000, 50000, 131072])
-def test_select_in_caches_of_long_rows(width):
+@pytest.mark.parametrize("width,G,D", [(700, 4, 64), (7000, 4, 64), (50000, 4, 64), (131072, 4, 64), (131072, 16, 256)])
+def test_select_in_caches_of_long_rows(width, G, D):
     """The cluster's size and the keys' place follow from max_pages."""
     lens, P, HK = [8 * 600 + 3, 20], 8, 1
-    c, K, _ = open_cache(lens, P, HK, 64, BF16, width=width)
-    q = torch.randn((2, 4, 64), device="cuda", generator=gen(7)).to(BF16)
+    c, K, _ = open_cache(lens, P, HK, D, BF16, width=width)
+    q = torch.randn((2, G, D), device="cuda", generator=gen(7)).to(BF16)
     got = c.select(0, q, i32([0, 1]), n_blocks=31).cpu().numpy()
     for s in (0, 1):
         assert (got[s] == plain_select(q[s], plain_bounds(K[s], P), lens[s], P, 31, 1, 1)).all()
@@ -515,3 +515,42 @@ def test_select_of_wide_rows_of_queries():
     got = c.select(0, q, i32([0, 1, 2, 3, 4]), n_blocks=20, first=2, recent=3).cpu().numpy()
     for s, n in enumerate(lens):
         assert (got[s] == plain_select(q[s], plain_bounds(K[s], P), n, P, 20, 2, 3)).all()
+
+
+def test_memory_is_charged_and_given_back():
+    import gc
+    from aero_b200.pages import PagedCache, plan_bytes
+    gc.collect()
+    lib = nc.lib()
+    before = [lib.aero_cuda_guard_committed(i) for i in range(5)]
+    c = PagedCache(2, 40, 16, 2, 128, 3, 9, bounds=True)
+    held = sum(lib.aero_cuda_guard_committed(i) for i in range(5)) - sum(before)
+    assert held == plan_bytes(2, 40, 16, 2, 128, 3, 9, bounds=True)["total"]
+    assert lib.aero_cuda_pages_keep_bounds(c.handle) == 0  # again: nothing more
+    assert sum(lib.aero_cuda_guard_committed(i) for i in range(5)) - sum(before) == held
+    c.close()
+    assert [lib.aero_cuda_guard_committed(i) for i in range(5)] == before
+
+
+def test_calls_on_other_streams_and_a_set_stream():
+    """The cache follows torch's current stream; what one stream wrote the next call on another waits for."""
+    c, K, V = open_cache([300, 90], 16, 2, 64, F16)
+    q = torch.randn((2, 8, 64), device="cuda", generator=gen(3)).half()
+    lists = c.select(0, q, i32([0, 1]), n_blocks=3)
+    want = c.attend_blocks(0, q, i32([0, 1]), lists)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    seqs, out = i32([0, 1]), torch.empty_like(lists)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(20000000)
+        c.select(0, q, seqs, n_blocks=3, out=out)
+    with torch.cuda.stream(b):  # the cache's calls run one after another
+        got = c.attend_blocks(0, q, seqs, out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, lists) and torch.equal(got, want)
+    c.set_stream(a)
+    got = c.attend_blocks(0, q, seqs, out)
+    a.synchronize()
+    assert torch.equal(got, want)
+    c.check()
