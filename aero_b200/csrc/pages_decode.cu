@@ -559,11 +559,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             const int parts = (int)(quotient(seg0 + sp.tiles - 1, w) - c0) + 1;
             asm volatile("bar.sync 1, 128;" ::: "memory");
             if (tid == 0) {
-                __threadfence();  // the CTA's stores, ordered before by the barrier
-                const bool last = atomicAdd(a.counters + c0, 1u) == (uint32_t)(parts - 1);
+                // the CTA's stores, ordered before by the barrier; what the others stored, ordered by the barrier below for the
+                // whole CTA
+                uint32_t before;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(a.counters + c0) : "memory");
+                const bool last = before == (uint32_t)(parts - 1);
                 if (last) a.counters[c0] = 0;  // for the next launch
                 joins[which] = make_int4(last ? parts : 0, (int)c0, e, h);
-                __threadfence();  // what the others stored, ordered by the barrier below for the whole CTA
             }
         }
         }
