@@ -9,8 +9,8 @@
 // bounds are finite, so the part that is zero adds nothing). A wrong order of two scores is a wrong block, so what is
 // chosen has to follow from sums in 64 bits; those cost 64 products a cycle and SM at best (m8n8k4 products: 48
 // sequences of up to 512 blocks, 32 query heads, 16 us of scores). So every score is computed first in f32 (m16n8k16
-// products, the operands as they are), off by at most e = 2^-13 max_g sum_d |q_gd| max |bounds|: 32 sums of 17 terms, each
-// term cut at 2^-23 of the largest. Only the blocks whose score lies within 2 e of where the least chosen one can
+// products, the operands as they are), off by at most e = 17 2^-23 D / 8 max_g sum_d |q_gd| max |bounds|: D / 8 sums of 17
+// terms one after another, each term cut at 2^-23 of the largest. Only the blocks whose score lies within 2 e of where the least chosen one can
 // be are computed again in 64 bits, a handful; where they are many (blocks alike) all are.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             number &= sizes[i] < INFINITY;
             size = fmaxf(size, sizes[i]);
         }
-        const float off = size * bound * 2.5e-4f;  // 2 e, rounded up
+        const float off = size * bound * (5.12e-7f * D);  // 2 e, rounded up
         if (number && off < 1e30f) {
             // ---- an interval that holds the least chosen score: a few blocks' or narrower than what they may be off
             int left = need;
