@@ -8,13 +8,15 @@ from __future__ import annotations
 from . import native_cuda as nc
 
 _KINDS = None  # torch types -> element types
+_TORCH = None  # torch, float32, int32
 
 
 def _kinds():
-    global _KINDS
+    global _KINDS, _TORCH
     if _KINDS is None:
         import torch
         nc.require_gpu()
+        _TORCH = torch, torch.float32, torch.int32
         _KINDS = {torch.float32: nc.TYPE_F32, torch.float16: nc.TYPE_F16, torch.bfloat16: nc.TYPE_BF16}
     return _KINDS
 
@@ -98,30 +100,28 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, l
     temperature, top_p, min_p: float32 (rows), top_k: int32 (rows); None, or a row's top_k of 0 or less, top_p of 1 or
     more, min_p of 0 or less: no such limit; a row's temperature of 0 or less: the largest logit. Logits of -infinity and
     those that are no number are never drawn; -1 for a row of nothing else. Runs on torch's current stream."""
-    import torch
     L, kinds = nc.lib(), _kinds()
-    index = logits.get_device()
-    if logits.dim() != 2 or logits.dtype not in kinds or index < 0 or logits.stride(1) != 1:
+    index, shape, kind = logits.get_device(), logits.shape, kinds.get(logits.dtype)
+    if len(shape) != 2 or kind is None or index < 0 or logits.stride(1) != 1:
         raise ValueError("logits must be a (rows, vocab) CUDA tensor of float32, float16 or bfloat16, contiguous along vocab")
-    rows, vocab = logits.shape
+    rows, vocab = shape
+    torch, f32, i32 = _TORCH
 
     def vec(t, name, dtype):
-        if t is None:
-            return None
         if t.dtype is not dtype or t.get_device() != index or t.numel() != rows or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous {dtype}, {rows} entries, on {logits.device}")
         return t.data_ptr()
 
-    f32, i32 = torch.float32, torch.int32
     if u is None:
         raise ValueError("u is required")
     if out is None:
         out = torch.empty(rows, dtype=i32, device=logits.device)
     logs = torch.empty(rows, dtype=f32, device=logits.device) if logprob else None
     if L.aero_cuda_logits_sample(
-            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kinds[logits.dtype], rows, vocab, vec(u, "u", f32),
-            vec(temperature, "temperature", f32), vec(top_k, "top_k", i32), vec(top_p, "top_p", f32),
-            vec(min_p, "min_p", f32), vec(out, "out", i32), None if logs is None else logs.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(index) or None) != 0:
+            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, kind, rows, vocab, vec(u, "u", f32),
+            None if temperature is None else vec(temperature, "temperature", f32),
+            None if top_k is None else vec(top_k, "top_k", i32), None if top_p is None else vec(top_p, "top_p", f32),
+            None if min_p is None else vec(min_p, "min_p", f32), vec(out, "out", i32),
+            None if logs is None else logs.data_ptr(), torch._C._cuda_getCurrentRawStream(index) or None) != 0:
         raise ValueError(f"logits_sample refused: {nc.last_error()}")
     return (out, logs) if logprob else out

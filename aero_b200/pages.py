@@ -324,14 +324,15 @@ class PagedCache:
         self._on()
         qp, q_token, q_head = self._rows(q, "q", None)
         T, H, _ = q.shape
-        if blocks.dim() != 3 or blocks.shape[0] != T or blocks.shape[1] != self.n_head_kv:
-            raise ValueError(f"blocks must be ({T}, {self.n_head_kv}, any), got {tuple(blocks.shape)}")
+        listed = blocks.shape
+        if len(listed) != 3 or listed[0] != T or listed[1] != self.n_head_kv:
+            raise ValueError(f"blocks must be ({T}, {self.n_head_kv}, any), got {tuple(listed)}")
         out, op, o_token, o_head = self._out(q, q_token, q_head, out)
         n = seqs.numel()
         if self._lib.aero_cuda_pages_attend_blocks(
                 self.handle, layer, qp, q_token, q_head, T, H, self._i32(seqs, "seqs"),
                 None if q_start is None else self._i32(q_start, "q_start", n + 1), n, self._i32(blocks, "blocks"),
-                blocks.shape[2], self._scale if scale is None else scale, op, o_token, o_head) != 0:
+                listed[2], self._scale if scale is None else scale, op, o_token, o_head) != 0:
             self._refused("attend_blocks")
         return out
 
