@@ -1073,6 +1073,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const int v0 = min(a.vocab, rank * a.slice), nv = min(a.vocab - v0, a.slice);
     const E* in = static_cast<const E*>(a.in) + (int64_t)row * a.ld + v0;
     Shared* const head = cluster.map_shared_rank(&s, 0);
+    cluster_begun(C);
     clear(s.first);
     clear(s.more);
     const double lift = __longlong_as_double((long long)(1023 + a.bits) << 52);
@@ -1099,6 +1100,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         for (int o = 1; o < 32; o <<= 1) e = fmaxf(e, __shfl_xor_sync(0xffffffffu, e, o));
         if (lane == 0) s.warp_ends[warp] = e;
         __syncthreads();
+        cluster_all_begun(C);
         if (warp == 0) {
             e = s.warp_ends[lane % kSampleWarps];
 #pragma unroll

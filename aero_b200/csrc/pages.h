@@ -68,8 +68,16 @@ __device__ __forceinline__ void cluster_barrier(int C) {
         __syncthreads();
         return;
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// In two halves: a CTA's memory may be reached by the cluster's others once it has begun, so each says so at its
+// beginning (cluster_begun), and nobody reaches for another's before all have (cluster_all_begun).
+__device__ __forceinline__ void cluster_begun(int C) {
+    if (C > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_all_begun(int C) {
+    if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void pages_flag(const PageView& c, int code) { atomicCAS(c.status, 0, code); }
 // Length of sequence s as kernels may use it: 0 for a number outside the table,

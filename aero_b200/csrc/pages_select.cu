@@ -235,6 +235,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
     const int tid = (int)threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int HK = a.c.HK, G = a.H / HK, P = 1 << a.c.page_shift;
     const int pair = (int)blockIdx.x / C, t = pair / HK, h = pair % HK;
+    cluster_begun(C);
     stream_turn();
     if (blockIdx.x == 0 && a.q_start) check_q_start(a);
     int seq, n;
@@ -249,15 +250,17 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
         // all of them, or no others
         for (int i = rank * kSelThreads + tid; i < W; i += C * kSelThreads)
             list[i] = nb <= W ? (i < nb ? i : -1) : i < f1 ? i : r0_ + i - f1;
+        cluster_all_begun(C);
         return;
     }
+    cluster_all_begun(C);
     const int per = ((nb + C - 1) / C + 15) & ~15;
     const int b0 = min(nb, rank * per), b1 = min(nb, b0 + per);
     const uint16_t* const q = static_cast<const uint16_t*>(a.q) + (int64_t)t * a.q_token + (int64_t)(h * G) * a.q_head;
     const uint16_t* const bounds = a.c.bounds + (int64_t)h * 2 * D;
     const auto page_of = [&](int b) { return b < b1 ? a.c.table[(int64_t)seq * a.c.max_pages + b] : -1; };
     const auto row_of = [&](int page) { return bounds + ((int64_t)a.layer * a.c.n_page + page) * HK * 2 * D; };
-    // an entry's place among the CTA's, and all of them, of 256 small numbers a thread each
+    // the sum of the numbers of the threads before this one, and of all
     const auto scan = [&](uint32_t v, uint32_t& all) {
         uint32_t incl = v;
 #pragma unroll
