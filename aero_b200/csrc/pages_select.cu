@@ -142,7 +142,9 @@ __global__ void __launch_bounds__(kBoundThreads, 4) set_bounds_kernel(PageView c
                 pages_flag(c, AERO_CUDA_PAGES_BAD_PAGE);
                 continue;
             }
-            bound<BF16>(c, layer, k, page, h, min(1 << c.page_shift, lj - (slot << c.page_shift)));
+            // (a page of several sequences, whose lengths may differ, whole: the warps that take it write the same)
+            const int rows = c.refs[page] > 1 ? 1 << c.page_shift : lj - (slot << c.page_shift);
+            bound<BF16>(c, layer, k, page, h, min(1 << c.page_shift, rows));
         }
         base += total;
     }

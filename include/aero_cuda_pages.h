@@ -133,7 +133,7 @@ int aero_cuda_pages_attend(void* cache, int layer, const void* q, int64_t q_toke
  * below the sequence's length (infinities count as the type's largest values, what is no
  * number is passed over, a column of nothing else has bounds 0). From keep_bounds on an append sets the bounds of
  * the pages that it writes to, a fork, a copy and a compaction move them with their pages, and
- * set_bounds makes them from the pool. */
+ * set_bounds makes them from the pool (of a page that several sequences hold, over all its positions). */
 
 /* Device bytes of the bounds. -1 for an invalid description. */
 int64_t aero_cuda_pages_bounds_bytes(const aero_cuda_pages_desc* desc);

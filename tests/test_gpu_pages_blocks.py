@@ -158,6 +158,26 @@ def test_bounds_step_by_step_and_refused_appends():
     assert c.status() != 0 and torch.equal(was, c.bounds())
 
 
+def test_bounds_of_a_page_that_sequences_of_several_lengths_hold():
+    """Adopted books may share a page that not all of its sequences fill: its bounds cover it whole, in any order."""
+    from aero_b200.pages import PagedCache
+    c = PagedCache(1, 9, 64, 2, 64, 3, 2, dtype=BF16, bounds=True)
+    rows = torch.randn((9, 2, 64, 64), device="cuda", generator=gen(2)).to(BF16)
+    c.k(0).copy_(rows.reshape(c.k(0).shape))
+    c.set_tables(i32([4, 7, 4, -1, 4, 2]), i32([70, 9, 128]), i32([0, 0, 1, 0, 3, 0, 0, 1, 0]))
+
+    def whole(page, n=64):
+        return plain_bounds(rows[page, :, :n].transpose(0, 1), 64)[0]
+
+    for order in ([0, 1, 2], [2, 1, 0], [1], [0, 2, 1]):
+        c.bounds().fill_(7)
+        c.set_bounds(0, i32(order))
+        c.check()
+        assert torch.equal(c.bounds(0)[4].double(), whole(4))
+        if 0 in order:
+            assert torch.equal(c.bounds(0)[7].double(), whole(7, 6)) and torch.equal(c.bounds(0)[2].double(), whole(2))
+
+
 # ------------------------------------------------------------------ the choice
 def plain_select(q, bounds, n, P, W, first, recent):
     """Block numbers (HK, W) of one token that sees n positions; bounds (blocks, HK, 2, D)."""
