@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             number &= sizes[i] < INFINITY;
             size = fmaxf(size, sizes[i]);
         }
-        const float off = size * bound * (5.12e-7f * D);  // 2 e, rounded up
+        const float off = size * bound * (5.12e-7f * D) + 2e-35f;  // 2 e, rounded up, and 2 * 17 * 32 times the least normal number for what underflows
         if (number && off < 1e30f) {
             // ---- an interval that holds the least chosen score: a few blocks' or narrower than what they may be off
             int left = need;

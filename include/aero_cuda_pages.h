@@ -150,7 +150,7 @@ int aero_cuda_pages_set_bounds(void* cache, int layer, const int32_t* seqs, int 
  * chosen always, and of the others those with the highest score, equal ones by the lower number, until there
  * are n_blocks (first + recent or more). score = the largest, over the kv head's query heads g, of sum_d max(q_gd *
  * lo_d, q_gd * hi_d): no key between the bounds has a larger product with g's query. Scores are summed
- * in 64 bits; one that is no number counts as +infinity. A block without a page is recorded and has bounds
+ * in 64 bits; one that is no number counts as +infinity. A block without a page is recorded where the choice needs scores, and has bounds
  * 0. An empty sequence has no blocks. For caches of max_pages at most 131072. */
 int aero_cuda_pages_select(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
                            const int32_t* seqs, const int32_t* q_start, int n, int first, int recent, int n_blocks,

@@ -524,6 +524,19 @@ def test_select_scores_next_to_one_another(dtype, alike):
         assert (got[0] == plain_select(q[0], plain_bounds(K[0], P), P * blocks, P, W, 1, 1)).all()
 
 
+@pytest.mark.parametrize("power", [-72, -66, -63, -60, -52, 55])
+def test_select_of_the_smallest_and_largest_values(power):
+    """Products around and below what f32 holds without loss, and sums near its largest."""
+    lens, P, HK, G, D = [4000, 640], 8, 2, 4, 128
+    values = torch.randn((sum(lens), HK, D), device="cuda", generator=gen(21)) * 2.0**power
+    c, K, _ = open_cache(lens, P, HK, D, BF16, values=values)
+    q = (torch.randn((2, HK * G, D), device="cuda", generator=gen(22)) * 2.0**power).to(BF16)
+    got = c.select(0, q, i32([0, 1]), n_blocks=30).cpu().numpy()
+    c.check()
+    for s, n in enumerate(lens):
+        assert (got[s] == plain_select(q[s], plain_bounds(K[s], P), n, P, 30, 1, 1)).all()
+
+
 def test_select_of_wide_rows_of_queries():
     """A batch with rows of zeros and of infinities beside ordinary ones, long and short sequences, over 16 query heads."""
     lens, P, HK, G, D = [3000, 5, 1111, 2048, 3000], 8, 2, 16, 192
