@@ -121,6 +121,19 @@ def test_equal_logits(dtype):
     assert check(same, us) is not None and check(same, [0.0] * 5).tolist() == [0] * 5
 
 
+@pytest.mark.parametrize("V", [32767, 32768, 40000, 65535, 65536, 65537, 100003, 131072, 151936, 300001, (1 << 20) + 7])
+def test_flat_rows_of_many_tokens(V):
+    """Sums as large as they can be: all weights the largest, or nearly."""
+    u = [0.0, 0.3, 0.71, 1 - 2.0**-24]
+    x = torch.full((4, V), 1.5, device="cuda")
+    check(x, u)
+    check(x, u, p=[0.9, 0.5, 1.0, 0.25], least=[1.0, 0.5, 0.0, 1e-9])
+    check(x, u, k=[0, V - 1, 3000, 40000], T=[1e-3, 1.0, 9.0, 1e9])
+    x += torch.rand(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(V)) * 1e-3
+    check(x.to(torch.bfloat16), u, p=[0.99, 1.0, 0.6, 0.999])
+    check(x, u, T=[1.0, 5.0, 0.1, 1e5])
+
+
 def test_values_of_every_kind():
     V = 9001
     x = logits(12, V, torch.float32, 5)
