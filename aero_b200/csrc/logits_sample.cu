@@ -61,7 +61,8 @@ struct SampleArgs {
     float* logprob;
 };
 
-// Keys in the values' order, -0 as 0.
+// Keys of numbers in their order, -0 as 0. (What is no number may have any key: the sign of an operation's result is not
+// said.)
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);
     return b >> 31 ? ~b : b | 0x80000000u;
@@ -512,7 +513,7 @@ __device__ __noinline__ void divide_pass(const E* in, int nv) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t key = key_of(x[e]);
-            const bool is = key >= lo && key <= hi;
+            const bool is = x[e] == x[e] && key >= lo && key <= hi;
             const float at = r.place(x[e]);
             const uint32_t to = is ? (hi - key) >> shift : 0u;
             b[e] = 0x4B000000u + to;
@@ -540,7 +541,7 @@ __device__ __noinline__ void gather_pass(const E* in, int v0, int nv) {
         for (int e = 0; e < 4; ++e) {
             if (KEYS) {
                 const uint32_t key = key_of(x[e]);
-                if (key >= lo && key <= hi) is |= 1u << e;
+                if (x[e] == x[e] && key >= lo && key <= hi) is |= 1u << e;
             } else {
                 if ((x[e] >= lo1 && x[e] <= hi1) || (x[e] >= lo2 && x[e] <= hi2)) is |= 1u << e;
             }

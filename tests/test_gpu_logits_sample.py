@@ -134,6 +134,23 @@ def test_flat_rows_of_many_tokens(V):
     check(x, u, T=[1.0, 5.0, 0.1, 1e5])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [2500, 30011])
+def test_no_numbers_among_tokens_nearly_alike(dtype, V):
+    """Slices that hold thousands of tokens, positive and negative ones, of which only the numbers count."""
+    T = [1.0, 30.0, 485.0, 1e5, 1e12]
+    x = torch.randn((5, V), device="cuda", generator=torch.Generator("cuda").manual_seed(12))
+    odd = torch.rand(x.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(13))
+    x[odd < 0.1] = math.nan
+    x[odd < 0.05] *= -1
+    x[odd > 0.99] = -math.inf
+    x = x.to(dtype)
+    x.view(torch.int32 if dtype == torch.float32 else torch.int16)[:, 7::50] = -1  # no number, its sign set
+    for u in (0.0, 0.5, 1 - 2.0**-24):
+        for limits in (dict(), dict(k=1300), dict(k=V * 2 // 3), dict(p=0.7), dict(k=2000, p=0.4), dict(least=0.99)):
+            check(x, [u] * 5, T=T, **{n: [v] * 5 for n, v in limits.items()})
+
+
 def test_values_of_every_kind():
     V = 9001
     x = logits(12, V, torch.float32, 5)
