@@ -7,8 +7,10 @@
 //
 // Bound by HBM: every visible K and V row is read once (up to 16 query heads share it,
 // at most 16 operations a byte). Measured, time on the GPU: 48 sequences of 8192 to 32768 positions, 32
-// query heads on 4 kv heads of 128, 281 us (1.85 GB: 6.6 TB/s); one sequence of 4096 13.6 us, of 20 5.3 us,
-// where a launch, the chain from lengths to pages to rows, and the join set the time.
+// query heads on 4 kv heads of 128, 281 us (1.85 GB: 6.6 TB/s); one sequence of 4096 12.5 us, of 20 5.3 us,
+// where a launch, the chain from lengths to pages to rows, and the join set the time. Over listed blocks: 48
+// sequences, 32 blocks of 64 positions a kv head, 42.5 us (199 MB: 4.7 TB/s); 2048 of one sequence's 32768
+// positions 10.5 us.
 //
 // Split: the work of the call is one line of units, unit = 64 positions of one
 // (sequence, kv head); each CTA takes an equal piece of the line, wherever it begins, so

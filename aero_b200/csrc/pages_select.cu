@@ -1,7 +1,8 @@
 // Bounds of a paged cache's keys and the choice of blocks by them (include/aero_cuda_pages.h).
 //
 // Bounds. lo[d] and hi[d], the smallest and the largest value in column d of a page's keys of one kv
-// head. Bound by HBM: the page's rows are read once, a warp a (page, kv head), 16 bytes a lane.
+// head. Bound by HBM: the page's rows are read once, a warp a (page, kv head), 16 bytes a lane
+// (32 sequences of 8192 to 16384 positions, 4 heads of 128: 413 MB in 72 us, 5.7 TB/s).
 //
 // Choice. score(b) = max over the kv head's query heads g of sum_d max(q_gd lo_bd, q_gd hi_bd): no key
 // between the bounds has a larger product with any of these heads' queries. As one product with
@@ -12,6 +13,12 @@
 // products, the operands as they are), off by at most e = 17 2^-23 D / 8 max_g sum_d |q_gd| max |bounds|: D / 8 sums of 17
 // terms one after another, each term cut at 2^-23 of the largest. Only the blocks whose score lies within 2 e of where the least chosen one can
 // be are computed again in 64 bits, a handful; where they are many (blocks alike) all are.
+//
+// Bound by a chain of steps, not by bytes: one sequence of 2048 blocks, 32 query heads on 4 kv heads of 128, 13.2 us, 48
+// sequences of up to 512 blocks 18.8 us, 8 sequences with 1 to 9 tokens each 15.6 us, a launch included (all in 64 bits: 18.8, 38.6
+// and 34.8 us). Cycles of the first, from HBM: lengths and queries 4500, page numbers, bounds and products 9000, ends 2700, a
+// histogram 4200, blocks near the border and their scores 2800, their exchange 3000, their order and the list
+// 3900.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
