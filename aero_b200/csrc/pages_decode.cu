@@ -46,6 +46,8 @@ constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kWhole = 8, kParts = 16;  // see piece_length
 constexpr int kHalf = kUnit * 128; // bytes of a unit's 64-column half
 constexpr int kNowhere = 1 << 30;  // a position that no token sees (sequences hold at most 2^30)
+constexpr int kNoMore = -1;        // in a stage's first position: this is no unit, and the list has no more
+constexpr int kLook = 4;           // entries of a list that a lane looks at at once
 
 template <int D>
 struct Cfg {
@@ -69,9 +71,11 @@ struct Span {
     int tiles;  // at least 1: an empty sequence has a unit that writes zeros
 };
 
-// Over listed blocks (SEL) a kv head's units are the list's: 64 positions of it in its order, `first`
-// entries of it at all. No list has more blocks that the token sees than there are, so of a
-// longer one the entries behind that many are not looked at.
+// Over listed blocks (SEL) a kv head's units are the list's: 64 positions of it in its order. The line has
+// units for as many entries of it as the token has blocks (`first`): most lists have no others that count. Of a longer list
+// whoever takes the last of these units goes on through the entries behind them and takes what they list (blocks
+// after -1s, listed again, after some that the token does not see), as units that the line does not know of. A list
+// that ends in -1s costs a look at them and no unit, while the units before are on their way.
 template <bool SEL>
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int e) {
     Span p;
@@ -89,6 +93,26 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int e) {
     p.first = min((p.sinks + kUnit - 1) / kUnit, p.tile0);
     p.tiles = p.n > 0 ? p.first + (p.n - 1) / kUnit + 1 - p.tile0 : 1;
     return p;
+}
+// Whether entries of a list lie behind units [t0, t0 + cnt) and behind the line's.
+__device__ __forceinline__ bool listed_behind(const AttendArgs& a, const Span& p, int t0, int cnt) {
+    return cnt > 0 && t0 + cnt == p.tiles && p.first < a.width && p.n > 0;
+}
+// By a warp: a list's first entry from i on that is a block which the token sees (up to `own`); `width`: none is. (A function of
+// its own: inside the producer's loop it costs a call of 11 us that never comes here 0.1 us more.)
+__device__ __noinline__ int seen_from(const int32_t* list, int i, int width, int own) {
+    const int lane = (int)threadIdx.x & 31;
+    for (; i < width; i += 32 * kLook) {
+        int block[kLook];
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) block[k] = i + 32 * k + lane < width ? list[i + 32 * k + lane] : -1;
+#pragma unroll
+        for (int k = 0; k < kLook; ++k) {
+            const uint32_t have = __ballot_sync(0xffffffffu, block[k] >= 0 && block[k] <= own);
+            if (have) return i + 32 * k + __ffs((int)have) - 1;
+        }
+    }
+    return width;
 }
 __device__ __forceinline__ int tile_at(const Span& p, int t) { return t < p.first ? t : p.tile0 + t - p.first; }
 __device__ __forceinline__ bool visible(const Span& p, int j) { return j < p.n && (j >= p.lo || j < p.sinks); }
@@ -225,18 +249,29 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
             // SEL: a box's first position and page for each lane, 32 boxes at once (the list and then the table are
             // two reads one after another; for each unit anew they held the first stages up)
             int at32 = kNowhere, page32 = 0;
-            for (int t = t0; t < t0 + cnt; ++t) {
+            const bool behind = SEL && listed_behind(a, sp, t0, cnt);
+            const int32_t* const list = SEL ? a.blocks + ((int64_t)e * HK + h) * a.width : nullptr;
+            int hand = t0;  // a unit at which 32 boxes were taken in hand
+            for (int t = t0; t < t0 + cnt || behind; ++t) {
                 // lane i brings box i, if a position in it is visible
                 int j0;
                 bool want;
                 int page = 0;
                 if constexpr (SEL) {
-                    const int slot = (t - t0) * boxes & 31;
+                    int slot = (t - hand) * boxes & 31;
+                    int left = (t0 + cnt - t) * boxes;  // (beyond the piece: boxes that no unit here takes)
+                    if (t >= t0 + cnt && (slot == 0 || t == t0 + cnt)) {
+                        // behind the line's units: on to the next one with an entry that counts, if there is one
+                        const int i = seen_from(list, (int)(((int64_t)t * kUnit) >> a.c.page_shift), a.width, (sp.n - 1) >> a.c.page_shift);
+                        t = max(t, (int)(((int64_t)i << a.c.page_shift) / kUnit));
+                        hand = t;
+                        slot = 0;
+                        left = i < a.width ? 32 : 0;
+                    }
                     if (slot == 0) {
                         const int64_t at = (int64_t)t * kUnit + lane * rows;  // in the list's positions
                         const int i = (int)(at >> a.c.page_shift);
-                        // (beyond the piece: a box that no unit here takes)
-                        const int block = i < sp.first && lane < (t0 + cnt - t) * boxes ? a.blocks[((int64_t)e * HK + h) * a.width + i] : -1;
+                        const int block = i < a.width && lane < left ? list[i] : -1;
                         at32 = kNowhere;
                         if (block >= 0 && block <= (sp.n - 1) >> a.c.page_shift) {
                             const int j = (block << a.c.page_shift) + (int)(at & (P - 1));
@@ -250,6 +285,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                     j0 = __shfl_sync(0xffffffffu, at32, slot + (lane & (boxes - 1)));
                     page = __shfl_sync(0xffffffffu, page32, slot + (lane & (boxes - 1)));
                     want = lane < boxes && j0 != kNowhere;
+                    if (t >= t0 + cnt && !__any_sync(0xffffffffu, want)) {
+                        if (left) continue;  // (nothing of it is seen)
+                        j0 = kNoMore;
+                    }
                 } else {
                     j0 = tile_at(sp, t) * kUnit + lane * rows;
                     want = lane < boxes && j0 < sp.n && (j0 + rows > sp.lo || j0 < sp.sinks);
@@ -291,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
                     stage = 0;
                     phase ^= 1u;
                 }
+                if (SEL && j0 == kNoMore) break;  // (in all lanes)
             }
             u += pc.line;
             if (u == base + (int64_t)(sp.tiles + a.over) * HK && u < u1) {
@@ -374,13 +414,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D>::ctas)
         float m[2 * NT], l[2 * NT];
 #pragma unroll
         for (int i = 0; i < 2 * NT; ++i) m[i] = -INFINITY, l[i] = 0.f;
-        for (int t = t0; t < t0 + cnt; ++t) {
+        const bool behind = SEL && listed_behind(a, sp, t0, cnt);
+        for (int t = t0; t < t0 + cnt || behind; ++t) {
             // a warp whose wait gave up goes on without waiting (its results are void, the status
             // says so): the other warps still meet it at the barriers below
             if (!dead && !warp_wait(smem_u32(bars + stage), phase, abort_flag)) {
                 dead = true;
                 *abort_flag = 1;
                 if (lane == 0) pages_flag(a.c, AERO_CUDA_PAGES_WAIT);
+            }
+            if (SEL && t >= t0 + cnt && (dead || box_at[stage * 8] == kNoMore)) {
+                __syncwarp();
+                if (lane == 0 && !dead) mbar_arrive(smem_u32(bars + ST + stage));
+                if (++stage == ST) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                break;
             }
             const uint32_t kb = ring + (uint32_t)stage * Cfg<D>::stage_bytes, vb = kb + (D / 64) * kHalf;
             // (two sums each, of the even and the odd steps: a shorter chain of products)

@@ -318,9 +318,8 @@ class PagedCache:
 
     def attend_blocks(self, layer: int, q, seqs, blocks, q_start=None, *, scale: Optional[float] = None, out=None):
         """Attention as `attend`'s, token by token, over the positions in the listed blocks: blocks (T, n_head_kv, any
-        number) int32 block numbers, in any order; negative ones and those past the token's own are passed over, one
-        listed twice counts twice, and no more entries are looked at than the token has blocks. A token
-        without a listed position has an output of zeros."""
+        number) int32 block numbers, in any order; negative ones and those past the token's own are passed over wherever
+        they stand, one listed twice counts twice. A token without a listed position has an output of zeros."""
         self._on()
         qp, q_token, q_head = self._rows(q, "q", None)
         T, H, _ = q.shape

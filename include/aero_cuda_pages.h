@@ -157,9 +157,9 @@ int aero_cuda_pages_select(void* cache, int layer, const void* q, int64_t q_toke
                            int32_t* blocks);
 /* Attention as attend's, token by token and exact as there, of kv head h's query heads of token t over the
  * positions up to the token's own in the blocks listed in blocks (T, n_head_kv, n_blocks), in any order.
- * Entries below 0 and past the token's own block are passed over, and of a list longer than the
- * number of the token's blocks only that many entries are looked at. A block listed twice counts twice. A
- * token none of whose positions is listed has an output of 0. */
+ * Every entry counts, wherever it stands: those below 0 and past the token's own block are passed over, a block listed
+ * twice counts twice. (Work is shared out by as many entries a list as the token has blocks; what is listed behind those,
+ * by one CTA a list.) A token none of whose positions is listed has an output of 0. */
 int aero_cuda_pages_attend_blocks(void* cache, int layer, const void* q, int64_t q_token, int64_t q_head, int T, int n_head,
                                   const int32_t* seqs, const int32_t* q_start, int n, const int32_t* blocks, int n_blocks,
                                   float scale, void* out, int64_t o_token, int64_t o_head);
