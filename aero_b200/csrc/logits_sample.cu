@@ -10,8 +10,9 @@
 //
 // Weights are whole numbers, multiples of 2^-B of the largest (B = 44 for a vocabulary of 2^18): their sums
 // are exact in any order, so histograms may be made by atomics and the answer does not depend on timing. Each weight is
-// computed in 64 bits and off by half of 2^-B at most, so a sum of V of them by V / 2 2^-B of the largest at the
-// very most (2^-27 for V = 2^18).
+// computed in 64 bits and off by half of 2^-B and by 2^-50 of the largest at most (y halvings below it by 2^-51 of itself for the
+// series, the table and the arithmetic, and by y 2^-52 for 1 / T's rounding), so a sum of V of them by V / 2 2^-B of the
+// largest and by 2^-47 of itself (in all 2^-27 of the largest for V = 2^18, if all weigh as much).
 //
 // A cluster of CTAs per row, each with an even share of the row, which it reads from HBM once, for the largest, and twice more
 // from L2, for the sums and for the members; the first CTA's shared memory holds the members. What crosses the cluster is 64
@@ -97,7 +98,7 @@ struct Row {
     float half_m, scale; // slice = (m / 2 - x / 2) * scale (halves: the difference of any two numbers is one)
     float step;          // a slice's width; infinity: m is too large for sums and differences of slices' ends
     float floor;         // a value of the last slice, next to its middle; -infinity: there is none
-    double per_t;        // 16 log2(e) / T
+    double per_t;        // 32 log2(e) / T
     double lift;         // 2^B
     u64 least;           // min_p 2^B
     __device__ __forceinline__ float open_place(float x) const { return fmaf(x, -0.5f, half_m) * scale; }
@@ -106,13 +107,13 @@ struct Row {
     __device__ __forceinline__ float slice(float x) const { return place(x) + 8388608.f; }
     __device__ __forceinline__ int bin(float x) const { return (int)(__float_as_uint(slice(x)) & (kBins - 1)); }
     // 2^52 + 2^B e^((x - m) / T), which leaves the weight's nearest whole number in the low bits (2^B is at most 2^48), for
-    // slices but the last. at = place(x). In sixteenths of a halving x lies z = 16 log2(e) (x - m) / T above m; with i the whole number
-    // next to -z and r = z + i, at most a half either way, the weight is 2^-(i / 16) 2^(r / 16): a table's value (2^B's sixteen parts,
-    // the halvings taken off its exponent) times the series of 2^(r / 16) to r^5, whose term in r^6 is made up for by Chebyshev's
-    // polynomial; what is left out is below 2^-46.
+    // slices but the last. at = place(x). In 32nds of a halving x lies z = 32 log2(e) (x - m) / T above m; with i the whole number
+    // next to -z and r = z + i, at most a half either way, the weight is 2^-(i / 32) 2^(r / 32): a table's value (2^B's 32 parts,
+    // the halvings taken off its exponent) times the series of 2^(r / 32) to r^5, whose term in r^6 is made up for by Chebyshev's
+    // polynomial; what is left out is below 2^-52 (with 16 parts 2^-46.6, 2.5 of 2^-48).
     __device__ __forceinline__ double beside(float x, float at, const double* table) const {
-        constexpr double L = 0.6931471805599453 / 16, h2 = 0.25, a5 = L * L * L * L * L * L / 720;
-        const float i = fmaf(at, 0.25f, 8388608.f);
+        constexpr double L = 0.6931471805599453 / 32, h2 = 0.25, a5 = L * L * L * L * L * L / 720;
+        const float i = fmaf(at, 0.5f, 8388608.f);
         const double z = fma((double)x - (double)m, per_t, (double)(i - 8388608.f));
         double p = fma(z, L * L * L * L * L / 120, L * L * L * L / 24 + 1.25 * h2 * a5);
         p = fma(p, z, L * L * L / 6);
@@ -120,8 +121,8 @@ struct Row {
         p = fma(p, z, L);
         p = fma(p, z, 1.0);
         const uint32_t n = __float_as_uint(i);
-        const double t = table[n & 15u];
-        return fma(p, __hiloint2double(__double2hiint(t) - (int)((n & ~15u) * 65536u), __double2loint(t)), kTwo52);
+        const double t = table[n & 31u];
+        return fma(p, __hiloint2double(__double2hiint(t) - (int)((n & ~31u) * 32768u), __double2loint(t)), kTwo52);
     }
     static __device__ __forceinline__ u64 whole(double beside) { return (u64)__double_as_longlong(beside) & 0xFFFFFFFFFFFFFull; }
     __device__ __forceinline__ u64 weight(float x, const double* table) const { return whole(beside(x, place(x), table)); }
@@ -167,7 +168,7 @@ struct Groups {
 };
 
 struct Shared {
-    double table[16];
+    double table[32];
     Slices first;             // of Row's slices
     Parts more;               // of one slice's keys, or of members' keys; the place of members on their way; else zero
     u64 member[kMembers];     // key, then all ones less the token's number (in the first CTA)
@@ -200,7 +201,7 @@ __device__ __forceinline__ Shared& shared() {
 }
 __device__ __noinline__ double log_of(double x) { return log(x); }
 __device__ __forceinline__ float logprob_of(const Row& r, float x, u64 kept) {
-    return (float)(((double)x - (double)r.m) * r.per_t * (0.6931471805599453 / 16) - log_of((double)kept / r.lift));
+    return (float)(((double)x - (double)r.m) * r.per_t * (0.6931471805599453 / 32) - log_of((double)kept / r.lift));
 }
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -1085,7 +1086,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     clear(s.first);
     clear(s.more);
     const double lift = __longlong_as_double((long long)(1023 + a.bits) << 52);
-    if (tid < 16) s.table[tid] = exp2(-tid / 16.0) * lift;
+    if (tid < 32) s.table[tid] = exp2(-tid / 32.0) * lift;
     stream_turn();
     const float T0 = a.temperature ? a.temperature[row] : 1.f, min_p = a.min_p ? a.min_p[row] : 0.f;
     const int k = a.top_k ? a.top_k[row] : 0;
@@ -1097,7 +1098,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         s.u = a.u[row];
         s.min_p = min_p;
         s.fresh = 1;
-        s.row.per_t = 23.083120654223414 / (double)fmaxf(T0, 7.8886091e-31f);  // 2^-100: what follows stays within f32's range
+        s.row.per_t = 46.166241308446828 / (double)fmaxf(T0, 7.8886091e-31f);  // 2^-100: what follows stays within f32's range
         s.find.k_slice = -1;
         s.find.k_before = s.find.k_members = 0;
     }
@@ -1136,8 +1137,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             r.per_t = s.row.per_t;
             r.lift = lift;
             r.least = min_p > 0.f ? min_p <= 1.f ? (u64)ceil((double)min_p * lift) : ~0ull : 0;
-            r.scale = (float)(8.0 * r.per_t);  // (64 slices to 16 sixteenths, for halves)
-            const float step = 0.25f / (float)r.per_t;
+            r.scale = (float)(4.0 * r.per_t);  // (64 slices to 32 parts, for halves)
+            const float step = 0.5f / (float)r.per_t;
             // (m a few million slices from 0 at most: sums and differences of slices' ends are off by a small part of one)
             const bool near = fabsf(r.m) < 4194304.f * step && step < 1e24f;
             r.step = near ? step : INFINITY;

@@ -206,8 +206,9 @@ int aero_cuda_logits_adjust_views(const void* logits, int64_t ld, int dtype, int
  * order (below 2^-100: as 2^-100). Logits of -infinity and those that are no number are never drawn; a row of nothing else gives -1 and
  * -infinity. With a logit of +infinity all others have weight 0. temperature (1), top_k, top_p and min_p may
  * be NULL. Weights are computed in 64 bits and summed as multiples of 2^-b of the largest, b = 62 less the bits of
- * vocab (48 at most, 44 for 2^18), so a weight below half of that is never drawn; the
- * result does not depend on timing. vocab is at most 2^22.
+ * vocab (48 at most, 44 for 2^18), so a weight below half of that is never drawn, and each is off by half of that and by
+ * 2^-50 of the largest at most: where u[r] times the sum, or the end of what a limit keeps, lies no further than these
+ * add up to from the border of two tokens, either may be taken. The result does not depend on timing. vocab is at most 2^22.
  * 0, or -1 with the reason in aero_cuda_moe_last_error(NULL). */
 int aero_cuda_logits_sample(const void* logits, int64_t ld, int dtype, int rows, int vocab, const float* u,
                             const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
