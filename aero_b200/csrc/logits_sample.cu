@@ -151,7 +151,7 @@ struct Search {
     uint32_t count_before;         // tokens before the slice in hand
     u64 limit;                     // the running sum, or number (kTopK, kPrefix), to be reached
     u64 mass_before, more_before;  // sums before the slice in hand; kBoth: and before slice b2
-    u64 total, kept, likely;       // sums: of the row, of the kept, of those that min_p keeps
+    u64 kept, likely;              // sums: of the kept, of those that min_p keeps
 };
 
 // A CTA's histogram of its tokens: sums as two words (or numbers, as the low one), numbers.
@@ -693,7 +693,6 @@ __device__ __noinline__ void look(bool first, bool sums, int C) {
                 } else {
                     u64 likely = 0;
                     for (int i = 0; i < C; ++i) likely += s.likely[i];
-                    f.total = total;
                     // (the first of the order is kept whatever min_p is)
                     f.likely = s.row.least ? max(likely, (u64)s.row.lift) : total;
                     if (f.k_slice < 0) next_goal(total);
