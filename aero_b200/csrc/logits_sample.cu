@@ -19,9 +19,9 @@
 // sums a CTA and 64 slices an answer: reads of another CTA's memory take some 13 cycles a warp's load (all
 // slices to all: 4000 to 14000 cycles).
 //
-// Bound, for many rows, by the weights' 64-bit arithmetic (64 rows of 151936, top-p: 52 us, of which 13 are the sums with 8
+// Bound, for many rows, by the weights' 64-bit arithmetic (64 rows of 151936, top-p: 51 us, of which 13 are the sums with 8
 // 64-bit operations in 32 instructions a token, 11 the other two passes from L2, some 11 the search, step after step);
-// for one row of 32000 by ten steps of some 2000 cycles one after another (12 us). Clusters of 16 gain 4 %
+// for one row of 32000 by ten steps of some 2000 cycles one after another (11.5 us). Clusters of 16 gain 4 %
 // for one row of 151936 and lose 10 % for 16 mixed ones.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -7,10 +7,11 @@
 //
 // Bound by HBM: every visible K and V row is read once (up to 16 query heads share it,
 // at most 16 operations a byte). Measured, time on the GPU: 48 sequences of 8192 to 32768 positions, 32
-// query heads on 4 kv heads of 128, 281 us (1.85 GB: 6.6 TB/s); one sequence of 4096 12.5 us, of 20 5.3 us,
+// query heads on 4 kv heads of 128, 289 us (1.85 GB: 6.4 TB/s); one sequence of 4096 12.9 us, of 20 5.3 us,
 // where a launch, the chain from lengths to pages to rows, and the join set the time. Over listed blocks: 48
-// sequences, 32 blocks of 64 positions a kv head, 42.5 us (199 MB: 4.7 TB/s); 2048 of one sequence's 32768
-// positions 10.5 us.
+// sequences, 32 blocks of 64 positions a kv head, 43.8 us (199 MB: 4.5 TB/s); 2048 of one sequence's 32768
+// positions 11.2 us. Lists wider than a sequence: 64 sequences of 20 positions, pages of 16, 6.1 us with lists as long as they are, 6.3
+// us with 128 entries, 8.1 us with 1000 (-1 behind).
 //
 // Split: the work of the call is one line of units, unit = 64 positions of one
 // (sequence, kv head); each CTA takes an equal piece of the line, wherever it begins, so

@@ -10,15 +10,21 @@
 // bounds are finite, so the part that is zero adds nothing). A wrong order of two scores is a wrong block, so what is
 // chosen has to follow from sums in 64 bits; those cost 64 products a cycle and SM at best (m8n8k4 products: 48
 // sequences of up to 512 blocks, 32 query heads, 16 us of scores). So every score is computed first in f32 (m16n8k16
-// products, the operands as they are), off by at most e = 17 2^-23 D / 8 max_g sum_d |q_gd| max |bounds|: D / 8 sums of 17
-// terms one after another, each term cut at 2^-23 of the largest. Only the blocks whose score lies within 2 e of where the least chosen one can
-// be are computed again in 64 bits, a handful; where they are many (blocks alike) all are.
+// products, the operands as they are), off by at most e = 17 2^-23 D / 8 M, M = max_g sum_d |q_gd| max |bounds|. A score is D / 8
+// sums of 17 terms (16 products, which are exact, and the sum so far) one after another, and no term or sum exceeds M. Terms are brought
+// to the largest one's exponent and cut there, each by 2^-23 of it at most. A sum with that exponent lies on the same grid and is cut no
+// further; of one with a higher exponent each of those cuts is half as much or less, so that with the sum's own they are
+// (17 / 2 + 1) 2^-23 of it. Measured on a B200, 4 10^8 sums (terms alike, spread, of one sign, one or the sum so far large): 4.0 2^-23 of the larger of the largest term and the sum, at
+// most. Only the blocks whose score lies within 2 e of where the least chosen one can be are computed again in 64 bits, a handful; where
+// they are many (blocks alike) all are.
 //
-// Bound by a chain of steps, not by bytes: one sequence of 2048 blocks, 32 query heads on 4 kv heads of 128, 13.2 us, 48
-// sequences of up to 512 blocks 18.8 us, 8 sequences with 1 to 9 tokens each 15.6 us, a launch included (all in 64 bits: 18.8, 38.6
-// and 34.8 us). Cycles of the first, from HBM: lengths and queries 4500, page numbers, bounds and products 9000, ends 2700, a
-// histogram 4200, blocks near the border and their scores 2800, their exchange 3000, their order and the list
-// 3900.
+// Bound by a chain of steps, not by bytes: one sequence of 2048 blocks, 32 query heads on 4 kv heads of 128, 12.7 us, 48
+// sequences of up to 512 blocks 18.6 us, 8 sequences with 1 to 9 tokens each 15.6 us, a launch included (all in 64 bits: 18.8, 38.6
+// and 34.8 us). Cycles of the first with its inputs in L2, as where that was measured (and from HBM): lengths and queries 2600
+// (4400), page numbers, bounds and products 4800 (7900), ends 2400 (2800), a histogram 3600 (3800), blocks near the border, their
+// scores and exchange 5800, their order 2800, the list 1100; in all 23,000 (28,500). So 7400 (12,300) of them, 12,600 of
+// 23,400 (23,100 of 34,100) for the 48 sequences, are reads one after another before the scores are there, of which the queries, the
+// page numbers and the bounds could be on their way at once; the rest are steps with a barrier each.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -401,7 +407,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const SelectArgs
             number &= sizes[i] < INFINITY;
             size = fmaxf(size, sizes[i]);
         }
-        const float off = size * bound * (5.12e-7f * D) + 2e-35f;  // 2 e, rounded up, and 2 * 17 * 32 times the least normal number for what underflows
+        const float off = size * bound * (5.12e-7f * D) + 2e-35f;  // 2 e (5.07e-7), rounded up, and 2 * 17 * 32 times the least normal number for what underflows
         if (number && off < 1e30f) {
             // ---- an interval that holds the least chosen score: a few blocks' or narrower than what they may be off
             int left = need;
